@@ -986,6 +986,19 @@ int cvae_decoder_backward_n(int nd, int cell, int B, int T, int E, int Hd, int64
   return decoder_backward_impl(nd, cell, B, T, E, Hd, go, q, demb, S(stream), (long)V);
 }
 
+// ------------------------------------------------------------------------------ gated linear recurrence
+int64_t cvae_linrnn_state_floats(int T, int B, int H) { return linrnn_bounds_floats(T, B, H); }
+int64_t cvae_linrnn_workspace(int dtype, int T, int B, int H) { return linrnn_workspace_floats(dtype, T, B, H); }
+int cvae_linrnn_forward(int dtype, int gates, int reverse, int T, int B, int H, const void* u, const float* h0,
+                        const int64_t* len, void* y, float* h_last, float* states, float* ws, void* stream) {
+  return launch_linrnn_forward(dtype, gates, reverse, T, B, H, u, h0, len, y, h_last, states, ws, S(stream));
+}
+int cvae_linrnn_backward(int dtype, int gates, int reverse, int T, int B, int H, const void* u, const int64_t* len,
+                         const float* states, const void* dy, const float* dh_last, void* du, float* dh0, float* ws,
+                         void* stream) {
+  return launch_linrnn_backward(dtype, gates, reverse, T, B, H, u, len, states, dy, dh_last, du, dh0, ws, S(stream));
+}
+
 // ------------------------------------------------------------------------------ projection + CE
 int64_t cvae_projce_workspace(int64_t N, int64_t E, int64_t V) {
   if (ce_fast_supported((int)E)) return ce_fast_workspace_floats(N, (int)V);

@@ -118,4 +118,13 @@ int launch_ce_fast_backward_n(int nd, const float* const* X, const float* const*
                               long N, long TR, int R, int E, int V, float* const* dX, float* const* dW,
                               float* const* db, float* ws, float* const* logits, hipStream_t s);
 
+// linrnn.hip: gated linear recurrence (dtype: dtype.hpp)
+long linrnn_bounds_floats(int T, int B, int H);
+long linrnn_workspace_floats(int dtype, int T, int B, int H);
+int launch_linrnn_forward(int dtype, int gates, int reverse, int T, int B, int H, const void* u, const float* h0,
+                          const int64_t* len, void* y, float* h_last, float* bounds, float* ws, hipStream_t s);
+int launch_linrnn_backward(int dtype, int gates, int reverse, int T, int B, int H, const void* u, const int64_t* len,
+                           const float* bounds, const void* dy, const float* dlast, void* du, float* dh0, float* ws,
+                           hipStream_t s);
+
 }  // namespace cvae

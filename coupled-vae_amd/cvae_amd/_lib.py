@@ -62,6 +62,10 @@ SIGNATURES = {
     'cvae_persist_status': [],
     'cvae_persist_status_peek': [],
     'cvae_persist_status_set': [I],
+    'cvae_linrnn_state_floats': [I, I, I],
+    'cvae_linrnn_workspace': [I, I, I, I],
+    'cvae_linrnn_forward': [I, I, I, I, I, I] + [P] * 8,
+    'cvae_linrnn_backward': [I, I, I, I, I, I] + [P] * 9,
     'cvae_projce_workspace': [L, L, L],
     'cvae_split_bf16': [I],
     'cvae_stream_rnn_min_bytes': [L],
@@ -98,7 +102,8 @@ SIGNATURES = {
 }
 _RESTYPE_LONG = {'cvae_encoder_backward_scratch', 'cvae_decoder_backward_scratch', 'cvae_projce_workspace',
                  'cvae_decoder_greedy_scratch', 'cvae_projce_logits_workspace', 'cvae_projce_backward_saved_n_workspace', 'cvae_decoder_beam_scratch',
-                 'cvae_projce_backward_workspace', 'cvae_mi_static_max_rows', 'cvae_stream_rnn_min_bytes'}
+                 'cvae_projce_backward_workspace', 'cvae_mi_static_max_rows', 'cvae_stream_rnn_min_bytes',
+                 'cvae_linrnn_state_floats', 'cvae_linrnn_workspace'}
 
 for _name, _args in SIGNATURES.items():
     _fn = getattr(lib, _name)          # AttributeError here = header and library out of sync

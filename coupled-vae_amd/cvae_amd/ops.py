@@ -1,7 +1,8 @@
 """torch.autograd wrappers around the C ABI (one Function per reference function on the path).
 
 torch is plumbing here: it owns device memory, the stream and the autograd tape; every
-number is produced by libcvae_hip kernels.  All tensors are fp32 / int64 on the GPU.
+number is produced by libcvae_hip kernels.  All tensors are fp32 / int64 on the GPU, unless an
+operator says that it takes bf16 / fp16 storage too.
 """
 import ctypes
 
@@ -26,6 +27,21 @@ def _c(t):
 
 def gates_of(cell):
     return 3 if cell == GRU else 4
+
+
+_DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # csrc/dtype.hpp
+
+
+def _need(ok, message):
+    if not ok:
+        raise ValueError(message)
+
+
+def _here(*tensors):
+    """Every tensor given is on the current GPU (the library launches on the current device's current stream)."""
+    for t in tensors:
+        if t is not None and (t.device.type != 'cuda' or t.device.index != torch.cuda.current_device()):
+            raise ValueError('tensor on %s, but the library works on the current GPU' % t.device)
 
 
 # --------------------------------------------------------------------------- a1 / a2
@@ -473,6 +489,83 @@ def decoder_pair(cell, go, emb, specs):
     for init, mi, mo, w in specs:
         flat += [init, mi, mo] + list(w)
     return DecoderPairFn.apply(cell, go, emb, *flat)
+
+
+# --------------------------------------------------------------------------- gated linear recurrence
+class LinearRnnFn(torch.autograd.Function):
+    """h_t = z h_(t-1) + (1 - z) n, y_t = o h_t over (T,B,gates*H) pre-activations (cvae_linrnn_*)."""
+
+    @staticmethod
+    def forward(ctx, u, gates, h0, length, reverse):
+        T, B, GH = u.shape
+        H = GH // gates
+        dt = _DTYPE[u.dtype]
+        y = torch.empty((T, B, H), dtype=u.dtype, device=u.device)
+        last = _f((B, H), u)
+        need_grad = any(ctx.needs_input_grad)
+        states = _f((query('cvae_linrnn_state_floats', T, B, H),), u) if need_grad else None
+        ws = _f((query('cvae_linrnn_workspace', dt, T, B, H),), u)
+        call('cvae_linrnn_forward', dt, gates, int(reverse), T, B, H, ptr(u), ptr(h0), ptr(length), ptr(y), ptr(last),
+             ptr(states), ptr(ws), stream())
+        if need_grad:
+            ctx.dims = (dt, gates, int(reverse), T, B, H)
+            ctx.save_for_backward(u, length, states)
+        return y, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dlast):
+        u, length, states = ctx.saved_tensors
+        T, B, H = ctx.dims[3:]
+        dy, dlast = _c(dy), _c(dlast)
+        du = torch.empty_like(u)
+        dh0 = _f((B, H), u) if ctx.needs_input_grad[2] else None
+        ws = _f((query('cvae_linrnn_workspace', ctx.dims[0], T, B, H),), u)
+        call('cvae_linrnn_backward', *ctx.dims, ptr(u), ptr(length), ptr(states), ptr(dy), ptr(dlast), ptr(du),
+             ptr(dh0), ptr(ws), stream())
+        return du, None, dh0, None, None
+
+
+def _linear_rnn_check(u, gates, h0, dims):
+    _need(gates in (2, 3), 'gates must be 2 or 3')
+    _need(u.dim() == dims, 'u must have %d dimensions' % dims)
+    _need(u.dtype in _DTYPE, 'u must be float32, bfloat16 or float16, not %s' % u.dtype)
+    _need(u.shape[-1] % gates == 0, 'the last dimension of u (%d) is no multiple of gates' % u.shape[-1])
+    if h0 is not None:
+        _need(h0.dtype == torch.float32 and tuple(h0.shape) == (u.shape[-2], u.shape[-1] // gates),
+              'the state must be float32 of shape (B, H)')
+
+
+def linear_rnn(u, gates, h0=None, length=None, reverse=False):
+    """Gated linear recurrence over time-major pre-activations u (T,B,gates*H) in fp32, bf16 or fp16:
+    rows z | n | o (gates = 3) or z | n (gates = 2, no output gate);
+    h_t = sigmoid(z) h_(t-1) + (1 - sigmoid(z)) tanh(n), y_t = sigmoid(o) h_t.
+    h0 (B,H) fp32 or None (zeros); length (B,) int64 or None: row b takes its first length[b] steps, backwards from
+    the last of them if `reverse`; y and the gradient are zero past them.
+    -> y (T,B,H) of u's type, the state after each row's last step (B,H) fp32.  Differentiable in u and h0."""
+    _linear_rnn_check(u, gates, h0, 3)
+    if length is not None:
+        _need(length.dtype == torch.int64 and tuple(length.shape) == (u.shape[1],), 'length must be int64 of shape (B,)')
+    _here(u, h0, length)
+    return LinearRnnFn.apply(_c(u), gates, _c(h0), _c(length), reverse)
+
+
+def linear_rnn_step(u, gates, h, out=None):
+    """One decoding step of linear_rnn: u (B,gates*H), state h (B,H) fp32 -> y (B,H) of u's type, the new state
+    (B,H) fp32 (written to `out` if given; out = h updates it in place).  No gradient."""
+    _linear_rnn_check(u, gates, h, 2)
+    _need(h is not None, 'the state is missing')
+    B, H = h.shape
+    if out is None:
+        out = _f((B, H), u)
+    _need(out.dtype == torch.float32 and out.shape == h.shape and out.is_contiguous(),
+          'out must be contiguous float32 of shape (B, H)')
+    _here(u, h, out)
+    u, h = _c(u), _c(h)
+    y = torch.empty((B, H), dtype=u.dtype, device=u.device)
+    call('cvae_linrnn_forward', _DTYPE[u.dtype], gates, 0, 1, B, H, ptr(u), ptr(h), None, ptr(y), ptr(out), None, None,
+         stream())
+    return y, out
 
 
 # --------------------------------------------------------------------------- projection + CE

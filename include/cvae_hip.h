@@ -196,6 +196,24 @@ int cvae_decoder_backward_n(int nd, int cell, int B, int T, int E, int Hd, int64
                             const float* const* dfinal, float* const* dinit, float* const* dw, float* demb,
                             float* const* scratch, void* stream);
 
+/* ---- gated linear recurrence (no reference counterpart: a layer beside GRU / LSTM whose step has no product with
+ * the state, so a sequence is a scan and long ones run in parallel over time):
+ *   z = sigmoid(u_z), n = tanh(u_n), o = sigmoid(u_o):  h_t = z h_(t-1) + (1 - z) n,  y_t = o h_t
+ * dtype: storage of u, y, dy, du: 0 = fp32, 1 = bf16, 2 = fp16 (the state, h0, h_last and their gradients are fp32).
+ * gates: 3 = rows z|n|o, 2 = rows z|n (y_t = h_t).  u[T,B,gates*H], h0[B,H] or NULL (zeros), len[B] or NULL (all T; a
+ * value outside [0,T] counts as the nearer end): row b takes steps t < len[b] -- upwards, or with reverse != 0 downwards
+ * from len[b]-1 -- and past them y = 0, the state is carried and du = 0.  y[T,B,H], h_last[B,H] (may be h0: in place).
+ * states: NULL, or cvae_linrnn_state_floats floats that the backward call reads (the state every 64 steps).
+ * ws: cvae_linrnn_workspace floats (0: may be NULL). */
+int64_t cvae_linrnn_state_floats(int T, int B, int H);
+int64_t cvae_linrnn_workspace(int dtype, int T, int B, int H);
+int cvae_linrnn_forward(int dtype, int gates, int reverse, int T, int B, int H, const void* u, const float* h0,
+                        const int64_t* len, void* y, float* h_last, float* states, float* ws, void* stream);
+/* dy[T,B,H], dh_last[B,H] or NULL (zeros) -> du[T,B,gates*H], dh0[B,H] (may be NULL), both overwritten. */
+int cvae_linrnn_backward(int dtype, int gates, int reverse, int T, int B, int H, const void* u, const int64_t* len,
+                         const float* states, const void* dy, const float* dh_last, void* du, float* dh0, float* ws,
+                         void* stream);
+
 /* ---- a7 tail + a8: ToVocab + SeqLoss(keep_batch=True) (Modules/vae_couple.py:119,
  * Modules/Losses/SeqLoss.py:36-44), fused: logits are never materialised, and rows whose target
  * is `pad` (loss 0, gradient 0 in the reference) are never multiplied.

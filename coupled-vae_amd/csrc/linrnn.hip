@@ -45,7 +45,7 @@ __device__ __forceinline__ void sigmoid_pair(float x, float& s, float& c) {
 }
 // tanh: its series to x^9 below 0.3 (next term < 6e-8 relative), else from exp (1 - 2 / (1 + e^2x) keeps only an
 // absolute 1e-7, too little near zero)
-__device__ __forceinline__ float tanh_pair(float x) {
+__device__ __forceinline__ float tanh_full(float x) {
   const float q = x * x;
   const float p = x * fmaf(q, fmaf(q, fmaf(q, fmaf(q, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
   return fabsf(x) < 0.3f ? p : tanh_fast(x);
@@ -59,15 +59,15 @@ template <typename T, int VW> __device__ __forceinline__ Packed<T, VW> ld(const 
 template <int VW> struct Lane {
   long c;            // first channel (b * H + j)
   bool valid;
-  long base, hbase;  // offset of (b, j) inside a step of u / of y
+  int base, hbase;   // offset of (b, j) inside a step of u / of y (below 2^31: checked by the launchers)
   int len;
   __device__ Lane(const LinRnnArgs& p, int lane) {
     c = ((long)blockIdx.x * 64 + lane) * VW;
     valid = c < p.n;
     if (!valid) c = 0;
     const long b = c / p.H, j = c - b * p.H;
-    base = b * p.gates * p.H + j;
-    hbase = c;
+    base = (int)(b * p.gates * p.H + j);
+    hbase = (int)c;
     long l = p.len ? p.len[b] : (long)p.T;
     len = (int)(l < 0 ? 0 : (l > p.T ? p.T : l));
   }
@@ -111,55 +111,67 @@ __device__ __forceinline__ void enter_segment(const LinRnnArgs& p, const Lane<VW
   __syncthreads();
 }
 
+// What a wave finds in its LR_C steps: every lane inside its row (addresses are then one scalar row pointer plus a lane
+// offset, nothing is masked), no lane (nothing is read), or a mixture.  The same for all lanes of the wave.
+enum Steps { ST_FULL, ST_MIXED, ST_DEAD };
+template <int VW> __device__ __forceinline__ Steps steps_of(const LinRnnArgs& p, const Lane<VW>& L, int w0, int w1) {
+  if (w0 >= w1) return ST_DEAD;
+  const int ta = time_of(p, w0), tb = time_of(p, w1 - 1), lo = ta < tb ? ta : tb, hi = ta < tb ? tb : ta;
+  if (w1 - w0 == LR_C && __all(hi < L.len)) return ST_FULL;
+  return __any(lo < L.len) ? ST_MIXED : ST_DEAD;
+}
+// rows of steps w0 .. w0 + LR_C of `src` (a lane's channels at `off` of a step): where not all are live, a step past a
+// row's end reads the row's last live step instead (in cache by then) and is masked by its reader
+template <typename T, int VW>
+__device__ __forceinline__ void load_steps(const LinRnnArgs& p, const Lane<VW>& L, bool full, const void* src,
+                                           long step, int off, int w0, Packed<T, VW> (&r)[LR_C]) {
+  const T* q = static_cast<const T*>(src);
+  if (full) {
+#pragma unroll
+    for (int i = 0; i < LR_C; ++i) r[i] = ld<T, VW>(q + (long)time_of(p, w0 + i) * step + (unsigned)off);
+  } else {
+#pragma unroll
+    for (int i = 0; i < LR_C; ++i) r[i] = ld<T, VW>(q + (long)clamp_time(time_of(p, w0 + i), L.len, p.T) * step + off);
+  }
+}
+
 // the maps of every segment.  BACK: of the backward carry (z, o, dy), else of the state (z, n).
-template <typename T, int VW, bool BACK>
+template <typename T, int VW, int G, bool BACK>
 __global__ __launch_bounds__(64 * LR_W) void linrnn_maps_kernel(LinRnnArgs p) {
   __shared__ float lds[LR_W][2][64 * VW];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
   const Lane<VW> L(p, lane);
   const int seg = blockIdx.y;
   const int s0 = seg * p.seg, s1 = min(p.T, s0 + p.seg);
   const int per = ((s1 - s0 + nw - 1) / nw + LR_C - 1) / LR_C * LR_C;
   const int w0 = s0 + wave * per, w1 = min(s1, w0 + per);
-  const T* u = static_cast<const T*>(p.u);
-  const T* dyp = static_cast<const T*>(p.dy);
-  const long ustep = (long)p.B * p.gates * p.H;
+  const long ustep = (long)p.B * G * p.H;
   float a[VW], x[VW];
 #pragma unroll
   for (int v = 0; v < VW; ++v) { a[v] = 1.f; x[v] = 0.f; }
-  for (int i0 = 0; w0 + i0 < w1; i0 += LR_C) {
+  const int rounds = w1 > w0 ? (w1 - w0 + LR_C - 1) / LR_C : 0;
+  for (int r = 0; r < rounds; ++r) {
+    const int c0 = w0 + (BACK ? rounds - 1 - r : r) * LR_C, c1 = min(w1, c0 + LR_C);
+    const Steps st = steps_of<VW>(p, L, c0, c1);
+    if (st == ST_DEAD) continue;
     Packed<T, VW> rz[LR_C], rn[LR_C], ro[LR_C];
-#pragma unroll
-    for (int i = 0; i < LR_C; ++i) {
-      const int k = i0 + i;
-      const int s = BACK ? w1 - 1 - k : w0 + k;
-      const long t = clamp_time(time_of(p, max(s, 0)), L.len, p.T);
-      const T* q = u + t * ustep + L.base;
-      rz[i] = ld<T, VW>(q);
-      if (BACK) {
-        rn[i] = ld<T, VW>(dyp + t * p.n + L.hbase);
-        if (p.gates == 3) ro[i] = ld<T, VW>(q + 2 * p.H);
-      } else {
-        rn[i] = ld<T, VW>(q + p.H);
-      }
+    load_steps<T, VW>(p, L, st == ST_FULL, p.u, ustep, L.base, c0, rz);
+    if (BACK) {
+      load_steps<T, VW>(p, L, st == ST_FULL, p.dy, p.n, L.hbase, c0, rn);
+      if (G == 3) load_steps<T, VW>(p, L, st == ST_FULL, p.u, ustep, L.base + 2 * p.H, c0, ro);
+    } else {
+      load_steps<T, VW>(p, L, st == ST_FULL, p.u, ustep, L.base + p.H, c0, rn);
     }
 #pragma unroll
-    for (int i = 0; i < LR_C; ++i) {
-      const int k = i0 + i;
-      const int s = BACK ? w1 - 1 - k : w0 + k;
-      const bool live = s >= w0 && s < w1 && time_of(p, s) < L.len;
+    for (int k = 0; k < LR_C; ++k) {
+      const int i = BACK ? LR_C - 1 - k : k;
+      const bool live = st == ST_FULL || (c0 + i < c1 && time_of(p, c0 + i) < L.len);
 #pragma unroll
       for (int v = 0; v < VW; ++v) {
-        float z, c;
+        float z, c, in;
         sigmoid_pair(rz[i].f(v), z, c);
-        float in;
-        if (BACK) {
-          in = rn[i].f(v);
-          if (p.gates == 3) { float o, oc; sigmoid_pair(ro[i].f(v), o, oc); in *= o; }
-          in *= z;
-        } else {
-          in = c * tanh_pair(rn[i].f(v));
-        }
+        if (BACK) in = z * (G == 3 ? rn[i].f(v) * sigmoid_fast(ro[i].f(v)) : rn[i].f(v));
+        else in = c * tanh_full(rn[i].f(v));
         if (live) { x[v] = fmaf(z, x[v], in); a[v] *= z; }
       }
     }
@@ -168,69 +180,72 @@ __global__ __launch_bounds__(64 * LR_W) void linrnn_maps_kernel(LinRnnArgs p) {
   for (int v = 0; v < VW; ++v) { lds[wave][0][lane * VW + v] = a[v]; lds[wave][1][lane * VW + v] = x[v]; }
   __syncthreads();
   if (wave == 0 && L.valid) {
-    for (int i = 1; i < nw; ++i) {
-      const int w = BACK ? nw - 1 - i : i;
-#pragma unroll
-      for (int v = 0; v < VW; ++v) {
-        if (i == 1 && BACK) { a[v] = lds[nw - 1][0][lane * VW + v]; x[v] = lds[nw - 1][1][lane * VW + v]; }
-        const float a2 = lds[w][0][lane * VW + v], x2 = lds[w][1][lane * VW + v];
-        x[v] = fmaf(a2, x[v], x2);
-        a[v] *= a2;
-      }
-    }
     float* g = p.agg + (long)seg * 2 * p.n + L.c;
 #pragma unroll
-    for (int v = 0; v < VW; ++v) { g[v] = a[v]; g[p.n + v] = x[v]; }
+    for (int v = 0; v < VW; ++v) {
+      float A = 1.f, X = 0.f;
+      for (int i = 0; i < nw; ++i) {
+        const int w = BACK ? nw - 1 - i : i;
+        const float a2 = lds[w][0][lane * VW + v], x2 = lds[w][1][lane * VW + v];
+        X = fmaf(a2, X, x2);
+        A *= a2;
+      }
+      g[v] = A;
+      g[p.n + v] = X;
+    }
   }
 }
 
-template <typename T, int VW>
+template <typename T, int VW, int G>
 __global__ __launch_bounds__(64 * LR_W) void linrnn_fwd_kernel(LinRnnArgs p) {
   __shared__ float lds[2][LR_W][2][64 * VW];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
   const Lane<VW> L(p, lane);
   const int seg = blockIdx.y;
   const int s0 = seg * p.seg, s1 = min(p.T, s0 + p.seg);
-  const T* u = static_cast<const T*>(p.u);
   T* y = static_cast<T*>(p.y);
-  const long ustep = (long)p.B * p.gates * p.H;
+  const long ustep = (long)p.B * G * p.H;
   float carry[VW];                                // the state before this block's next 64 steps, in every wave
 #pragma unroll
   for (int v = 0; v < VW; ++v) carry[v] = p.h0 ? p.h0[L.c + v] : 0.f;
   if (seg > 0) enter_segment<VW>(p, L, seg, false, wave, nw, lane, lds[0], carry);
   int buf = 0;
   for (int sc = s0; sc < s1; sc += LR_C * nw, buf ^= 1) {
-    const int w0 = sc + wave * LR_C;
-    Packed<T, VW> rz[LR_C], rn[LR_C], ro[LR_C];
+    const int w0 = sc + wave * LR_C, w1 = min(s1, w0 + LR_C);
+    const Steps st = steps_of<VW>(p, L, w0, w1);
+    float a[LR_C][VW], x[LR_C][VW], A[VW], X[VW];
+    Packed<T, VW> ro[LR_C];
 #pragma unroll
-    for (int i = 0; i < LR_C; ++i) {
-      const long t = clamp_time(time_of(p, w0 + i), L.len, p.T);
-      const T* q = u + t * ustep + L.base;
-      rz[i] = ld<T, VW>(q);
-      rn[i] = ld<T, VW>(q + p.H);
-      if (p.gates == 3) ro[i] = ld<T, VW>(q + 2 * p.H);
+    for (int v = 0; v < VW; ++v) { A[v] = 1.f; X[v] = 0.f; }
+    if (st != ST_DEAD) {
+      Packed<T, VW> rz[LR_C], rn[LR_C];
+      load_steps<T, VW>(p, L, st == ST_FULL, p.u, ustep, L.base, w0, rz);
+      load_steps<T, VW>(p, L, st == ST_FULL, p.u, ustep, L.base + p.H, w0, rn);
+      if (G == 3) load_steps<T, VW>(p, L, st == ST_FULL, p.u, ustep, L.base + 2 * p.H, w0, ro);
+#pragma unroll
+      for (int i = 0; i < LR_C; ++i)
+#pragma unroll
+        for (int v = 0; v < VW; ++v) {
+          float c;
+          sigmoid_pair(rz[i].f(v), a[i][v], c);
+          x[i][v] = c * tanh_full(rn[i].f(v));
+        }
+      if (st == ST_MIXED) {
+#pragma unroll
+        for (int i = 0; i < LR_C; ++i)
+          if (!(w0 + i < w1 && time_of(p, w0 + i) < L.len)) {
+#pragma unroll
+            for (int v = 0; v < VW; ++v) { a[i][v] = 1.f; x[i][v] = 0.f; }
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < LR_C; ++i)
+#pragma unroll
+        for (int v = 0; v < VW; ++v) { X[v] = fmaf(a[i][v], X[v], x[i][v]); A[v] *= a[i][v]; }
     }
     if (p.bounds && wave == 0 && L.valid && sc % (LR_C * LR_W) == 0) {
 #pragma unroll
       for (int v = 0; v < VW; ++v) p.bounds[(long)(sc / (LR_C * LR_W)) * p.n + L.c + v] = carry[v];
-    }
-    float a[LR_C][VW], x[LR_C][VW], A[VW], X[VW];
-#pragma unroll
-    for (int v = 0; v < VW; ++v) { A[v] = 1.f; X[v] = 0.f; }
-#pragma unroll
-    for (int i = 0; i < LR_C; ++i) {
-      const int s = w0 + i;
-      const bool live = s < s1 && time_of(p, s) < L.len;
-#pragma unroll
-      for (int v = 0; v < VW; ++v) {
-        float z, c;
-        sigmoid_pair(rz[i].f(v), z, c);
-        const float in = c * tanh_pair(rn[i].f(v));
-        a[i][v] = live ? z : 1.f;
-        x[i][v] = live ? in : 0.f;
-        X[v] = fmaf(a[i][v], X[v], x[i][v]);
-        A[v] *= a[i][v];
-      }
     }
 #pragma unroll
     for (int v = 0; v < VW; ++v) { lds[buf][wave][0][lane * VW + v] = A[v]; lds[buf][wave][1][lane * VW + v] = X[v]; }
@@ -245,19 +260,22 @@ __global__ __launch_bounds__(64 * LR_W) void linrnn_fwd_kernel(LinRnnArgs p) {
       for (int v = 0; v < VW; ++v)
         carry[v] = fmaf(lds[buf][w][0][lane * VW + v], carry[v], lds[buf][w][1][lane * VW + v]);
     }
+    if (st == ST_DEAD) {
+      for (int s = w0; s < w1; ++s)
+        if (L.valid) *reinterpret_cast<Packed<T, VW>*>(y + (long)time_of(p, s) * p.n + (unsigned)L.hbase) = Packed<T, VW>{};
+      continue;
+    }
 #pragma unroll
     for (int i = 0; i < LR_C; ++i) {
       const int s = w0 + i, t = time_of(p, s);
-      const bool live = s < s1 && t < L.len;
       Packed<T, VW> out;
 #pragma unroll
       for (int v = 0; v < VW; ++v) {
         h[v] = fmaf(a[i][v], h[v], x[i][v]);
-        float o = 1.f;
-        if (p.gates == 3) { float oc; sigmoid_pair(ro[i].f(v), o, oc); }
-        out.set(v, live ? o * h[v] : 0.f);
+        out.set(v, G == 3 ? sigmoid_fast(ro[i].f(v)) * h[v] : h[v]);
       }
-      if (s < s1 && L.valid) *reinterpret_cast<Packed<T, VW>*>(y + (long)t * p.n + L.hbase) = out;
+      if (st == ST_MIXED && t >= L.len) out = Packed<T, VW>{};
+      if (s < w1 && L.valid) *reinterpret_cast<Packed<T, VW>*>(y + (long)t * p.n + (unsigned)L.hbase) = out;
     }
   }
   if (seg == p.nseg - 1 && wave == 0 && L.valid) {
@@ -266,17 +284,16 @@ __global__ __launch_bounds__(64 * LR_W) void linrnn_fwd_kernel(LinRnnArgs p) {
   }
 }
 
-template <typename T, int VW>
-__global__ __launch_bounds__(64 * LR_W) void linrnn_bwd_kernel(LinRnnArgs p) {
+// four waves on a SIMD (two blocks on a CU): 128 registers
+template <typename T, int VW, int G>
+__global__ __launch_bounds__(64 * LR_W, 4) void linrnn_bwd_kernel(LinRnnArgs p) {
   __shared__ float lds[2][LR_W][3][64 * VW];      // A (both directions), X of the state, X of the carry
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
   const Lane<VW> L(p, lane);
   const int seg = blockIdx.y;
   const int s0 = seg * p.seg, s1 = min(p.T, s0 + p.seg);
-  const T* u = static_cast<const T*>(p.u);
-  const T* dyp = static_cast<const T*>(p.dy);
   T* du = static_cast<T*>(p.du);
-  const long ustep = (long)p.B * p.gates * p.H;
+  const long ustep = (long)p.B * G * p.H;
   float carry[VW];                                // gradient of the state after this block's steps
 #pragma unroll
   for (int v = 0; v < VW; ++v) carry[v] = p.dlast ? p.dlast[L.c + v] : 0.f;
@@ -285,42 +302,47 @@ __global__ __launch_bounds__(64 * LR_W) void linrnn_bwd_kernel(LinRnnArgs p) {
   int buf = 0;
   const int R = LR_C * nw;                        // steps of a round: 64, or the whole of a shorter sequence
   for (int sc = s0 + (s1 - s0 - 1) / R * R; sc >= s0; sc -= R, buf ^= 1) {
-    const int w0 = sc + wave * LR_C;
-    Packed<T, VW> rz[LR_C], rn[LR_C], ro[LR_C], rd[LR_C];
-#pragma unroll
-    for (int i = 0; i < LR_C; ++i) {
-      const long t = clamp_time(time_of(p, w0 + i), L.len, p.T);
-      const T* q = u + t * ustep + L.base;
-      rz[i] = ld<T, VW>(q);
-      rn[i] = ld<T, VW>(q + p.H);
-      rd[i] = ld<T, VW>(dyp + t * p.n + L.hbase);
-      if (p.gates == 3) ro[i] = ld<T, VW>(q + 2 * p.H);
-    }
+    const int w0 = sc + wave * LR_C, w1 = min(s1, w0 + LR_C);
+    const Steps st = steps_of<VW>(p, L, w0, w1);
     float hin[VW];
 #pragma unroll
     for (int v = 0; v < VW; ++v) hin[v] = p.bounds[(long)(sc / (LR_C * LR_W)) * p.n + L.c + v];
     float z[LR_C][VW], c[LR_C][VW], n[LR_C][VW], o[LR_C][VW], A[VW], X[VW], Q[VW];
+    Packed<T, VW> rd[LR_C];
 #pragma unroll
     for (int v = 0; v < VW; ++v) { A[v] = 1.f; X[v] = 0.f; Q[v] = 0.f; }
+    if (st != ST_DEAD) {
+      Packed<T, VW> rz[LR_C], rn[LR_C], ro[LR_C];
+      load_steps<T, VW>(p, L, st == ST_FULL, p.u, ustep, L.base, w0, rz);
+      load_steps<T, VW>(p, L, st == ST_FULL, p.u, ustep, L.base + p.H, w0, rn);
+      if (G == 3) load_steps<T, VW>(p, L, st == ST_FULL, p.u, ustep, L.base + 2 * p.H, w0, ro);
+      load_steps<T, VW>(p, L, st == ST_FULL, p.dy, p.n, L.hbase, w0, rd);
 #pragma unroll
-    for (int i = 0; i < LR_C; ++i) {
-      const int s = w0 + i;
-      const bool live = s < s1 && time_of(p, s) < L.len;
+      for (int i = 0; i < LR_C; ++i)
 #pragma unroll
-      for (int v = 0; v < VW; ++v) {
-        sigmoid_pair(rz[i].f(v), z[i][v], c[i][v]);
-        n[i][v] = tanh_pair(rn[i].f(v));
-        o[i][v] = 1.f;
-        if (p.gates == 3) { float oc; sigmoid_pair(ro[i].f(v), o[i][v], oc); }
-        if (!live) { z[i][v] = 1.f; c[i][v] = 0.f; n[i][v] = 0.f; o[i][v] = 0.f; rd[i].set(v, 0.f); }
-        X[v] = fmaf(z[i][v], X[v], c[i][v] * n[i][v]);
-        A[v] *= z[i][v];
+        for (int v = 0; v < VW; ++v) {
+          sigmoid_pair(rz[i].f(v), z[i][v], c[i][v]);
+          n[i][v] = tanh_full(rn[i].f(v));
+          o[i][v] = G == 3 ? sigmoid_fast(ro[i].f(v)) : 1.f;
+        }
+      if (st == ST_MIXED) {
+#pragma unroll
+        for (int i = 0; i < LR_C; ++i)
+          if (!(w0 + i < w1 && time_of(p, w0 + i) < L.len)) {
+#pragma unroll
+            for (int v = 0; v < VW; ++v) { z[i][v] = 1.f; c[i][v] = 0.f; n[i][v] = 0.f; o[i][v] = 0.f; }
+            rd[i] = Packed<T, VW>{};
+          }
       }
+#pragma unroll
+      for (int i = 0; i < LR_C; ++i)
+#pragma unroll
+        for (int v = 0; v < VW; ++v) { X[v] = fmaf(z[i][v], X[v], c[i][v] * n[i][v]); A[v] *= z[i][v]; }
+#pragma unroll
+      for (int i = LR_C - 1; i >= 0; --i)
+#pragma unroll
+        for (int v = 0; v < VW; ++v) Q[v] = z[i][v] * (G == 3 ? fmaf(rd[i].f(v), o[i][v], Q[v]) : rd[i].f(v) + Q[v]);
     }
-#pragma unroll
-    for (int i = LR_C - 1; i >= 0; --i)
-#pragma unroll
-      for (int v = 0; v < VW; ++v) Q[v] = z[i][v] * fmaf(rd[i].f(v), o[i][v], Q[v]);
 #pragma unroll
     for (int v = 0; v < VW; ++v) {
       lds[buf][wave][0][lane * VW + v] = A[v];
@@ -342,35 +364,42 @@ __global__ __launch_bounds__(64 * LR_W) void linrnn_bwd_kernel(LinRnnArgs p) {
       for (int v = 0; v < VW; ++v)
         carry[v] = fmaf(lds[buf][w][0][lane * VW + v], carry[v], lds[buf][w][2][lane * VW + v]);
     }
-    float hp[LR_C][VW];                           // h before each step
+    if (st == ST_DEAD) {
+      for (int s = w0; s < w1; ++s)
+        if (L.valid) {
+          T* q = du + (long)time_of(p, s) * ustep + (unsigned)L.base;
+#pragma unroll
+          for (int g = 0; g < G; ++g) *reinterpret_cast<Packed<T, VW>*>(q + g * p.H) = Packed<T, VW>{};
+        }
+      continue;
+    }
+    float hp[LR_C + 1][VW];                       // h before each step
+#pragma unroll
+    for (int v = 0; v < VW; ++v) hp[0][v] = hin[v];
 #pragma unroll
     for (int i = 0; i < LR_C; ++i)
 #pragma unroll
-      for (int v = 0; v < VW; ++v) {
-        hp[i][v] = hin[v];
-        hin[v] = fmaf(z[i][v], hin[v], c[i][v] * n[i][v]);
-      }
+      for (int v = 0; v < VW; ++v) hp[i + 1][v] = fmaf(z[i][v], hp[i][v], c[i][v] * n[i][v]);
 #pragma unroll
     for (int i = LR_C - 1; i >= 0; --i) {
       const int s = w0 + i, t = time_of(p, s);
-      const bool live = s < s1 && t < L.len;
       Packed<T, VW> gz, gn, go;
 #pragma unroll
       for (int v = 0; v < VW; ++v) {
-        const float dyv = rd[i].f(v), zz = z[i][v], cc = c[i][v], nn = n[i][v];
-        const float delta = fmaf(dyv, o[i][v], d[v]);
-        const float hh = fmaf(zz, hp[i][v], cc * nn);
-        // a step past the row's end gives exact zeros, whatever its carry holds
-        gz.set(v, live ? delta * (hp[i][v] - nn) * zz * cc : 0.f);
-        gn.set(v, live ? delta * cc * fmaf(-nn, nn, 1.f) : 0.f);
-        go.set(v, live ? dyv * hh * o[i][v] * (1.f - o[i][v]) : 0.f);
+        const float dyo = rd[i].f(v) * o[i][v], zz = z[i][v], cc = c[i][v], nn = n[i][v];
+        const float delta = (G == 3 ? dyo : rd[i].f(v)) + d[v];
+        const float into = delta * cc;
+        gz.set(v, into * (hp[i][v] - nn) * zz);
+        gn.set(v, into * fmaf(-nn, nn, 1.f));
+        if (G == 3) go.set(v, dyo * hp[i + 1][v] * (1.f - o[i][v]));
         d[v] = zz * delta;
       }
-      if (s < s1 && L.valid) {
-        T* q = du + (long)t * ustep + L.base;
+      if (st == ST_MIXED && t >= L.len) gz = gn = go = Packed<T, VW>{};   // exact zeros, whatever the carry holds
+      if (s < w1 && L.valid) {
+        T* q = du + (long)t * ustep + (unsigned)L.base;
         *reinterpret_cast<Packed<T, VW>*>(q) = gz;
         *reinterpret_cast<Packed<T, VW>*>(q + p.H) = gn;
-        if (p.gates == 3) *reinterpret_cast<Packed<T, VW>*>(q + 2 * p.H) = go;
+        if (G == 3) *reinterpret_cast<Packed<T, VW>*>(q + 2 * p.H) = go;
       }
     }
   }
@@ -397,7 +426,7 @@ __global__ __launch_bounds__(256) void linrnn_step_kernel(LinRnnArgs p) {
   for (int v = 0; v < VW; ++v) {
     float z, k, o = 1.f, oc;
     sigmoid_pair(rz.f(v), z, k);
-    h[v] = fmaf(z, h[v], k * tanh_pair(rn.f(v)));
+    h[v] = fmaf(z, h[v], k * tanh_full(rn.f(v)));
     if (p.gates == 3) sigmoid_pair(ro.f(v), o, oc);
     out.set(v, o * h[v]);
     p.h_last[c + v] = h[v];
@@ -426,7 +455,7 @@ long linrnn_workspace_floats(int dtype, int T, int B, int H) {
   return nseg > 1 ? 2L * nseg * B * H : 0;
 }
 
-template <typename T, int VW> static int lr_launch(LinRnnArgs a, bool back, hipStream_t s) {
+template <typename T, int VW, int G> static int lr_launch(LinRnnArgs a, bool back, hipStream_t s) {
   const dim3 grid((unsigned)((a.n + 64 * VW - 1) / (64 * VW)), a.nseg);
   const int nw = a.T >= LR_C * LR_W ? LR_W : (a.T > 0 ? cdiv(a.T, LR_C) : 1);
   if (!back && a.T == 1 && !a.bounds && !a.len) {
@@ -435,23 +464,27 @@ template <typename T, int VW> static int lr_launch(LinRnnArgs a, bool back, hipS
     return 0;
   }
   if (a.nseg > 1) {
-    if (back) hipLaunchKernelGGL((linrnn_maps_kernel<T, VW, true>), grid, dim3(64 * nw), 0, s, a);
-    else hipLaunchKernelGGL((linrnn_maps_kernel<T, VW, false>), grid, dim3(64 * nw), 0, s, a);
+    if (back) hipLaunchKernelGGL((linrnn_maps_kernel<T, VW, G, true>), grid, dim3(64 * nw), 0, s, a);
+    else hipLaunchKernelGGL((linrnn_maps_kernel<T, VW, G, false>), grid, dim3(64 * nw), 0, s, a);
     CVAE_LAUNCH_CHECK("linrnn_maps_kernel");
   }
-  if (back) hipLaunchKernelGGL((linrnn_bwd_kernel<T, VW>), grid, dim3(64 * nw), 0, s, a);
-  else hipLaunchKernelGGL((linrnn_fwd_kernel<T, VW>), grid, dim3(64 * nw), 0, s, a);
+  if (back) hipLaunchKernelGGL((linrnn_bwd_kernel<T, VW, G>), grid, dim3(64 * nw), 0, s, a);
+  else hipLaunchKernelGGL((linrnn_fwd_kernel<T, VW, G>), grid, dim3(64 * nw), 0, s, a);
   CVAE_LAUNCH_CHECK("linrnn kernel");
   return 0;
+}
+
+template <typename T, int VW> static int lr_gates(const LinRnnArgs& a, bool back, hipStream_t s) {
+  return a.gates == 3 ? lr_launch<T, VW, 3>(a, back, s) : lr_launch<T, VW, 2>(a, back, s);
 }
 
 static int lr_dispatch(int dtype, const LinRnnArgs& a, bool back, hipStream_t s) {
   // two channels a lane need rows that stay 4-byte aligned: an even H and operands on 4-byte boundaries
   const uintptr_t at = (uintptr_t)a.u | (uintptr_t)a.y | (uintptr_t)a.dy | (uintptr_t)a.du;
   const bool two = a.H % 2 == 0 && (at & 3) == 0;
-  if (dtype == DT_F32) return lr_launch<float, 1>(a, back, s);
-  if (dtype == DT_BF16) return two ? lr_launch<bf16_t, 2>(a, back, s) : lr_launch<bf16_t, 1>(a, back, s);
-  return two ? lr_launch<f16_t, 2>(a, back, s) : lr_launch<f16_t, 1>(a, back, s);
+  if (dtype == DT_F32) return lr_gates<float, 1>(a, back, s);
+  if (dtype == DT_BF16) return two ? lr_gates<bf16_t, 2>(a, back, s) : lr_gates<bf16_t, 1>(a, back, s);
+  return two ? lr_gates<f16_t, 2>(a, back, s) : lr_gates<f16_t, 1>(a, back, s);
 }
 
 static int lr_check(const char* what, int dtype, int gates, int T, int B, int H) {

@@ -1,0 +1,985 @@
+// Losses of projected logits S = X W^T + b over a large vocabulary, for fp32, bf16 and fp16 storage and any width E:
+//   hard[n] = lse(S[n]) - S[n][target]                                   (softmax cross-entropy)
+//   soft[n] = tau^2 sum_k p_k (log p_k - S[n][id_k] / tau + lse(S[n] / tau)),  p = softmax(teacher's top logits / tau)
+// and their gradients.  The (rows, V) array is never formed: the forward pass folds 128 x 128 tiles of S into running
+// (max, sum) pairs; the backward pass forms d loss / d S again in pieces of the vocabulary that stay in the chip's
+// caches, and multiplies each piece with W and X before the next one is made.  Rows whose target is `pad` are dropped
+// first (their loss and gradient are zero): everything below works on the compact list of live rows.
+//
+// Number format.  All four products run on v_mfma_f32_32x32x16_f16 with fp32 accumulation.  X and W are first laid out
+// as images: a power-of-two scale brings the tensor's largest element to [2^13, 2^14), 16-bit inputs are then one fp16
+// plane (exact: bf16 and fp16 have at most 11 significant bits; elements below 2^-28 of the largest lose bits, an
+// absolute 2^-38 of it), fp32 inputs are two planes hi + lo (22 bits), multiplied as hi.lo + lo.hi + hi.hi, which drops
+// at most 2^-22 of a product (bf16 planes would drop 2^-16).  The gradient's tile P = dS / s is stored the same way (s: the
+// row's power of two above |dS|, carried by the other operand), one plane for 16-bit outputs: half a step of fp16,
+// 2^-11, is an eighth of bf16's own rounding.
+//
+// Image layout: rows of 128-byte pieces, one plane: 64 values, two planes: 32 hi values then 32 lo values.  A piece is
+// what one row adds to a pipeline stage, so one loop serves both.  Rows are padded to 128 with zeros, columns to 64.
+// Both orders that the products need are read from this one layout: rows along K with ds_read_b128, and K down the
+// rows with ds_read_b64_tr_b16, which transposes on its way to the registers.
+#include "common.hpp"
+#include "misc.hpp"
+#include "dtype.hpp"
+
+namespace cvae {
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4 lds_s4;
+
+constexpr int DT_TILE = 128;               // rows / columns of a tile, both ways
+constexpr int DT_STAGE = 16384;            // bytes of one operand's stage: 128 rows x 128 bytes
+constexpr int DT_AMAX = 256;               // partial maxima of |X| and |W|
+constexpr int DT_CROWS = 256;              // rows of one count of the live-row scan
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int P_EXP = 13;                  // |P| <= 1 is stored times 2^13
+
+struct DistillArgs {
+  int N, T, R, B, E, V, K;
+  int Np, Vp, Kp, Kg;                      // N and V up to 128, E up to 64, E + 1 up to 64
+  float tau, itau;
+  int two;                                 // tau != 1 and K > 0: a second normaliser
+  const void* X; const void* W; const void* bias;
+  const int64_t* tgt; int64_t pad;
+  const int64_t* ids; const float* top;
+  float* hard; float* soft;                // [N]
+  // kept for the backward pass
+  int* counts; int* rows; int* inv; int* nlive; int* slive;   // slive[R]: the sentence has a live row
+  float* amax;                             // [2][DT_AMAX]
+  _Float16* Ximg; _Float16* Wimg; float* b2;
+  float* L1; float* L2; float* pick; float* pk;   // by live row: normalisers (base 2), picked logits [K+1], p [K]
+  float* part; int splits_cap;             // [3][splits][Np]
+  // backward
+  const float* ghard; const float* gsoft;  // [R]
+  _Float16* Gimg; float* coef;             // s X image with a column of s; [3][Np]: a, b, s / gmax
+  float* gmax;
+  _Float16* P; int v0, vc; long ldp;       // a piece of the vocabulary
+  float* slab; int xsplits;
+  void* dX; void* dW; void* db;
+};
+
+// ------------------------------------------------------------------------------------------------- scales and images
+__device__ __forceinline__ int scale_exp(float amax) {          // amax * 2^e in [2^13, 2^14)
+  if (!(amax > 0.f)) return 0;
+  const int e = P_EXP - (int)floorf(log2f(amax));
+  return e < -60 ? -60 : (e > 60 ? 60 : e);
+}
+// largest finite magnitude of a tensor from its partials, by every thread of a block of >= 256 threads
+__device__ __forceinline__ float block_amax(const float* part, float* red) {
+  float m = threadIdx.x < DT_AMAX ? part[threadIdx.x] : 0.f;
+  m = wave_max(m);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = 0.f;
+  for (int i = 0; i < (int)blockDim.x / 64; ++i) m = fmaxf(m, red[i]);
+  __syncthreads();
+  return m;
+}
+// four elements at columns k .. k+3 of a row (zero past E), times 2^e, as fp16 planes
+template <typename T> __device__ __forceinline__ void load4(const T* row, int k, int E, bool vec, float (&x)[4]) {
+  if (vec && k + 3 < E) {
+    const Packed<T, 4> r = *reinterpret_cast<const Packed<T, 4>*>(row + k);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = r.f(i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = k + i < E ? (float)row[k + i] : 0.f;
+  }
+}
+template <int NP> __device__ __forceinline__ long image_at(int k) { return NP == 1 ? k : (long)(k >> 5) * 64 + (k & 31); }
+template <int NP> __device__ __forceinline__ void store4(_Float16* row, int k, const float (&x)[4]) {
+  Packed<f16_t, 4> hi, lo;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    hi.set(i, x[i]);
+    if (NP == 2) {
+      const float r = x[i] - hi.f(i);
+      lo.set(i, fabsf(x[i]) < 3.0e38f ? r : 0.f);                // an infinity has no remainder
+    }
+  }
+  _Float16* q = row + image_at<NP>(k);
+  *reinterpret_cast<Packed<f16_t, 4>*>(q) = hi;
+  if (NP == 2) *reinterpret_cast<Packed<f16_t, 4>*>(q + 32) = lo;
+}
+
+// live rows per DT_CROWS rows, zero losses, and (the blocks after those) partial maxima of |X| and |W|
+template <typename T> __global__ __launch_bounds__(256) void dt_count_kernel(DistillArgs p, int nb) {
+  __shared__ float red[4];
+  if ((int)blockIdx.x < nb) {
+    const int n = blockIdx.x * DT_CROWS + threadIdx.x;
+    const bool live = n < p.N && p.tgt[n] != p.pad;
+    if (n < p.N) {
+      p.hard[n] = 0.f;
+      if (p.K) p.soft[n] = 0.f;
+      if (n < p.R) p.slive[n] = 0;
+    }
+    const int c = __popcll(__ballot(live));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = (float)c;
+    __syncthreads();
+    if (threadIdx.x == 0) p.counts[blockIdx.x] = (int)(red[0] + red[1] + red[2] + red[3]);
+    return;
+  }
+  // (what stands in dropped rows does not set the scale of the others)
+  const int b = blockIdx.x - nb, which = b / DT_AMAX, slot = b % DT_AMAX;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const T* x = static_cast<const T*>(which ? p.W : p.X);
+  const int rows = which ? p.V : p.N;
+  const bool vec = p.E % 4 == 0 && ((uintptr_t)x % (4 * sizeof(T))) == 0;
+  float m = 0.f;
+  for (int n = slot * 4 + wave; n < rows; n += DT_AMAX * 4) {
+    if (!which && p.tgt[n] == p.pad) continue;
+    for (int k = lane * 4; k < p.E; k += 256) {
+      float v[4];
+      load4<T>(x + (long)n * p.E, k, p.E, vec, v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float a = fabsf(v[j]);
+        if (a < 3.4e38f) m = fmaxf(m, a);
+      }
+    }
+  }
+  m = wave_max(m);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) p.amax[which * DT_AMAX + slot] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
+// the row list and the images.  Blocks [0, nb): DT_CROWS rows of X each, to their places in the compact order; the
+// next Np / 64: zeros of the compact rows past the last live one; the rest: 16 rows of W and its bias each.
+template <typename T, int NP> __global__ __launch_bounds__(256) void dt_image_kernel(DistillArgs p, int nb) {
+  __shared__ float red[4];
+  __shared__ int sred[4], swave[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long ld = (long)p.Kp * NP;
+  const int k4 = p.Kp / 4;
+  int blk = blockIdx.x;
+  if (blk < nb + p.Np / 64) {
+    const bool tail = blk >= nb;
+    const int upto = tail ? nb : blk;
+    int s = 0;
+    for (int i = threadIdx.x; i < upto; i += 256) s += p.counts[i];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if (lane == 0) sred[wave] = s;
+    if (tail) {
+      __syncthreads();
+      const int nl = sred[0] + sred[1] + sred[2] + sred[3];
+      if (blk == nb && threadIdx.x == 0) *p.nlive = nl;
+      for (int i = (blk - nb) * 64 + wave; i < (blk - nb) * 64 + 64; i += 4)
+        if (i >= nl)
+          for (int k = lane; k < k4 * NP; k += 64) reinterpret_cast<Packed<f16_t, 4>*>(p.Ximg + i * ld)[k] = Packed<f16_t, 4>{};
+      return;
+    }
+    __shared__ int slot[DT_CROWS];
+    const int n = blk * DT_CROWS + threadIdx.x;
+    const bool live = n < p.N && p.tgt[n] != p.pad;
+    const unsigned long long b = __ballot(live);
+    if (lane == 0) swave[wave] = __popcll(b);
+    __syncthreads();
+    int off = sred[0] + sred[1] + sred[2] + sred[3];
+    for (int i = 0; i < wave; ++i) off += swave[i];
+    off += __popcll(b & ((1ull << lane) - 1ull));
+    slot[threadIdx.x] = live ? off : -1;
+    if (n < p.N) p.inv[n] = live ? off : -1;
+    if (live) p.rows[off] = n;
+    const int e = scale_exp(block_amax(p.amax, red));            // (its barriers also publish slot[])
+    const bool vec = p.E % 4 == 0 && ((uintptr_t)p.X % (4 * sizeof(T))) == 0;
+    for (int i = wave; i < DT_CROWS; i += 4) {
+      const int to = slot[i];
+      if (to < 0) continue;
+      const T* row = static_cast<const T*>(p.X) + (long)(blk * DT_CROWS + i) * p.E;
+      for (int k = lane; k < k4; k += 64) {
+        float x[4];
+        load4<T>(row, 4 * k, p.E, vec, x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = ldexpf(x[j], e);
+        store4<NP>(p.Ximg + to * ld, 4 * k, x);
+      }
+    }
+    return;
+  }
+  blk -= nb + p.Np / 64;
+  const int e = scale_exp(block_amax(p.amax + DT_AMAX, red));
+  const bool vec = p.E % 4 == 0 && ((uintptr_t)p.W % (4 * sizeof(T))) == 0;
+  for (int v = blk * 16 + wave; v < blk * 16 + 16; v += 4) {
+    const T* row = static_cast<const T*>(p.W) + (long)v * p.E;
+    for (int k = lane; k < k4; k += 64) {
+      float x[4] = {0.f, 0.f, 0.f, 0.f};
+      if (v < p.V) load4<T>(row, 4 * k, p.E, vec, x);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = ldexpf(x[j], e);
+      store4<NP>(p.Wimg + v * ld, 4 * k, x);
+    }
+    if (lane == 0) p.b2[v] = v < p.V ? (float)static_cast<const T*>(p.bias)[v] * LOG2E : -INFINITY;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------- the product loop
+// One operand's tile: `base` the first byte of its stage 0, `ld` bytes from row to row.
+//   K along the row (KS = false): 128 rows; stage s is bytes [128 s, 128 s + 128) of each.
+//   K down the rows (KS = true): 128 columns; stage s is 64 (two planes: 32) rows of 256 (512) bytes.
+// In LDS, 16-byte chunk c of row r sits at chunk c ^ (r & 7) of its 128 bytes (KS: c ^ 4 (r & 3) of its 256): the
+// chunks that the lanes of a read take lie in different banks.
+template <int NP, bool KS> struct Operand {
+  const char* base;
+  long ld;
+  unsigned off[4];
+  __device__ __forceinline__ void init(const void* p, long ld_bytes, int lane, int wave) {
+    base = static_cast<const char*>(p);
+    ld = ld_bytes;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int piece = wave * 4 + i;                             // 1 KiB of the stage
+      if (!KS) {
+        const int r = piece * 8 + (lane >> 3);
+        off[i] = (unsigned)(r * ld + (((lane & 7) ^ (r & 7)) << 4));
+      } else {
+        constexpr int LPR = NP == 1 ? 16 : 32;                    // lanes (chunks) of a row
+        const int r = piece * (64 / LPR) + lane / LPR, c = lane % LPR;
+        off[i] = (unsigned)(r * ld + ((c ^ ((r & 3) << 2)) << 4));
+      }
+    }
+  }
+  __device__ __forceinline__ void issue(int stage, char* lds, int wave) const {
+    const char* b = base + (KS ? (long)stage * (64 / NP) * ld : (long)stage * 128);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(b + off[i]),
+                                       (__attribute__((address_space(3))) void*)(lds + (wave * 4 + i) * 1024), 16, 0, 0);
+  }
+  // the 32 rows / columns from `c0`, K block `ks` of the stage, plane `pl`, as one MFMA operand
+  static __device__ __forceinline__ h8 frag(const char* lds, int c0, int ks, int pl, int lane) {
+    if (!KS) {
+      const int r = c0 + (lane & 31), c = (NP == 1 ? 0 : pl * 4) + ks * 2 + (lane >> 5);
+      return *reinterpret_cast<const h8*>(lds + r * 128 + ((c ^ (r & 7)) << 4));
+    }
+    constexpr int ROW = 256 * NP;
+    const int k = ks * 16 + (lane >> 5) * 8 + ((lane >> 2) & 3);
+    const int col = c0 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+    const int byte = NP == 1 ? col * 2 : (col >> 5) * 128 + pl * 64 + (col & 31) * 2;
+    const char* q = lds + k * ROW + ((((byte >> 4) ^ ((k & 3) << 2)) << 4) | (byte & 15));
+    union { s4 s[2]; h8 h; } u;
+    u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(q));
+    u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(q + 4 * ROW));
+    return u.h;
+  }
+};
+
+// acc[i][j] += (rows am + 32 i of A) x (rows bn + 32 j of B) over K block ks of the stage in LDS
+template <int NP, bool AKS, bool BKS>
+__device__ __forceinline__ void mfma_block(const char* la, const char* lb, int am, int bn, int ks, int lane,
+                                           f32x16 (&acc)[2][2]) {
+  h8 a[2][NP], b[2][NP];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int q = 0; q < NP; ++q) {
+      a[i][q] = Operand<NP, AKS>::frag(la, am + 32 * i, ks, q, lane);
+      b[i][q] = Operand<NP, BKS>::frag(lb, bn + 32 * i, ks, q, lane);
+    }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (NP == 2) {                                              // the small products first
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][NP - 1], acc[i][j], 0, 0, 0);
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][NP - 1], b[j][0], acc[i][j], 0, 0, 0);
+      }
+      acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][0], acc[i][j], 0, 0, 0);
+    }
+}
+template <int NP, bool AKS, bool BKS>
+__device__ __forceinline__ void stage_product(const char* la, const char* lb, int am, int bn, int blocks, int lane,
+                                              f32x16 (&acc)[2][2]) {
+  constexpr int KB = 4 / NP;                                      // K blocks of 16 in a stage
+  if (blocks >= KB) {
+#pragma unroll
+    for (int ks = 0; ks < KB; ++ks) mfma_block<NP, AKS, BKS>(la, lb, am, bn, ks, lane, acc);
+  } else {
+    for (int ks = 0; ks < blocks; ++ks) mfma_block<NP, AKS, BKS>(la, lb, am, bn, ks, lane, acc);
+  }
+}
+__device__ __forceinline__ void clear(f32x16 (&acc)[2][2]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+}
+// this block's loads into LDS have arrived, and every wave has left the buffer that is filled next
+__device__ __forceinline__ void stage_barrier() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+// stages [0, n) of one tile; `last` K blocks of the last stage are used
+template <int NP, bool AKS, bool BKS>
+__device__ __forceinline__ void product(const Operand<NP, AKS>& A, const Operand<NP, BKS>& B, int n, int last, char* lds,
+                                        int am, int bn, int lane, int wave, f32x16 (&acc)[2][2]) {
+  clear(acc);
+  if (n > 0) { A.issue(0, lds, wave); B.issue(0, lds + DT_STAGE, wave); }
+  for (int s = 0; s < n; ++s) {
+    char* cur = lds + (s & 1) * 2 * DT_STAGE;
+    char* nxt = lds + ((s + 1) & 1) * 2 * DT_STAGE;
+    stage_barrier();
+    if (s + 1 < n) { A.issue(s + 1, nxt, wave); B.issue(s + 1, nxt + DT_STAGE, wave); }
+    stage_product<NP, AKS, BKS>(cur, cur + DT_STAGE, am, bn, s + 1 < n ? 4 : last, lane, acc);
+  }
+}
+// value r of an accumulator tile: row 4 (lane / 32) + 8 (r / 4) + r % 4, column lane % 32
+__device__ __forceinline__ int acc_row(int r, int lane) { return (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5); }
+
+// ------------------------------------------------------------------------------------------------- forward
+// Vocabulary splits for nt tiles of live rows: the blocks of an XCD (block % 8) share a range of W, and the splits are
+// as many as fill 512 blocks (two on every CU).  Computed alike by the product and the merge.
+__host__ __device__ inline int dt_splits(int nt, int vt) {
+  int s = nt > 0 ? 64 / nt : 1;
+  if (s < 1) s = 1;
+  s *= 8;
+  return s < vt ? s : (vt + 7) / 8 * 8;
+}
+constexpr int DT_FWD_BLOCKS = 512;
+
+template <int NP, bool TWO>
+__global__ __launch_bounds__(256, 2) void dt_forward_kernel(DistillArgs p) {
+  __shared__ __attribute__((aligned(16))) char lds[4 * DT_STAGE];
+  __shared__ float red[4];
+  const int nl = *p.nlive, nt = (nl + DT_TILE - 1) / DT_TILE, vt = p.Vp / DT_TILE;
+  const int splits = dt_splits(nt, vt), per = (vt + splits - 1) / splits;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int am = (wave >> 1) * 64, bn = (wave & 1) * 64;
+  const int e = scale_exp(block_amax(p.amax, red)) + scale_exp(block_amax(p.amax + DT_AMAX, red));
+  const float c = ldexpf(LOG2E, -e);
+  const long ld = (long)p.Kp * NP * 2;
+  const int nst = (p.E + 64 / NP - 1) / (64 / NP), last = ((p.E + 15) / 16) - (nst - 1) * (4 / NP);
+  const int xcd = blockIdx.x & 7, per_xcd = nt * (splits / 8);
+  for (int q = blockIdx.x >> 3; q < per_xcd; q += DT_FWD_BLOCKS / 8) {
+    const int split = xcd + 8 * (q / nt), n0 = (q % nt) * DT_TILE;
+    const int t0 = split * per, t1 = min(vt, t0 + per);
+    Operand<NP, false> A, B;
+    A.init(p.Wimg, ld, lane, wave);
+    B.init(reinterpret_cast<const char*>(p.Ximg) + n0 * ld, ld, lane, wave);
+    float m[2], s1[2], s2[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) { m[j] = -1e30f; s1[j] = s2[j] = 0.f; }
+    f32x16 acc[2][2];
+    const int total = (t1 - t0) * nst;
+    const char* wbase = A.base;
+    A.base = wbase + (long)t0 * DT_TILE * ld;
+    __syncthreads();                                              // the last item's reads are over
+    if (total > 0) { A.issue(0, lds, wave); B.issue(0, lds + DT_STAGE, wave); }
+    int st = 0, tile = t0;
+    clear(acc);
+    for (int s = 0; s < total; ++s) {
+      char* cur = lds + (s & 1) * 2 * DT_STAGE;
+      char* nxt = lds + ((s + 1) & 1) * 2 * DT_STAGE;
+      const bool end = st + 1 == nst;
+      stage_barrier();
+      if (s + 1 < total) {
+        if (end) A.base = wbase + (long)(tile + 1) * DT_TILE * ld;
+        A.issue(end ? 0 : st + 1, nxt, wave);
+        B.issue(end ? 0 : st + 1, nxt + DT_STAGE, wave);
+      }
+      stage_product<NP, false, false>(cur, cur + DT_STAGE, am, bn, end ? last : 4, lane, acc);
+      ++st;
+      if (!end) continue;
+      // fold the tile: a lane owns two rows (columns of the product) and 32 of the tile's 64 vocabulary entries
+      const float* b2 = p.b2 + tile * DT_TILE + am;
+      float4 bias[2][4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) bias[i][g] = *reinterpret_cast<const float4*>(b2 + 32 * i + 8 * g + 4 * (lane >> 5));
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float mx = m[j];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float4& bb = bias[i][r >> 2];
+            const float bv = (r & 3) == 0 ? bb.x : (r & 3) == 1 ? bb.y : (r & 3) == 2 ? bb.z : bb.w;
+            acc[i][j][r] = fmaf(acc[i][j][r], c, bv);
+            mx = fmaxf(mx, acc[i][j][r]);
+          }
+        const float back = m[j] - mx;
+        float a = s1[j] * __builtin_amdgcn_exp2f(back), b = 0.f;
+        if (TWO) b = s2[j] * __builtin_amdgcn_exp2f(back * p.itau);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float d = acc[i][j][r] - mx;
+            a += __builtin_amdgcn_exp2f(d);
+            if (TWO) b += __builtin_amdgcn_exp2f(d * p.itau);
+          }
+        m[j] = mx; s1[j] = a; s2[j] = b;
+      }
+      clear(acc);
+      st = 0;
+      ++tile;
+    }
+    // join the two half-waves and the two waves that share a row, and store the split's pair
+    __syncthreads();
+    float* x = reinterpret_cast<float*>(lds);                     // [2 (am)][128][3]
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float m2 = __shfl_xor(m[j], 32, 64), mm = fmaxf(m[j], m2);
+      const float f = __builtin_amdgcn_exp2f(m[j] - mm), f2 = __builtin_amdgcn_exp2f(m2 - mm);
+      const float a = s1[j] * f + __shfl_xor(s1[j], 32, 64) * f2;
+      float b = 0.f;
+      if (TWO) b = s2[j] * __builtin_amdgcn_exp2f((m[j] - mm) * p.itau) +
+                   __shfl_xor(s2[j], 32, 64) * __builtin_amdgcn_exp2f((m2 - mm) * p.itau);
+      if (lane < 32) {
+        float* y = x + ((wave >> 1) * 128 + bn + 32 * j + lane) * 3;
+        y[0] = mm; y[1] = a; y[2] = b;
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x < 128) {
+      const float* y = x + threadIdx.x * 3;
+      const float* z = y + 128 * 3;
+      const float mm = fmaxf(y[0], z[0]), d = y[0] - mm, d2 = z[0] - mm;
+      float* out = p.part + (long)split * p.Np + n0 + threadIdx.x;
+      const long plane = (long)p.splits_cap * p.Np;
+      out[0] = mm;
+      out[plane] = y[1] * __builtin_amdgcn_exp2f(d) + z[1] * __builtin_amdgcn_exp2f(d2);
+      if (TWO) out[2 * plane] = y[2] * __builtin_amdgcn_exp2f(d * p.itau) + z[2] * __builtin_amdgcn_exp2f(d2 * p.itau);
+    }
+  }
+}
+
+// One block per live row: merge the splits, form the picked logits (16 lanes a dot product), the teacher's distribution
+// and the two losses.
+template <typename T, bool TWO>
+__global__ __launch_bounds__(256) void dt_combine_kernel(DistillArgs p) {
+  const int i = blockIdx.x;
+  const int nl = *p.nlive;
+  if (i >= nl) return;
+  __shared__ float red[4][3];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int n = p.rows[i], r = n % p.R, t = n / p.R;
+  const int64_t* ids = p.K ? p.ids + ((long)(r % p.B) * p.T + t) * p.K : nullptr;
+  const float* top = p.K ? p.top + ((long)(r % p.B) * p.T + t) * p.K : nullptr;
+  const int64_t tg = p.tgt[n];
+  float* pick = p.pick + (long)i * (p.K + 1);
+  // picked logits, base 2
+  const T* x = static_cast<const T*>(p.X) + (long)n * p.E;
+  const bool vec = p.E % 4 == 0 && ((uintptr_t)p.X % (4 * sizeof(T))) == 0 && ((uintptr_t)p.W % (4 * sizeof(T))) == 0;
+  const int l16 = threadIdx.x & 15;
+  for (int k = threadIdx.x >> 4; k <= p.K; k += 16) {
+    const int64_t id = k < p.K ? ids[k] : tg;
+    float dot = 0.f;
+    if (id >= 0 && id < p.V) {
+      const T* w = static_cast<const T*>(p.W) + id * p.E;
+      for (int e = l16 * 4; e < p.E; e += 64) {
+        float a[4], b[4];
+        load4<T>(x, e, p.E, vec, a);
+        load4<T>(w, e, p.E, vec, b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dot = fmaf(a[j], b[j], dot);
+      }
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
+    if (l16 == 0) pick[k] = (id >= 0 && id < p.V) ? (dot + (float)static_cast<const T*>(p.bias)[id]) * LOG2E : 0.f;
+  }
+  // normalisers
+  const int nt = (nl + DT_TILE - 1) / DT_TILE, splits = dt_splits(nt, p.Vp / DT_TILE);
+  const long plane = (long)p.splits_cap * p.Np;
+  float m = -1e30f, a = 0.f, b = 0.f;
+  for (int s = threadIdx.x; s < splits; s += 256) {
+    const float* q = p.part + (long)s * p.Np + i;
+    const float m2 = q[0], mm = fmaxf(m, m2);
+    a = a * __builtin_amdgcn_exp2f(m - mm) + q[plane] * __builtin_amdgcn_exp2f(m2 - mm);
+    if (TWO) b = b * __builtin_amdgcn_exp2f((m - mm) * p.itau) + q[2 * plane] * __builtin_amdgcn_exp2f((m2 - mm) * p.itau);
+    m = mm;
+  }
+  {
+    const float mm = wave_max(m);
+    a = wave_sum(a * __builtin_amdgcn_exp2f(m - mm));
+    if (TWO) b = wave_sum(b * __builtin_amdgcn_exp2f((m - mm) * p.itau));
+    if (lane == 0) { red[wave][0] = mm; red[wave][1] = a; red[wave][2] = b; }
+  }
+  __threadfence_block();
+  __syncthreads();                                                // also: pick[] is written
+  if (wave != 0) return;
+  m = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
+  a = b = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float d = red[w][0] - m;
+    a += red[w][1] * __builtin_amdgcn_exp2f(d);
+    if (TWO) b += red[w][2] * __builtin_amdgcn_exp2f(d * p.itau);
+  }
+  const float L1 = m + log2f(a), L2 = TWO ? fmaf(m, p.itau, log2f(b)) : L1;
+  if (lane == 0) {
+    p.L1[i] = L1;
+    p.L2[i] = L2;
+    p.slive[r] = 1;
+    p.hard[n] = (L1 - pick[p.K]) * LN2;
+  }
+  if (!p.K) return;
+  float tm = -INFINITY;
+  bool bad = false;                                               // a NaN among the teacher's logits
+  for (int k = lane; k < p.K; k += 64) {
+    const int64_t id = ids[k];
+    if (id >= 0 && id < p.V) { tm = fmaxf(tm, top[k]); bad |= top[k] != top[k]; }
+  }
+  tm = wave_max(tm);
+  if (__any(bad)) tm = NAN;
+  float sum = 0.f;
+  if (tm != -INFINITY)
+    for (int k = lane; k < p.K; k += 64) {
+      const int64_t id = ids[k];
+      if (id >= 0 && id < p.V) sum += __builtin_amdgcn_exp2f((top[k] - tm) * p.itau * LOG2E);
+    }
+  sum = wave_sum(sum);
+  const float lsum = log2f(sum), inv = 1.0f / sum;
+  float loss = 0.f;
+  for (int k = lane; k < p.K; k += 64) {
+    const int64_t id = ids[k];
+    float pk = 0.f;
+    if (id >= 0 && id < p.V && tm != -INFINITY) {
+      const float lp = (top[k] - tm) * p.itau * LOG2E;
+      pk = __builtin_amdgcn_exp2f(lp) * inv;
+      if (pk != 0.f) loss += pk * (lp - lsum - (pick[k] * p.itau - L2));
+    }
+    p.pk[(long)i * p.K + k] = pk;
+  }
+  loss = wave_sum(loss);
+  if (lane == 0) p.soft[n] = p.tau * p.tau * LN2 * loss;
+}
+
+// ------------------------------------------------------------------------------------------------- backward
+// Per live row: the two coefficients of its gradient over the row's power of two s, and the image of s X (with a column
+// of s itself: the product with P gives the bias gradient beside the weights').  Zeros: dX of dead rows, image rows past
+// the last live one.  Blocks [0, cdiv(N, 64)): 64 original rows; the next Np / 64: the image's tail.
+template <typename T, int NP> __global__ __launch_bounds__(256) void dt_gimage_kernel(DistillArgs p, int nb) {
+  __shared__ float red[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long ld = (long)p.Kg * NP;
+  const int k4 = p.Kg / 4;
+  const int nl = *p.nlive;
+  if ((int)blockIdx.x >= nb) {
+    const int b0 = (blockIdx.x - nb) * 64;
+    for (int i = b0 + wave; i < b0 + 64; i += 4)
+      if (i >= nl)
+        for (int k = lane; k < k4 * NP; k += 64) reinterpret_cast<Packed<f16_t, 4>*>(p.Gimg + i * ld)[k] = Packed<f16_t, 4>{};
+    return;
+  }
+  float g = 0.f;
+  for (int r = threadIdx.x; r < p.R; r += 256) {
+    if (!p.slive[r]) continue;
+    const float x = fabsf(p.ghard[r]) + (p.K ? fabsf(p.gsoft[r]) * p.tau : 0.f);
+    if (x < 3.4e38f) g = fmaxf(g, x);
+  }
+  g = wave_max(g);
+  if (lane == 0) red[wave] = g;
+  __syncthreads();
+  g = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  __syncthreads();
+  const int eg = g > 0.f ? (int)ceilf(log2f(g)) : 0;              // gmax = 2^eg
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.gmax = ldexpf(1.f, eg);
+  const int ex = scale_exp(block_amax(p.amax, red));
+  const bool vec = p.E % 4 == 0 && ((uintptr_t)p.X % (4 * sizeof(T))) == 0;
+  for (int j = wave; j < 64; j += 4) {
+    const int n = blockIdx.x * 64 + j;
+    if (n >= p.N) break;
+    const int i = p.inv[n];
+    if (i < 0) {
+      T* q = static_cast<T*>(p.dX) + (long)n * p.E;
+      for (int k = lane; k < p.E; k += 64) q[k] = (T)0.f;
+      continue;
+    }
+    const int r = n % p.R;
+    const float gh = p.ghard[r];
+    float gs = 0.f;
+    if (p.K) {                                                    // rows whose teacher lists nothing have no soft part
+      float any = 0.f;
+      for (int k = lane; k < p.K; k += 64) any += p.pk[(long)i * p.K + k];
+      any = wave_sum(any);
+      gs = any != 0.f ? p.gsoft[r] * p.tau : 0.f;
+      if (any != any) gs = any;
+    }
+    const float mag = fabsf(gh) + fabsf(gs);
+    const bool fin = mag < 3.4e38f;
+    int es = (mag > 0.f && fin) ? (int)ceilf(log2f(mag)) : eg;
+    es = es > eg ? eg : (es < eg - 40 ? eg - 40 : es);
+    if (lane == 0) {
+      p.coef[i] = ldexpf(gh, P_EXP - es);
+      p.coef[p.Np + i] = ldexpf(gs, P_EXP - es);
+      p.coef[2 * (long)p.Np + i] = ldexpf(1.f, es);
+    }
+    const T* row = static_cast<const T*>(p.X) + (long)n * p.E;
+    for (int k = lane; k < k4; k += 64) {
+      float x[4];
+      load4<T>(row, 4 * k, p.E, vec, x);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        x[q] = ldexpf(x[q], ex + es - eg);
+        if (4 * k + q == p.E) x[q] = ldexpf(1.f, P_EXP + es - eg);
+      }
+      store4<NP>(p.Gimg + i * ld, 4 * k, x);
+    }
+  }
+}
+
+// P[n][v] of a piece of the vocabulary without the picked entries: a 2^(t - L1) + b 2^(t / tau - L2)
+template <int NP, bool TWO>
+__global__ __launch_bounds__(256, 2) void dt_grad_kernel(DistillArgs p) {
+  __shared__ __attribute__((aligned(16))) char lds[4 * DT_STAGE];
+  __shared__ float red[4];
+  const int nl = *p.nlive, nt = (nl + DT_TILE - 1) / DT_TILE, vt = (p.vc + DT_TILE - 1) / DT_TILE;
+  // block -> (vocabulary tile, row tile): an XCD walks its own range of W, all row tiles of one tile of W in turn
+  const int pv = (vt + 7) / 8, j0 = blockIdx.x >> 3, tv = (blockIdx.x & 7) * pv + (nt > 0 ? j0 / nt : 0);
+  if (nt == 0 || j0 / nt >= pv || tv >= vt) return;
+  const int n0 = (j0 % nt) * DT_TILE, w0 = p.v0 + tv * DT_TILE;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int am = (wave >> 1) * 64, bn = (wave & 1) * 64;
+  const long ld = (long)p.Kp * NP * 2;
+  Operand<NP, false> A, B;
+  A.init(reinterpret_cast<const char*>(p.Wimg) + w0 * ld, ld, lane, wave);
+  B.init(reinterpret_cast<const char*>(p.Ximg) + n0 * ld, ld, lane, wave);
+  const int nst = (p.E + 64 / NP - 1) / (64 / NP), last = ((p.E + 15) / 16) - (nst - 1) * (4 / NP);
+  const int e = scale_exp(block_amax(p.amax, red)) + scale_exp(block_amax(p.amax + DT_AMAX, red));
+  const float c = ldexpf(LOG2E, -e);
+  f32x16 acc[2][2];
+  product<NP, false, false>(A, B, nst, last, lds, am, bn, lane, wave, acc);
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int nn = bn + 32 * j + (lane & 31), i = n0 + nn;
+    const bool in = i < nl;
+    const float L1 = in ? p.L1[i] : 0.f, L2 = (TWO && in) ? p.L2[i] : 0.f;
+    const float ca = in ? p.coef[i] + (TWO ? 0.f : p.coef[p.Np + i]) : 0.f, cb = (TWO && in) ? p.coef[p.Np + i] : 0.f;
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int v = am + 32 * q + 8 * g + 4 * (lane >> 5);
+        const float4 bb = *reinterpret_cast<const float4*>(p.b2 + w0 + v);
+        const float bv[4] = {bb.x, bb.y, bb.z, bb.w};
+        Packed<f16_t, 4> hi, lo;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float t = fmaf(acc[q][j][4 * g + k], c, bv[k]);
+          float x = ca * __builtin_amdgcn_exp2f(t - L1);
+          if (TWO) x = fmaf(cb, __builtin_amdgcn_exp2f(fmaf(t, p.itau, -L2)), x);
+          x = in ? x : 0.f;
+          hi.set(k, x);
+          if (NP == 2) lo.set(k, x - hi.f(k));
+        }
+        const int byte = NP == 1 ? v * 2 : (v >> 5) * 128 + (v & 31) * 2;
+        char* row = lds + nn * 256 * NP;
+        *reinterpret_cast<Packed<f16_t, 4>*>(row + ((((byte >> 4) ^ (nn & 15)) << 4) | (byte & 15))) = hi;
+        if (NP == 2) {
+          const int bl = byte + 64;
+          *reinterpret_cast<Packed<f16_t, 4>*>(row + ((((bl >> 4) ^ (nn & 15)) << 4) | (bl & 15))) = lo;
+        }
+      }
+  }
+  __syncthreads();
+  constexpr int CPR = 16 * NP;                                    // 16-byte chunks of a row
+  for (int k = threadIdx.x; k < DT_TILE * CPR; k += 256) {
+    const int nn = k / CPR, ch = k % CPR;
+    const uint4 x = *reinterpret_cast<const uint4*>(lds + nn * 256 * NP + ((ch ^ (nn & 15)) << 4));
+    *reinterpret_cast<uint4*>(reinterpret_cast<char*>(p.P + (long)(n0 + nn) * p.ldp) + (long)tv * 256 * NP + ch * 16) = x;
+  }
+}
+
+// The picked entries of a row, from their own fp32 logits: softmax minus the target / the teacher's share.  An id that a
+// teacher lists twice, or that is the target too, is one entry: its first place writes it.
+template <int NP, bool TWO>
+__global__ __launch_bounds__(256) void dt_pick_kernel(DistillArgs p) {
+  const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (i >= *p.nlive) return;
+  const int n = p.rows[i], r = n % p.R, t = n / p.R;
+  const int64_t* ids = p.K ? p.ids + ((long)(r % p.B) * p.T + t) * p.K : nullptr;
+  const int64_t tg = p.tgt[n];
+  const float* pick = p.pick + (long)i * (p.K + 1);
+  const float a = p.coef[i], b = p.coef[p.Np + i], L1 = p.L1[i], L2 = p.L2[i];
+  for (int k = lane; k <= p.K; k += 64) {
+    const int64_t id = k < p.K ? ids[k] : tg;
+    if (id < p.v0 || id >= (int64_t)p.v0 + p.vc || id >= p.V) continue;
+    float share = 0.f;
+    bool first = true;
+    for (int q = 0; q < p.K; ++q)
+      if (ids[q] == id) {
+        if (q < k) first = false;
+        share += p.pk[(long)i * p.K + q];
+      }
+    if (!first) continue;
+    float x = a * (__builtin_amdgcn_exp2f(pick[k] - L1) - (id == tg ? 1.f : 0.f));
+    if (p.K) x = fmaf(b, __builtin_amdgcn_exp2f(fmaf(pick[k], TWO ? p.itau : 1.f, -L2)) - share, x);
+    const int v = (int)(id - p.v0);
+    _Float16* q = p.P + (long)i * p.ldp + image_at<NP>(v);
+    const _Float16 hi = (_Float16)x;
+    q[0] = hi;
+    if (NP == 2) q[32] = (_Float16)(x - (float)hi);
+  }
+}
+
+// dX: (W down its rows: K = vocabulary) x (P along its rows).  Blocks (row tile, column tile of E, split of the piece):
+// partial tiles in accumulator order, added to what an earlier piece left there.
+template <int NP>
+__global__ __launch_bounds__(256, 2) void dt_dx_kernel(DistillArgs p, int et, int add) {
+  __shared__ __attribute__((aligned(16))) char lds[4 * DT_STAGE];
+  const int nl = *p.nlive, nt = (nl + DT_TILE - 1) / DT_TILE;
+  const int split = blockIdx.x % p.xsplits, rest = blockIdx.x / p.xsplits, te = rest % et, tn = rest / et;
+  if (tn >= nt) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int am = (wave >> 1) * 64, bn = (wave & 1) * 64;
+  constexpr int BK = 64 / NP;
+  const int stages = (p.vc + DT_TILE - 1) / DT_TILE * (DT_TILE / BK), per = (stages + p.xsplits - 1) / p.xsplits;
+  const int s0 = split * per, s1 = min(stages, s0 + per);
+  const long ldw = (long)p.Kp * NP * 2, ldp = p.ldp * 2;
+  Operand<NP, true> A;
+  Operand<NP, false> B;
+  A.init(reinterpret_cast<const char*>(p.Wimg) + (p.v0 + (long)s0 * BK) * ldw + (long)te * 256 * NP, ldw, lane, wave);
+  B.init(reinterpret_cast<const char*>(p.P) + (long)tn * DT_TILE * ldp + (long)s0 * 128, ldp, lane, wave);
+  f32x16 acc[2][2];
+  product<NP, true, false>(A, B, s1 - s0, 4, lds, am, bn, lane, wave, acc);
+  float4* out = reinterpret_cast<float4*>(p.slab) + (((long)split * (p.Np / DT_TILE) + tn) * et + te) * (DT_TILE * DT_TILE / 4) + wave * 1024 + lane;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float4* q = out + ((i * 2 + j) * 4 + g) * 64;
+        float4 x = make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
+        if (add) { const float4 y = *q; x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w; }
+        *q = x;
+      }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void dt_dx_sum_kernel(DistillArgs p, int et) {
+  __shared__ float red[4];
+  const int nl = *p.nlive, nt = (nl + DT_TILE - 1) / DT_TILE;
+  const int tile = blockIdx.x >> 4;                               // 16 blocks a tile
+  if (tile / et >= nt) return;
+  const float w = ldexpf(1.f, -scale_exp(block_amax(p.amax + DT_AMAX, red)) - P_EXP);
+  const int slot = (blockIdx.x & 15) * 256 + threadIdx.x;
+  const long step = (long)(p.Np / DT_TILE) * et * (DT_TILE * DT_TILE / 4);
+  const float4* q = reinterpret_cast<const float4*>(p.slab) + (long)tile * (DT_TILE * DT_TILE / 4) + slot;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int k = 0; k < p.xsplits; ++k) { const float4 y = q[k * step]; s.x += y.x; s.y += y.y; s.z += y.z; s.w += y.w; }
+  const int lane = slot & 63, frag = (slot >> 6) & 15, wave = slot >> 10;
+  const int i = (tile / et) * DT_TILE + (wave & 1) * 64 + ((frag >> 2) & 1) * 32 + (lane & 31);
+  const int e = (tile % et) * DT_TILE + (wave >> 1) * 64 + (frag >> 3) * 32 + (frag & 3) * 8 + (lane >> 5) * 4;
+  if (i >= nl) return;
+  const float f = w * p.coef[2 * (long)p.Np + i];
+  T* out = static_cast<T*>(p.dX) + (long)p.rows[i] * p.E + e;
+  const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (e + k < p.E) out[k] = (T)(v[k] * f);
+}
+
+// dW and db: (s X down its rows: K = live rows) x (P down its rows), whole K in one block
+template <typename T, int NP>
+__global__ __launch_bounds__(256, 2) void dt_dw_kernel(DistillArgs p, int et) {
+  __shared__ __attribute__((aligned(16))) char lds[4 * DT_STAGE];
+  __shared__ float red[4];
+  const int nl = *p.nlive, vt = (p.vc + DT_TILE - 1) / DT_TILE;
+  const int pv = (vt + 7) / 8, j0 = blockIdx.x >> 3, tv = (blockIdx.x & 7) * pv + j0 / et, te = j0 % et;
+  if (j0 / et >= pv || tv >= vt) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int am = (wave >> 1) * 64, bn = (wave & 1) * 64;
+  constexpr int BK = 64 / NP;
+  Operand<NP, true> A, B;
+  A.init(reinterpret_cast<const char*>(p.Gimg) + (long)te * 256 * NP, (long)p.Kg * NP * 2, lane, wave);
+  B.init(reinterpret_cast<const char*>(p.P) + (long)tv * 256 * NP, p.ldp * 2, lane, wave);
+  const int ex = scale_exp(block_amax(p.amax, red));
+  const float fw = *p.gmax * ldexpf(1.f, -P_EXP - ex), fb = *p.gmax * ldexpf(1.f, -2 * P_EXP);
+  f32x16 acc[2][2];
+  product<NP, true, true>(A, B, (nl + BK - 1) / BK, 4, lds, am, bn, lane, wave, acc);
+  __syncthreads();
+  // through LDS: rows of the vocabulary, 128 columns each, chunk c of row r at c ^ (r & 31)
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int row = bn + 32 * j + (lane & 31);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int ch = (am + 32 * i + 8 * g + 4 * (lane >> 5)) >> 2;
+        *reinterpret_cast<float4*>(lds + row * 512 + ((ch ^ (row & 31)) << 4)) =
+            make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
+      }
+    }
+  __syncthreads();
+  for (int row = wave; row < DT_TILE; row += 4) {
+    const int v = p.v0 + tv * DT_TILE + row;
+    if (v >= p.V) break;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int el = h * 64 + lane, e = te * DT_TILE + el;
+      const float x = *reinterpret_cast<const float*>(lds + row * 512 + (((el >> 2) ^ (row & 31)) << 4) + (el & 3) * 4);
+      if (e < p.E) static_cast<T*>(p.dW)[(long)v * p.E + e] = (T)(x * fw);
+      else if (e == p.E) static_cast<T*>(p.db)[v] = (T)(x * fb);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------- host side
+constexpr long DT_PIECE_BYTES = 192L << 20;        // of P: it is written, then read twice, from the last-level cache
+
+struct DistillPlan {
+  long bytes, back_bytes;
+  long counts, rows, inv, nlive, slive, amax, Ximg, Wimg, b2, L1, L2, pick, pk, part;   // offsets in bytes
+  long Gimg, coef, gmax, P, slab;
+  int np, Np, Vp, Kp, Kg, nb, splits_cap, et, etw, xsplits;
+  long vc;
+};
+static DistillPlan dt_plan(int dtype, long N, int E, int V, int K) {
+  DistillPlan d = {};
+  d.np = dtype == DT_F32 ? 2 : 1;
+  d.Np = (int)((N + 127) / 128 * 128); d.Vp = (V + 127) / 128 * 128; d.Kp = (E + 63) / 64 * 64; d.Kg = (E + 64) / 64 * 64;
+  d.nb = cdiv(N, DT_CROWS);
+  d.et = cdiv(E, DT_TILE); d.etw = cdiv(E + 1, DT_TILE);
+  const int nt = d.Np / DT_TILE, vt = d.Vp / DT_TILE;
+  d.splits_cap = 8;                                 // live tiles are 1 .. nt: fewer tiles, more splits
+  for (int t = 1; t <= (nt < 64 ? nt : 64); ++t) { const int s = dt_splits(t, vt); if (s > d.splits_cap) d.splits_cap = s; }
+  auto take = [](long& at, long bytes) { const long o = at; at += (bytes + 255) / 256 * 256; return o; };
+  long at = 0;
+  d.counts = take(at, 4L * d.nb); d.rows = take(at, 4 * N); d.inv = take(at, 4 * N); d.nlive = take(at, 4);
+  d.slive = take(at, 4 * N);
+  d.amax = take(at, 8L * DT_AMAX);
+  const long slack = 1024;                          // a column tile of the last row may be read past the row's end
+  d.Ximg = take(at, 2L * d.Np * d.Kp * d.np); d.Wimg = take(at, 2L * d.Vp * d.Kp * d.np + slack);
+  d.b2 = take(at, 4L * d.Vp);
+  d.L1 = take(at, 4L * d.Np); d.L2 = take(at, 4L * d.Np);
+  d.pick = take(at, 4L * N * (K + 1)); d.pk = take(at, 4L * N * K);
+  d.part = take(at, 12L * d.splits_cap * d.Np);
+  d.bytes = at;
+  long vc = DT_PIECE_BYTES / (2L * d.np * d.Np) / 128 * 128;
+  if (vc < 1024) vc = 1024;
+  const int pieces = cdiv(d.Vp, vc);
+  d.vc = ((long)d.Vp / 128 + pieces - 1) / pieces * 128;          // pieces of equal size
+  const int stages = (int)(d.vc / (64 / d.np));
+  d.xsplits = 1024 / (8 * nt * d.et) * 8;           // about 1024 blocks
+  if (d.xsplits < 8) d.xsplits = 8;
+  while (d.xsplits > 8 && stages / d.xsplits < 4) d.xsplits -= 8;
+  at = 0;
+  d.Gimg = take(at, 2L * d.Np * d.Kg * d.np + slack); d.coef = take(at, 12L * d.Np); d.gmax = take(at, 4);
+  d.P = take(at, 2L * d.Np * d.vc * d.np);
+  d.slab = take(at, 4L * d.xsplits * nt * d.et * DT_TILE * DT_TILE);
+  d.back_bytes = at;
+  return d;
+}
+static bool dt_sizes_ok(long N, long E, long V, long K) {
+  return N < (1L << 30) && E > 0 && E <= 65536 && V > 0 && V < (1L << 30) && K >= 0 && K <= V && K <= 65536;
+}
+// 0 where there are no rows, or for sizes that the calls refuse
+long distill_workspace_floats(int dtype, long N, long E, long V, long K) {
+  return N > 0 && dt_sizes_ok(N, E, V, K) ? dt_plan(dtype, N, (int)E, (int)V, (int)K).bytes / 4 : 0;
+}
+long distill_backward_workspace_floats(int dtype, long N, long E, long V, long K) {
+  return N > 0 && dt_sizes_ok(N, E, V, K) ? dt_plan(dtype, N, (int)E, (int)V, (int)K).back_bytes / 4 : 0;
+}
+
+static int dt_check(const char* what, const DistillCall& c) {
+  CVAE_REQUIRE(c.dtype >= DT_F32 && c.dtype <= DT_F16, "%s: dtype %d is none of 0 (fp32), 1 (bf16), 2 (fp16)", what, c.dtype);
+  CVAE_REQUIRE(c.B > 0 && c.T >= 0 && c.R >= 0 && c.R % c.B == 0, "%s: R = %d must be a multiple of B = %d", what, c.R, c.B);
+  CVAE_REQUIRE(dt_sizes_ok((int64_t)c.T * c.R, c.E, c.V, c.K), "%s: bad shape T=%d R=%d E=%d V=%lld K=%d", what, c.T, c.R,
+               c.E, (long long)c.V, c.K);
+  CVAE_REQUIRE(c.K == 0 || (c.tau > 0.f && c.tau < 1e6f), "%s: tau must be positive", what);
+  return 0;
+}
+static void dt_fill(DistillArgs& a, const DistillPlan& d, const DistillCall& c, void* ws) {
+  a.N = c.T * c.R; a.T = c.T; a.R = c.R; a.B = c.B; a.E = c.E; a.V = (int)c.V; a.K = c.K;
+  a.Np = d.Np; a.Vp = d.Vp; a.Kp = d.Kp; a.Kg = d.Kg;
+  a.tau = c.K ? c.tau : 1.f; a.itau = 1.f / a.tau;
+  a.two = c.K > 0 && a.tau != 1.f;
+  a.X = c.X; a.W = c.W; a.bias = c.b; a.tgt = c.tgt; a.pad = c.pad; a.ids = c.ids; a.top = c.top;
+  char* w = static_cast<char*>(ws);
+  a.counts = (int*)(w + d.counts); a.rows = (int*)(w + d.rows); a.inv = (int*)(w + d.inv); a.nlive = (int*)(w + d.nlive); a.slive = (int*)(w + d.slive);
+  a.amax = (float*)(w + d.amax); a.Ximg = (_Float16*)(w + d.Ximg); a.Wimg = (_Float16*)(w + d.Wimg); a.b2 = (float*)(w + d.b2);
+  a.L1 = (float*)(w + d.L1); a.L2 = (float*)(w + d.L2); a.pick = (float*)(w + d.pick); a.pk = (float*)(w + d.pk);
+  a.part = (float*)(w + d.part); a.splits_cap = d.splits_cap;
+}
+
+template <typename T, int NP, bool TWO> static int dt_forward(const DistillPlan& d, const DistillArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((dt_count_kernel<T>), dim3(d.nb + 2 * DT_AMAX), dim3(256), 0, s, a, d.nb);
+  CVAE_LAUNCH_CHECK("dt_count_kernel");
+  hipLaunchKernelGGL((dt_image_kernel<T, NP>), dim3(d.nb + d.Np / 64 + d.Vp / 16), dim3(256), 0, s, a, d.nb);
+  CVAE_LAUNCH_CHECK("dt_image_kernel");
+  hipLaunchKernelGGL((dt_forward_kernel<NP, TWO>), dim3(DT_FWD_BLOCKS), dim3(256), 0, s, a);
+  CVAE_LAUNCH_CHECK("dt_forward_kernel");
+  hipLaunchKernelGGL((dt_combine_kernel<T, TWO>), dim3(a.N), dim3(256), 0, s, a);
+  CVAE_LAUNCH_CHECK("dt_combine_kernel");
+  return 0;
+}
+template <typename T, int NP, bool TWO> static int dt_backward(const DistillPlan& d, DistillArgs a, hipStream_t s) {
+  const int nb = cdiv(a.N, 64), nt = d.Np / DT_TILE;
+  hipLaunchKernelGGL((dt_gimage_kernel<T, NP>), dim3(nb + d.Np / 64), dim3(256), 0, s, a, nb);
+  CVAE_LAUNCH_CHECK("dt_gimage_kernel");
+  a.ldp = d.vc * NP;
+  for (long v0 = 0; v0 < d.Vp; v0 += d.vc) {
+    a.v0 = (int)v0;
+    a.vc = (int)(d.Vp - v0 < d.vc ? d.Vp - v0 : d.vc);
+    const int vt = cdiv(a.vc, DT_TILE);
+    hipLaunchKernelGGL((dt_grad_kernel<NP, TWO>), dim3((unsigned)((long)cdiv(vt, 8) * 8 * nt)), dim3(256), 0, s, a);
+    CVAE_LAUNCH_CHECK("dt_grad_kernel");
+    hipLaunchKernelGGL((dt_pick_kernel<NP, TWO>), dim3(cdiv(a.N, 4)), dim3(256), 0, s, a);
+    CVAE_LAUNCH_CHECK("dt_pick_kernel");
+    hipLaunchKernelGGL((dt_dx_kernel<NP>), dim3((unsigned)((long)nt * d.et * d.xsplits)), dim3(256), 0, s, a, d.et, v0 > 0 ? 1 : 0);
+    CVAE_LAUNCH_CHECK("dt_dx_kernel");
+    hipLaunchKernelGGL((dt_dw_kernel<T, NP>), dim3((unsigned)((long)cdiv(vt, 8) * 8 * d.etw)), dim3(256), 0, s, a, d.etw);
+    CVAE_LAUNCH_CHECK("dt_dw_kernel");
+  }
+  hipLaunchKernelGGL((dt_dx_sum_kernel<T>), dim3((unsigned)((long)nt * d.et * 16)), dim3(256), 0, s, a, d.et);
+  CVAE_LAUNCH_CHECK("dt_dx_sum_kernel");
+  return 0;
+}
+template <typename T, int NP> static int dt_run(const DistillPlan& d, const DistillArgs& a, bool back, hipStream_t s) {
+  if (back) return a.two ? dt_backward<T, NP, true>(d, a, s) : dt_backward<T, NP, false>(d, a, s);
+  return a.two ? dt_forward<T, NP, true>(d, a, s) : dt_forward<T, NP, false>(d, a, s);
+}
+static int dt_dispatch(int dtype, const DistillPlan& d, const DistillArgs& a, bool back, hipStream_t s) {
+  if (dtype == DT_F32) return dt_run<float, 2>(d, a, back, s);
+  return dtype == DT_BF16 ? dt_run<bf16_t, 1>(d, a, back, s) : dt_run<f16_t, 1>(d, a, back, s);
+}
+
+int launch_distill_forward(const DistillCall& c, float* hard_row, float* soft_row, float* hard, float* soft, void* ws,
+                           hipStream_t s) {
+  CVAE_TRY(dt_check("distill_forward", c));
+  if (c.R == 0) return 0;
+  CVAE_REQUIRE(hard && (c.K == 0 || soft), "distill_forward: null operand");
+  if (c.T > 0) {
+    CVAE_REQUIRE(c.X && c.W && c.b && c.tgt && hard_row && ws && (c.K == 0 || (c.ids && c.top && soft_row)),
+                 "distill_forward: null operand");
+    CVAE_REQUIRE(((uintptr_t)ws & 15) == 0, "distill_forward: the workspace must be 16-byte aligned");
+    const DistillPlan d = dt_plan(c.dtype, (long)c.T * c.R, c.E, (int)c.V, c.K);
+    DistillArgs a = {};
+    dt_fill(a, d, c, ws);
+    a.hard = hard_row; a.soft = soft_row;
+    CVAE_TRY(dt_dispatch(c.dtype, d, a, false, s));
+  }
+  CVAE_TRY(launch_sum_time(hard_row, c.T, c.R, hard, s));
+  if (c.K) CVAE_TRY(launch_sum_time(soft_row, c.T, c.R, soft, s));
+  return 0;
+}
+
+int launch_distill_backward(const DistillCall& c, const float* ghard, const float* gsoft, const void* saved, void* dX,
+                            void* dW, void* db, void* ws, hipStream_t s) {
+  CVAE_TRY(dt_check("distill_backward", c));
+  CVAE_REQUIRE((int64_t)c.T * c.R > 0, "distill_backward: no rows");
+  CVAE_REQUIRE(c.X && c.W && c.b && c.tgt && ghard && saved && dX && dW && db && ws && (c.K == 0 || (c.ids && c.top && gsoft)),
+               "distill_backward: null operand");
+  CVAE_REQUIRE((((uintptr_t)ws | (uintptr_t)saved) & 15) == 0, "distill_backward: the workspaces must be 16-byte aligned");
+  const DistillPlan d = dt_plan(c.dtype, (long)c.T * c.R, c.E, (int)c.V, c.K);
+  DistillArgs a = {};
+  dt_fill(a, d, c, const_cast<void*>(saved));
+  a.ghard = ghard; a.gsoft = gsoft; a.dX = dX; a.dW = dW; a.db = db;
+  char* w = static_cast<char*>(ws);
+  a.Gimg = (_Float16*)(w + d.Gimg); a.coef = (float*)(w + d.coef); a.gmax = (float*)(w + d.gmax);
+  a.P = (_Float16*)(w + d.P); a.slab = (float*)(w + d.slab); a.xsplits = d.xsplits;
+  return dt_dispatch(c.dtype, d, a, true, s);
+}
+
+}  // namespace cvae

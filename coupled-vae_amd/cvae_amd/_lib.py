@@ -78,6 +78,10 @@ SIGNATURES = {
     'cvae_projce_forward_train_n': [I, P, P, P, P, L, I, I, I, L, P, P, P, P, P, P],
     'cvae_projce_backward_saved_n_workspace': [L],
     'cvae_projce_backward_saved_n': [I, P, P, P, P, L, P, P, I, I, I, L, P, P, P, P, P, P],
+    'cvae_distill_workspace': [I, L, L, L, I],
+    'cvae_distill_backward_workspace': [I, L, L, L, I],
+    'cvae_distill_forward': [I, P, P, P, P, L, I, I, I, I, L, I, P, P, F, P, P, P, P, P, P],
+    'cvae_distill_backward': [I, P, P, P, P, L, I, I, I, I, L, I, P, P, F] + [P] * 8,
     'cvae_targets_time_major': [P, I, I, I, P, P],
     'cvae_logits': [P, P, P, I, I, I, L, P, P, P],
     'cvae_reparam_forward': [P, P, P, I, I, I, P, P],
@@ -103,7 +107,8 @@ SIGNATURES = {
 _RESTYPE_LONG = {'cvae_encoder_backward_scratch', 'cvae_decoder_backward_scratch', 'cvae_projce_workspace',
                  'cvae_decoder_greedy_scratch', 'cvae_projce_logits_workspace', 'cvae_projce_backward_saved_n_workspace', 'cvae_decoder_beam_scratch',
                  'cvae_projce_backward_workspace', 'cvae_mi_static_max_rows', 'cvae_stream_rnn_min_bytes',
-                 'cvae_linrnn_state_floats', 'cvae_linrnn_workspace'}
+                 'cvae_linrnn_state_floats', 'cvae_linrnn_workspace', 'cvae_distill_workspace',
+                 'cvae_distill_backward_workspace'}
 
 for _name, _args in SIGNATURES.items():
     _fn = getattr(lib, _name)          # AttributeError here = header and library out of sync

@@ -632,19 +632,93 @@ class ProjCEFn(torch.autograd.Function):
         return dfinal, dW, db, None, None
 
 
-def proj_ce(final, W, b, eos, pad, cache=None):
-    """final (T,R,E), eos (B,T) with R % B == 0 -> (R,).  `cache`: a dict shared by the losses of one forward pass
-    (the two decoders of a training step read the same targets): the time-major targets are built once."""
-    R = final.shape[1]
+class ProjDistillFn(torch.autograd.Function):
+    """Per-sentence hard (cross-entropy) and soft (teacher's top logits) losses of projected logits that are never
+    stored (cvae_distill_*); fp32, bf16 or fp16 storage.  ids = None: the hard loss alone."""
+
+    @staticmethod
+    def forward(ctx, final, W, b, tgt_tm, pad, B, ids, top, tau):
+        T, R, E = final.shape
+        V, K = W.shape[0], 0 if ids is None else ids.shape[2]
+        dt, N = _DTYPE[final.dtype], T * R
+        rows, hard, soft = _f((2 * N,), final), _f((R,), final), _f((R,), final)
+        ws = _f((query('cvae_distill_workspace', dt, N, E, V, K),), final)
+        ctx.args = (pad, B, T, R, E, V, K)
+        ctx.tau = tau
+        call('cvae_distill_forward', dt, ptr(final), ptr(W), ptr(b), ptr(tgt_tm), *ctx.args, ptr(ids), ptr(top), tau,
+             ptr(rows), rows.data_ptr() + 4 * N, ptr(hard), ptr(soft) if K else None, ptr(ws), stream())
+        if any(ctx.needs_input_grad):
+            ctx.save_for_backward(final, W, b, tgt_tm, ids, top, ws)
+        return hard, soft
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, ghard, gsoft):
+        final, W, b, tgt_tm, ids, top, saved = ctx.saved_tensors
+        pad, B, T, R, E, V, K = ctx.args
+        dt, N = _DTYPE[final.dtype], T * R
+        if N == 0:
+            return (torch.zeros_like(final), torch.zeros_like(W), torch.zeros_like(b)) + (None,) * 6
+        ghard, gsoft = _c(ghard), _c(gsoft)
+        dfinal, dW, db = torch.empty_like(final), torch.empty_like(W), torch.empty_like(b)
+        ws = _f((query('cvae_distill_backward_workspace', dt, N, E, V, K),), final)
+        call('cvae_distill_backward', dt, ptr(final), ptr(W), ptr(b), ptr(tgt_tm), *ctx.args, ptr(ids), ptr(top), ctx.tau,
+             ptr(ghard), ptr(gsoft), ptr(saved), ptr(dfinal), ptr(dW), ptr(db), ptr(ws), stream())
+        return (dfinal, dW, db) + (None,) * 6
+
+
+def _proj_check(final, W, b, eos):
+    _need(final.dim() == 3 and W.dim() == 2 and tuple(b.shape) == (W.shape[0],) and final.shape[2] == W.shape[1],
+          'final must be (T,R,E), W (V,E) and b (V,)')
+    _need(final.dtype in _DTYPE and W.dtype == final.dtype and b.dtype == final.dtype,
+          'final, W and b must share one of float32, bfloat16, float16')
+    _need(W.shape[0] > 0 and W.shape[1] > 0, 'W is empty')
+    _need(eos.dim() == 2 and eos.dtype == torch.int64 and eos.shape[0] > 0 and eos.shape[1] == final.shape[0] and
+          final.shape[1] % eos.shape[0] == 0, 'eos must be int64 (B,T) with R a multiple of B')
+
+
+def proj_distill(final, W, b, eos, pad, teacher_ids, teacher_logits, tau, cache=None):
+    """Cross-entropy and distillation of one student projection, logits never stored: final (T,R,E), W (V,E), b (V,) in
+    fp32, bf16 or fp16; eos (B,T) int64 targets (rows at `pad` count nothing), R % B == 0; the teacher's K best of every
+    position: teacher_ids (B,T,K) int64, teacher_logits (B,T,K) float (ids outside the vocabulary and logits of -inf are
+    absent entries).  With p = softmax(teacher_logits / tau) over the K entries and q_tau = softmax(logits / tau) over
+    the whole vocabulary:
+      hard (R,) = sum_t -log softmax(logits)[target],   soft (R,) = sum_t tau^2 KL(p || q_tau)
+    -> (hard, soft) fp32, differentiable in final, W and b.  `cache` as in proj_ce."""
+    _proj_check(final, W, b, eos)
+    _need(teacher_ids.dim() == 3 and teacher_ids.dtype == torch.int64 and
+          tuple(teacher_ids.shape[:2]) == tuple(eos.shape) and 0 < teacher_ids.shape[2] <= W.shape[0],
+          'teacher_ids must be int64 (B,T,K) with 0 < K <= V')
+    _need(teacher_logits.shape == teacher_ids.shape and teacher_logits.is_floating_point(),
+          'teacher_logits must be a float tensor of the shape of teacher_ids')
+    _need(0.0 < tau < 1e6, 'tau must be positive')
+    _here(final, W, b, eos, teacher_ids, teacher_logits)
+    tgt = _targets(eos, final.shape[1], cache)
+    return ProjDistillFn.apply(_c(final), _c(W), _c(b), tgt, pad, eos.shape[0], _c(teacher_ids),
+                               _c(teacher_logits.float()), float(tau))
+
+
+def _targets(eos, R, cache):
+    """Time-major targets, built once for the losses that share `cache`."""
     if cache is None:
-        tgt = targets_time_major(eos, R)
-    else:
-        key = ('tgt_tm', eos.data_ptr(), tuple(eos.shape), tuple(eos.stride()), eos._version, R)
-        hit = cache.get(key)
-        if hit is None:
-            hit = cache[key] = (targets_time_major(eos, R), eos)      # holds `eos`: its storage stays pinned
-        tgt = hit[0]
-    return ProjCEFn.apply(final, W, b, tgt, pad)
+        return targets_time_major(eos, R)
+    key = ('tgt_tm', eos.data_ptr(), tuple(eos.shape), tuple(eos.stride()), eos._version, R)
+    hit = cache.get(key)
+    if hit is None:
+        hit = cache[key] = (targets_time_major(eos, R), eos)      # holds `eos`: its storage stays pinned
+    return hit[0]
+
+
+def proj_ce(final, W, b, eos, pad, cache=None):
+    """final (T,R,E), W (V,E), b (V,), eos (B,T) with R % B == 0 -> (R,) fp32.  fp32, or bf16 / fp16 throughout (then
+    through the kernels of proj_distill).  `cache`: a dict shared by the losses of one forward pass
+    (the two decoders of a training step read the same targets): the time-major targets are built once."""
+    if final.dtype != torch.float32:
+        _proj_check(final, W, b, eos)
+        _here(final, W, b, eos)
+        tgt = _targets(eos, final.shape[1], cache)
+        return ProjDistillFn.apply(_c(final), _c(W), _c(b), tgt, pad, eos.shape[0], None, None, 1.0)[0]
+    return ProjCEFn.apply(final, W, b, _targets(eos, final.shape[1], cache), pad)
 
 
 class ProjCEPairFn(torch.autograd.Function):
@@ -701,6 +775,8 @@ def proj_ce_pair_ok(finals, Ws):
     """The paired path covers a training step whose decoders have one shape and whose logits fit the save budget."""
     if not (settings.ce_pair and settings.ce_save_logits and torch.is_grad_enabled()):
         return False
+    if any(f.dtype != torch.float32 for f in finals):
+        return False
     T, R, E = finals[0].shape
     V = Ws[0].shape[0]
     if any(f.shape != finals[0].shape for f in finals) or any(w.shape != Ws[0].shape for w in Ws):
@@ -710,23 +786,21 @@ def proj_ce_pair_ok(finals, Ws):
 
 
 def proj_ce_pair(finals, Ws, bs, eos, pad, cache=None):
-    """[final (T,R,E)] * nd, eos (B,T) -> nd per-sentence sums (R,), as nd proj_ce calls."""
-    R = finals[0].shape[1]
-    if cache is None:
-        tgt = targets_time_major(eos, R)
-    else:
-        key = ('tgt_tm', eos.data_ptr(), tuple(eos.shape), tuple(eos.stride()), eos._version, R)
-        hit = cache.get(key)
-        if hit is None:
-            hit = cache[key] = (targets_time_major(eos, R), eos)
-        tgt = hit[0]
+    """[final (T,R,E)] * nd, eos (B,T) -> nd per-sentence sums (R,), as nd proj_ce calls.  fp32."""
+    _need(all(t.dtype == torch.float32 for t in (*finals, *Ws, *bs)), 'proj_ce_pair takes float32 (16-bit: proj_ce)')
+    tgt = _targets(eos, finals[0].shape[1], cache)
     flat = [t for d in range(len(finals)) for t in (finals[d], Ws[d], bs[d])]
     return ProjCEPairFn.apply(pad, tgt, *flat)
 
 
 def proj_ce_sorted(final, W, b, eos, pad):
-    """final (T,B*K,E) on sentence-major rows, eos (B,T) -> (B*K,)."""
+    """final (T,B*K,E) on sentence-major rows, eos (B,T) -> (B*K,).  fp32, or bf16 / fp16 throughout."""
     B = eos.shape[0]
+    if final.dtype != torch.float32:
+        _proj_check(final, W, b, eos)
+        _here(final, W, b, eos)
+        tgt = targets_sentence_major(eos, final.shape[1] // B)
+        return ProjDistillFn.apply(_c(final), _c(W), _c(b), tgt, pad, B, None, None, 1.0)[0]
     tgt = targets_sentence_major(eos, final.shape[1] // B)
     return ProjCEFn.apply(final, W, b, tgt, pad)
 

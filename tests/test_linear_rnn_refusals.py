@@ -61,3 +61,5 @@ def test_c_entries_refuse_bad_arguments():
     for name in ('cvae_linrnn_forward', 'cvae_linrnn_backward'):         # nothing to do
         n = len(_lib.SIGNATURES[name]) - 6
         _lib.call(name, 0, 3, 0, 4, 0, 8, *([None] * n))
+    for sizes in ((0, 2, 8), (4, 0, 8), (4, 2, 0), (0, 0, 0), (1, 1, 1)):
+        assert _lib.query('cvae_linrnn_workspace', 0, *sizes) == 0

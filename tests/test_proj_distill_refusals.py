@@ -1,0 +1,80 @@
+"""Calls of the 16-bit cross-entropy and of the distillation loss that have to be refused before anything is launched."""
+import pytest
+import torch
+
+from cvae_amd import _lib, ops
+
+T, B, E, V, K = 4, 2, 8, 10, 3
+
+
+def good():
+    return dict(final=torch.zeros(T, B, E), W=torch.zeros(V, E), b=torch.zeros(V), eos=torch.ones(B, T, dtype=torch.int64), pad=0,
+                teacher_ids=torch.zeros(B, T, K, dtype=torch.int64), teacher_logits=torch.zeros(B, T, K), tau=2.0)
+
+
+@pytest.mark.parametrize('what,change', [
+    ('must be \\(T,R,E\\)', dict(final=torch.zeros(T, B, E + 1))),
+    ('must be \\(T,R,E\\)', dict(final=torch.zeros(T, E))),
+    ('must be \\(T,R,E\\)', dict(b=torch.zeros(V + 1))),
+    ('must share', dict(W=torch.zeros(V, E, dtype=torch.bfloat16))),
+    ('must share', dict(final=torch.zeros(T, B, E, dtype=torch.float64), W=torch.zeros(V, E, dtype=torch.float64),
+                        b=torch.zeros(V, dtype=torch.float64))),
+    ('W is empty', dict(W=torch.zeros(0, E), b=torch.zeros(0))),
+    ('eos must be', dict(eos=torch.ones(B, T + 1, dtype=torch.int64))),
+    ('eos must be', dict(eos=torch.ones(3, T, dtype=torch.int64))),
+    ('eos must be', dict(eos=torch.ones(B, T, dtype=torch.int32))),
+    ('teacher_ids', dict(teacher_ids=torch.zeros(B, T, K, dtype=torch.int32))),
+    ('teacher_ids', dict(teacher_ids=torch.zeros(T, B, K, dtype=torch.int64))),
+    ('teacher_ids', dict(teacher_ids=torch.zeros(B, T, V + 1, dtype=torch.int64))),
+    ('teacher_ids', dict(teacher_ids=torch.zeros(B, T, 0, dtype=torch.int64))),
+    ('teacher_logits', dict(teacher_logits=torch.zeros(B, T, K + 1))),
+    ('teacher_logits', dict(teacher_logits=torch.zeros(B, T, K, dtype=torch.int64))),
+    ('tau', dict(tau=0.0)), ('tau', dict(tau=-1.0)), ('tau', dict(tau=float('nan'))), ('tau', dict(tau=float('inf'))),
+    ('current GPU', dict()),
+])
+def test_proj_distill_refuses(what, change, monkeypatch):
+    monkeypatch.setattr(torch.cuda, 'current_device', lambda: 0)
+    with pytest.raises(ValueError, match=what):
+        ops.proj_distill(**dict(good(), **change))
+
+
+@pytest.mark.parametrize('what,change', [
+    ('must share', dict(W=torch.zeros(V, E))),
+    ('eos must be', dict(eos=torch.ones(3, T, dtype=torch.int64))),
+    ('current GPU', dict()),
+])
+def test_proj_ce_16_bit_refuses(what, change, monkeypatch):
+    monkeypatch.setattr(torch.cuda, 'current_device', lambda: 0)
+    a = good()
+    a = {k: a[k].to(torch.bfloat16) if k in ('final', 'W', 'b') else a[k] for k in ('final', 'W', 'b', 'eos', 'pad')}
+    for f in (ops.proj_ce, ops.proj_ce_sorted):
+        with pytest.raises(ValueError, match=what):
+            f(**dict(a, **change))
+    with pytest.raises(ValueError, match='float32'):
+        ops.proj_ce_pair([a['final']], [a['W']], [a['b']], a['eos'], 0)
+    assert not ops.proj_ce_pair_ok([a['final']], [a['W']])
+
+
+def test_c_entries_refuse_bad_arguments():
+    one = 16                                   # never dereferenced: the call is refused first
+    ok = dict(dtype=0, B=2, T=4, R=2, E=8, V=10, K=3, tau=2.0, ws=one)
+
+    def forward(**kw):
+        a = dict(ok, **kw)
+        _lib.call('cvae_distill_forward', a['dtype'], one, one, one, one, 0, a['B'], a['T'], a['R'], a['E'], a['V'], a['K'],
+                  one, one, a['tau'], one, one, one, one, a['ws'], None)
+
+    def backward(**kw):
+        a = dict(ok, **kw)
+        _lib.call('cvae_distill_backward', a['dtype'], one, one, one, one, 0, a['B'], a['T'], a['R'], a['E'], a['V'], a['K'],
+                  one, one, a['tau'], one, one, one, one, one, one, a['ws'], None)
+    for f in (forward, backward):
+        for bad in (dict(dtype=3), dict(B=0), dict(R=3), dict(T=-1), dict(T=1 << 20, R=1 << 12), dict(E=0), dict(V=0),
+                    dict(V=1 << 31), dict(K=-1), dict(K=11), dict(tau=0.0), dict(tau=float('nan')), dict(ws=None), dict(ws=24)):
+            with pytest.raises(_lib.CvaeHipError, match='distill_'):
+                f(**bad)
+    for name in ('cvae_distill_workspace', 'cvae_distill_backward_workspace'):      # sizes of nothing, or refused ones: 0
+        assert _lib.query(name, 1, 5, 8, 10, 3) > 0
+        for sizes in ((0, 8, 10, 3), (-1, 8, 10, 3), (5, 0, 10, 3), (5, 8, 0, 0), (5, 8, 10, 11), (5, 8, 10, -1),
+                      (1 << 40, 8, 10, 3), (5, 1 << 40, 10, 3), (5, 8, 1 << 40, 3)):
+            assert _lib.query(name, 1, *sizes) == 0, sizes

@@ -30,7 +30,7 @@ typedef __attribute__((address_space(3))) s4 lds_s4;
 
 constexpr int DT_TILE = 128;               // rows / columns of a tile, both ways
 constexpr int DT_STAGE = 16384;            // bytes of one operand's stage: 128 rows x 128 bytes
-constexpr int DT_AMAX = 256;               // partial maxima of |X| and |W|
+constexpr int DT_AMAX = 512;               // partial maxima of |X| and |W|, each
 constexpr int DT_CROWS = 256;              // rows of one count of the live-row scan
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int P_EXP = 13;                  // |P| <= 1 is stored times 2^13
@@ -46,9 +46,10 @@ struct DistillArgs {
   float* hard; float* soft;                // [N]
   // kept for the backward pass
   int* counts; int* rows; int* inv; int* nlive; int* slive;   // slive[R]: the sentence has a live row
-  float* amax;                             // [2][DT_AMAX]
+  float* amax; int* sexp;                  // [2][DT_AMAX]; [2] scale exponents of X and W
   _Float16* Ximg; _Float16* Wimg; float* b2;
-  float* L1; float* L2; float* pick; float* pk;   // by live row: normalisers (base 2), picked logits [K+1], p [K]
+  float* L1; float* L2; float* some;       // by live row: normalisers (base 2), 1 where the teacher lists anything
+  float* pick; float* share;               // picked logits (base 2) and the teacher's share of them, [K + 1]
   float* part; int splits_cap;             // [3][splits][Np]
   // backward
   const float* ghard; const float* gsoft;  // [R]
@@ -65,14 +66,14 @@ __device__ __forceinline__ int scale_exp(float amax) {          // amax * 2^e in
   const int e = P_EXP - (int)floorf(log2f(amax));
   return e < -60 ? -60 : (e > 60 ? 60 : e);
 }
-// largest finite magnitude of a tensor from its partials, by every thread of a block of >= 256 threads
+// largest finite magnitude of a tensor from its partials, by every thread of a block of 256
 __device__ __forceinline__ float block_amax(const float* part, float* red) {
-  float m = threadIdx.x < DT_AMAX ? part[threadIdx.x] : 0.f;
-  m = wave_max(m);
+  static_assert(DT_AMAX == 512, "two partials a thread");
+  float m = wave_max(fmaxf(part[threadIdx.x], part[threadIdx.x + 256]));
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
   __syncthreads();
   m = 0.f;
-  for (int i = 0; i < (int)blockDim.x / 64; ++i) m = fmaxf(m, red[i]);
+  for (int i = 0; i < 4; ++i) m = fmaxf(m, red[i]);
   __syncthreads();
   return m;
 }
@@ -121,21 +122,40 @@ template <typename T> __global__ __launch_bounds__(256) void dt_count_kernel(Dis
     return;
   }
   // (what stands in dropped rows does not set the scale of the others)
+  // (what stands in dropped rows does not set the scale of the others)
   const int b = blockIdx.x - nb, which = b / DT_AMAX, slot = b % DT_AMAX;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const T* x = static_cast<const T*>(which ? p.W : p.X);
-  const int rows = which ? p.V : p.N;
-  const bool vec = p.E % 4 == 0 && ((uintptr_t)x % (4 * sizeof(T))) == 0;
   float m = 0.f;
-  for (int n = slot * 4 + wave; n < rows; n += DT_AMAX * 4) {
-    if (!which && p.tgt[n] == p.pad) continue;
-    for (int k = lane * 4; k < p.E; k += 256) {
-      float v[4];
-      load4<T>(x + (long)n * p.E, k, p.E, vec, v);
+  const auto take = [&](float v) { v = fabsf(v); m = v < 3.4e38f ? fmaxf(m, v) : m; };
+  if (which) {
+    const T* x = static_cast<const T*>(p.W);
+    constexpr int VN = 16 / sizeof(T);
+    const long n = (long)p.V * p.E;
+    long head = (long)((16 - ((uintptr_t)x & 15)) & 15) / (long)sizeof(T);      // elements before a 16-byte boundary
+    if (head > n) head = n;
+    const long nv = (n - head) / VN, tail = head + nv * VN;
+    if (slot == 0) {
+      for (long i = threadIdx.x; i < head; i += 256) take((float)x[i]);
+      for (long i = tail + threadIdx.x; i < n; i += 256) take((float)x[i]);
+    }
+    const Packed<T, VN>* xv = reinterpret_cast<const Packed<T, VN>*>(x + head);
+#pragma unroll 4
+    for (long i = (long)slot * 256 + threadIdx.x; i < nv; i += (long)DT_AMAX * 256) {
+      const Packed<T, VN> r = xv[i];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float a = fabsf(v[j]);
-        if (a < 3.4e38f) m = fmaxf(m, a);
+      for (int j = 0; j < VN; ++j) take(r.f(j));
+    }
+  } else {
+    const T* x = static_cast<const T*>(p.X);
+    const bool vec = p.E % 4 == 0 && ((uintptr_t)x % (4 * sizeof(T))) == 0;
+#pragma unroll 2
+    for (int n = slot * 4 + wave; n < p.N; n += DT_AMAX * 4) {
+      if (p.tgt[n] == p.pad) continue;
+      for (int k = lane * 4; k < p.E; k += 256) {
+        float v[4];
+        load4<T>(x + (long)n * p.E, k, p.E, vec, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) take(v[j]);
       }
     }
   }
@@ -145,34 +165,66 @@ template <typename T> __global__ __launch_bounds__(256) void dt_count_kernel(Dis
   if (threadIdx.x == 0) p.amax[which * DT_AMAX + slot] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
 
-// the row list and the images.  Blocks [0, nb): DT_CROWS rows of X each, to their places in the compact order; the
-// next Np / 64: zeros of the compact rows past the last live one; the rest: 16 rows of W and its bias each.
-template <typename T, int NP> __global__ __launch_bounds__(256) void dt_image_kernel(DistillArgs p, int nb) {
+// four rows of an image by a wave, loaded together: row[q] (null: zeros, when `to` is not) -> to[q] (null: none)
+template <typename T, int NP>
+__device__ __forceinline__ void image_rows(const T* const (&row)[4], _Float16* const (&to)[4], int E, int K4, bool vec,
+                                           const int (&e)[4], int lane, float one) {
+  for (int k = lane; k < K4; k += 64) {
+    float x[4][4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[q][j] = 0.f;
+      if (row[q]) load4<T>(row[q], 4 * k, E, vec, x[q]);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (!to[q]) continue;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[q][j] = ldexpf(x[q][j], e[q]);
+        if (one != 0.f && 4 * k + j == E && row[q]) x[q][j] = ldexpf(one, e[q]);
+      }
+      store4<NP>(to[q], 4 * k, x[q]);
+    }
+  }
+}
+
+// The row list and the images, 16 rows a block.  Blocks [0, cdiv(N, 16)): rows of X to their places in the compact
+// order; the next Np / 16: zeros of the compact rows past the last live one; the rest: rows of W and its bias.
+template <typename T, int NP> __global__ __launch_bounds__(256) void dt_image_kernel(DistillArgs p, int nx) {
   __shared__ float red[4];
-  __shared__ int sred[4], swave[4];
+  __shared__ int sred[4], swave[4], slot[DT_CROWS];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const long ld = (long)p.Kp * NP;
-  const int k4 = p.Kp / 4;
+  const int nb = (p.N + DT_CROWS - 1) / DT_CROWS;
   int blk = blockIdx.x;
-  if (blk < nb + p.Np / 64) {
-    const bool tail = blk >= nb;
-    const int upto = tail ? nb : blk;
+  const T* row[4];
+  _Float16* to[4];
+  int ee[4];
+  if (blk < nx + p.Np / 16) {
+    const bool tail = blk >= nx;
+    const int group = tail ? nb : blk * 16 / DT_CROWS;
     int s = 0;
-    for (int i = threadIdx.x; i < upto; i += 256) s += p.counts[i];
+    for (int i = threadIdx.x; i < group; i += 256) s += p.counts[i];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if (lane == 0) sred[wave] = s;
     if (tail) {
       __syncthreads();
       const int nl = sred[0] + sred[1] + sred[2] + sred[3];
-      if (blk == nb && threadIdx.x == 0) *p.nlive = nl;
-      for (int i = (blk - nb) * 64 + wave; i < (blk - nb) * 64 + 64; i += 4)
-        if (i >= nl)
-          for (int k = lane; k < k4 * NP; k += 64) reinterpret_cast<Packed<f16_t, 4>*>(p.Ximg + i * ld)[k] = Packed<f16_t, 4>{};
+      if (blk == nx && threadIdx.x == 0) *p.nlive = nl;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int i = (blk - nx) * 16 + wave * 4 + q;
+        row[q] = nullptr;
+        to[q] = i >= nl ? p.Ximg + i * ld : nullptr;
+        ee[q] = 0;
+      }
+      image_rows<T, NP>(row, to, p.E, p.Kp / 4, false, ee, lane, 0.f);
       return;
     }
-    __shared__ int slot[DT_CROWS];
-    const int n = blk * DT_CROWS + threadIdx.x;
+    const int n = group * DT_CROWS + threadIdx.x;
     const bool live = n < p.N && p.tgt[n] != p.pad;
     const unsigned long long b = __ballot(live);
     if (lane == 0) swave[wave] = __popcll(b);
@@ -181,38 +233,39 @@ template <typename T, int NP> __global__ __launch_bounds__(256) void dt_image_ke
     for (int i = 0; i < wave; ++i) off += swave[i];
     off += __popcll(b & ((1ull << lane) - 1ull));
     slot[threadIdx.x] = live ? off : -1;
-    if (n < p.N) p.inv[n] = live ? off : -1;
-    if (live) p.rows[off] = n;
-    const int e = scale_exp(block_amax(p.amax, red));            // (its barriers also publish slot[])
-    const bool vec = p.E % 4 == 0 && ((uintptr_t)p.X % (4 * sizeof(T))) == 0;
-    for (int i = wave; i < DT_CROWS; i += 4) {
-      const int to = slot[i];
-      if (to < 0) continue;
-      const T* row = static_cast<const T*>(p.X) + (long)(blk * DT_CROWS + i) * p.E;
-      for (int k = lane; k < k4; k += 64) {
-        float x[4];
-        load4<T>(row, 4 * k, p.E, vec, x);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = ldexpf(x[j], e);
-        store4<NP>(p.Ximg + to * ld, 4 * k, x);
-      }
+    if (blk * 16 == group * DT_CROWS) {                           // the group's first block writes its lists
+      if (n < p.N) p.inv[n] = live ? off : -1;
+      if (live) p.rows[off] = n;
     }
+    const int e = scale_exp(block_amax(p.amax, red));             // (its barriers also publish slot[])
+    if (blk == 0 && threadIdx.x == 0) p.sexp[0] = e;
+    const bool vec = p.E % 4 == 0 && ((uintptr_t)p.X % (4 * sizeof(T))) == 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int nn = blk * 16 + wave * 4 + q, at = slot[nn - group * DT_CROWS];
+      row[q] = at >= 0 ? static_cast<const T*>(p.X) + (long)nn * p.E : nullptr;
+      to[q] = at >= 0 ? p.Ximg + at * ld : nullptr;
+      ee[q] = e;
+    }
+    image_rows<T, NP>(row, to, p.E, p.Kp / 4, vec, ee, lane, 0.f);
     return;
   }
-  blk -= nb + p.Np / 64;
+  blk -= nx + p.Np / 16;
   const int e = scale_exp(block_amax(p.amax + DT_AMAX, red));
+  if (blk == 0 && threadIdx.x == 0) p.sexp[1] = e;
   const bool vec = p.E % 4 == 0 && ((uintptr_t)p.W % (4 * sizeof(T))) == 0;
-  for (int v = blk * 16 + wave; v < blk * 16 + 16; v += 4) {
-    const T* row = static_cast<const T*>(p.W) + (long)v * p.E;
-    for (int k = lane; k < k4; k += 64) {
-      float x[4] = {0.f, 0.f, 0.f, 0.f};
-      if (v < p.V) load4<T>(row, 4 * k, p.E, vec, x);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = ldexpf(x[j], e);
-      store4<NP>(p.Wimg + v * ld, 4 * k, x);
-    }
-    if (lane == 0) p.b2[v] = v < p.V ? (float)static_cast<const T*>(p.bias)[v] * LOG2E : -INFINITY;
+  for (int q = 0; q < 4; ++q) {
+    const int v = blk * 16 + wave * 4 + q;
+    row[q] = v < p.V ? static_cast<const T*>(p.W) + (long)v * p.E : nullptr;
+    to[q] = p.Wimg + v * ld;
+    ee[q] = e;
   }
+  if (threadIdx.x < 16) {
+    const int v = blk * 16 + threadIdx.x;
+    p.b2[v] = v < p.V ? (float)static_cast<const T*>(p.bias)[v] * LOG2E : -INFINITY;
+  }
+  image_rows<T, NP>(row, to, p.E, p.Kp / 4, vec, ee, lane, 0.f);
 }
 
 // ------------------------------------------------------------------------------------------------- the product loop
@@ -308,24 +361,61 @@ __device__ __forceinline__ void clear(f32x16 (&acc)[2][2]) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 }
-// this block's loads into LDS have arrived, and every wave has left the buffer that is filled next
+// this wave's copies into LDS have arrived and its reads of the other buffers are over; then those of all waves
 __device__ __forceinline__ void stage_barrier() {
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070);                             // vmcnt(0) lgkmcnt(0), where the compiler sees it
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
-// stages [0, n) of one tile; `last` K blocks of the last stage are used
-template <int NP, bool AKS, bool BKS>
-__device__ __forceinline__ void product(const Operand<NP, AKS>& A, const Operand<NP, BKS>& B, int n, int last, char* lds,
-                                        int am, int bn, int lane, int wave, f32x16 (&acc)[2][2]) {
-  clear(acc);
-  if (n > 0) { A.issue(0, lds, wave); B.issue(0, lds + DT_STAGE, wave); }
-  for (int s = 0; s < n; ++s) {
-    char* cur = lds + (s & 1) * 2 * DT_STAGE;
-    char* nxt = lds + ((s + 1) & 1) * 2 * DT_STAGE;
+// Two buffers of two operands as four arrays: the compiler then sees that a copy into one is no reason for a read of
+// another to wait (it waits for every copy in flight when buffers share an array, and nothing overlaps).
+#define DT_LDS \
+  __shared__ __attribute__((aligned(16))) char la0[DT_STAGE]; \
+  __shared__ __attribute__((aligned(16))) char lb0[DT_STAGE]; \
+  __shared__ __attribute__((aligned(16))) char la1[DT_STAGE]; \
+  __shared__ __attribute__((aligned(16))) char lb1[DT_STAGE];
+// the four together as one area of 64 KiB for an epilogue, in units of 16 KiB
+#define DT_AREA(i) ((i) == 0 ? la0 : (i) == 1 ? lb0 : (i) == 2 ? la1 : lb1)
+
+// Stages [0, n), n > 0, of one tile, stage 0 already on its way into (la, lb); `last` K blocks of the last stage are used.
+// While a stage is multiplied the next one loads: behind the last one, whatever then(a, b) asks for the free pair.
+// (No stage is left out of the loop's middle: a `break` there cost 64 register moves a round.)
+template <int NP, bool AKS, bool BKS, typename Then>
+__device__ __forceinline__ void stages(const Operand<NP, AKS>& A, const Operand<NP, BKS>& B, int n, int last, char* la,
+                                       char* lb, char* na, char* nb, int am, int bn, int lane, int wave,
+                                       f32x16 (&acc)[2][2], const Then& then) {
+  int s = 0;
+  for (; s + 3 <= n; s += 2) {
     stage_barrier();
-    if (s + 1 < n) { A.issue(s + 1, nxt, wave); B.issue(s + 1, nxt + DT_STAGE, wave); }
-    stage_product<NP, AKS, BKS>(cur, cur + DT_STAGE, am, bn, s + 1 < n ? 4 : last, lane, acc);
+    A.issue(s + 1, na, wave); B.issue(s + 1, nb, wave);
+    stage_product<NP, AKS, BKS>(la, lb, am, bn, 4, lane, acc);
+    stage_barrier();
+    A.issue(s + 2, la, wave); B.issue(s + 2, lb, wave);
+    stage_product<NP, AKS, BKS>(na, nb, am, bn, 4, lane, acc);
   }
+  if (s + 2 == n) {
+    stage_barrier();
+    A.issue(s + 1, na, wave); B.issue(s + 1, nb, wave);
+    stage_product<NP, AKS, BKS>(la, lb, am, bn, 4, lane, acc);
+    stage_barrier();
+    then(la, lb);
+    stage_product<NP, AKS, BKS>(na, nb, am, bn, last, lane, acc);
+  } else {
+    stage_barrier();
+    then(na, nb);
+    stage_product<NP, AKS, BKS>(la, lb, am, bn, last, lane, acc);
+  }
+}
+template <int NP, bool AKS, bool BKS>
+__device__ __forceinline__ void product(const Operand<NP, AKS>& A, const Operand<NP, BKS>& B, int n, int last, char* la0,
+                                        char* lb0, char* la1, char* lb1, int am, int bn, int lane, int wave,
+                                        f32x16 (&acc)[2][2]) {
+  clear(acc);
+  if (n <= 0) return;
+  A.issue(0, la0, wave);
+  B.issue(0, lb0, wave);
+  stages<NP, AKS, BKS>(A, B, n, last, la0, lb0, la1, lb1, am, bn, lane, wave, acc, [](char*, char*) {});
 }
 // value r of an accumulator tile: row 4 (lane / 32) + 8 (r / 4) + r % 4, column lane % 32
 __device__ __forceinline__ int acc_row(int r, int lane) { return (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5); }
@@ -343,13 +433,12 @@ constexpr int DT_FWD_BLOCKS = 512;
 
 template <int NP, bool TWO>
 __global__ __launch_bounds__(256, 2) void dt_forward_kernel(DistillArgs p) {
-  __shared__ __attribute__((aligned(16))) char lds[4 * DT_STAGE];
-  __shared__ float red[4];
+  DT_LDS
   const int nl = *p.nlive, nt = (nl + DT_TILE - 1) / DT_TILE, vt = p.Vp / DT_TILE;
   const int splits = dt_splits(nt, vt), per = (vt + splits - 1) / splits;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int am = (wave >> 1) * 64, bn = (wave & 1) * 64;
-  const int e = scale_exp(block_amax(p.amax, red)) + scale_exp(block_amax(p.amax + DT_AMAX, red));
+  const int e = p.sexp[0] + p.sexp[1];
   const float c = ldexpf(LOG2E, -e);
   const long ld = (long)p.Kp * NP * 2;
   const int nst = (p.E + 64 / NP - 1) / (64 / NP), last = ((p.E + 15) / 16) - (nst - 1) * (4 / NP);
@@ -364,26 +453,19 @@ __global__ __launch_bounds__(256, 2) void dt_forward_kernel(DistillArgs p) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) { m[j] = -1e30f; s1[j] = s2[j] = 0.f; }
     f32x16 acc[2][2];
-    const int total = (t1 - t0) * nst;
     const char* wbase = A.base;
     A.base = wbase + (long)t0 * DT_TILE * ld;
     __syncthreads();                                              // the last item's reads are over
-    if (total > 0) { A.issue(0, lds, wave); B.issue(0, lds + DT_STAGE, wave); }
-    int st = 0, tile = t0;
-    clear(acc);
-    for (int s = 0; s < total; ++s) {
-      char* cur = lds + (s & 1) * 2 * DT_STAGE;
-      char* nxt = lds + ((s + 1) & 1) * 2 * DT_STAGE;
-      const bool end = st + 1 == nst;
-      stage_barrier();
-      if (s + 1 < total) {
-        if (end) A.base = wbase + (long)(tile + 1) * DT_TILE * ld;
-        A.issue(end ? 0 : st + 1, nxt, wave);
-        B.issue(end ? 0 : st + 1, nxt + DT_STAGE, wave);
-      }
-      stage_product<NP, false, false>(cur, cur + DT_STAGE, am, bn, end ? last : 4, lane, acc);
-      ++st;
-      if (!end) continue;
+    if (t0 < t1) { A.issue(0, la0, wave); B.issue(0, lb0, wave); }
+    const auto do_tile = [&](int tile, char* la, char* lb, char* na, char* nb) {
+      clear(acc);
+      stages<NP, false, false>(A, B, nst, last, la, lb, na, nb, am, bn, lane, wave, acc, [&](char* fa, char* fb) {
+        if (tile + 1 < t1) {                                      // the next tile of W loads under this one's fold
+          A.base = wbase + (long)(tile + 1) * DT_TILE * ld;
+          A.issue(0, fa, wave);
+          B.issue(0, fb, wave);
+        }
+      });
       // fold the tile: a lane owns two rows (columns of the product) and 32 of the tile's 64 vocabulary entries
       const float* b2 = p.b2 + tile * DT_TILE + am;
       float4 bias[2][4];
@@ -416,13 +498,14 @@ __global__ __launch_bounds__(256, 2) void dt_forward_kernel(DistillArgs p) {
           }
         m[j] = mx; s1[j] = a; s2[j] = b;
       }
-      clear(acc);
-      st = 0;
-      ++tile;
+    };
+    for (int tile = t0; tile < t1; ++tile) {                      // an odd number of stages swaps the pairs
+      do_tile(tile, la0, lb0, la1, lb1);
+      if ((nst & 1) && tile + 1 < t1) do_tile(++tile, la1, lb1, la0, lb0);
     }
     // join the two half-waves and the two waves that share a row, and store the split's pair
     __syncthreads();
-    float* x = reinterpret_cast<float*>(lds);                     // [2 (am)][128][3]
+    float* x = reinterpret_cast<float*>(la0);                     // [2 (am)][128][3]
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const float m2 = __shfl_xor(m[j], 32, 64), mm = fmaxf(m[j], m2);
@@ -464,26 +547,48 @@ __global__ __launch_bounds__(256) void dt_combine_kernel(DistillArgs p) {
   const float* top = p.K ? p.top + ((long)(r % p.B) * p.T + t) * p.K : nullptr;
   const int64_t tg = p.tgt[n];
   float* pick = p.pick + (long)i * (p.K + 1);
-  // picked logits, base 2
+  // Picked logits, base 2: 32 lanes a dot product, four of them in flight.  16 bytes a lane where rows allow it (a W row
+  // of E = 200 in 16 bits is then one access), else single elements.
   const T* x = static_cast<const T*>(p.X) + (long)n * p.E;
-  const bool vec = p.E % 4 == 0 && ((uintptr_t)p.X % (4 * sizeof(T))) == 0 && ((uintptr_t)p.W % (4 * sizeof(T))) == 0;
-  const int l16 = threadIdx.x & 15;
-  for (int k = threadIdx.x >> 4; k <= p.K; k += 16) {
-    const int64_t id = k < p.K ? ids[k] : tg;
-    float dot = 0.f;
-    if (id >= 0 && id < p.V) {
-      const T* w = static_cast<const T*>(p.W) + id * p.E;
-      for (int e = l16 * 4; e < p.E; e += 64) {
-        float a[4], b[4];
-        load4<T>(x, e, p.E, vec, a);
-        load4<T>(w, e, p.E, vec, b);
+  const T* W = static_cast<const T*>(p.W);
+  constexpr int VN = 16 / sizeof(T);
+  const bool vec = p.E % VN == 0 && (((uintptr_t)p.X | (uintptr_t)p.W) & 15) == 0;
+  const int l32 = threadIdx.x & 31;
+  for (int k0 = threadIdx.x >> 5; k0 <= p.K; k0 += 32) {
+    int64_t id[4];
+    float dot[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) dot = fmaf(a[j], b[j], dot);
+    for (int q = 0; q < 4; ++q) {
+      const int k = k0 + 8 * q;
+      id[q] = k < p.K ? ids[k] : k == p.K ? tg : -1;
+      if (id[q] < 0 || id[q] >= p.V) id[q] = -1;
+      dot[q] = 0.f;
+    }
+    if (vec) {
+      for (int e = l32 * VN; e < p.E; e += 32 * VN) {
+        const Packed<T, VN> a = *reinterpret_cast<const Packed<T, VN>*>(x + e);
+        Packed<T, VN> w[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) w[q] = *reinterpret_cast<const Packed<T, VN>*>(W + (id[q] < 0 ? 0 : id[q]) * p.E + e);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int j = 0; j < VN; ++j) dot[q] = fmaf(a.f(j), w[q].f(j), dot[q]);
+      }
+    } else {
+      for (int e = l32; e < p.E; e += 32) {
+        const float a = (float)x[e];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) dot[q] = fmaf(a, (float)W[(id[q] < 0 ? 0 : id[q]) * p.E + e], dot[q]);
       }
     }
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
-    if (l16 == 0) pick[k] = (id >= 0 && id < p.V) ? (dot + (float)static_cast<const T*>(p.bias)[id]) * LOG2E : 0.f;
+    for (int q = 0; q < 4; ++q) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) dot[q] += __shfl_xor(dot[q], o, 64);
+      if (l32 == 0 && k0 + 8 * q <= p.K)
+        pick[k0 + 8 * q] = id[q] >= 0 ? (dot[q] + (float)static_cast<const T*>(p.bias)[id[q]]) * LOG2E : 0.f;
+    }
   }
   // normalisers
   const int nt = (nl + DT_TILE - 1) / DT_TILE, splits = dt_splits(nt, p.Vp / DT_TILE);
@@ -520,7 +625,11 @@ __global__ __launch_bounds__(256) void dt_combine_kernel(DistillArgs p) {
     p.slive[r] = 1;
     p.hard[n] = (L1 - pick[p.K]) * LN2;
   }
-  if (!p.K) return;
+  float* share = p.share + (long)i * (p.K + 1);
+  if (!p.K) {
+    if (lane == 0) { share[0] = 0.f; p.some[i] = 0.f; }
+    return;
+  }
   float tm = -INFINITY;
   bool bad = false;                                               // a NaN among the teacher's logits
   for (int k = lane; k < p.K; k += 64) {
@@ -538,35 +647,83 @@ __global__ __launch_bounds__(256) void dt_combine_kernel(DistillArgs p) {
   sum = wave_sum(sum);
   const float lsum = log2f(sum), inv = 1.0f / sum;
   float loss = 0.f;
+  const auto prob = [&](int k) { return __builtin_amdgcn_exp2f((top[k] - tm) * p.itau * LOG2E) * inv; };
+  bool listed = false;
   for (int k = lane; k < p.K; k += 64) {
     const int64_t id = ids[k];
-    float pk = 0.f;
-    if (id >= 0 && id < p.V && tm != -INFINITY) {
-      const float lp = (top[k] - tm) * p.itau * LOG2E;
-      pk = __builtin_amdgcn_exp2f(lp) * inv;
+    const bool in = id >= 0 && id < p.V, some = tm != -INFINITY;
+    if (in && some) {
+      const float lp = (top[k] - tm) * p.itau * LOG2E, pk = prob(k);
       if (pk != 0.f) loss += pk * (lp - lsum - (pick[k] * p.itau - L2));
     }
-    p.pk[(long)i * p.K + k] = pk;
+    listed |= id == tg;
   }
+  // an id listed several times is one entry of the gradient: its first place holds the sum of the shares, the others -1
+  // (as does the target's own place, K, if the teacher lists it)
+  const int ne = (p.K + 63) / 64;
+  for (int c = 0; c < ne; ++c) {
+    const int k = c * 64 + lane;
+    const int64_t id = k < p.K ? ids[k] : -1;
+    const bool in = id >= 0 && id < p.V;
+    float sum2 = 0.f;
+    bool first = true;
+    for (int d = 0; d < ne; ++d) {
+      const int kq = d * 64 + lane;
+      const int64_t idq = kq < p.K ? ids[kq] : -1;
+      const float pq = (idq >= 0 && idq < p.V && tm != -INFINITY) ? prob(kq) : 0.f;
+      for (int q = 0; q < 64 && d * 64 + q < p.K; ++q) {
+        const int iq = __builtin_amdgcn_readlane((int)idq, q);    // ids inside the vocabulary fit 31 bits
+        const float sq = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, pq), q));
+        const int hq = __builtin_amdgcn_readlane((int)(idq >> 32), q);
+        if (in && hq == 0 && iq == (int)id) {
+          sum2 += sq;
+          if (d * 64 + q < k) first = false;
+        }
+      }
+    }
+    if (k < p.K) share[k] = in && first ? sum2 : -1.f;
+  }
+  const bool tgt_listed = __any(listed);
+  if (lane == 0) share[p.K] = tgt_listed ? -1.f : 0.f;
+  const float some = bad || tm != tm ? NAN : tm != -INFINITY ? 1.f : 0.f;
+  if (lane == 0) p.some[i] = some;
   loss = wave_sum(loss);
   if (lane == 0) p.soft[n] = p.tau * p.tau * LN2 * loss;
+}
+
+// a wave per sentence: out[r] = sum over t, of the hard rows and (blockIdx.y = 1) the soft ones
+__global__ __launch_bounds__(256) void dt_sum_kernel(int T, int R, const float* __restrict__ h, const float* __restrict__ f,
+                                                     float* __restrict__ hard, float* __restrict__ soft) {
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (r >= R) return;
+  const float* x = blockIdx.y ? f : h;
+  float s = 0.f;
+  for (int t = lane; t < T; t += 64) s += x[(long)t * R + r];
+  s = wave_sum(s);
+  if (lane == 0) (blockIdx.y ? soft : hard)[r] = s;
 }
 
 // ------------------------------------------------------------------------------------------------- backward
 // Per live row: the two coefficients of its gradient over the row's power of two s, and the image of s X (with a column
 // of s itself: the product with P gives the bias gradient beside the weights').  Zeros: dX of dead rows, image rows past
-// the last live one.  Blocks [0, cdiv(N, 64)): 64 original rows; the next Np / 64: the image's tail.
-template <typename T, int NP> __global__ __launch_bounds__(256) void dt_gimage_kernel(DistillArgs p, int nb) {
+// the last live one.  16 rows a block: blocks [0, nx) original rows, the next Np / 16 the image's tail.
+template <typename T, int NP> __global__ __launch_bounds__(256) void dt_gimage_kernel(DistillArgs p, int nx) {
   __shared__ float red[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const long ld = (long)p.Kg * NP;
-  const int k4 = p.Kg / 4;
   const int nl = *p.nlive;
-  if ((int)blockIdx.x >= nb) {
-    const int b0 = (blockIdx.x - nb) * 64;
-    for (int i = b0 + wave; i < b0 + 64; i += 4)
-      if (i >= nl)
-        for (int k = lane; k < k4 * NP; k += 64) reinterpret_cast<Packed<f16_t, 4>*>(p.Gimg + i * ld)[k] = Packed<f16_t, 4>{};
+  const T* row[4];
+  _Float16* to[4];
+  int ee[4];
+  if ((int)blockIdx.x >= nx) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int i = (blockIdx.x - nx) * 16 + wave * 4 + q;
+      row[q] = nullptr;
+      to[q] = i >= nl ? p.Gimg + i * ld : nullptr;
+      ee[q] = 0;
+    }
+    image_rows<T, NP>(row, to, p.E, p.Kg / 4, false, ee, lane, 0.f);
     return;
   }
   float g = 0.f;
@@ -579,58 +736,45 @@ template <typename T, int NP> __global__ __launch_bounds__(256) void dt_gimage_k
   if (lane == 0) red[wave] = g;
   __syncthreads();
   g = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  __syncthreads();
   const int eg = g > 0.f ? (int)ceilf(log2f(g)) : 0;              // gmax = 2^eg
   if (blockIdx.x == 0 && threadIdx.x == 0) *p.gmax = ldexpf(1.f, eg);
-  const int ex = scale_exp(block_amax(p.amax, red));
+  const int ex = p.sexp[0];
   const bool vec = p.E % 4 == 0 && ((uintptr_t)p.X % (4 * sizeof(T))) == 0;
-  for (int j = wave; j < 64; j += 4) {
-    const int n = blockIdx.x * 64 + j;
-    if (n >= p.N) break;
-    const int i = p.inv[n];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int n = blockIdx.x * 16 + wave * 4 + q;
+    const int i = n < p.N ? p.inv[n] : -1;
+    row[q] = nullptr;
+    to[q] = nullptr;
+    ee[q] = 0;
     if (i < 0) {
-      T* q = static_cast<T*>(p.dX) + (long)n * p.E;
-      for (int k = lane; k < p.E; k += 64) q[k] = (T)0.f;
+      T* z = static_cast<T*>(p.dX) + (long)n * p.E;
+      if (n < p.N)
+        for (int k = lane; k < p.E; k += 64) z[k] = (T)0.f;
       continue;
     }
     const int r = n % p.R;
-    const float gh = p.ghard[r];
-    float gs = 0.f;
-    if (p.K) {                                                    // rows whose teacher lists nothing have no soft part
-      float any = 0.f;
-      for (int k = lane; k < p.K; k += 64) any += p.pk[(long)i * p.K + k];
-      any = wave_sum(any);
-      gs = any != 0.f ? p.gsoft[r] * p.tau : 0.f;
-      if (any != any) gs = any;
-    }
+    const float gh = p.ghard[r], some = p.some[i];                // no soft part where the teacher lists nothing
+    const float gs = !p.K || some == 0.f ? 0.f : some != some ? some : p.gsoft[r] * p.tau;
     const float mag = fabsf(gh) + fabsf(gs);
-    const bool fin = mag < 3.4e38f;
-    int es = (mag > 0.f && fin) ? (int)ceilf(log2f(mag)) : eg;
+    int es = (mag > 0.f && mag < 3.4e38f) ? (int)ceilf(log2f(mag)) : eg;
     es = es > eg ? eg : (es < eg - 40 ? eg - 40 : es);
     if (lane == 0) {
       p.coef[i] = ldexpf(gh, P_EXP - es);
       p.coef[p.Np + i] = ldexpf(gs, P_EXP - es);
       p.coef[2 * (long)p.Np + i] = ldexpf(1.f, es);
     }
-    const T* row = static_cast<const T*>(p.X) + (long)n * p.E;
-    for (int k = lane; k < k4; k += 64) {
-      float x[4];
-      load4<T>(row, 4 * k, p.E, vec, x);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        x[q] = ldexpf(x[q], ex + es - eg);
-        if (4 * k + q == p.E) x[q] = ldexpf(1.f, P_EXP + es - eg);
-      }
-      store4<NP>(p.Gimg + i * ld, 4 * k, x);
-    }
+    row[q] = static_cast<const T*>(p.X) + (long)n * p.E;
+    to[q] = p.Gimg + i * ld;
+    ee[q] = ex + es - eg;
   }
+  image_rows<T, NP>(row, to, p.E, p.Kg / 4, vec, ee, lane, ldexpf(1.f, P_EXP - ex));
 }
 
 // P[n][v] of a piece of the vocabulary without the picked entries: a 2^(t - L1) + b 2^(t / tau - L2)
 template <int NP, bool TWO>
 __global__ __launch_bounds__(256, 2) void dt_grad_kernel(DistillArgs p) {
-  __shared__ __attribute__((aligned(16))) char lds[4 * DT_STAGE];
-  __shared__ float red[4];
+  DT_LDS
   const int nl = *p.nlive, nt = (nl + DT_TILE - 1) / DT_TILE, vt = (p.vc + DT_TILE - 1) / DT_TILE;
   // block -> (vocabulary tile, row tile): an XCD walks its own range of W, all row tiles of one tile of W in turn
   const int pv = (vt + 7) / 8, j0 = blockIdx.x >> 3, tv = (blockIdx.x & 7) * pv + (nt > 0 ? j0 / nt : 0);
@@ -643,10 +787,10 @@ __global__ __launch_bounds__(256, 2) void dt_grad_kernel(DistillArgs p) {
   A.init(reinterpret_cast<const char*>(p.Wimg) + w0 * ld, ld, lane, wave);
   B.init(reinterpret_cast<const char*>(p.Ximg) + n0 * ld, ld, lane, wave);
   const int nst = (p.E + 64 / NP - 1) / (64 / NP), last = ((p.E + 15) / 16) - (nst - 1) * (4 / NP);
-  const int e = scale_exp(block_amax(p.amax, red)) + scale_exp(block_amax(p.amax + DT_AMAX, red));
+  const int e = p.sexp[0] + p.sexp[1];
   const float c = ldexpf(LOG2E, -e);
   f32x16 acc[2][2];
-  product<NP, false, false>(A, B, nst, last, lds, am, bn, lane, wave, acc);
+  product<NP, false, false>(A, B, nst, last, la0, lb0, la1, lb1, am, bn, lane, wave, acc);
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -672,7 +816,7 @@ __global__ __launch_bounds__(256, 2) void dt_grad_kernel(DistillArgs p) {
           if (NP == 2) lo.set(k, x - hi.f(k));
         }
         const int byte = NP == 1 ? v * 2 : (v >> 5) * 128 + (v & 31) * 2;
-        char* row = lds + nn * 256 * NP;
+        char* row = DT_AREA(nn * NP >> 6) + (nn * 256 * NP & (DT_STAGE - 1));
         *reinterpret_cast<Packed<f16_t, 4>*>(row + ((((byte >> 4) ^ (nn & 15)) << 4) | (byte & 15))) = hi;
         if (NP == 2) {
           const int bl = byte + 64;
@@ -684,13 +828,13 @@ __global__ __launch_bounds__(256, 2) void dt_grad_kernel(DistillArgs p) {
   constexpr int CPR = 16 * NP;                                    // 16-byte chunks of a row
   for (int k = threadIdx.x; k < DT_TILE * CPR; k += 256) {
     const int nn = k / CPR, ch = k % CPR;
-    const uint4 x = *reinterpret_cast<const uint4*>(lds + nn * 256 * NP + ((ch ^ (nn & 15)) << 4));
+    const uint4 x = *reinterpret_cast<const uint4*>(DT_AREA(nn * NP >> 6) + (nn * 256 * NP & (DT_STAGE - 1)) + ((ch ^ (nn & 15)) << 4));
     *reinterpret_cast<uint4*>(reinterpret_cast<char*>(p.P + (long)(n0 + nn) * p.ldp) + (long)tv * 256 * NP + ch * 16) = x;
   }
 }
 
-// The picked entries of a row, from their own fp32 logits: softmax minus the target / the teacher's share.  An id that a
-// teacher lists twice, or that is the target too, is one entry: its first place writes it.
+// The picked entries of a row, from their own fp32 logits: softmax minus the target / the teacher's share (an id that
+// was listed before, or a target that the teacher lists, has share -1 here: its first place writes it).
 template <int NP, bool TWO>
 __global__ __launch_bounds__(256) void dt_pick_kernel(DistillArgs p) {
   const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -698,21 +842,13 @@ __global__ __launch_bounds__(256) void dt_pick_kernel(DistillArgs p) {
   const int n = p.rows[i], r = n % p.R, t = n / p.R;
   const int64_t* ids = p.K ? p.ids + ((long)(r % p.B) * p.T + t) * p.K : nullptr;
   const int64_t tg = p.tgt[n];
-  const float* pick = p.pick + (long)i * (p.K + 1);
   const float a = p.coef[i], b = p.coef[p.Np + i], L1 = p.L1[i], L2 = p.L2[i];
   for (int k = lane; k <= p.K; k += 64) {
     const int64_t id = k < p.K ? ids[k] : tg;
-    if (id < p.v0 || id >= (int64_t)p.v0 + p.vc || id >= p.V) continue;
-    float share = 0.f;
-    bool first = true;
-    for (int q = 0; q < p.K; ++q)
-      if (ids[q] == id) {
-        if (q < k) first = false;
-        share += p.pk[(long)i * p.K + q];
-      }
-    if (!first) continue;
-    float x = a * (__builtin_amdgcn_exp2f(pick[k] - L1) - (id == tg ? 1.f : 0.f));
-    if (p.K) x = fmaf(b, __builtin_amdgcn_exp2f(fmaf(pick[k], TWO ? p.itau : 1.f, -L2)) - share, x);
+    const float share = p.share[(long)i * (p.K + 1) + k], pick = p.pick[(long)i * (p.K + 1) + k];
+    if (id < p.v0 || id >= (int64_t)p.v0 + p.vc || id >= p.V || share == -1.f) continue;
+    float x = a * (__builtin_amdgcn_exp2f(pick - L1) - (id == tg ? 1.f : 0.f));
+    if (p.K) x = fmaf(b, __builtin_amdgcn_exp2f(fmaf(pick, TWO ? p.itau : 1.f, -L2)) - share, x);
     const int v = (int)(id - p.v0);
     _Float16* q = p.P + (long)i * p.ldp + image_at<NP>(v);
     const _Float16 hi = (_Float16)x;
@@ -725,7 +861,7 @@ __global__ __launch_bounds__(256) void dt_pick_kernel(DistillArgs p) {
 // partial tiles in accumulator order, added to what an earlier piece left there.
 template <int NP>
 __global__ __launch_bounds__(256, 2) void dt_dx_kernel(DistillArgs p, int et, int add) {
-  __shared__ __attribute__((aligned(16))) char lds[4 * DT_STAGE];
+  DT_LDS
   const int nl = *p.nlive, nt = (nl + DT_TILE - 1) / DT_TILE;
   const int split = blockIdx.x % p.xsplits, rest = blockIdx.x / p.xsplits, te = rest % et, tn = rest / et;
   if (tn >= nt) return;
@@ -740,7 +876,7 @@ __global__ __launch_bounds__(256, 2) void dt_dx_kernel(DistillArgs p, int et, in
   A.init(reinterpret_cast<const char*>(p.Wimg) + (p.v0 + (long)s0 * BK) * ldw + (long)te * 256 * NP, ldw, lane, wave);
   B.init(reinterpret_cast<const char*>(p.P) + (long)tn * DT_TILE * ldp + (long)s0 * 128, ldp, lane, wave);
   f32x16 acc[2][2];
-  product<NP, true, false>(A, B, s1 - s0, 4, lds, am, bn, lane, wave, acc);
+  product<NP, true, false>(A, B, s1 - s0, 4, la0, lb0, la1, lb1, am, bn, lane, wave, acc);
   float4* out = reinterpret_cast<float4*>(p.slab) + (((long)split * (p.Np / DT_TILE) + tn) * et + te) * (DT_TILE * DT_TILE / 4) + wave * 1024 + lane;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -756,11 +892,10 @@ __global__ __launch_bounds__(256, 2) void dt_dx_kernel(DistillArgs p, int et, in
 }
 template <typename T>
 __global__ __launch_bounds__(256) void dt_dx_sum_kernel(DistillArgs p, int et) {
-  __shared__ float red[4];
   const int nl = *p.nlive, nt = (nl + DT_TILE - 1) / DT_TILE;
   const int tile = blockIdx.x >> 4;                               // 16 blocks a tile
   if (tile / et >= nt) return;
-  const float w = ldexpf(1.f, -scale_exp(block_amax(p.amax + DT_AMAX, red)) - P_EXP);
+  const float w = ldexpf(1.f, -p.sexp[1] - P_EXP);
   const int slot = (blockIdx.x & 15) * 256 + threadIdx.x;
   const long step = (long)(p.Np / DT_TILE) * et * (DT_TILE * DT_TILE / 4);
   const float4* q = reinterpret_cast<const float4*>(p.slab) + (long)tile * (DT_TILE * DT_TILE / 4) + slot;
@@ -782,8 +917,7 @@ __global__ __launch_bounds__(256) void dt_dx_sum_kernel(DistillArgs p, int et) {
 // dW and db: (s X down its rows: K = live rows) x (P down its rows), whole K in one block
 template <typename T, int NP>
 __global__ __launch_bounds__(256, 2) void dt_dw_kernel(DistillArgs p, int et) {
-  __shared__ __attribute__((aligned(16))) char lds[4 * DT_STAGE];
-  __shared__ float red[4];
+  DT_LDS
   const int nl = *p.nlive, vt = (p.vc + DT_TILE - 1) / DT_TILE;
   const int pv = (vt + 7) / 8, j0 = blockIdx.x >> 3, tv = (blockIdx.x & 7) * pv + j0 / et, te = j0 % et;
   if (j0 / et >= pv || tv >= vt) return;
@@ -793,10 +927,10 @@ __global__ __launch_bounds__(256, 2) void dt_dw_kernel(DistillArgs p, int et) {
   Operand<NP, true> A, B;
   A.init(reinterpret_cast<const char*>(p.Gimg) + (long)te * 256 * NP, (long)p.Kg * NP * 2, lane, wave);
   B.init(reinterpret_cast<const char*>(p.P) + (long)tv * 256 * NP, p.ldp * 2, lane, wave);
-  const int ex = scale_exp(block_amax(p.amax, red));
+  const int ex = p.sexp[0];
   const float fw = *p.gmax * ldexpf(1.f, -P_EXP - ex), fb = *p.gmax * ldexpf(1.f, -2 * P_EXP);
   f32x16 acc[2][2];
-  product<NP, true, true>(A, B, (nl + BK - 1) / BK, 4, lds, am, bn, lane, wave, acc);
+  product<NP, true, true>(A, B, (nl + BK - 1) / BK, 4, la0, lb0, la1, lb1, am, bn, lane, wave, acc);
   __syncthreads();
   // through LDS: rows of the vocabulary, 128 columns each, chunk c of row r at c ^ (r & 31)
 #pragma unroll
@@ -807,7 +941,7 @@ __global__ __launch_bounds__(256, 2) void dt_dw_kernel(DistillArgs p, int et) {
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int ch = (am + 32 * i + 8 * g + 4 * (lane >> 5)) >> 2;
-        *reinterpret_cast<float4*>(lds + row * 512 + ((ch ^ (row & 31)) << 4)) =
+        *reinterpret_cast<float4*>(DT_AREA(row >> 5) + (row & 31) * 512 + ((ch ^ (row & 31)) << 4)) =
             make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
       }
     }
@@ -818,7 +952,7 @@ __global__ __launch_bounds__(256, 2) void dt_dw_kernel(DistillArgs p, int et) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int el = h * 64 + lane, e = te * DT_TILE + el;
-      const float x = *reinterpret_cast<const float*>(lds + row * 512 + (((el >> 2) ^ (row & 31)) << 4) + (el & 3) * 4);
+      const float x = *reinterpret_cast<const float*>(DT_AREA(row >> 5) + (row & 31) * 512 + (((el >> 2) ^ (row & 31)) << 4) + (el & 3) * 4);
       if (e < p.E) static_cast<T*>(p.dW)[(long)v * p.E + e] = (T)(x * fw);
       else if (e == p.E) static_cast<T*>(p.db)[v] = (T)(x * fb);
     }
@@ -830,7 +964,7 @@ constexpr long DT_PIECE_BYTES = 192L << 20;        // of P: it is written, then 
 
 struct DistillPlan {
   long bytes, back_bytes;
-  long counts, rows, inv, nlive, slive, amax, Ximg, Wimg, b2, L1, L2, pick, pk, part;   // offsets in bytes
+  long counts, rows, inv, nlive, slive, amax, sexp, Ximg, Wimg, b2, L1, L2, some, pick, share, part;   // offsets in bytes
   long Gimg, coef, gmax, P, slab;
   int np, Np, Vp, Kp, Kg, nb, splits_cap, et, etw, xsplits;
   long vc;
@@ -848,12 +982,13 @@ static DistillPlan dt_plan(int dtype, long N, int E, int V, int K) {
   long at = 0;
   d.counts = take(at, 4L * d.nb); d.rows = take(at, 4 * N); d.inv = take(at, 4 * N); d.nlive = take(at, 4);
   d.slive = take(at, 4 * N);
-  d.amax = take(at, 8L * DT_AMAX);
+  d.amax = take(at, 8L * DT_AMAX); d.sexp = take(at, 8);
   const long slack = 1024;                          // a column tile of the last row may be read past the row's end
   d.Ximg = take(at, 2L * d.Np * d.Kp * d.np); d.Wimg = take(at, 2L * d.Vp * d.Kp * d.np + slack);
   d.b2 = take(at, 4L * d.Vp);
   d.L1 = take(at, 4L * d.Np); d.L2 = take(at, 4L * d.Np);
-  d.pick = take(at, 4L * N * (K + 1)); d.pk = take(at, 4L * N * K);
+  d.some = take(at, 4L * d.Np);
+  d.pick = take(at, 4L * N * (K + 1)); d.share = take(at, 4L * N * (K + 1));
   d.part = take(at, 12L * d.splits_cap * d.Np);
   d.bytes = at;
   long vc = DT_PIECE_BYTES / (2L * d.np * d.Np) / 128 * 128;
@@ -861,8 +996,9 @@ static DistillPlan dt_plan(int dtype, long N, int E, int V, int K) {
   const int pieces = cdiv(d.Vp, vc);
   d.vc = ((long)d.Vp / 128 + pieces - 1) / pieces * 128;          // pieces of equal size
   const int stages = (int)(d.vc / (64 / d.np));
-  d.xsplits = 1024 / (8 * nt * d.et) * 8;           // about 1024 blocks
-  if (d.xsplits < 8) d.xsplits = 8;
+  // about 1024 blocks; 1, 2, 4 or a multiple of 8 splits, so that an XCD (block % 8) reads one range of W
+  const int want = 1024 / (nt * d.et);
+  d.xsplits = want >= 8 ? want / 8 * 8 : want >= 4 ? 4 : want >= 2 ? 2 : 1;
   while (d.xsplits > 8 && stages / d.xsplits < 4) d.xsplits -= 8;
   at = 0;
   d.Gimg = take(at, 2L * d.Np * d.Kg * d.np + slack); d.coef = take(at, 12L * d.Np); d.gmax = take(at, 4);
@@ -898,15 +1034,16 @@ static void dt_fill(DistillArgs& a, const DistillPlan& d, const DistillCall& c, 
   a.X = c.X; a.W = c.W; a.bias = c.b; a.tgt = c.tgt; a.pad = c.pad; a.ids = c.ids; a.top = c.top;
   char* w = static_cast<char*>(ws);
   a.counts = (int*)(w + d.counts); a.rows = (int*)(w + d.rows); a.inv = (int*)(w + d.inv); a.nlive = (int*)(w + d.nlive); a.slive = (int*)(w + d.slive);
-  a.amax = (float*)(w + d.amax); a.Ximg = (_Float16*)(w + d.Ximg); a.Wimg = (_Float16*)(w + d.Wimg); a.b2 = (float*)(w + d.b2);
-  a.L1 = (float*)(w + d.L1); a.L2 = (float*)(w + d.L2); a.pick = (float*)(w + d.pick); a.pk = (float*)(w + d.pk);
+  a.amax = (float*)(w + d.amax); a.sexp = (int*)(w + d.sexp); a.Ximg = (_Float16*)(w + d.Ximg); a.Wimg = (_Float16*)(w + d.Wimg); a.b2 = (float*)(w + d.b2);
+  a.L1 = (float*)(w + d.L1); a.L2 = (float*)(w + d.L2); a.some = (float*)(w + d.some);
+  a.pick = (float*)(w + d.pick); a.share = (float*)(w + d.share);
   a.part = (float*)(w + d.part); a.splits_cap = d.splits_cap;
 }
 
 template <typename T, int NP, bool TWO> static int dt_forward(const DistillPlan& d, const DistillArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((dt_count_kernel<T>), dim3(d.nb + 2 * DT_AMAX), dim3(256), 0, s, a, d.nb);
   CVAE_LAUNCH_CHECK("dt_count_kernel");
-  hipLaunchKernelGGL((dt_image_kernel<T, NP>), dim3(d.nb + d.Np / 64 + d.Vp / 16), dim3(256), 0, s, a, d.nb);
+  hipLaunchKernelGGL((dt_image_kernel<T, NP>), dim3(cdiv(a.N, 16) + d.Np / 16 + d.Vp / 16), dim3(256), 0, s, a, cdiv(a.N, 16));
   CVAE_LAUNCH_CHECK("dt_image_kernel");
   hipLaunchKernelGGL((dt_forward_kernel<NP, TWO>), dim3(DT_FWD_BLOCKS), dim3(256), 0, s, a);
   CVAE_LAUNCH_CHECK("dt_forward_kernel");
@@ -915,8 +1052,8 @@ template <typename T, int NP, bool TWO> static int dt_forward(const DistillPlan&
   return 0;
 }
 template <typename T, int NP, bool TWO> static int dt_backward(const DistillPlan& d, DistillArgs a, hipStream_t s) {
-  const int nb = cdiv(a.N, 64), nt = d.Np / DT_TILE;
-  hipLaunchKernelGGL((dt_gimage_kernel<T, NP>), dim3(nb + d.Np / 64), dim3(256), 0, s, a, nb);
+  const int nx = cdiv(a.N, 16), nt = d.Np / DT_TILE;
+  hipLaunchKernelGGL((dt_gimage_kernel<T, NP>), dim3(nx + d.Np / 16), dim3(256), 0, s, a, nx);
   CVAE_LAUNCH_CHECK("dt_gimage_kernel");
   a.ldp = d.vc * NP;
   for (long v0 = 0; v0 < d.Vp; v0 += d.vc) {
@@ -960,8 +1097,8 @@ int launch_distill_forward(const DistillCall& c, float* hard_row, float* soft_ro
     a.hard = hard_row; a.soft = soft_row;
     CVAE_TRY(dt_dispatch(c.dtype, d, a, false, s));
   }
-  CVAE_TRY(launch_sum_time(hard_row, c.T, c.R, hard, s));
-  if (c.K) CVAE_TRY(launch_sum_time(soft_row, c.T, c.R, soft, s));
+  hipLaunchKernelGGL(dt_sum_kernel, dim3(cdiv(c.R, 4), c.K ? 2 : 1), dim3(256), 0, s, c.T, c.R, hard_row, soft_row, hard, soft);
+  CVAE_LAUNCH_CHECK("dt_sum_kernel");
   return 0;
 }
 

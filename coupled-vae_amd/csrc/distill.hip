@@ -37,7 +37,7 @@ constexpr int P_EXP = 13;                  // |P| <= 1 is stored times 2^13
 
 struct DistillArgs {
   int N, T, R, B, E, V, K;
-  int Np, Vp, Kp, Kg;                      // N and V up to 128, E up to 64, E + 1 up to 64
+  int Np, Vp, Kp, Kg;                      // N and V up to 256, E up to 64, E + 1 up to 64
   float tau, itau;
   int two;                                 // tau != 1 and K > 0: a second normaliser
   const void* X; const void* W; const void* bias;
@@ -55,7 +55,7 @@ struct DistillArgs {
   const float* ghard; const float* gsoft;  // [R]
   _Float16* Gimg; float* coef;             // s X image with a column of s; [3][Np]: a, b, s / gmax
   float* gmax;
-  _Float16* P; int v0, vc; long ldp;       // a piece of the vocabulary
+  _Float16* P; int v0, vc;                 // a range of the vocabulary: [vc NP / 64 pieces][Np rows][128 bytes]
   float* slab; int xsplits;
   void* dX; void* dW; void* db;
 };
@@ -269,37 +269,42 @@ template <typename T, int NP> __global__ __launch_bounds__(256) void dt_image_ke
 }
 
 // ------------------------------------------------------------------------------------------------- the product loop
-// One operand's tile: `base` the first byte of its stage 0, `ld` bytes from row to row.
-//   K along the row (KS = false): 128 rows; stage s is bytes [128 s, 128 s + 128) of each.
-//   K down the rows (KS = true): 128 columns; stage s is 64 (two planes: 32) rows of 256 (512) bytes.
-// In LDS, 16-byte chunk c of row r sits at chunk c ^ (r & 7) of its 128 bytes (KS: c ^ 4 (r & 3) of its 256): the
-// chunks that the lanes of a read take lie in different banks.
-template <int NP, bool KS> struct Operand {
+// One operand's tile of RT rows / columns, copied to LDS by NW waves.  Memory holds 128-byte pieces: `row` bytes from a
+// row's piece to the next row's, `grp` bytes from a piece to the next one of the same row (images: grp = 128, a row is
+// contiguous; P: row = 128, the rows of one piece are contiguous).
+//   K along the rows (KS = false): RT rows; stage s is piece s of each.
+//   K down the rows (KS = true): RT columns, that is RT NP / 64 pieces, of 64 (two planes: 32) rows a stage.
+// In LDS, 16-byte chunk c of row r sits at chunk c ^ (r & 7) of its 128 bytes (KS: c ^ 4 (r & 3)): the chunks that the
+// lanes of a read take lie in different banks.
+template <int NP, bool KS, int RT, int NW> struct Operand {
+  static constexpr int PI = RT / 8 / NW;                          // copies of 1 KiB a wave and stage
+  static constexpr int ROW = RT * 2 * NP;                         // bytes of a K row in LDS (KS)
   const char* base;
-  long ld;
-  unsigned off[4];
-  __device__ __forceinline__ void init(const void* p, long ld_bytes, int lane, int wave) {
+  long row, grp;
+  unsigned off[PI];
+  __device__ __forceinline__ void init(const void* p, long row_bytes, long grp_bytes, int lane, int wave) {
     base = static_cast<const char*>(p);
-    ld = ld_bytes;
+    row = row_bytes;
+    grp = grp_bytes;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int piece = wave * 4 + i;                             // 1 KiB of the stage
+    for (int i = 0; i < PI; ++i) {
+      const int piece = wave * PI + i;
       if (!KS) {
         const int r = piece * 8 + (lane >> 3);
-        off[i] = (unsigned)(r * ld + (((lane & 7) ^ (r & 7)) << 4));
+        off[i] = (unsigned)(r * row + (((lane & 7) ^ (r & 7)) << 4));
       } else {
-        constexpr int LPR = NP == 1 ? 16 : 32;                    // lanes (chunks) of a row
-        const int r = piece * (64 / LPR) + lane / LPR, c = lane % LPR;
-        off[i] = (unsigned)(r * ld + ((c ^ ((r & 3) << 2)) << 4));
+        constexpr int LPR = ROW / 16;                             // lanes (chunks) of a row
+        const int r = piece * (64 / LPR) + lane / LPR, c = (lane % LPR) ^ ((r & 3) << 2);
+        off[i] = (unsigned)(r * row + (c >> 3) * grp + ((c & 7) << 4));
       }
     }
   }
   __device__ __forceinline__ void issue(int stage, char* lds, int wave) const {
-    const char* b = base + (KS ? (long)stage * (64 / NP) * ld : (long)stage * 128);
+    const char* b = base + (KS ? (long)stage * (64 / NP) * row : (long)stage * grp);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < PI; ++i)
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(b + off[i]),
-                                       (__attribute__((address_space(3))) void*)(lds + (wave * 4 + i) * 1024), 16, 0, 0);
+                                       (__attribute__((address_space(3))) void*)(lds + (wave * PI + i) * 1024), 16, 0, 0);
   }
   // the 32 rows / columns from `c0`, K block `ks` of the stage, plane `pl`, as one MFMA operand
   static __device__ __forceinline__ h8 frag(const char* lds, int c0, int ks, int pl, int lane) {
@@ -307,7 +312,6 @@ template <int NP, bool KS> struct Operand {
       const int r = c0 + (lane & 31), c = (NP == 1 ? 0 : pl * 4) + ks * 2 + (lane >> 5);
       return *reinterpret_cast<const h8*>(lds + r * 128 + ((c ^ (r & 7)) << 4));
     }
-    constexpr int ROW = 256 * NP;
     const int k = ks * 16 + (lane >> 5) * 8 + ((lane >> 2) & 3);
     const int col = c0 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
     const int byte = NP == 1 ? col * 2 : (col >> 5) * 128 + pl * 64 + (col & 31) * 2;
@@ -320,7 +324,7 @@ template <int NP, bool KS> struct Operand {
 };
 
 // acc[i][j] += (rows am + 32 i of A) x (rows bn + 32 j of B) over K block ks of the stage in LDS
-template <int NP, bool AKS, bool BKS>
+template <int NP, typename OA, typename OB>
 __device__ __forceinline__ void mfma_block(const char* la, const char* lb, int am, int bn, int ks, int lane,
                                            f32x16 (&acc)[2][2]) {
   h8 a[2][NP], b[2][NP];
@@ -328,8 +332,8 @@ __device__ __forceinline__ void mfma_block(const char* la, const char* lb, int a
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int q = 0; q < NP; ++q) {
-      a[i][q] = Operand<NP, AKS>::frag(la, am + 32 * i, ks, q, lane);
-      b[i][q] = Operand<NP, BKS>::frag(lb, bn + 32 * i, ks, q, lane);
+      a[i][q] = OA::frag(la, am + 32 * i, ks, q, lane);
+      b[i][q] = OB::frag(lb, bn + 32 * i, ks, q, lane);
     }
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -342,15 +346,15 @@ __device__ __forceinline__ void mfma_block(const char* la, const char* lb, int a
       acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][0], acc[i][j], 0, 0, 0);
     }
 }
-template <int NP, bool AKS, bool BKS>
+template <int NP, typename OA, typename OB>
 __device__ __forceinline__ void stage_product(const char* la, const char* lb, int am, int bn, int blocks, int lane,
                                               f32x16 (&acc)[2][2]) {
   constexpr int KB = 4 / NP;                                      // K blocks of 16 in a stage
   if (blocks >= KB) {
 #pragma unroll
-    for (int ks = 0; ks < KB; ++ks) mfma_block<NP, AKS, BKS>(la, lb, am, bn, ks, lane, acc);
+    for (int ks = 0; ks < KB; ++ks) mfma_block<NP, OA, OB>(la, lb, am, bn, ks, lane, acc);
   } else {
-    for (int ks = 0; ks < blocks; ++ks) mfma_block<NP, AKS, BKS>(la, lb, am, bn, ks, lane, acc);
+    for (int ks = 0; ks < blocks; ++ks) mfma_block<NP, OA, OB>(la, lb, am, bn, ks, lane, acc);
   }
 }
 __device__ __forceinline__ void clear(f32x16 (&acc)[2][2]) {
@@ -381,42 +385,77 @@ __device__ __forceinline__ void stage_barrier() {
 // Stages [0, n), n > 0, of one tile, stage 0 already on its way into (la, lb); `last` K blocks of the last stage are used.
 // While a stage is multiplied the next one loads: behind the last one, whatever then(a, b) asks for the free pair.
 // (No stage is left out of the loop's middle: a `break` there cost 64 register moves a round.)
-template <int NP, bool AKS, bool BKS, typename Then>
-__device__ __forceinline__ void stages(const Operand<NP, AKS>& A, const Operand<NP, BKS>& B, int n, int last, char* la,
+template <int NP, typename OA, typename OB, typename Then>
+__device__ __forceinline__ void stages(const OA& A, const OB& B, int n, int last, char* la,
                                        char* lb, char* na, char* nb, int am, int bn, int lane, int wave,
                                        f32x16 (&acc)[2][2], const Then& then) {
   int s = 0;
   for (; s + 3 <= n; s += 2) {
     stage_barrier();
     A.issue(s + 1, na, wave); B.issue(s + 1, nb, wave);
-    stage_product<NP, AKS, BKS>(la, lb, am, bn, 4, lane, acc);
+    stage_product<NP, OA, OB>(la, lb, am, bn, 4, lane, acc);
     stage_barrier();
     A.issue(s + 2, la, wave); B.issue(s + 2, lb, wave);
-    stage_product<NP, AKS, BKS>(na, nb, am, bn, 4, lane, acc);
+    stage_product<NP, OA, OB>(na, nb, am, bn, 4, lane, acc);
   }
   if (s + 2 == n) {
     stage_barrier();
     A.issue(s + 1, na, wave); B.issue(s + 1, nb, wave);
-    stage_product<NP, AKS, BKS>(la, lb, am, bn, 4, lane, acc);
+    stage_product<NP, OA, OB>(la, lb, am, bn, 4, lane, acc);
     stage_barrier();
     then(la, lb);
-    stage_product<NP, AKS, BKS>(na, nb, am, bn, last, lane, acc);
+    stage_product<NP, OA, OB>(na, nb, am, bn, last, lane, acc);
   } else {
     stage_barrier();
     then(na, nb);
-    stage_product<NP, AKS, BKS>(la, lb, am, bn, last, lane, acc);
+    stage_product<NP, OA, OB>(la, lb, am, bn, last, lane, acc);
   }
 }
-template <int NP, bool AKS, bool BKS>
-__device__ __forceinline__ void product(const Operand<NP, AKS>& A, const Operand<NP, BKS>& B, int n, int last, char* la0,
-                                        char* lb0, char* la1, char* lb1, int am, int bn, int lane, int wave,
-                                        f32x16 (&acc)[2][2]) {
+
+// The same with three buffers, for tiles of 256 x 128 on 8 waves (one block on a CU): two stages are in flight under the
+// one that is multiplied.  Every step copies a stage (the last ones a stage that is already there), so that the count of
+// copies to wait for is a constant.
+template <int C> __device__ __forceinline__ void ring_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070 | C);                         // vmcnt(C) lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+template <int NP, typename OA, typename OB>
+__device__ __forceinline__ void ring_product(const OA& A, const OB& B, int n, char* la0, char* lb0, char* la1, char* lb1,
+                                             char* la2, char* lb2, int am, int bn, int lane, int wave, f32x16 (&acc)[2][2]) {
+  constexpr int C = OA::PI + OB::PI;
   clear(acc);
   if (n <= 0) return;
-  A.issue(0, la0, wave);
-  B.issue(0, lb0, wave);
-  stages<NP, AKS, BKS>(A, B, n, last, la0, lb0, la1, lb1, am, bn, lane, wave, acc, [](char*, char*) {});
+  const auto issue = [&](int s, char* la, char* lb) {
+    s = s < n ? s : n - 1;
+    A.issue(s, la, wave);
+    B.issue(s, lb, wave);
+  };
+  const auto step = [&](int s, char* la, char* lb, char* fa, char* fb) {
+    ring_barrier<C>();
+    issue(s + 2, fa, fb);
+    stage_product<NP, OA, OB>(la, lb, am, bn, 4, lane, acc);
+  };
+  issue(0, la0, lb0);
+  issue(1, la1, lb1);
+  int s = 0;
+  for (; s + 3 <= n; s += 3) {
+    step(s, la0, lb0, la2, lb2);
+    step(s + 1, la1, lb1, la0, lb0);
+    step(s + 2, la2, lb2, la1, lb1);
+  }
+  if (s < n) step(s, la0, lb0, la2, lb2);
+  if (s + 1 < n) step(s + 1, la1, lb1, la0, lb0);
+  ring_barrier<0>();                                              // no copy may land in LDS that the next block owns
 }
+#define DT_RING(RA, RB) \
+  __shared__ __attribute__((aligned(16))) char la0[(RA) * 128]; \
+  __shared__ __attribute__((aligned(16))) char la1[(RA) * 128]; \
+  __shared__ __attribute__((aligned(16))) char la2[(RA) * 128]; \
+  __shared__ __attribute__((aligned(16))) char lb0[(RB) * 128]; \
+  __shared__ __attribute__((aligned(16))) char lb1[(RB) * 128]; \
+  __shared__ __attribute__((aligned(16))) char lb2[(RB) * 128];
 // value r of an accumulator tile: row 4 (lane / 32) + 8 (r / 4) + r % 4, column lane % 32
 __device__ __forceinline__ int acc_row(int r, int lane) { return (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5); }
 
@@ -446,9 +485,10 @@ __global__ __launch_bounds__(256, 2) void dt_forward_kernel(DistillArgs p) {
   for (int q = blockIdx.x >> 3; q < per_xcd; q += DT_FWD_BLOCKS / 8) {
     const int split = xcd + 8 * (q / nt), n0 = (q % nt) * DT_TILE;
     const int t0 = split * per, t1 = min(vt, t0 + per);
-    Operand<NP, false> A, B;
-    A.init(p.Wimg, ld, lane, wave);
-    B.init(reinterpret_cast<const char*>(p.Ximg) + n0 * ld, ld, lane, wave);
+    using Op = Operand<NP, false, DT_TILE, 4>;
+    Op A, B;
+    A.init(p.Wimg, ld, 128, lane, wave);
+    B.init(reinterpret_cast<const char*>(p.Ximg) + n0 * ld, ld, 128, lane, wave);
     float m[2], s1[2], s2[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) { m[j] = -1e30f; s1[j] = s2[j] = 0.f; }
@@ -459,7 +499,7 @@ __global__ __launch_bounds__(256, 2) void dt_forward_kernel(DistillArgs p) {
     if (t0 < t1) { A.issue(0, la0, wave); B.issue(0, lb0, wave); }
     const auto do_tile = [&](int tile, char* la, char* lb, char* na, char* nb) {
       clear(acc);
-      stages<NP, false, false>(A, B, nst, last, la, lb, na, nb, am, bn, lane, wave, acc, [&](char* fa, char* fb) {
+      stages<NP, Op, Op>(A, B, nst, last, la, lb, na, nb, am, bn, lane, wave, acc, [&](char* fa, char* fb) {
         if (tile + 1 < t1) {                                      // the next tile of W loads under this one's fold
           A.base = wbase + (long)(tile + 1) * DT_TILE * ld;
           A.issue(0, fa, wave);
@@ -783,14 +823,18 @@ __global__ __launch_bounds__(256, 2) void dt_grad_kernel(DistillArgs p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int am = (wave >> 1) * 64, bn = (wave & 1) * 64;
   const long ld = (long)p.Kp * NP * 2;
-  Operand<NP, false> A, B;
-  A.init(reinterpret_cast<const char*>(p.Wimg) + w0 * ld, ld, lane, wave);
-  B.init(reinterpret_cast<const char*>(p.Ximg) + n0 * ld, ld, lane, wave);
+  using Op = Operand<NP, false, DT_TILE, 4>;
+  Op A, B;
+  A.init(reinterpret_cast<const char*>(p.Wimg) + w0 * ld, ld, 128, lane, wave);
+  B.init(reinterpret_cast<const char*>(p.Ximg) + n0 * ld, ld, 128, lane, wave);
   const int nst = (p.E + 64 / NP - 1) / (64 / NP), last = ((p.E + 15) / 16) - (nst - 1) * (4 / NP);
   const int e = p.sexp[0] + p.sexp[1];
   const float c = ldexpf(LOG2E, -e);
   f32x16 acc[2][2];
-  product<NP, false, false>(A, B, nst, last, la0, lb0, la1, lb1, am, bn, lane, wave, acc);
+  clear(acc);
+  A.issue(0, la0, wave);
+  B.issue(0, lb0, wave);
+  stages<NP, Op, Op>(A, B, nst, last, la0, lb0, la1, lb1, am, bn, lane, wave, acc, [](char*, char*) {});
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -825,11 +869,11 @@ __global__ __launch_bounds__(256, 2) void dt_grad_kernel(DistillArgs p) {
       }
   }
   __syncthreads();
-  constexpr int CPR = 16 * NP;                                    // 16-byte chunks of a row
-  for (int k = threadIdx.x; k < DT_TILE * CPR; k += 256) {
-    const int nn = k / CPR, ch = k % CPR;
+  char* P = reinterpret_cast<char*>(p.P) + ((long)tv * 2 * NP * p.Np + n0) * 128;
+  for (int k = threadIdx.x; k < DT_TILE * 16 * NP; k += 256) {    // piece by piece, its 128 rows in one run of memory
+    const int g = k >> 10, nn = (k >> 3) & 127, ch = g * 8 + (k & 7);
     const uint4 x = *reinterpret_cast<const uint4*>(DT_AREA(nn * NP >> 6) + (nn * 256 * NP & (DT_STAGE - 1)) + ((ch ^ (nn & 15)) << 4));
-    *reinterpret_cast<uint4*>(reinterpret_cast<char*>(p.P + (long)(n0 + nn) * p.ldp) + (long)tv * 256 * NP + ch * 16) = x;
+    *reinterpret_cast<uint4*>(P + (long)g * p.Np * 128 + (k & 1023) * 16) = x;
   }
 }
 
@@ -850,34 +894,36 @@ __global__ __launch_bounds__(256) void dt_pick_kernel(DistillArgs p) {
     float x = a * (__builtin_amdgcn_exp2f(pick - L1) - (id == tg ? 1.f : 0.f));
     if (p.K) x = fmaf(b, __builtin_amdgcn_exp2f(fmaf(pick, TWO ? p.itau : 1.f, -L2)) - share, x);
     const int v = (int)(id - p.v0);
-    _Float16* q = p.P + (long)i * p.ldp + image_at<NP>(v);
+    _Float16* q = p.P + ((long)(v * NP >> 6) * p.Np + i) * 64 + (v & (64 / NP - 1));
     const _Float16 hi = (_Float16)x;
     q[0] = hi;
     if (NP == 2) q[32] = (_Float16)(x - (float)hi);
   }
 }
 
-// dX: (W down its rows: K = vocabulary) x (P along its rows).  Blocks (row tile, column tile of E, split of the piece):
-// partial tiles in accumulator order, added to what an earlier piece left there.
-template <int NP>
-__global__ __launch_bounds__(256, 2) void dt_dx_kernel(DistillArgs p, int et, int add) {
-  DT_LDS
-  const int nl = *p.nlive, nt = (nl + DT_TILE - 1) / DT_TILE;
+// dX: (W down its rows: K = vocabulary) x (P along its rows), tiles of RA columns of E x RB rows.  Blocks (row tile,
+// column tile, split of the range): partial tiles in accumulator order, added to what an earlier range left there.
+template <int NP, int RA>
+__global__ __launch_bounds__(512, 2) void dt_dx_kernel(DistillArgs p, int et, int add) {
+  constexpr int RB = 384 - RA, BK = 64 / NP;
+  DT_RING(RA, RB)
+  const int nl = *p.nlive, nt = (nl + RB - 1) / RB;
   const int split = blockIdx.x % p.xsplits, rest = blockIdx.x / p.xsplits, te = rest % et, tn = rest / et;
   if (tn >= nt) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int am = (wave >> 1) * 64, bn = (wave & 1) * 64;
-  constexpr int BK = 64 / NP;
-  const int stages = (p.vc + DT_TILE - 1) / DT_TILE * (DT_TILE / BK), per = (stages + p.xsplits - 1) / p.xsplits;
+  const int am = (RA == 256 ? wave >> 1 : wave & 1) * 64, bn = (RA == 256 ? wave & 1 : wave >> 1) * 64;
+  const int stages = p.vc / BK, per = (stages + p.xsplits - 1) / p.xsplits;
   const int s0 = split * per, s1 = min(stages, s0 + per);
-  const long ldw = (long)p.Kp * NP * 2, ldp = p.ldp * 2;
-  Operand<NP, true> A;
-  Operand<NP, false> B;
-  A.init(reinterpret_cast<const char*>(p.Wimg) + (p.v0 + (long)s0 * BK) * ldw + (long)te * 256 * NP, ldw, lane, wave);
-  B.init(reinterpret_cast<const char*>(p.P) + (long)tn * DT_TILE * ldp + (long)s0 * 128, ldp, lane, wave);
+  const long ldw = (long)p.Kp * NP * 2;
+  using OA = Operand<NP, true, RA, 8>;
+  using OB = Operand<NP, false, RB, 8>;
+  OA A;
+  OB B;
+  A.init(reinterpret_cast<const char*>(p.Wimg) + (p.v0 + (long)s0 * BK) * ldw + (long)te * RA * 2 * NP, ldw, 128, lane, wave);
+  B.init(reinterpret_cast<const char*>(p.P) + ((long)s0 * p.Np + tn * RB) * 128, 128, (long)p.Np * 128, lane, wave);
   f32x16 acc[2][2];
-  product<NP, true, false>(A, B, s1 - s0, 4, la0, lb0, la1, lb1, am, bn, lane, wave, acc);
-  float4* out = reinterpret_cast<float4*>(p.slab) + (((long)split * (p.Np / DT_TILE) + tn) * et + te) * (DT_TILE * DT_TILE / 4) + wave * 1024 + lane;
+  ring_product<NP, OA, OB>(A, B, s1 - s0, la0, lb0, la1, lb1, la2, lb2, am, bn, lane, wave, acc);
+  float4* out = reinterpret_cast<float4*>(p.slab) + (((long)split * (p.Np / RB) + tn) * et + te) * (RA * RB / 4) + wave * 1024 + lane;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -890,21 +936,23 @@ __global__ __launch_bounds__(256, 2) void dt_dx_kernel(DistillArgs p, int et, in
         *q = x;
       }
 }
-template <typename T>
+template <typename T, int RA>
 __global__ __launch_bounds__(256) void dt_dx_sum_kernel(DistillArgs p, int et) {
-  const int nl = *p.nlive, nt = (nl + DT_TILE - 1) / DT_TILE;
-  const int tile = blockIdx.x >> 4;                               // 16 blocks a tile
+  constexpr int RB = 384 - RA;
+  const int nl = *p.nlive, nt = (nl + RB - 1) / RB;
+  const int tile = blockIdx.x >> 5;                               // 32 blocks a tile
   if (tile / et >= nt) return;
   const float w = ldexpf(1.f, -p.sexp[1] - P_EXP);
-  const int slot = (blockIdx.x & 15) * 256 + threadIdx.x;
-  const long step = (long)(p.Np / DT_TILE) * et * (DT_TILE * DT_TILE / 4);
-  const float4* q = reinterpret_cast<const float4*>(p.slab) + (long)tile * (DT_TILE * DT_TILE / 4) + slot;
+  const int slot = (blockIdx.x & 31) * 256 + threadIdx.x;
+  const long step = (long)(p.Np / RB) * et * (RA * RB / 4);
+  const float4* q = reinterpret_cast<const float4*>(p.slab) + (long)tile * (RA * RB / 4) + slot;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
   for (int k = 0; k < p.xsplits; ++k) { const float4 y = q[k * step]; s.x += y.x; s.y += y.y; s.z += y.z; s.w += y.w; }
   const int lane = slot & 63, frag = (slot >> 6) & 15, wave = slot >> 10;
-  const int i = (tile / et) * DT_TILE + (wave & 1) * 64 + ((frag >> 2) & 1) * 32 + (lane & 31);
-  const int e = (tile % et) * DT_TILE + (wave >> 1) * 64 + (frag >> 3) * 32 + (frag & 3) * 8 + (lane >> 5) * 4;
+  const int am = (RA == 256 ? wave >> 1 : wave & 1) * 64, bn = (RA == 256 ? wave & 1 : wave >> 1) * 64;
+  const int i = (tile / et) * RB + bn + ((frag >> 2) & 1) * 32 + (lane & 31);
+  const int e = (tile % et) * RA + am + (frag >> 3) * 32 + (frag & 3) * 8 + (lane >> 5) * 4;
   if (i >= nl) return;
   const float f = w * p.coef[2 * (long)p.Np + i];
   T* out = static_cast<T*>(p.dX) + (long)p.rows[i] * p.E + e;
@@ -914,67 +962,73 @@ __global__ __launch_bounds__(256) void dt_dx_sum_kernel(DistillArgs p, int et) {
     if (e + k < p.E) out[k] = (T)(v[k] * f);
 }
 
-// dW and db: (s X down its rows: K = live rows) x (P down its rows), whole K in one block
-template <typename T, int NP>
-__global__ __launch_bounds__(256, 2) void dt_dw_kernel(DistillArgs p, int et) {
-  DT_LDS
-  const int nl = *p.nlive, vt = (p.vc + DT_TILE - 1) / DT_TILE;
+// dW and db: (s X down its rows: K = live rows) x (P down its rows), tiles of RA columns of E x RB words, whole K in one
+// block
+template <typename T, int NP, int RA>
+__global__ __launch_bounds__(512, 2) void dt_dw_kernel(DistillArgs p, int et) {
+  constexpr int RB = 384 - RA, BK = 64 / NP;
+  DT_RING(RA, RB)
+  const int nl = *p.nlive, vt = p.vc / RB;
   const int pv = (vt + 7) / 8, j0 = blockIdx.x >> 3, tv = (blockIdx.x & 7) * pv + j0 / et, te = j0 % et;
   if (j0 / et >= pv || tv >= vt) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int am = (wave >> 1) * 64, bn = (wave & 1) * 64;
-  constexpr int BK = 64 / NP;
-  Operand<NP, true> A, B;
-  A.init(reinterpret_cast<const char*>(p.Gimg) + (long)te * 256 * NP, (long)p.Kg * NP * 2, lane, wave);
-  B.init(reinterpret_cast<const char*>(p.P) + (long)tv * 256 * NP, p.ldp * 2, lane, wave);
-  const int ex = p.sexp[0];
-  const float fw = *p.gmax * ldexpf(1.f, -P_EXP - ex), fb = *p.gmax * ldexpf(1.f, -2 * P_EXP);
+  const int am = (RA == 256 ? wave >> 1 : wave & 1) * 64, bn = (RA == 256 ? wave & 1 : wave >> 1) * 64;
+  using OA = Operand<NP, true, RA, 8>;
+  using OB = Operand<NP, true, RB, 8>;
+  OA A;
+  OB B;
+  A.init(reinterpret_cast<const char*>(p.Gimg) + (long)te * RA * 2 * NP, (long)p.Kg * NP * 2, 128, lane, wave);
+  B.init(reinterpret_cast<const char*>(p.P) + (long)(tv * RB / BK) * p.Np * 128, 128, (long)p.Np * 128, lane, wave);
+  const float fw = *p.gmax * ldexpf(1.f, -P_EXP - p.sexp[0]), fb = *p.gmax * ldexpf(1.f, -2 * P_EXP);
   f32x16 acc[2][2];
-  product<NP, true, true>(A, B, (nl + BK - 1) / BK, 4, la0, lb0, la1, lb1, am, bn, lane, wave, acc);
-  __syncthreads();
-  // through LDS: rows of the vocabulary, 128 columns each, chunk c of row r at c ^ (r & 31)
+  ring_product<NP, OA, OB>(A, B, (nl + BK - 1) / BK, la0, lb0, la1, lb1, la2, lb2, am, bn, lane, wave, acc);
+  // a lane holds four neighbouring columns of a word's row at a time
+  const bool vec = p.E % 4 == 0 && ((uintptr_t)p.dW % (4 * sizeof(T))) == 0;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int j = 0; j < 2; ++j) {
+    const int v = p.v0 + tv * RB + bn + 32 * j + (lane & 31);
+    if (v >= p.V) continue;
+    T* out = static_cast<T*>(p.dW) + (long)v * p.E;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int row = bn + 32 * j + (lane & 31);
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int ch = (am + 32 * i + 8 * g + 4 * (lane >> 5)) >> 2;
-        *reinterpret_cast<float4*>(DT_AREA(row >> 5) + (row & 31) * 512 + ((ch ^ (row & 31)) << 4)) =
-            make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
-      }
-    }
-  __syncthreads();
-  for (int row = wave; row < DT_TILE; row += 4) {
-    const int v = p.v0 + tv * DT_TILE + row;
-    if (v >= p.V) break;
+        const int e = te * RA + am + 32 * i + 8 * g + 4 * (lane >> 5);
+        if (vec && e + 3 < p.E) {
+          Packed<T, 4> x;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int el = h * 64 + lane, e = te * DT_TILE + el;
-      const float x = *reinterpret_cast<const float*>(DT_AREA(row >> 5) + (row & 31) * 512 + (((el >> 2) ^ (row & 31)) << 4) + (el & 3) * 4);
-      if (e < p.E) static_cast<T*>(p.dW)[(long)v * p.E + e] = (T)(x * fw);
-      else if (e == p.E) static_cast<T*>(p.db)[v] = (T)(x * fb);
-    }
+          for (int k = 0; k < 4; ++k) x.set(k, acc[i][j][4 * g + k] * fw);
+          *reinterpret_cast<Packed<T, 4>*>(out + e) = x;
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (e + k < p.E) out[e + k] = (T)(acc[i][j][4 * g + k] * fw);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (e + k == p.E) static_cast<T*>(p.db)[v] = (T)(acc[i][j][4 * g + k] * fb);
+      }
   }
 }
 
 // ------------------------------------------------------------------------------------------------- host side
-constexpr long DT_PIECE_BYTES = 192L << 20;        // of P: it is written, then read twice, from the last-level cache
+constexpr long DT_PIECE_BYTES = 400L << 20;        // of P: it is written, then read twice
 
 struct DistillPlan {
   long bytes, back_bytes;
   long counts, rows, inv, nlive, slive, amax, sexp, Ximg, Wimg, b2, L1, L2, some, pick, share, part;   // offsets in bytes
   long Gimg, coef, gmax, P, slab;
-  int np, Np, Vp, Kp, Kg, nb, splits_cap, et, etw, xsplits;
+  int np, Np, Vp, Kp, Kg, nb, splits_cap, rax, raw, et, etw, xsplits;
   long vc;
 };
 static DistillPlan dt_plan(int dtype, long N, int E, int V, int K) {
   DistillPlan d = {};
   d.np = dtype == DT_F32 ? 2 : 1;
-  d.Np = (int)((N + 127) / 128 * 128); d.Vp = (V + 127) / 128 * 128; d.Kp = (E + 63) / 64 * 64; d.Kg = (E + 64) / 64 * 64;
+  d.Np = (int)((N + 255) / 256 * 256); d.Vp = (V + 255) / 256 * 256; d.Kp = (E + 63) / 64 * 64; d.Kg = (E + 64) / 64 * 64;
   d.nb = cdiv(N, DT_CROWS);
-  d.et = cdiv(E, DT_TILE); d.etw = cdiv(E + 1, DT_TILE);
+  // the gradient products' tiles: 256 columns of E x 128 rows or words where E needs more than 128, else 128 x 256
+  d.rax = E > 128 ? 256 : 128; d.raw = E + 1 > 128 ? 256 : 128;
+  d.et = cdiv(E, d.rax); d.etw = cdiv(E + 1, d.raw);
   const int nt = d.Np / DT_TILE, vt = d.Vp / DT_TILE;
   d.splits_cap = 8;                                 // live tiles are 1 .. nt: fewer tiles, more splits
   for (int t = 1; t <= (nt < 64 ? nt : 64); ++t) { const int s = dt_splits(t, vt); if (s > d.splits_cap) d.splits_cap = s; }
@@ -983,7 +1037,7 @@ static DistillPlan dt_plan(int dtype, long N, int E, int V, int K) {
   d.counts = take(at, 4L * d.nb); d.rows = take(at, 4 * N); d.inv = take(at, 4 * N); d.nlive = take(at, 4);
   d.slive = take(at, 4 * N);
   d.amax = take(at, 8L * DT_AMAX); d.sexp = take(at, 8);
-  const long slack = 1024;                          // a column tile of the last row may be read past the row's end
+  const long slack = 2048;                          // a column tile of the last row may be read past the row's end
   d.Ximg = take(at, 2L * d.Np * d.Kp * d.np); d.Wimg = take(at, 2L * d.Vp * d.Kp * d.np + slack);
   d.b2 = take(at, 4L * d.Vp);
   d.L1 = take(at, 4L * d.Np); d.L2 = take(at, 4L * d.Np);
@@ -991,19 +1045,20 @@ static DistillPlan dt_plan(int dtype, long N, int E, int V, int K) {
   d.pick = take(at, 4L * N * (K + 1)); d.share = take(at, 4L * N * (K + 1));
   d.part = take(at, 12L * d.splits_cap * d.Np);
   d.bytes = at;
-  long vc = DT_PIECE_BYTES / (2L * d.np * d.Np) / 128 * 128;
+  long vc = DT_PIECE_BYTES / (2L * d.np * d.Np) / 256 * 256;
   if (vc < 1024) vc = 1024;
   const int pieces = cdiv(d.Vp, vc);
-  d.vc = ((long)d.Vp / 128 + pieces - 1) / pieces * 128;          // pieces of equal size
+  d.vc = ((long)d.Vp / 256 + pieces - 1) / pieces * 256;          // ranges of equal size
   const int stages = (int)(d.vc / (64 / d.np));
-  // about 1024 blocks; 1, 2, 4 or a multiple of 8 splits, so that an XCD (block % 8) reads one range of W
-  const int want = 1024 / (nt * d.et);
+  // about 512 blocks (two rounds of one a CU); 1, 2, 4 or a multiple of 8 splits, so that an XCD (block % 8) reads one
+  // range of W
+  const int tiles = d.Np / (384 - d.rax) * d.et, want = 512 / tiles;
   d.xsplits = want >= 8 ? want / 8 * 8 : want >= 4 ? 4 : want >= 2 ? 2 : 1;
-  while (d.xsplits > 8 && stages / d.xsplits < 4) d.xsplits -= 8;
+  while (d.xsplits > 8 && stages / d.xsplits < 6) d.xsplits -= 8;
   at = 0;
   d.Gimg = take(at, 2L * d.Np * d.Kg * d.np + slack); d.coef = take(at, 12L * d.Np); d.gmax = take(at, 4);
   d.P = take(at, 2L * d.Np * d.vc * d.np);
-  d.slab = take(at, 4L * d.xsplits * nt * d.et * DT_TILE * DT_TILE);
+  d.slab = take(at, 4L * d.xsplits * tiles * 32768);
   d.back_bytes = at;
   return d;
 }
@@ -1055,7 +1110,6 @@ template <typename T, int NP, bool TWO> static int dt_backward(const DistillPlan
   const int nx = cdiv(a.N, 16), nt = d.Np / DT_TILE;
   hipLaunchKernelGGL((dt_gimage_kernel<T, NP>), dim3(nx + d.Np / 16), dim3(256), 0, s, a, nx);
   CVAE_LAUNCH_CHECK("dt_gimage_kernel");
-  a.ldp = d.vc * NP;
   for (long v0 = 0; v0 < d.Vp; v0 += d.vc) {
     a.v0 = (int)v0;
     a.vc = (int)(d.Vp - v0 < d.vc ? d.Vp - v0 : d.vc);
@@ -1064,12 +1118,18 @@ template <typename T, int NP, bool TWO> static int dt_backward(const DistillPlan
     CVAE_LAUNCH_CHECK("dt_grad_kernel");
     hipLaunchKernelGGL((dt_pick_kernel<NP, TWO>), dim3(cdiv(a.N, 4)), dim3(256), 0, s, a);
     CVAE_LAUNCH_CHECK("dt_pick_kernel");
-    hipLaunchKernelGGL((dt_dx_kernel<NP>), dim3((unsigned)((long)nt * d.et * d.xsplits)), dim3(256), 0, s, a, d.et, v0 > 0 ? 1 : 0);
+    const dim3 gx((unsigned)((long)(d.Np / (384 - d.rax)) * d.et * d.xsplits));
+    if (d.rax == 256) hipLaunchKernelGGL((dt_dx_kernel<NP, 256>), gx, dim3(512), 0, s, a, d.et, v0 > 0 ? 1 : 0);
+    else hipLaunchKernelGGL((dt_dx_kernel<NP, 128>), gx, dim3(512), 0, s, a, d.et, v0 > 0 ? 1 : 0);
     CVAE_LAUNCH_CHECK("dt_dx_kernel");
-    hipLaunchKernelGGL((dt_dw_kernel<T, NP>), dim3((unsigned)((long)cdiv(vt, 8) * 8 * d.etw)), dim3(256), 0, s, a, d.etw);
+    const dim3 gw((unsigned)((long)cdiv(a.vc / (384 - d.raw), 8) * 8 * d.etw));
+    if (d.raw == 256) hipLaunchKernelGGL((dt_dw_kernel<T, NP, 256>), gw, dim3(512), 0, s, a, d.etw);
+    else hipLaunchKernelGGL((dt_dw_kernel<T, NP, 128>), gw, dim3(512), 0, s, a, d.etw);
     CVAE_LAUNCH_CHECK("dt_dw_kernel");
   }
-  hipLaunchKernelGGL((dt_dx_sum_kernel<T>), dim3((unsigned)((long)nt * d.et * 16)), dim3(256), 0, s, a, d.et);
+  const dim3 gs((unsigned)((long)(d.Np / (384 - d.rax)) * d.et * 32));
+  if (d.rax == 256) hipLaunchKernelGGL((dt_dx_sum_kernel<T, 256>), gs, dim3(256), 0, s, a, d.et);
+  else hipLaunchKernelGGL((dt_dx_sum_kernel<T, 128>), gs, dim3(256), 0, s, a, d.et);
   CVAE_LAUNCH_CHECK("dt_dx_sum_kernel");
   return 0;
 }
@@ -1106,6 +1166,7 @@ int launch_distill_backward(const DistillCall& c, const float* ghard, const floa
                             void* dW, void* db, void* ws, hipStream_t s) {
   CVAE_TRY(dt_check("distill_backward", c));
   CVAE_REQUIRE((int64_t)c.T * c.R > 0, "distill_backward: no rows");
+  CVAE_REQUIRE((int64_t)c.T * c.R <= (1 << 22), "distill_backward: more than %d rows", 1 << 22);   // 32-bit lane offsets in P
   CVAE_REQUIRE(c.X && c.W && c.b && c.tgt && ghard && saved && dX && dW && db && ws && (c.K == 0 || (c.ids && c.top && gsoft)),
                "distill_backward: null operand");
   CVAE_REQUIRE((((uintptr_t)ws | (uintptr_t)saved) & 15) == 0, "distill_backward: the workspaces must be 16-byte aligned");

@@ -1122,17 +1122,17 @@ int64_t cvae_distill_workspace(int dtype, int64_t N, int64_t E, int64_t V, int K
 int64_t cvae_distill_backward_workspace(int dtype, int64_t N, int64_t E, int64_t V, int K) {
   return distill_backward_workspace_floats(dtype, N, E, V, K);
 }
-int cvae_distill_forward(int dtype, const void* final, const void* W, const void* b, const int64_t* tgt, int64_t pad,
-                         int B, int T, int R, int E, int64_t V, int K, const int64_t* ids, const float* top, float tau,
-                         float* hard_row, float* soft_row, float* hard, float* soft, float* ws, void* stream) {
-  const DistillCall c = {dtype, B, T, R, E, V, K, tau, final, W, b, tgt, pad, ids, top};
-  return launch_distill_forward(c, hard_row, soft_row, hard, soft, ws, S(stream));
+int cvae_distill_forward(int dtype, const void* final, const void* W, const void* b, const int64_t* eos, int64_t pad,
+                         int sentence_major, int B, int T, int R, int E, int64_t V, int K, const int64_t* ids,
+                         const float* top, float tau, float* hard, float* soft, float* ws, void* stream) {
+  const DistillCall c = {dtype, B, T, R, E, V, K, tau, final, W, b, eos, pad, sentence_major, ids, top};
+  return launch_distill_forward(c, hard, soft, ws, S(stream));
 }
-int cvae_distill_backward(int dtype, const void* final, const void* W, const void* b, const int64_t* tgt, int64_t pad,
-                          int B, int T, int R, int E, int64_t V, int K, const int64_t* ids, const float* top, float tau,
-                          const float* ghard, const float* gsoft, const float* saved, void* dfinal, void* dW, void* db,
-                          float* ws, void* stream) {
-  const DistillCall c = {dtype, B, T, R, E, V, K, tau, final, W, b, tgt, pad, ids, top};
+int cvae_distill_backward(int dtype, const void* final, const void* W, const void* b, const int64_t* eos, int64_t pad,
+                          int sentence_major, int B, int T, int R, int E, int64_t V, int K, const int64_t* ids,
+                          const float* top, float tau, const float* ghard, const float* gsoft, const float* saved,
+                          void* dfinal, void* dW, void* db, float* ws, void* stream) {
+  const DistillCall c = {dtype, B, T, R, E, V, K, tau, final, W, b, eos, pad, sentence_major, ids, top};
   return launch_distill_backward(c, ghard, gsoft, saved, dfinal, dW, db, ws, S(stream));
 }
 

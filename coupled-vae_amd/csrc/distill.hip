@@ -41,9 +41,9 @@ struct DistillArgs {
   float tau, itau;
   int two;                                 // tau != 1 and K > 0: a second normaliser
   const void* X; const void* W; const void* bias;
-  const int64_t* tgt; int64_t pad;
+  const int64_t* eos; int64_t pad; int per;   // targets [B,T]; rows per sentence of sentence-major rows, else 0
   const int64_t* ids; const float* top;
-  float* hard; float* soft;                // [N]
+  float* hard; float* soft;                // [N], in the workspace
   // kept for the backward pass
   int* counts; int* rows; int* inv; int* nlive; int* slive;   // slive[R]: the sentence has a live row
   float* amax; int* sexp;                  // [2][DT_AMAX]; [2] scale exponents of X and W
@@ -59,6 +59,12 @@ struct DistillArgs {
   float* slab; int xsplits;
   void* dX; void* dW; void* db;
 };
+
+// row n = t R + r reads position (sentence, t): r % B, or r / (R / B) for sentence-major rows
+__device__ __forceinline__ long position(const DistillArgs& p, int n) {
+  const int t = n / p.R, r = n - t * p.R, b = p.per ? r / p.per : r % p.B;
+  return (long)b * p.T + t;
+}
 
 // ------------------------------------------------------------------------------------------------- scales and images
 __device__ __forceinline__ int scale_exp(float amax) {          // amax * 2^e in [2^13, 2^14)
@@ -109,7 +115,7 @@ template <typename T> __global__ __launch_bounds__(256) void dt_count_kernel(Dis
   __shared__ float red[4];
   if ((int)blockIdx.x < nb) {
     const int n = blockIdx.x * DT_CROWS + threadIdx.x;
-    const bool live = n < p.N && p.tgt[n] != p.pad;
+    const bool live = n < p.N && p.eos[position(p, n)] != p.pad;
     if (n < p.N) {
       p.hard[n] = 0.f;
       if (p.K) p.soft[n] = 0.f;
@@ -150,7 +156,7 @@ template <typename T> __global__ __launch_bounds__(256) void dt_count_kernel(Dis
     const bool vec = p.E % 4 == 0 && ((uintptr_t)x % (4 * sizeof(T))) == 0;
 #pragma unroll 2
     for (int n = slot * 4 + wave; n < p.N; n += DT_AMAX * 4) {
-      if (p.tgt[n] == p.pad) continue;
+      if (p.eos[position(p, n)] == p.pad) continue;
       for (int k = lane * 4; k < p.E; k += 256) {
         float v[4];
         load4<T>(x + (long)n * p.E, k, p.E, vec, v);
@@ -225,7 +231,7 @@ template <typename T, int NP> __global__ __launch_bounds__(256) void dt_image_ke
       return;
     }
     const int n = group * DT_CROWS + threadIdx.x;
-    const bool live = n < p.N && p.tgt[n] != p.pad;
+    const bool live = n < p.N && p.eos[position(p, n)] != p.pad;
     const unsigned long long b = __ballot(live);
     if (lane == 0) swave[wave] = __popcll(b);
     __syncthreads();
@@ -582,10 +588,11 @@ __global__ __launch_bounds__(256) void dt_combine_kernel(DistillArgs p) {
   if (i >= nl) return;
   __shared__ float red[4][3];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int n = p.rows[i], r = n % p.R, t = n / p.R;
-  const int64_t* ids = p.K ? p.ids + ((long)(r % p.B) * p.T + t) * p.K : nullptr;
-  const float* top = p.K ? p.top + ((long)(r % p.B) * p.T + t) * p.K : nullptr;
-  const int64_t tg = p.tgt[n];
+  const int n = p.rows[i], r = n % p.R;
+  const long at = position(p, n);
+  const int64_t* ids = p.K ? p.ids + at * p.K : nullptr;
+  const float* top = p.K ? p.top + at * p.K : nullptr;
+  const int64_t tg = p.eos[at];
   float* pick = p.pick + (long)i * (p.K + 1);
   // Picked logits, base 2: 32 lanes a dot product, four of them in flight.  16 bytes a lane where rows allow it (a W row
   // of E = 200 in 16 bits is then one access), else single elements.
@@ -883,9 +890,9 @@ template <int NP, bool TWO>
 __global__ __launch_bounds__(256) void dt_pick_kernel(DistillArgs p) {
   const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (i >= *p.nlive) return;
-  const int n = p.rows[i], r = n % p.R, t = n / p.R;
-  const int64_t* ids = p.K ? p.ids + ((long)(r % p.B) * p.T + t) * p.K : nullptr;
-  const int64_t tg = p.tgt[n];
+  const long at = position(p, p.rows[i]);
+  const int64_t* ids = p.K ? p.ids + at * p.K : nullptr;
+  const int64_t tg = p.eos[at];
   const float a = p.coef[i], b = p.coef[p.Np + i], L1 = p.L1[i], L2 = p.L2[i];
   for (int k = lane; k <= p.K; k += 64) {
     const int64_t id = k < p.K ? ids[k] : tg;
@@ -1016,7 +1023,7 @@ constexpr long DT_PIECE_BYTES = 400L << 20;        // of P: it is written, then 
 
 struct DistillPlan {
   long bytes, back_bytes;
-  long counts, rows, inv, nlive, slive, amax, sexp, Ximg, Wimg, b2, L1, L2, some, pick, share, part;   // offsets in bytes
+  long hard, soft, counts, rows, inv, nlive, slive, amax, sexp, Ximg, Wimg, b2, L1, L2, some, pick, share, part;   // offsets in bytes
   long Gimg, coef, gmax, P, slab;
   int np, Np, Vp, Kp, Kg, nb, splits_cap, rax, raw, et, etw, xsplits;
   long vc;
@@ -1034,6 +1041,7 @@ static DistillPlan dt_plan(int dtype, long N, int E, int V, int K) {
   for (int t = 1; t <= (nt < 64 ? nt : 64); ++t) { const int s = dt_splits(t, vt); if (s > d.splits_cap) d.splits_cap = s; }
   auto take = [](long& at, long bytes) { const long o = at; at += (bytes + 255) / 256 * 256; return o; };
   long at = 0;
+  d.hard = take(at, 4 * N); d.soft = take(at, K ? 4 * N : 0);
   d.counts = take(at, 4L * d.nb); d.rows = take(at, 4 * N); d.inv = take(at, 4 * N); d.nlive = take(at, 4);
   d.slive = take(at, 4 * N);
   d.amax = take(at, 8L * DT_AMAX); d.sexp = take(at, 8);
@@ -1086,8 +1094,9 @@ static void dt_fill(DistillArgs& a, const DistillPlan& d, const DistillCall& c, 
   a.Np = d.Np; a.Vp = d.Vp; a.Kp = d.Kp; a.Kg = d.Kg;
   a.tau = c.K ? c.tau : 1.f; a.itau = 1.f / a.tau;
   a.two = c.K > 0 && a.tau != 1.f;
-  a.X = c.X; a.W = c.W; a.bias = c.b; a.tgt = c.tgt; a.pad = c.pad; a.ids = c.ids; a.top = c.top;
+  a.X = c.X; a.W = c.W; a.bias = c.b; a.eos = c.eos; a.pad = c.pad; a.per = c.sentence_major ? c.R / c.B : 0; a.ids = c.ids; a.top = c.top;
   char* w = static_cast<char*>(ws);
+  a.hard = (float*)(w + d.hard); a.soft = (float*)(w + d.soft);
   a.counts = (int*)(w + d.counts); a.rows = (int*)(w + d.rows); a.inv = (int*)(w + d.inv); a.nlive = (int*)(w + d.nlive); a.slive = (int*)(w + d.slive);
   a.amax = (float*)(w + d.amax); a.sexp = (int*)(w + d.sexp); a.Ximg = (_Float16*)(w + d.Ximg); a.Wimg = (_Float16*)(w + d.Wimg); a.b2 = (float*)(w + d.b2);
   a.L1 = (float*)(w + d.L1); a.L2 = (float*)(w + d.L2); a.some = (float*)(w + d.some);
@@ -1142,22 +1151,19 @@ static int dt_dispatch(int dtype, const DistillPlan& d, const DistillArgs& a, bo
   return dtype == DT_BF16 ? dt_run<bf16_t, 1>(d, a, back, s) : dt_run<f16_t, 1>(d, a, back, s);
 }
 
-int launch_distill_forward(const DistillCall& c, float* hard_row, float* soft_row, float* hard, float* soft, void* ws,
-                           hipStream_t s) {
+int launch_distill_forward(const DistillCall& c, float* hard, float* soft, void* ws, hipStream_t s) {
   CVAE_TRY(dt_check("distill_forward", c));
   if (c.R == 0) return 0;
   CVAE_REQUIRE(hard && (c.K == 0 || soft), "distill_forward: null operand");
+  DistillArgs a = {};
   if (c.T > 0) {
-    CVAE_REQUIRE(c.X && c.W && c.b && c.tgt && hard_row && ws && (c.K == 0 || (c.ids && c.top && soft_row)),
-                 "distill_forward: null operand");
+    CVAE_REQUIRE(c.X && c.W && c.b && c.eos && ws && (c.K == 0 || (c.ids && c.top)), "distill_forward: null operand");
     CVAE_REQUIRE(((uintptr_t)ws & 15) == 0, "distill_forward: the workspace must be 16-byte aligned");
     const DistillPlan d = dt_plan(c.dtype, (long)c.T * c.R, c.E, (int)c.V, c.K);
-    DistillArgs a = {};
     dt_fill(a, d, c, ws);
-    a.hard = hard_row; a.soft = soft_row;
     CVAE_TRY(dt_dispatch(c.dtype, d, a, false, s));
   }
-  hipLaunchKernelGGL(dt_sum_kernel, dim3(cdiv(c.R, 4), c.K ? 2 : 1), dim3(256), 0, s, c.T, c.R, hard_row, soft_row, hard, soft);
+  hipLaunchKernelGGL(dt_sum_kernel, dim3(cdiv(c.R, 4), c.K ? 2 : 1), dim3(256), 0, s, c.T, c.R, a.hard, a.soft, hard, soft);
   CVAE_LAUNCH_CHECK("dt_sum_kernel");
   return 0;
 }
@@ -1167,7 +1173,7 @@ int launch_distill_backward(const DistillCall& c, const float* ghard, const floa
   CVAE_TRY(dt_check("distill_backward", c));
   CVAE_REQUIRE((int64_t)c.T * c.R > 0, "distill_backward: no rows");
   CVAE_REQUIRE((int64_t)c.T * c.R <= (1 << 22), "distill_backward: more than %d rows", 1 << 22);   // 32-bit lane offsets in P
-  CVAE_REQUIRE(c.X && c.W && c.b && c.tgt && ghard && saved && dX && dW && db && ws && (c.K == 0 || (c.ids && c.top && gsoft)),
+  CVAE_REQUIRE(c.X && c.W && c.b && c.eos && ghard && saved && dX && dW && db && ws && (c.K == 0 || (c.ids && c.top && gsoft)),
                "distill_backward: null operand");
   CVAE_REQUIRE((((uintptr_t)ws | (uintptr_t)saved) & 15) == 0, "distill_backward: the workspaces must be 16-byte aligned");
   const DistillPlan d = dt_plan(c.dtype, (long)c.T * c.R, c.E, (int)c.V, c.K);

@@ -131,13 +131,12 @@ int launch_linrnn_backward(int dtype, int gates, int reverse, int T, int B, int 
 struct DistillCall {
   int dtype, B, T, R, E; int64_t V; int K; float tau;
   const void* X; const void* W; const void* b;      // [T*R,E] [V,E] [V]
-  const int64_t* tgt; int64_t pad;                  // [T*R] time-major
+  const int64_t* eos; int64_t pad; int sentence_major;   // [B,T]
   const int64_t* ids; const float* top;             // [B,T,K]
 };
 long distill_workspace_floats(int dtype, long N, long E, long V, long K);
 long distill_backward_workspace_floats(int dtype, long N, long E, long V, long K);
-int launch_distill_forward(const DistillCall& c, float* hard_row, float* soft_row, float* hard, float* soft, void* ws,
-                           hipStream_t s);
+int launch_distill_forward(const DistillCall& c, float* hard, float* soft, void* ws, hipStream_t s);
 int launch_distill_backward(const DistillCall& c, const float* ghard, const float* gsoft, const void* saved, void* dX,
                             void* dW, void* db, void* ws, hipStream_t s);
 

@@ -80,8 +80,8 @@ SIGNATURES = {
     'cvae_projce_backward_saved_n': [I, P, P, P, P, L, P, P, I, I, I, L, P, P, P, P, P, P],
     'cvae_distill_workspace': [I, L, L, L, I],
     'cvae_distill_backward_workspace': [I, L, L, L, I],
-    'cvae_distill_forward': [I, P, P, P, P, L, I, I, I, I, L, I, P, P, F, P, P, P, P, P, P],
-    'cvae_distill_backward': [I, P, P, P, P, L, I, I, I, I, L, I, P, P, F] + [P] * 8,
+    'cvae_distill_forward': [I, P, P, P, P, L, I, I, I, I, I, L, I, P, P, F, P, P, P, P],
+    'cvae_distill_backward': [I, P, P, P, P, L, I, I, I, I, I, L, I, P, P, F] + [P] * 8,
     'cvae_targets_time_major': [P, I, I, I, P, P],
     'cvae_logits': [P, P, P, I, I, I, L, P, P, P],
     'cvae_reparam_forward': [P, P, P, I, I, I, P, P],

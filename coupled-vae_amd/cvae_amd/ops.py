@@ -39,8 +39,9 @@ def _need(ok, message):
 
 def _here(*tensors):
     """Every tensor given is on the current GPU (the library launches on the current device's current stream)."""
+    here = torch.cuda.current_device()
     for t in tensors:
-        if t is not None and (t.device.type != 'cuda' or t.device.index != torch.cuda.current_device()):
+        if t is not None and t.get_device() != here:               # -1: on the host
             raise ValueError('tensor on %s, but the library works on the current GPU' % t.device)
 
 
@@ -637,33 +638,33 @@ class ProjDistillFn(torch.autograd.Function):
     stored (cvae_distill_*); fp32, bf16 or fp16 storage.  ids = None: the hard loss alone."""
 
     @staticmethod
-    def forward(ctx, final, W, b, tgt_tm, pad, B, ids, top, tau):
+    def forward(ctx, final, W, b, eos, pad, sentence_major, ids, top, tau):
         T, R, E = final.shape
         V, K = W.shape[0], 0 if ids is None else ids.shape[2]
-        dt, N = _DTYPE[final.dtype], T * R
-        rows, hard, soft = _f((2 * N,), final), _f((R,), final), _f((R,), final)
-        ws = _f((query('cvae_distill_workspace', dt, N, E, V, K),), final)
-        ctx.args = (pad, B, T, R, E, V, K)
-        ctx.tau = tau
-        call('cvae_distill_forward', dt, ptr(final), ptr(W), ptr(b), ptr(tgt_tm), *ctx.args, ptr(ids), ptr(top), tau,
-             ptr(rows), rows.data_ptr() + 4 * N, ptr(hard), ptr(soft) if K else None, ptr(ws), stream())
+        dt = _DTYPE[final.dtype]
+        hard, soft = _f((R,), final), _f((R,), final) if K else None
+        ws = _f((query('cvae_distill_workspace', dt, T * R, E, V, K),), final)
+        args = (pad, sentence_major, eos.shape[0], T, R, E, V, K)
+        call('cvae_distill_forward', dt, ptr(final), ptr(W), ptr(b), ptr(eos), *args, ptr(ids), ptr(top), tau, ptr(hard),
+             ptr(soft), ptr(ws), stream())
         if any(ctx.needs_input_grad):
-            ctx.save_for_backward(final, W, b, tgt_tm, ids, top, ws)
-        return hard, soft
+            ctx.args = (dt, tau) + args
+            ctx.save_for_backward(final, W, b, eos, ids, top, ws)
+        return (hard, soft) if K else hard
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, ghard, gsoft):
-        final, W, b, tgt_tm, ids, top, saved = ctx.saved_tensors
-        pad, B, T, R, E, V, K = ctx.args
-        dt, N = _DTYPE[final.dtype], T * R
-        if N == 0:
+    def backward(ctx, ghard, gsoft=None):
+        final, W, b, eos, ids, top, saved = ctx.saved_tensors
+        dt, tau, *args = ctx.args
+        T, R, E, V, K = args[3:]
+        if T * R == 0:
             return (torch.zeros_like(final), torch.zeros_like(W), torch.zeros_like(b)) + (None,) * 6
         ghard, gsoft = _c(ghard), _c(gsoft)
         dfinal, dW, db = torch.empty_like(final), torch.empty_like(W), torch.empty_like(b)
-        ws = _f((query('cvae_distill_backward_workspace', dt, N, E, V, K),), final)
-        call('cvae_distill_backward', dt, ptr(final), ptr(W), ptr(b), ptr(tgt_tm), *ctx.args, ptr(ids), ptr(top), ctx.tau,
-             ptr(ghard), ptr(gsoft), ptr(saved), ptr(dfinal), ptr(dW), ptr(db), ptr(ws), stream())
+        ws = _f((query('cvae_distill_backward_workspace', dt, T * R, E, V, K),), final)
+        call('cvae_distill_backward', dt, ptr(final), ptr(W), ptr(b), ptr(eos), *args, ptr(ids), ptr(top), tau, ptr(ghard),
+             ptr(gsoft), ptr(saved), ptr(dfinal), ptr(dW), ptr(db), ptr(ws), stream())
         return (dfinal, dW, db) + (None,) * 6
 
 
@@ -677,14 +678,14 @@ def _proj_check(final, W, b, eos):
           final.shape[1] % eos.shape[0] == 0, 'eos must be int64 (B,T) with R a multiple of B')
 
 
-def proj_distill(final, W, b, eos, pad, teacher_ids, teacher_logits, tau, cache=None):
+def proj_distill(final, W, b, eos, pad, teacher_ids, teacher_logits, tau):
     """Cross-entropy and distillation of one student projection, logits never stored: final (T,R,E), W (V,E), b (V,) in
     fp32, bf16 or fp16; eos (B,T) int64 targets (rows at `pad` count nothing), R % B == 0; the teacher's K best of every
     position: teacher_ids (B,T,K) int64, teacher_logits (B,T,K) float (ids outside the vocabulary and logits of -inf are
     absent entries).  With p = softmax(teacher_logits / tau) over the K entries and q_tau = softmax(logits / tau) over
     the whole vocabulary:
       hard (R,) = sum_t -log softmax(logits)[target],   soft (R,) = sum_t tau^2 KL(p || q_tau)
-    -> (hard, soft) fp32, differentiable in final, W and b.  `cache` as in proj_ce."""
+    -> (hard, soft) fp32, differentiable in final, W and b."""
     _proj_check(final, W, b, eos)
     _need(teacher_ids.dim() == 3 and teacher_ids.dtype == torch.int64 and
           tuple(teacher_ids.shape[:2]) == tuple(eos.shape) and 0 < teacher_ids.shape[2] <= W.shape[0],
@@ -693,9 +694,8 @@ def proj_distill(final, W, b, eos, pad, teacher_ids, teacher_logits, tau, cache=
           'teacher_logits must be a float tensor of the shape of teacher_ids')
     _need(0.0 < tau < 1e6, 'tau must be positive')
     _here(final, W, b, eos, teacher_ids, teacher_logits)
-    tgt = _targets(eos, final.shape[1], cache)
-    return ProjDistillFn.apply(_c(final), _c(W), _c(b), tgt, pad, eos.shape[0], _c(teacher_ids),
-                               _c(teacher_logits.float()), float(tau))
+    return ProjDistillFn.apply(_c(final), _c(W), _c(b), _c(eos), pad, 0, _c(teacher_ids), _c(teacher_logits.float()),
+                               float(tau))
 
 
 def _targets(eos, R, cache):
@@ -716,8 +716,7 @@ def proj_ce(final, W, b, eos, pad, cache=None):
     if final.dtype != torch.float32:
         _proj_check(final, W, b, eos)
         _here(final, W, b, eos)
-        tgt = _targets(eos, final.shape[1], cache)
-        return ProjDistillFn.apply(_c(final), _c(W), _c(b), tgt, pad, eos.shape[0], None, None, 1.0)[0]
+        return ProjDistillFn.apply(_c(final), _c(W), _c(b), _c(eos), pad, 0, None, None, 1.0)
     return ProjCEFn.apply(final, W, b, _targets(eos, final.shape[1], cache), pad)
 
 
@@ -799,8 +798,7 @@ def proj_ce_sorted(final, W, b, eos, pad):
     if final.dtype != torch.float32:
         _proj_check(final, W, b, eos)
         _here(final, W, b, eos)
-        tgt = targets_sentence_major(eos, final.shape[1] // B)
-        return ProjDistillFn.apply(_c(final), _c(W), _c(b), tgt, pad, B, None, None, 1.0)[0]
+        return ProjDistillFn.apply(_c(final), _c(W), _c(b), _c(eos), pad, 1, None, None, 1.0)
     tgt = targets_sentence_major(eos, final.shape[1] // B)
     return ProjCEFn.apply(final, W, b, tgt, pad)
 

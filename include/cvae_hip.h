@@ -266,24 +266,25 @@ int cvae_projce_backward_saved_n(int nd, const float* const* final, const float*
  * distillation from a teacher's top logits).  With q = softmax(S), q_tau = softmax(S / tau), p = softmax(top / tau):
  *   hard = -log q[tgt],   soft = tau^2 sum_k p_k (log p_k - log q_tau[ids_k])          (tau^2 KL(p || q_tau))
  * dtype: storage of final, W, b and their gradients: 0 = fp32, 1 = bf16, 2 = fp16; losses, sums and softmax statistics
- * are fp32.  final[T*R,E] (rows n = t*R + r), W[V,E], b[V], tgt[T*R]: rows whose target is `pad` have no loss and no
- * gradient; a target outside [0,V) that is not `pad` counts as a logit of 0 (as in cvae_projce_*).
- * K >= 0 entries of the teacher: ids[B,T,K], top[B,T,K] (batch-major; row r reads sentence r % B, R % B == 0); an entry
- * whose id is outside [0,V) or whose logit is -inf is absent, a row with no entry has soft = 0; an id may be listed
- * twice.  K = 0: ids, top, soft_row, soft are NULL and tau is ignored.
- * -> hard_row[T*R], soft_row[T*R]; hard[R], soft[R] = their sums over t.
- * ws: cvae_distill_workspace(dtype, T*R, E, V, K) floats, 16-byte aligned; the backward call reads it (`saved`). */
+ * are fp32.  final[T*R,E] (rows n = t*R + r), W[V,E], b[V], eos[B,T] targets: row r reads sentence r % B, or r / (R / B)
+ * if sentence_major (R % B == 0).  Rows whose target is `pad` have no loss and no gradient; a target outside [0,V) that
+ * is not `pad` counts as a logit of 0 (as in cvae_projce_*).
+ * K >= 0 entries of the teacher at every position: ids[B,T,K], top[B,T,K]; an entry whose id is outside [0,V) or whose
+ * logit is -inf is absent, a row with no entry has soft = 0; an id may be listed twice.  K = 0: ids, top, soft (and
+ * gsoft) are not read and tau is ignored.
+ * -> hard[R], soft[R]: sums over t.  ws: cvae_distill_workspace(dtype, T*R, E, V, K) floats, 16-byte aligned; the backward
+ * call reads it (`saved`). */
 int64_t cvae_distill_workspace(int dtype, int64_t N, int64_t E, int64_t V, int K);
-int cvae_distill_forward(int dtype, const void* final, const void* W, const void* b, const int64_t* tgt, int64_t pad,
-                         int B, int T, int R, int E, int64_t V, int K, const int64_t* ids, const float* top, float tau,
-                         float* hard_row, float* soft_row, float* hard, float* soft, float* ws, void* stream);
+int cvae_distill_forward(int dtype, const void* final, const void* W, const void* b, const int64_t* eos, int64_t pad,
+                         int sentence_major, int B, int T, int R, int E, int64_t V, int K, const int64_t* ids,
+                         const float* top, float tau, float* hard, float* soft, float* ws, void* stream);
 /* ghard[R], gsoft[R] = dL/dhard, dL/dsoft -> dfinal[T*R,E], dW[V,E], db[V] of `dtype`, overwritten.  The other arguments
- * as in the forward call.  ws: cvae_distill_backward_workspace floats, 16-byte aligned. */
+ * as in the forward call; at most 2^22 rows.  ws: cvae_distill_backward_workspace floats, 16-byte aligned. */
 int64_t cvae_distill_backward_workspace(int dtype, int64_t N, int64_t E, int64_t V, int K);
-int cvae_distill_backward(int dtype, const void* final, const void* W, const void* b, const int64_t* tgt, int64_t pad,
-                          int B, int T, int R, int E, int64_t V, int K, const int64_t* ids, const float* top, float tau,
-                          const float* ghard, const float* gsoft, const float* saved, void* dfinal, void* dW, void* db,
-                          float* ws, void* stream);
+int cvae_distill_backward(int dtype, const void* final, const void* W, const void* b, const int64_t* eos, int64_t pad,
+                          int sentence_major, int B, int T, int R, int E, int64_t V, int K, const int64_t* ids,
+                          const float* top, float tau, const float* ghard, const float* gsoft, const float* saved,
+                          void* dfinal, void* dW, void* db, float* ws, void* stream);
 /* tgt_tm[t*R + r] = eos[(r % B)*T + t]: time-major targets for R = n*B rows. */
 int cvae_targets_time_major(const int64_t* eos, int B, int T, int R, int64_t* tgt_tm, void* stream);
 /* tgt_tm[t*B*K + r] = eos[(r / K)*T + t]: the same for sentence-major rows r = b*K + k. */

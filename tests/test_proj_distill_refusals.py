@@ -61,18 +61,20 @@ def test_c_entries_refuse_bad_arguments():
 
     def forward(**kw):
         a = dict(ok, **kw)
-        _lib.call('cvae_distill_forward', a['dtype'], one, one, one, one, 0, a['B'], a['T'], a['R'], a['E'], a['V'], a['K'],
-                  one, one, a['tau'], one, one, one, one, a['ws'], None)
+        _lib.call('cvae_distill_forward', a['dtype'], one, one, one, one, 0, 0, a['B'], a['T'], a['R'], a['E'], a['V'], a['K'],
+                  one, one, a['tau'], one, one, a['ws'], None)
 
     def backward(**kw):
         a = dict(ok, **kw)
-        _lib.call('cvae_distill_backward', a['dtype'], one, one, one, one, 0, a['B'], a['T'], a['R'], a['E'], a['V'], a['K'],
+        _lib.call('cvae_distill_backward', a['dtype'], one, one, one, one, 0, 0, a['B'], a['T'], a['R'], a['E'], a['V'], a['K'],
                   one, one, a['tau'], one, one, one, one, one, one, a['ws'], None)
     for f in (forward, backward):
         for bad in (dict(dtype=3), dict(B=0), dict(R=3), dict(T=-1), dict(T=1 << 20, R=1 << 12), dict(E=0), dict(V=0),
                     dict(V=1 << 31), dict(K=-1), dict(K=11), dict(tau=0.0), dict(tau=float('nan')), dict(ws=None), dict(ws=24)):
             with pytest.raises(_lib.CvaeHipError, match='distill_'):
                 f(**bad)
+    with pytest.raises(_lib.CvaeHipError, match='rows'):
+        backward(T=1 << 14, R=1 << 9)
     for name in ('cvae_distill_workspace', 'cvae_distill_backward_workspace'):      # sizes of nothing, or refused ones: 0
         assert _lib.query(name, 1, 5, 8, 10, 3) > 0
         for sizes in ((0, 8, 10, 3), (-1, 8, 10, 3), (5, 0, 10, 3), (5, 8, 0, 0), (5, 8, 10, 11), (5, 8, 10, -1),

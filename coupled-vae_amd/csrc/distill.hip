@@ -50,7 +50,7 @@ struct DistillArgs {
   _Float16* Ximg; _Float16* Wimg; float* b2;
   float* L1; float* L2; float* some;       // by live row: normalisers (base 2), 1 where the teacher lists anything
   float* pick; float* share;               // picked logits (base 2) and the teacher's share of them, [K + 1]
-  float* part; int splits_cap;             // [3][splits][Np]
+  float* part; long pplane; int fvt;       // [3][splits][tiles of live rows][128]; floats of one; vocabulary tiles of the walk
   // backward
   const float* ghard; const float* gsoft;  // [R]
   _Float16* Gimg; float* coef;             // s X image with a column of s; [3][Np]: a, b, s / gmax
@@ -423,7 +423,7 @@ __device__ __forceinline__ void stages(const OA& A, const OB& B, int n, int last
 // copies to wait for is a constant.
 template <int C> __device__ __forceinline__ void ring_barrier() {
   asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0x0070 | C);                         // vmcnt(C) lgkmcnt(0)
+  __builtin_amdgcn_s_waitcnt(0x0070 | (C & 15) | (C >> 4) << 14);  // vmcnt(C) lgkmcnt(0)
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
@@ -466,20 +466,86 @@ __device__ __forceinline__ void ring_product(const OA& A, const OB& B, int n, ch
 __device__ __forceinline__ int acc_row(int r, int lane) { return (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5); }
 
 // ------------------------------------------------------------------------------------------------- forward
-// Vocabulary splits for nt tiles of live rows: the blocks of an XCD (block % 8) share a range of W, and the splits are
-// as many as fill 512 blocks (two on every CU).  Computed alike by the product and the merge.
-__host__ __device__ inline int dt_splits(int nt, int vt) {
-  int s = nt > 0 ? 64 / nt : 1;
-  if (s < 1) s = 1;
-  s *= 8;
-  return s < vt ? s : (vt + 7) / 8 * 8;
+// Work items of the kernels that walk the vocabulary: (tile of 128 live rows) x (range of its vt tiles).  512 blocks, two
+// on a CU; the 64 of an XCD (block % 8) take every eighth range, so that they share W's tiles in its L2.  The number of
+// ranges, 8 k, is what the live rows (known on the device alone) make cheapest: rounds of 64 items times the tiles of an
+// item, and one tile's time for its start.  One wave's lanes try one k each; every kernel that needs it gets the same.
+constexpr int DT_WALK_BLOCKS = 512, DT_MOST_ITEMS = 1024;         // the latter: per XCD, for more than one range
+__device__ __forceinline__ int dt_splits(int nt, int vt) {
+  const int k = (threadIdx.x & 63) + 1;
+  const bool ok = k == 1 || (k * 8 <= vt && nt * k <= DT_MOST_ITEMS);
+  int best = 0x7fffffff;
+  if (ok) best = min(((nt * k + 63) / 64) * ((vt + 8 * k - 1) / (8 * k) + 1), 0x1ffffff) * 64 + (k - 1);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) best = min(best, __shfl_xor(best, o, 64));
+  return __builtin_amdgcn_readfirstlane(((best & 63) + 1) * 8);
 }
-constexpr int DT_FWD_BLOCKS = 512;
+
+// Fold 64 vocabulary entries of a lane's row into its running (max, sum) pairs, base 2: two accumulator tiles of 32
+// entries, of which the lane holds 16 each, and their biases.
+template <bool TWO>
+__device__ __forceinline__ void fold(f32x16& t0, f32x16& t1, const float4 (&bias)[2][4], float c, float itau, float& m,
+                                     float& s1, float& s2) {
+  float mx = m;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const float4 &ba = bias[0][r >> 2], &bb = bias[1][r >> 2];
+    t0[r] = fmaf(t0[r], c, (r & 3) == 0 ? ba.x : (r & 3) == 1 ? ba.y : (r & 3) == 2 ? ba.z : ba.w);
+    t1[r] = fmaf(t1[r], c, (r & 3) == 0 ? bb.x : (r & 3) == 1 ? bb.y : (r & 3) == 2 ? bb.z : bb.w);
+    mx = fmaxf(mx, fmaxf(t0[r], t1[r]));
+  }
+  const float back = m - mx;
+  float a = s1 * __builtin_amdgcn_exp2f(back), b = 0.f;
+  if (TWO) b = s2 * __builtin_amdgcn_exp2f(back * itau);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const float d0 = t0[r] - mx, d1 = t1[r] - mx;
+    a += __builtin_amdgcn_exp2f(d0) + __builtin_amdgcn_exp2f(d1);
+    if (TWO) b += __builtin_amdgcn_exp2f(d0 * itau) + __builtin_amdgcn_exp2f(d1 * itau);
+  }
+  m = mx; s1 = a; s2 = b;
+}
+// Join the pairs of the lanes (and of the `waves` waves) that share a row, and store them for the merge:
+// part[3][splits][nt * 128].  x: [waves][128][3] floats of LDS.
+template <int NJ, bool TWO>
+__device__ __forceinline__ void store_pairs(const DistillArgs& p, float* x, const float* m, const float* s1, const float* s2,
+                                            int split, int nt, int n0, int bn, int who, int waves, int lane) {
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    const float m2 = __shfl_xor(m[j], 32, 64), mm = fmaxf(m[j], m2);
+    const float f = __builtin_amdgcn_exp2f(m[j] - mm), f2 = __builtin_amdgcn_exp2f(m2 - mm);
+    const float a = s1[j] * f + __shfl_xor(s1[j], 32, 64) * f2;
+    float b = 0.f;
+    if (TWO) b = s2[j] * __builtin_amdgcn_exp2f((m[j] - mm) * p.itau) +
+                 __shfl_xor(s2[j], 32, 64) * __builtin_amdgcn_exp2f((m2 - mm) * p.itau);
+    if (lane < 32) {
+      float* y = x + (who * 128 + bn + 32 * j + lane) * 3;
+      y[0] = mm; y[1] = a; y[2] = b;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < 128) {
+    const float* y = x + threadIdx.x * 3;
+    float mm = y[0], a = y[1], b = y[2];
+    if (waves == 2) {
+      const float* z = y + 128 * 3;
+      const float m1 = mm;
+      mm = fmaxf(m1, z[0]);
+      a = a * __builtin_amdgcn_exp2f(m1 - mm) + z[1] * __builtin_amdgcn_exp2f(z[0] - mm);
+      if (TWO) b = b * __builtin_amdgcn_exp2f((m1 - mm) * p.itau) + z[2] * __builtin_amdgcn_exp2f((z[0] - mm) * p.itau);
+    }
+    float* out = p.part + (long)split * nt * 128 + n0 + threadIdx.x;
+    out[0] = mm;
+    out[p.pplane] = a;
+    if (TWO) out[2 * p.pplane] = b;
+  }
+}
 
 template <int NP, bool TWO>
 __global__ __launch_bounds__(256, 2) void dt_forward_kernel(DistillArgs p) {
   DT_LDS
-  const int nl = *p.nlive, nt = (nl + DT_TILE - 1) / DT_TILE, vt = p.Vp / DT_TILE;
+  const int nl = *p.nlive, nt = (nl + DT_TILE - 1) / DT_TILE, vt = p.fvt;
+  if (nt == 0) return;
   const int splits = dt_splits(nt, vt), per = (vt + splits - 1) / splits;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int am = (wave >> 1) * 64, bn = (wave & 1) * 64;
@@ -488,7 +554,7 @@ __global__ __launch_bounds__(256, 2) void dt_forward_kernel(DistillArgs p) {
   const long ld = (long)p.Kp * NP * 2;
   const int nst = (p.E + 64 / NP - 1) / (64 / NP), last = ((p.E + 15) / 16) - (nst - 1) * (4 / NP);
   const int xcd = blockIdx.x & 7, per_xcd = nt * (splits / 8);
-  for (int q = blockIdx.x >> 3; q < per_xcd; q += DT_FWD_BLOCKS / 8) {
+  for (int q = blockIdx.x >> 3; q < per_xcd; q += DT_WALK_BLOCKS / 8) {
     const int split = xcd + 8 * (q / nt), n0 = (q % nt) * DT_TILE;
     const int t0 = split * per, t1 = min(vt, t0 + per);
     using Op = Operand<NP, false, DT_TILE, 4>;
@@ -512,7 +578,6 @@ __global__ __launch_bounds__(256, 2) void dt_forward_kernel(DistillArgs p) {
           B.issue(0, fb, wave);
         }
       });
-      // fold the tile: a lane owns two rows (columns of the product) and 32 of the tile's 64 vocabulary entries
       const float* b2 = p.b2 + tile * DT_TILE + am;
       float4 bias[2][4];
 #pragma unroll
@@ -520,62 +585,201 @@ __global__ __launch_bounds__(256, 2) void dt_forward_kernel(DistillArgs p) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) bias[i][g] = *reinterpret_cast<const float4*>(b2 + 32 * i + 8 * g + 4 * (lane >> 5));
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float mx = m[j];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float4& bb = bias[i][r >> 2];
-            const float bv = (r & 3) == 0 ? bb.x : (r & 3) == 1 ? bb.y : (r & 3) == 2 ? bb.z : bb.w;
-            acc[i][j][r] = fmaf(acc[i][j][r], c, bv);
-            mx = fmaxf(mx, acc[i][j][r]);
-          }
-        const float back = m[j] - mx;
-        float a = s1[j] * __builtin_amdgcn_exp2f(back), b = 0.f;
-        if (TWO) b = s2[j] * __builtin_amdgcn_exp2f(back * p.itau);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float d = acc[i][j][r] - mx;
-            a += __builtin_amdgcn_exp2f(d);
-            if (TWO) b += __builtin_amdgcn_exp2f(d * p.itau);
-          }
-        m[j] = mx; s1[j] = a; s2[j] = b;
-      }
+      for (int j = 0; j < 2; ++j) fold<TWO>(acc[0][j], acc[1][j], bias, c, p.itau, m[j], s1[j], s2[j]);
     };
     for (int tile = t0; tile < t1; ++tile) {                      // an odd number of stages swaps the pairs
       do_tile(tile, la0, lb0, la1, lb1);
       if ((nst & 1) && tile + 1 < t1) do_tile(++tile, la1, lb1, la0, lb0);
     }
-    // join the two half-waves and the two waves that share a row, and store the split's pair
     __syncthreads();
-    float* x = reinterpret_cast<float*>(la0);                     // [2 (am)][128][3]
+    store_pairs<2, TWO>(p, reinterpret_cast<float*>(la0), m, s1, s2, split, nt, n0, bn, wave >> 1, 2, lane);
+  }
+}
+
+// The same walk for E <= 208 with the rows of X in registers: a wave holds 64 (two planes: 32) of the 128 rows, all K, as
+// MFMA operands, and only W streams through LDS -- half the LDS reads and half the copies of the general kernel, which
+// at E = 200 spends its time on them.  Stages of 64 K values x 128 (64) words, four buffers, three in flight; K blocks
+// of 16: NK = 4, 8 or 13 (E up to 64, 128, 208; every shipped model has E = 200).  GRAD: instead of folding, the tile
+// leaves as P = a 2^(t - L1) + b 2^(t / tau - L2), through 2 KiB of LDS a wave so that rows leave in runs of 64 bytes.
+template <int NP, bool TWO, bool GRAD, int NK>
+__global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
+  constexpr int NST = NK <= 4 ? 1 : NK <= 8 ? 2 : 4, VT = 128 / NP, NJ = 2 / NP, RB = 128 * NP;   // RB: bytes of a row's stage
+  __shared__ __attribute__((aligned(16))) char w0[DT_STAGE + 512];
+  __shared__ __attribute__((aligned(16))) char w1[DT_STAGE + 512];
+  __shared__ __attribute__((aligned(16))) char w2[DT_STAGE + 512];
+  __shared__ __attribute__((aligned(16))) char w3[DT_STAGE + 512];
+  __shared__ __attribute__((aligned(16))) char turn[GRAD ? 8192 : 3072];
+  const int nl = *p.nlive, nt = (nl + DT_TILE - 1) / DT_TILE, vt = GRAD ? p.vc / VT : p.fvt;
+  if (nt == 0) return;
+  const int splits = dt_splits(nt, vt), per = (vt + splits - 1) / splits;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int am = NP == 1 ? (wave >> 1) * 64 : 0, bn = NP == 1 ? (wave & 1) * 64 : wave * 32;
+  const int l31 = lane & 31, lhi = lane >> 5;
+  const float c = ldexpf(LOG2E, -(p.sexp[0] + p.sexp[1]));
+  const long ld = (long)p.Kp * NP * 2;
+  unsigned off[4];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const float m2 = __shfl_xor(m[j], 32, 64), mm = fmaxf(m[j], m2);
-      const float f = __builtin_amdgcn_exp2f(m[j] - mm), f2 = __builtin_amdgcn_exp2f(m2 - mm);
-      const float a = s1[j] * f + __shfl_xor(s1[j], 32, 64) * f2;
-      float b = 0.f;
-      if (TWO) b = s2[j] * __builtin_amdgcn_exp2f((m[j] - mm) * p.itau) +
-                   __shfl_xor(s2[j], 32, 64) * __builtin_amdgcn_exp2f((m2 - mm) * p.itau);
-      if (lane < 32) {
-        float* y = x + ((wave >> 1) * 128 + bn + 32 * j + lane) * 3;
-        y[0] = mm; y[1] = a; y[2] = b;
+  for (int i = 0; i < 4; ++i) {
+    const int piece = wave * 4 + i;
+    const int r = NP == 1 ? piece * 8 + (lane >> 3) : piece * 4 + (lane >> 4);
+    const int ch = NP == 1 ? (lane & 7) ^ (r & 7) : (lane & 15) ^ (r & 15);
+    off[i] = (unsigned)(r * ld + ch * 16);
+  }
+  const int boff = NP == 1 ? (wave & 1) * 256 : 0;                // each wave copies 64 of the tile's biases
+  const int xcd = blockIdx.x & 7, per_xcd = nt * (splits / 8);
+  for (int q = blockIdx.x >> 3; q < per_xcd; q += DT_WALK_BLOCKS / 8) {
+    const int split = xcd + 8 * (q / nt), n0 = (q % nt) * DT_TILE;
+    const int t0 = split * per, t1 = min(vt, t0 + per);
+    if (GRAD && t0 >= t1) continue;
+    float m[NJ], s1[NJ], s2[NJ];                                  // GRAD: L1, a, then L2, b
+    float La[NJ], Lb[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      m[j] = -1e30f; s1[j] = s2[j] = La[j] = Lb[j] = 0.f;
+      const int i = n0 + bn + 32 * j + l31;
+      if (GRAD && i < nl) {
+        La[j] = p.L1[i]; Lb[j] = p.L2[i];
+        s1[j] = p.coef[i]; s2[j] = p.coef[p.Np + i];
+        if (!TWO) s1[j] += s2[j];
       }
     }
-    __syncthreads();
-    if (threadIdx.x < 128) {
-      const float* y = x + threadIdx.x * 3;
-      const float* z = y + 128 * 3;
-      const float mm = fmaxf(y[0], z[0]), d = y[0] - mm, d2 = z[0] - mm;
-      float* out = p.part + (long)split * p.Np + n0 + threadIdx.x;
-      const long plane = (long)p.splits_cap * p.Np;
-      out[0] = mm;
-      out[plane] = y[1] * __builtin_amdgcn_exp2f(d) + z[1] * __builtin_amdgcn_exp2f(d2);
-      if (TWO) out[2 * plane] = y[2] * __builtin_amdgcn_exp2f(d * p.itau) + z[2] * __builtin_amdgcn_exp2f(d2 * p.itau);
+    if (t0 < t1) {
+      h8 xf[NJ][NP][NK];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int pl = 0; pl < NP; ++pl)
+#pragma unroll
+          for (int kb = 0; kb < NK; ++kb) {
+            const int k = kb * 16 + lhi * 8;
+            xf[j][pl][kb] = *reinterpret_cast<const h8*>(reinterpret_cast<const char*>(p.Ximg) + (n0 + bn + 32 * j + l31) * ld +
+                                                         (NP == 1 ? k * 2 : (k >> 5) * 128 + pl * 64 + (k & 31) * 2));
+          }
+      const char* W = reinterpret_cast<const char*>(p.Wimg) + (long)(GRAD ? p.v0 : 0) * ld;
+      const float* b2 = p.b2 + (GRAD ? p.v0 : 0);
+      const auto issue = [&](int tile, int st, char* w) {         // (past the range: its last tile again)
+        tile = tile < t1 ? tile : t1 - 1;
+        const char* b = W + (long)tile * VT * ld + st * RB;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(b + off[i]),
+                                           (__attribute__((address_space(3))) void*)(w + (wave * 4 + i) * 1024), 16, 0, 0);
+        if (st == NST - 1)
+          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(
+                                               reinterpret_cast<const char*>(b2 + tile * VT) + boff + lane * 4),
+                                           (__attribute__((address_space(3))) void*)(w + DT_STAGE + boff), 4, 0, 0);
+      };
+      const auto ring = [&](int g) -> char* { return (g & 3) == 0 ? w0 : (g & 3) == 1 ? w1 : (g & 3) == 2 ? w2 : w3; };
+#pragma unroll
+      for (int g = 0; g < 3; ++g) issue(t0 + g / NST, g % NST, ring(g));
+      for (int tile = t0; tile < t1; tile += 4 / NST) {
+#pragma unroll
+        for (int u = 0; u < 4 / NST; ++u) {
+          const int tl = tile + u;
+          if (tl >= t1) continue;
+          f32x16 acc[2][NJ];
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+#pragma unroll
+          for (int st = 0; st < NST; ++st) {
+            const int g = u * NST + st;
+            // Stages g + 1 and g + 2 stay in flight: four copies each, one more for a tile's last stage (its biases);
+            // and the 8 stores of every tile that ended within the last three steps (they count like copies, in order;
+            // at an item's first three steps there are none to count).
+            constexpr int two = 8 + (NST == 1 ? 2 : NST == 2 ? 1 : 0);
+            if (GRAD && (tl - t0) * NST + st >= 3) {
+              if (NST == 4) { if (st == 0) ring_barrier<16>(); else if (st == 3) ring_barrier<8>(); else ring_barrier<17>(); }
+              else if (NST == 2) { if (st == 0) ring_barrier<25>(); else ring_barrier<17>(); }
+              else ring_barrier<34>();
+            } else if (NST == 4 && (st == 1 || st == 2)) {
+              ring_barrier<9>();
+            } else {
+              ring_barrier<two>();
+            }
+            issue(tile + (g + 3) / NST, (g + 3) % NST, ring(g + 3));
+            const char* w = ring(g);
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+              if (st * 4 + ks >= NK) continue;
+              h8 a[2][NP];
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int pl = 0; pl < NP; ++pl) {
+                  const int r = am + 32 * i + l31;
+                  const int ch = NP == 1 ? (ks * 2 + lhi) ^ (r & 7) : ((ks >> 1) * 8 + pl * 4 + (ks & 1) * 2 + lhi) ^ (r & 15);
+                  a[i][pl] = *reinterpret_cast<const h8*>(w + r * RB + ch * 16);
+                }
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                  const int kb = st * 4 + ks;
+                  if (NP == 2) {
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], xf[j][NP - 1][kb], acc[i][j], 0, 0, 0);
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][NP - 1], xf[j][0][kb], acc[i][j], 0, 0, 0);
+                  }
+                  acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], xf[j][0][kb], acc[i][j], 0, 0, 0);
+                }
+            }
+          }
+          const float* bl = reinterpret_cast<const float*>(ring(u * NST + NST - 1) + DT_STAGE) + am;
+          float4 bias[2][4];
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) bias[i][g] = *reinterpret_cast<const float4*>(bl + 32 * i + 8 * g + 4 * lhi);
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) {
+            if (!GRAD) {
+              fold<TWO>(acc[0][j], acc[1][j], bias, c, p.itau, m[j], s1[j], s2[j]);
+              continue;
+            }
+            const bool in = n0 + bn + 32 * j + l31 < nl;
+            char* tr = turn + wave * 2048;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int v = tl * VT + am + 32 * i;                // in the range
+              char* out = reinterpret_cast<char*>(p.P) +
+                          ((long)(v * NP >> 6) * p.Np + n0 + bn + 32 * j + (lane >> 2)) * 128 + (NP == 1 ? (v & 32) * 2 : 0) + (lane & 3) * 16;
+              Packed<f16_t, 4> hi[4], lo[4];
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                const float bv[4] = {bias[i][g].x, bias[i][g].y, bias[i][g].z, bias[i][g].w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  const float t = fmaf(acc[i][j][4 * g + k], c, bv[k]);
+                  float x = s1[j] * __builtin_amdgcn_exp2f(t - La[j]);
+                  if (TWO) x = fmaf(s2[j], __builtin_amdgcn_exp2f(fmaf(t, p.itau, -Lb[j])), x);
+                  x = in ? x : 0.f;
+                  hi[g].set(k, x);
+                  if (NP == 2) lo[g].set(k, x - hi[g].f(k));
+                }
+              }
+#pragma unroll
+              for (int pl = 0; pl < NP; ++pl) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                  *reinterpret_cast<Packed<f16_t, 4>*>(tr + l31 * 64 + ((g ^ ((l31 >> 1) & 3)) << 4) + lhi * 8) = pl ? lo[g] : hi[g];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  const int r = h * 16 + (lane >> 2);
+                  const uint4 x = *reinterpret_cast<const uint4*>(tr + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
+                  *reinterpret_cast<uint4*>(out + h * 16 * 128 + pl * 64) = x;
+                }
+              }
+            }
+          }
+        }
+      }
+      ring_barrier<0>();                                          // the next item's copies go where the last ones landed
     }
+    if (!GRAD) store_pairs<NJ, TWO>(p, reinterpret_cast<float*>(turn), m, s1, s2, split, nt, n0, bn, NP == 1 ? wave >> 1 : 0, 2 / NP, lane);
+    if (!GRAD) __syncthreads();                                   // turn is read before the next item writes it
   }
 }
 
@@ -638,11 +842,11 @@ __global__ __launch_bounds__(256) void dt_combine_kernel(DistillArgs p) {
     }
   }
   // normalisers
-  const int nt = (nl + DT_TILE - 1) / DT_TILE, splits = dt_splits(nt, p.Vp / DT_TILE);
-  const long plane = (long)p.splits_cap * p.Np;
+  const int nt = (nl + DT_TILE - 1) / DT_TILE, splits = dt_splits(nt, p.fvt);
+  const long plane = p.pplane;
   float m = -1e30f, a = 0.f, b = 0.f;
   for (int s = threadIdx.x; s < splits; s += 256) {
-    const float* q = p.part + (long)s * p.Np + i;
+    const float* q = p.part + (long)s * nt * 128 + i;
     const float m2 = q[0], mm = fmaxf(m, m2);
     a = a * __builtin_amdgcn_exp2f(m - mm) + q[plane] * __builtin_amdgcn_exp2f(m2 - mm);
     if (TWO) b = b * __builtin_amdgcn_exp2f((m - mm) * p.itau) + q[2 * plane] * __builtin_amdgcn_exp2f((m2 - mm) * p.itau);
@@ -1025,20 +1229,21 @@ struct DistillPlan {
   long bytes, back_bytes;
   long hard, soft, counts, rows, inv, nlive, slive, amax, sexp, Ximg, Wimg, b2, L1, L2, some, pick, share, part;   // offsets in bytes
   long Gimg, coef, gmax, P, slab;
-  int np, Np, Vp, Kp, Kg, nb, splits_cap, rax, raw, et, etw, xsplits;
-  long vc;
+  int np, Np, Vp, Kp, Kg, nb, nk, fvt, rax, raw, et, etw, xsplits;
+  long vc, pplane;
 };
 static DistillPlan dt_plan(int dtype, long N, int E, int V, int K) {
   DistillPlan d = {};
   d.np = dtype == DT_F32 ? 2 : 1;
-  d.Np = (int)((N + 255) / 256 * 256); d.Vp = (V + 255) / 256 * 256; d.Kp = (E + 63) / 64 * 64; d.Kg = (E + 64) / 64 * 64;
+  d.Np = (int)((N + 255) / 256 * 256); d.Vp = (V + 255) / 256 * 256; d.nk = E <= 64 ? 4 : E <= 128 ? 8 : E <= 208 ? 13 : 0;
+  d.Kp = d.nk == 13 ? 256 : (E + 63) / 64 * 64; d.Kg = (E + 64) / 64 * 64;
   d.nb = cdiv(N, DT_CROWS);
   // the gradient products' tiles: 256 columns of E x 128 rows or words where E needs more than 128, else 128 x 256
   d.rax = E > 128 ? 256 : 128; d.raw = E + 1 > 128 ? 256 : 128;
   d.et = cdiv(E, d.rax); d.etw = cdiv(E + 1, d.raw);
-  const int nt = d.Np / DT_TILE, vt = d.Vp / DT_TILE;
-  d.splits_cap = 8;                                 // live tiles are 1 .. nt: fewer tiles, more splits
-  for (int t = 1; t <= (nt < 64 ? nt : 64); ++t) { const int s = dt_splits(t, vt); if (s > d.splits_cap) d.splits_cap = s; }
+  const int nt = d.Np / DT_TILE;
+  d.fvt = d.Vp / (d.nk ? DT_TILE / d.np : DT_TILE);
+  d.pplane = 8L * (nt > DT_MOST_ITEMS ? nt : DT_MOST_ITEMS) * 128;
   auto take = [](long& at, long bytes) { const long o = at; at += (bytes + 255) / 256 * 256; return o; };
   long at = 0;
   d.hard = take(at, 4 * N); d.soft = take(at, K ? 4 * N : 0);
@@ -1051,7 +1256,7 @@ static DistillPlan dt_plan(int dtype, long N, int E, int V, int K) {
   d.L1 = take(at, 4L * d.Np); d.L2 = take(at, 4L * d.Np);
   d.some = take(at, 4L * d.Np);
   d.pick = take(at, 4L * N * (K + 1)); d.share = take(at, 4L * N * (K + 1));
-  d.part = take(at, 12L * d.splits_cap * d.Np);
+  d.part = take(at, 12L * d.pplane);
   d.bytes = at;
   long vc = DT_PIECE_BYTES / (2L * d.np * d.Np) / 256 * 256;
   if (vc < 1024) vc = 1024;
@@ -1101,15 +1306,22 @@ static void dt_fill(DistillArgs& a, const DistillPlan& d, const DistillCall& c, 
   a.amax = (float*)(w + d.amax); a.sexp = (int*)(w + d.sexp); a.Ximg = (_Float16*)(w + d.Ximg); a.Wimg = (_Float16*)(w + d.Wimg); a.b2 = (float*)(w + d.b2);
   a.L1 = (float*)(w + d.L1); a.L2 = (float*)(w + d.L2); a.some = (float*)(w + d.some);
   a.pick = (float*)(w + d.pick); a.share = (float*)(w + d.share);
-  a.part = (float*)(w + d.part); a.splits_cap = d.splits_cap;
+  a.part = (float*)(w + d.part); a.pplane = d.pplane; a.fvt = d.fvt;
 }
 
+template <int NP, bool TWO, bool GRAD> static void dt_rows(int nk, const DistillArgs& a, hipStream_t s) {
+  const dim3 grid(DT_WALK_BLOCKS);
+  if (nk == 4) hipLaunchKernelGGL((dt_rows_kernel<NP, TWO, GRAD, 4>), grid, dim3(256), 0, s, a);
+  else if (nk == 8) hipLaunchKernelGGL((dt_rows_kernel<NP, TWO, GRAD, 8>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((dt_rows_kernel<NP, TWO, GRAD, 13>), grid, dim3(256), 0, s, a);
+}
 template <typename T, int NP, bool TWO> static int dt_forward(const DistillPlan& d, const DistillArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((dt_count_kernel<T>), dim3(d.nb + 2 * DT_AMAX), dim3(256), 0, s, a, d.nb);
   CVAE_LAUNCH_CHECK("dt_count_kernel");
   hipLaunchKernelGGL((dt_image_kernel<T, NP>), dim3(cdiv(a.N, 16) + d.Np / 16 + d.Vp / 16), dim3(256), 0, s, a, cdiv(a.N, 16));
   CVAE_LAUNCH_CHECK("dt_image_kernel");
-  hipLaunchKernelGGL((dt_forward_kernel<NP, TWO>), dim3(DT_FWD_BLOCKS), dim3(256), 0, s, a);
+  if (d.nk) dt_rows<NP, TWO, false>(d.nk, a, s);
+  else hipLaunchKernelGGL((dt_forward_kernel<NP, TWO>), dim3(DT_WALK_BLOCKS), dim3(256), 0, s, a);
   CVAE_LAUNCH_CHECK("dt_forward_kernel");
   hipLaunchKernelGGL((dt_combine_kernel<T, TWO>), dim3(a.N), dim3(256), 0, s, a);
   CVAE_LAUNCH_CHECK("dt_combine_kernel");
@@ -1123,7 +1335,8 @@ template <typename T, int NP, bool TWO> static int dt_backward(const DistillPlan
     a.v0 = (int)v0;
     a.vc = (int)(d.Vp - v0 < d.vc ? d.Vp - v0 : d.vc);
     const int vt = cdiv(a.vc, DT_TILE);
-    hipLaunchKernelGGL((dt_grad_kernel<NP, TWO>), dim3((unsigned)((long)cdiv(vt, 8) * 8 * nt)), dim3(256), 0, s, a);
+    if (d.nk) dt_rows<NP, TWO, true>(d.nk, a, s);
+    else hipLaunchKernelGGL((dt_grad_kernel<NP, TWO>), dim3((unsigned)((long)cdiv(vt, 8) * 8 * nt)), dim3(256), 0, s, a);
     CVAE_LAUNCH_CHECK("dt_grad_kernel");
     hipLaunchKernelGGL((dt_pick_kernel<NP, TWO>), dim3(cdiv(a.N, 4)), dim3(256), 0, s, a);
     CVAE_LAUNCH_CHECK("dt_pick_kernel");

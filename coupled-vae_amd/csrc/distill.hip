@@ -56,7 +56,7 @@ struct DistillArgs {
   _Float16* Gimg; float* coef;             // s X image with a column of s; [3][Np]: a, b, s / gmax
   float* gmax;
   _Float16* P; int v0, vc;                 // a range of the vocabulary: [vc NP / 64 pieces][Np rows][128 bytes]
-  float* slab; int xsplits;
+  float* slab; int vfull;                  // partial tiles of dX; words of a full range
   void* dX; void* dW; void* db;
 };
 
@@ -280,8 +280,8 @@ template <typename T, int NP> __global__ __launch_bounds__(256) void dt_image_ke
 // contiguous; P: row = 128, the rows of one piece are contiguous).
 //   K along the rows (KS = false): RT rows; stage s is piece s of each.
 //   K down the rows (KS = true): RT columns, that is RT NP / 64 pieces, of 64 (two planes: 32) rows a stage.
-// In LDS, 16-byte chunk c of row r sits at chunk c ^ (r & 7) of its 128 bytes (KS: c ^ 4 (r & 3)): the chunks that the
-// lanes of a read take lie in different banks.
+// In LDS, 16-byte chunk c of row r sits at chunk c ^ (r / 2 & 7) of its 128 bytes (KS: c ^ 4 (r & 3)): the chunks that
+// 16 lanes of a read take lie in different banks of the 64 (c ^ (r & 7) left two rows in each: half of all LDS cycles).
 template <int NP, bool KS, int RT, int NW> struct Operand {
   static constexpr int PI = RT / 8 / NW;                          // copies of 1 KiB a wave and stage
   static constexpr int ROW = RT * 2 * NP;                         // bytes of a K row in LDS (KS)
@@ -297,7 +297,7 @@ template <int NP, bool KS, int RT, int NW> struct Operand {
       const int piece = wave * PI + i;
       if (!KS) {
         const int r = piece * 8 + (lane >> 3);
-        off[i] = (unsigned)(r * row + (((lane & 7) ^ (r & 7)) << 4));
+        off[i] = (unsigned)(r * row + (((lane & 7) ^ ((r >> 1) & 7)) << 4));
       } else {
         constexpr int LPR = ROW / 16;                             // lanes (chunks) of a row
         const int r = piece * (64 / LPR) + lane / LPR, c = (lane % LPR) ^ ((r & 3) << 2);
@@ -316,7 +316,7 @@ template <int NP, bool KS, int RT, int NW> struct Operand {
   static __device__ __forceinline__ h8 frag(const char* lds, int c0, int ks, int pl, int lane) {
     if (!KS) {
       const int r = c0 + (lane & 31), c = (NP == 1 ? 0 : pl * 4) + ks * 2 + (lane >> 5);
-      return *reinterpret_cast<const h8*>(lds + r * 128 + ((c ^ (r & 7)) << 4));
+      return *reinterpret_cast<const h8*>(lds + r * 128 + ((c ^ ((r >> 1) & 7)) << 4));
     }
     const int k = ks * 16 + (lane >> 5) * 8 + ((lane >> 2) & 3);
     const int col = c0 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
@@ -622,7 +622,7 @@ __global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
   for (int i = 0; i < 4; ++i) {
     const int piece = wave * 4 + i;
     const int r = NP == 1 ? piece * 8 + (lane >> 3) : piece * 4 + (lane >> 4);
-    const int ch = NP == 1 ? (lane & 7) ^ (r & 7) : (lane & 15) ^ (r & 15);
+    const int ch = NP == 1 ? (lane & 7) ^ ((r >> 1) & 7) : (lane & 15) ^ (r & 15);
     off[i] = (unsigned)(r * ld + ch * 16);
   }
   const int boff = NP == 1 ? (wave & 1) * 256 : 0;                // each wave copies 64 of the tile's biases
@@ -711,7 +711,7 @@ __global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
 #pragma unroll
                 for (int pl = 0; pl < NP; ++pl) {
                   const int r = am + 32 * i + l31;
-                  const int ch = NP == 1 ? (ks * 2 + lhi) ^ (r & 7) : ((ks >> 1) * 8 + pl * 4 + (ks & 1) * 2 + lhi) ^ (r & 15);
+                  const int ch = NP == 1 ? (ks * 2 + lhi) ^ ((r >> 1) & 7) : ((ks >> 1) * 8 + pl * 4 + (ks & 1) * 2 + lhi) ^ (r & 15);
                   a[i][pl] = *reinterpret_cast<const h8*>(w + r * RB + ch * 16);
                 }
 #pragma unroll
@@ -1112,54 +1112,72 @@ __global__ __launch_bounds__(256) void dt_pick_kernel(DistillArgs p) {
   }
 }
 
-// dX: (W down its rows: K = vocabulary) x (P along its rows), tiles of RA columns of E x RB rows.  Blocks (row tile,
-// column tile, split of the range): partial tiles in accumulator order, added to what an earlier range left there.
+// Splits of the vocabulary for the dX product's tiles (known on the device alone): a block a CU, items in rounds of 256;
+// an item costs its stages and about 14 more for its partial tile's way out and back.
+constexpr int DT_DX_BLOCKS = 256, DT_DX_MOST = 1024;
+__device__ __forceinline__ int dt_dx_splits(int tiles, int stages) {
+  const int k = (threadIdx.x & 63) + 1;
+  int best = 0x7fffffff;
+  if (k == 1 || (tiles * k <= DT_DX_MOST && k * 4 <= stages))
+    best = min(((tiles * k + DT_DX_BLOCKS - 1) / DT_DX_BLOCKS) * ((stages + k - 1) / k + 14), 0x1ffffff) * 64 + (k - 1);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) best = min(best, __shfl_xor(best, o, 64));
+  return __builtin_amdgcn_readfirstlane((best & 63) + 1);
+}
+
+// dX: (W down its rows: K = vocabulary) x (P along its rows), tiles of RA columns of E x RB rows.  Items (tile, split of
+// the range): partial tiles in accumulator order, added to what an earlier range left there.
 template <int NP, int RA>
 __global__ __launch_bounds__(512, 2) void dt_dx_kernel(DistillArgs p, int et, int add) {
   constexpr int RB = 384 - RA, BK = 64 / NP;
   DT_RING(RA, RB)
-  const int nl = *p.nlive, nt = (nl + RB - 1) / RB;
-  const int split = blockIdx.x % p.xsplits, rest = blockIdx.x / p.xsplits, te = rest % et, tn = rest / et;
-  if (tn >= nt) return;
+  const int nl = *p.nlive, tiles = (nl + RB - 1) / RB * et;
+  const int splits = dt_dx_splits(tiles, p.vfull / BK);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int am = (RA == 256 ? wave >> 1 : wave & 1) * 64, bn = (RA == 256 ? wave & 1 : wave >> 1) * 64;
-  const int stages = p.vc / BK, per = (stages + p.xsplits - 1) / p.xsplits;
-  const int s0 = split * per, s1 = min(stages, s0 + per);
+  const int stages = p.vc / BK, per = (stages + splits - 1) / splits;
   const long ldw = (long)p.Kp * NP * 2;
   using OA = Operand<NP, true, RA, 8>;
   using OB = Operand<NP, false, RB, 8>;
   OA A;
   OB B;
-  A.init(reinterpret_cast<const char*>(p.Wimg) + (p.v0 + (long)s0 * BK) * ldw + (long)te * RA * 2 * NP, ldw, 128, lane, wave);
-  B.init(reinterpret_cast<const char*>(p.P) + ((long)s0 * p.Np + tn * RB) * 128, 128, (long)p.Np * 128, lane, wave);
-  f32x16 acc[2][2];
-  ring_product<NP, OA, OB>(A, B, s1 - s0, la0, lb0, la1, lb1, la2, lb2, am, bn, lane, wave, acc);
-  float4* out = reinterpret_cast<float4*>(p.slab) + (((long)split * (p.Np / RB) + tn) * et + te) * (RA * RB / 4) + wave * 1024 + lane;
+  A.init(nullptr, ldw, 128, lane, wave);
+  B.init(nullptr, 128, (long)p.Np * 128, lane, wave);
+  for (int item = blockIdx.x; item < tiles * splits; item += DT_DX_BLOCKS) {
+    const int split = item % splits, tile = item / splits, te = tile % et, tn = tile / et;
+    const int s0 = split * per, s1 = min(stages, s0 + per);
+    A.base = reinterpret_cast<const char*>(p.Wimg) + (p.v0 + (long)s0 * BK) * ldw + (long)te * RA * 2 * NP;
+    B.base = reinterpret_cast<const char*>(p.P) + ((long)s0 * p.Np + tn * RB) * 128;
+    f32x16 acc[2][2];
+    ring_product<NP, OA, OB>(A, B, s1 - s0, la0, lb0, la1, lb1, la2, lb2, am, bn, lane, wave, acc);
+    float4* out = reinterpret_cast<float4*>(p.slab) + ((long)split * tiles + tile) * (RA * RB / 4) + wave * 1024 + lane;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        float4* q = out + ((i * 2 + j) * 4 + g) * 64;
-        float4 x = make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
-        if (add) { const float4 y = *q; x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w; }
-        *q = x;
-      }
+        for (int g = 0; g < 4; ++g) {
+          float4* q = out + ((i * 2 + j) * 4 + g) * 64;
+          float4 x = make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
+          if (add) { const float4 y = *q; x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w; }
+          *q = x;
+        }
+  }
 }
-template <typename T, int RA>
+template <typename T, int NP, int RA>
 __global__ __launch_bounds__(256) void dt_dx_sum_kernel(DistillArgs p, int et) {
   constexpr int RB = 384 - RA;
-  const int nl = *p.nlive, nt = (nl + RB - 1) / RB;
+  const int nl = *p.nlive, tiles = (nl + RB - 1) / RB * et;
   const int tile = blockIdx.x >> 5;                               // 32 blocks a tile
-  if (tile / et >= nt) return;
+  if (tile >= tiles) return;
+  const int splits = dt_dx_splits(tiles, p.vfull / (64 / NP));
   const float w = ldexpf(1.f, -p.sexp[1] - P_EXP);
   const int slot = (blockIdx.x & 31) * 256 + threadIdx.x;
-  const long step = (long)(p.Np / RB) * et * (RA * RB / 4);
+  const long step = (long)tiles * (RA * RB / 4);
   const float4* q = reinterpret_cast<const float4*>(p.slab) + (long)tile * (RA * RB / 4) + slot;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int k = 0; k < p.xsplits; ++k) { const float4 y = q[k * step]; s.x += y.x; s.y += y.y; s.z += y.z; s.w += y.w; }
+  for (int k = 0; k < splits; ++k) { const float4 y = q[k * step]; s.x += y.x; s.y += y.y; s.z += y.z; s.w += y.w; }
   const int lane = slot & 63, frag = (slot >> 6) & 15, wave = slot >> 10;
   const int am = (RA == 256 ? wave >> 1 : wave & 1) * 64, bn = (RA == 256 ? wave & 1 : wave >> 1) * 64;
   const int i = (tile / et) * RB + bn + ((frag >> 2) & 1) * 32 + (lane & 31);
@@ -1229,7 +1247,7 @@ struct DistillPlan {
   long bytes, back_bytes;
   long hard, soft, counts, rows, inv, nlive, slive, amax, sexp, Ximg, Wimg, b2, L1, L2, some, pick, share, part;   // offsets in bytes
   long Gimg, coef, gmax, P, slab;
-  int np, Np, Vp, Kp, Kg, nb, nk, fvt, rax, raw, et, etw, xsplits;
+  int np, Np, Vp, Kp, Kg, nb, nk, fvt, rax, raw, et, etw;
   long vc, pplane;
 };
 static DistillPlan dt_plan(int dtype, long N, int E, int V, int K) {
@@ -1262,16 +1280,11 @@ static DistillPlan dt_plan(int dtype, long N, int E, int V, int K) {
   if (vc < 1024) vc = 1024;
   const int pieces = cdiv(d.Vp, vc);
   d.vc = ((long)d.Vp / 256 + pieces - 1) / pieces * 256;          // ranges of equal size
-  const int stages = (int)(d.vc / (64 / d.np));
-  // about 512 blocks (two rounds of one a CU); 1, 2, 4 or a multiple of 8 splits, so that an XCD (block % 8) reads one
-  // range of W
-  const int tiles = d.Np / (384 - d.rax) * d.et, want = 512 / tiles;
-  d.xsplits = want >= 8 ? want / 8 * 8 : want >= 4 ? 4 : want >= 2 ? 2 : 1;
-  while (d.xsplits > 8 && stages / d.xsplits < 6) d.xsplits -= 8;
+  const int tiles = d.Np / (384 - d.rax) * d.et;
   at = 0;
   d.Gimg = take(at, 2L * d.Np * d.Kg * d.np + slack); d.coef = take(at, 12L * d.Np); d.gmax = take(at, 4);
   d.P = take(at, 2L * d.Np * d.vc * d.np);
-  d.slab = take(at, 4L * d.xsplits * tiles * 32768);
+  d.slab = take(at, 4L * 32768 * (tiles > DT_DX_MOST ? tiles : DT_DX_MOST));
   d.back_bytes = at;
   return d;
 }
@@ -1340,7 +1353,7 @@ template <typename T, int NP, bool TWO> static int dt_backward(const DistillPlan
     CVAE_LAUNCH_CHECK("dt_grad_kernel");
     hipLaunchKernelGGL((dt_pick_kernel<NP, TWO>), dim3(cdiv(a.N, 4)), dim3(256), 0, s, a);
     CVAE_LAUNCH_CHECK("dt_pick_kernel");
-    const dim3 gx((unsigned)((long)(d.Np / (384 - d.rax)) * d.et * d.xsplits));
+    const dim3 gx(DT_DX_BLOCKS);
     if (d.rax == 256) hipLaunchKernelGGL((dt_dx_kernel<NP, 256>), gx, dim3(512), 0, s, a, d.et, v0 > 0 ? 1 : 0);
     else hipLaunchKernelGGL((dt_dx_kernel<NP, 128>), gx, dim3(512), 0, s, a, d.et, v0 > 0 ? 1 : 0);
     CVAE_LAUNCH_CHECK("dt_dx_kernel");
@@ -1350,8 +1363,8 @@ template <typename T, int NP, bool TWO> static int dt_backward(const DistillPlan
     CVAE_LAUNCH_CHECK("dt_dw_kernel");
   }
   const dim3 gs((unsigned)((long)(d.Np / (384 - d.rax)) * d.et * 32));
-  if (d.rax == 256) hipLaunchKernelGGL((dt_dx_sum_kernel<T, 256>), gs, dim3(256), 0, s, a, d.et);
-  else hipLaunchKernelGGL((dt_dx_sum_kernel<T, 128>), gs, dim3(256), 0, s, a, d.et);
+  if (d.rax == 256) hipLaunchKernelGGL((dt_dx_sum_kernel<T, NP, 256>), gs, dim3(256), 0, s, a, d.et);
+  else hipLaunchKernelGGL((dt_dx_sum_kernel<T, NP, 128>), gs, dim3(256), 0, s, a, d.et);
   CVAE_LAUNCH_CHECK("dt_dx_sum_kernel");
   return 0;
 }
@@ -1395,7 +1408,7 @@ int launch_distill_backward(const DistillCall& c, const float* ghard, const floa
   a.ghard = ghard; a.gsoft = gsoft; a.dX = dX; a.dW = dW; a.db = db;
   char* w = static_cast<char*>(ws);
   a.Gimg = (_Float16*)(w + d.Gimg); a.coef = (float*)(w + d.coef); a.gmax = (float*)(w + d.gmax);
-  a.P = (_Float16*)(w + d.P); a.slab = (float*)(w + d.slab); a.xsplits = d.xsplits;
+  a.P = (_Float16*)(w + d.P); a.slab = (float*)(w + d.slab); a.vfull = (int)d.vc;
   return dt_dispatch(c.dtype, d, a, true, s);
 }
 

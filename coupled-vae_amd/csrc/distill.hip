@@ -50,7 +50,8 @@ struct DistillArgs {
   _Float16* Ximg; _Float16* Wimg; float* b2;
   float* L1; float* L2; float* some;       // by live row: normalisers (base 2), 1 where the teacher lists anything
   float* pick; float* share;               // picked logits (base 2) and the teacher's share of them, [K + 1]
-  float* part; long pplane; int fvt;       // [3][splits][tiles of live rows][128]; floats of one; vocabulary tiles of the walk
+  float* part; long pplane;                // [3][splits][tiles of live rows][128]; floats of one
+  int fvt, least;                          // vocabulary tiles of the forward walk, ranges an XCD takes at least
   // backward
   const float* ghard; const float* gsoft;  // [R]
   _Float16* Gimg; float* coef;             // s X image with a column of s; [3][Np]: a, b, s / gmax
@@ -468,17 +469,26 @@ __device__ __forceinline__ int acc_row(int r, int lane) { return (r & 3) + 8 * (
 // ------------------------------------------------------------------------------------------------- forward
 // Work items of the kernels that walk the vocabulary: (tile of 128 live rows) x (range of its vt tiles).  512 blocks, two
 // on a CU; the 64 of an XCD (block % 8) take every eighth range, so that they share W's tiles in its L2.  The number of
-// ranges, 8 k, is what the live rows (known on the device alone) make cheapest: rounds of 64 items times the tiles of an
-// item, and one tile's time for its start.  One wave's lanes try one k each; every kernel that needs it gets the same.
+// ranges, 8 k with k >= least, is what the live rows (known on the device alone) make cheapest: rounds of 64 items times the
+// tiles of an item, and one tile's time for its start.  One wave's lanes try one k each; every kernel that needs it gets the same.
 constexpr int DT_WALK_BLOCKS = 512, DT_MOST_ITEMS = 1024;         // the latter: per XCD, for more than one range
-__device__ __forceinline__ int dt_splits(int nt, int vt) {
+__device__ __forceinline__ int dt_splits(int nt, int vt, int least) {
   const int k = (threadIdx.x & 63) + 1;
-  const bool ok = k == 1 || (k * 8 <= vt && nt * k <= DT_MOST_ITEMS);
+  const bool ok = k == 1 || (k * 8 <= vt && nt * k <= DT_MOST_ITEMS && k >= least);
   int best = 0x7fffffff;
   if (ok) best = min(((nt * k + 63) / 64) * ((vt + 8 * k - 1) / (8 * k) + 1), 0x1ffffff) * 64 + (k - 1);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) best = min(best, __shfl_xor(best, o, 64));
   return __builtin_amdgcn_readfirstlane(((best & 63) + 1) * 8);
+}
+
+// An XCD's item q of (row tile, range of W): eight row tiles at a time over all its ranges, so that the rows that are
+// walked at once (8 x 128 x K) stay in its L2 beside the tiles of W (E = 1024, V = 50000, with at least 8 ranges: 469 us,
+// all 29 row tiles at once: 504).
+__device__ __forceinline__ void walk_order(int q, int nt, int ranges, int& tn, int& range) {
+  const int group = q / (8 * ranges), rem = q - group * 8 * ranges, size = min(8, nt - 8 * group);
+  range = rem / size;
+  tn = group * 8 + rem - range * size;
 }
 
 // Fold 64 vocabulary entries of a lane's row into its running (max, sum) pairs, base 2: two accumulator tiles of 32
@@ -546,7 +556,7 @@ __global__ __launch_bounds__(256, 2) void dt_forward_kernel(DistillArgs p) {
   DT_LDS
   const int nl = *p.nlive, nt = (nl + DT_TILE - 1) / DT_TILE, vt = p.fvt;
   if (nt == 0) return;
-  const int splits = dt_splits(nt, vt), per = (vt + splits - 1) / splits;
+  const int splits = dt_splits(nt, vt, p.least), per = (vt + splits - 1) / splits;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int am = (wave >> 1) * 64, bn = (wave & 1) * 64;
   const int e = p.sexp[0] + p.sexp[1];
@@ -555,7 +565,9 @@ __global__ __launch_bounds__(256, 2) void dt_forward_kernel(DistillArgs p) {
   const int nst = (p.E + 64 / NP - 1) / (64 / NP), last = ((p.E + 15) / 16) - (nst - 1) * (4 / NP);
   const int xcd = blockIdx.x & 7, per_xcd = nt * (splits / 8);
   for (int q = blockIdx.x >> 3; q < per_xcd; q += DT_WALK_BLOCKS / 8) {
-    const int split = xcd + 8 * (q / nt), n0 = (q % nt) * DT_TILE;
+    int tn, range;
+    walk_order(q, nt, splits / 8, tn, range);
+    const int split = xcd + 8 * range, n0 = tn * DT_TILE;
     const int t0 = split * per, t1 = min(vt, t0 + per);
     using Op = Operand<NP, false, DT_TILE, 4>;
     Op A, B;
@@ -611,7 +623,7 @@ __global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
   __shared__ __attribute__((aligned(16))) char turn[GRAD ? 8192 : 3072];
   const int nl = *p.nlive, nt = (nl + DT_TILE - 1) / DT_TILE, vt = GRAD ? p.vc / VT : p.fvt;
   if (nt == 0) return;
-  const int splits = dt_splits(nt, vt), per = (vt + splits - 1) / splits;
+  const int splits = dt_splits(nt, vt, 1), per = (vt + splits - 1) / splits;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int am = NP == 1 ? (wave >> 1) * 64 : 0, bn = NP == 1 ? (wave & 1) * 64 : wave * 32;
   const int l31 = lane & 31, lhi = lane >> 5;
@@ -842,7 +854,7 @@ __global__ __launch_bounds__(256) void dt_combine_kernel(DistillArgs p) {
     }
   }
   // normalisers
-  const int nt = (nl + DT_TILE - 1) / DT_TILE, splits = dt_splits(nt, p.fvt);
+  const int nt = (nl + DT_TILE - 1) / DT_TILE, splits = dt_splits(nt, p.fvt, p.least);
   const long plane = p.pplane;
   float m = -1e30f, a = 0.f, b = 0.f;
   for (int s = threadIdx.x; s < splits; s += 256) {
@@ -1028,9 +1040,13 @@ __global__ __launch_bounds__(256, 2) void dt_grad_kernel(DistillArgs p) {
   DT_LDS
   const int nl = *p.nlive, nt = (nl + DT_TILE - 1) / DT_TILE, vt = (p.vc + DT_TILE - 1) / DT_TILE;
   // block -> (vocabulary tile, row tile): an XCD walks its own range of W, all row tiles of one tile of W in turn
-  const int pv = (vt + 7) / 8, j0 = blockIdx.x >> 3, tv = (blockIdx.x & 7) * pv + (nt > 0 ? j0 / nt : 0);
-  if (nt == 0 || j0 / nt >= pv || tv >= vt) return;
-  const int n0 = (j0 % nt) * DT_TILE, w0 = p.v0 + tv * DT_TILE;
+  const int pv = (vt + 7) / 8, j0 = blockIdx.x >> 3;
+  if (j0 >= nt * pv) return;
+  int tn, tv;
+  walk_order(j0, nt, pv, tn, tv);
+  tv += (blockIdx.x & 7) * pv;
+  if (tv >= vt) return;
+  const int n0 = tn * DT_TILE, w0 = p.v0 + tv * DT_TILE;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int am = (wave >> 1) * 64, bn = (wave & 1) * 64;
   const long ld = (long)p.Kp * NP * 2;
@@ -1256,8 +1272,9 @@ static DistillPlan dt_plan(int dtype, long N, int E, int V, int K) {
   d.Np = (int)((N + 255) / 256 * 256); d.Vp = (V + 255) / 256 * 256; d.nk = E <= 64 ? 4 : E <= 128 ? 8 : E <= 208 ? 13 : 0;
   d.Kp = d.nk == 13 ? 256 : (E + 63) / 64 * 64; d.Kg = (E + 64) / 64 * 64;
   d.nb = cdiv(N, DT_CROWS);
-  // the gradient products' tiles: 256 columns of E x 128 rows or words where E needs more than 128, else 128 x 256
-  d.rax = E > 128 ? 256 : 128; d.raw = E + 1 > 128 ? 256 : 128;
+  // the gradient products' tiles, 256 columns of E x 128 rows or words or 128 x 256: what pads E less
+  d.rax = (E + 255) / 256 * 256 == (E + 127) / 128 * 128 ? 256 : 128;
+  d.raw = (E + 256) / 256 * 256 == (E + 128) / 128 * 128 ? 256 : 128;
   d.et = cdiv(E, d.rax); d.etw = cdiv(E + 1, d.raw);
   const int nt = d.Np / DT_TILE;
   d.fvt = d.Vp / (d.nk ? DT_TILE / d.np : DT_TILE);
@@ -1319,7 +1336,7 @@ static void dt_fill(DistillArgs& a, const DistillPlan& d, const DistillCall& c, 
   a.amax = (float*)(w + d.amax); a.sexp = (int*)(w + d.sexp); a.Ximg = (_Float16*)(w + d.Ximg); a.Wimg = (_Float16*)(w + d.Wimg); a.b2 = (float*)(w + d.b2);
   a.L1 = (float*)(w + d.L1); a.L2 = (float*)(w + d.L2); a.some = (float*)(w + d.some);
   a.pick = (float*)(w + d.pick); a.share = (float*)(w + d.share);
-  a.part = (float*)(w + d.part); a.pplane = d.pplane; a.fvt = d.fvt;
+  a.part = (float*)(w + d.part); a.pplane = d.pplane; a.fvt = d.fvt; a.least = d.nk ? 1 : 8;
 }
 
 template <int NP, bool TWO, bool GRAD> static void dt_rows(int nk, const DistillArgs& a, hipStream_t s) {

@@ -647,7 +647,8 @@ __global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
     float La[NJ], Lb[NJ];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-      m[j] = -1e30f; s1[j] = s2[j] = La[j] = Lb[j] = 0.f;
+      m[j] = -1e30f; s1[j] = s2[j] = 0.f;
+      La[j] = Lb[j] = INFINITY;                                   // rows past the last live one: 0 * 2^-inf
       const int i = n0 + bn + 32 * j + l31;
       if (GRAD && i < nl) {
         La[j] = p.L1[i]; Lb[j] = p.L2[i];
@@ -751,7 +752,6 @@ __global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
               fold<TWO>(acc[0][j], acc[1][j], bias, c, p.itau, m[j], s1[j], s2[j]);
               continue;
             }
-            const bool in = n0 + bn + 32 * j + l31 < nl;
             char* tr = turn + wave * 2048;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -767,7 +767,6 @@ __global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
                   const float t = fmaf(acc[i][j][4 * g + k], c, bv[k]);
                   float x = s1[j] * __builtin_amdgcn_exp2f(t - La[j]);
                   if (TWO) x = fmaf(s2[j], __builtin_amdgcn_exp2f(fmaf(t, p.itau, -Lb[j])), x);
-                  x = in ? x : 0.f;
                   hi[g].set(k, x);
                   if (NP == 2) lo[g].set(k, x - hi[g].f(k));
                 }
@@ -795,74 +794,92 @@ __global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
   }
 }
 
-// One block per live row: merge the splits, form the picked logits (16 lanes a dot product), the teacher's distribution
-// and the two losses.
+// sum over the 32 lanes of a half-wave: four steps inside rows of 16 lanes on the vector ALU, one through LDS
+__device__ __forceinline__ float half_sum(float v) {
+  const auto step = [](float x, int y) { return x + __builtin_bit_cast(float, y); };
+  v = step(v, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, true));    // lane ^ 1
+  v = step(v, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, true));    // lane ^ 2
+  v = step(v, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x141, 0xF, 0xF, true));   // mirrored within 8
+  v = step(v, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x140, 0xF, 0xF, true));   // mirrored within 16
+  return v + __shfl_xor(v, 16, 64);
+}
+
+// One block per live row: the picked logits, the merge of the walk's pairs, the teacher's distribution, the two losses,
+// and the teacher's shares as the backward pass wants them.  A row is one chain of dependent loads, so everything that
+// does not wait for another load is asked for at once: the ids and teacher logits first.  (Two picked rows of W in flight
+// a group of lanes: with 64 entries a row 49 us for 4815 rows, four 54, eight 74.)
+constexpr int DT_MOST_K = 1024;
 template <typename T, bool TWO>
 __global__ __launch_bounds__(256) void dt_combine_kernel(DistillArgs p) {
+  __shared__ float red[4][3];
+  __shared__ int sid[DT_MOST_K + 1];                              // ids inside the vocabulary, else -1; [K]: the target
+  __shared__ float slog[DT_MOST_K], spick[DT_MOST_K + 1];
   const int i = blockIdx.x;
   const int nl = *p.nlive;
   if (i >= nl) return;
-  __shared__ float red[4][3];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int n = p.rows[i], r = n % p.R;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, K = p.K;
+  const int n = p.rows[i];
   const long at = position(p, n);
-  const int64_t* ids = p.K ? p.ids + at * p.K : nullptr;
-  const float* top = p.K ? p.top + at * p.K : nullptr;
-  const int64_t tg = p.eos[at];
-  float* pick = p.pick + (long)i * (p.K + 1);
-  // Picked logits, base 2: 32 lanes a dot product, four of them in flight.  16 bytes a lane where rows allow it (a W row
-  // of E = 200 in 16 bits is then one access), else single elements.
-  const T* x = static_cast<const T*>(p.X) + (long)n * p.E;
-  const T* W = static_cast<const T*>(p.W);
-  constexpr int VN = 16 / sizeof(T);
-  const bool vec = p.E % VN == 0 && (((uintptr_t)p.X | (uintptr_t)p.W) & 15) == 0;
-  const int l32 = threadIdx.x & 31;
-  for (int k0 = threadIdx.x >> 5; k0 <= p.K; k0 += 32) {
-    int64_t id[4];
-    float dot[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int k = k0 + 8 * q;
-      id[q] = k < p.K ? ids[k] : k == p.K ? tg : -1;
-      if (id[q] < 0 || id[q] >= p.V) id[q] = -1;
-      dot[q] = 0.f;
-    }
-    if (vec) {
-      for (int e = l32 * VN; e < p.E; e += 32 * VN) {
-        const Packed<T, VN> a = *reinterpret_cast<const Packed<T, VN>*>(x + e);
-        Packed<T, VN> w[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) w[q] = *reinterpret_cast<const Packed<T, VN>*>(W + (id[q] < 0 ? 0 : id[q]) * p.E + e);
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int j = 0; j < VN; ++j) dot[q] = fmaf(a.f(j), w[q].f(j), dot[q]);
-      }
-    } else {
-      for (int e = l32; e < p.E; e += 32) {
-        const float a = (float)x[e];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) dot[q] = fmaf(a, (float)W[(id[q] < 0 ? 0 : id[q]) * p.E + e], dot[q]);
-      }
-    }
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) dot[q] += __shfl_xor(dot[q], o, 64);
-      if (l32 == 0 && k0 + 8 * q <= p.K)
-        pick[k0 + 8 * q] = id[q] >= 0 ? (dot[q] + (float)static_cast<const T*>(p.bias)[id[q]]) * LOG2E : 0.f;
-    }
+  for (int k = threadIdx.x; k <= K; k += 256) {
+    const int64_t id = k < K ? p.ids[at * K + k] : p.eos[at];
+    sid[k] = id >= 0 && id < p.V ? (int)id : -1;
+    if (k < K) slog[k] = p.top[at * K + k];
   }
-  // normalisers
+  // normalisers: every thread a share of the walk's ranges
   const int nt = (nl + DT_TILE - 1) / DT_TILE, splits = dt_splits(nt, p.fvt, p.least);
-  const long plane = p.pplane;
   float m = -1e30f, a = 0.f, b = 0.f;
   for (int s = threadIdx.x; s < splits; s += 256) {
     const float* q = p.part + (long)s * nt * 128 + i;
     const float m2 = q[0], mm = fmaxf(m, m2);
-    a = a * __builtin_amdgcn_exp2f(m - mm) + q[plane] * __builtin_amdgcn_exp2f(m2 - mm);
-    if (TWO) b = b * __builtin_amdgcn_exp2f((m - mm) * p.itau) + q[2 * plane] * __builtin_amdgcn_exp2f((m2 - mm) * p.itau);
+    a = a * __builtin_amdgcn_exp2f(m - mm) + q[p.pplane] * __builtin_amdgcn_exp2f(m2 - mm);
+    if (TWO) b = b * __builtin_amdgcn_exp2f((m - mm) * p.itau) + q[2 * p.pplane] * __builtin_amdgcn_exp2f((m2 - mm) * p.itau);
     m = mm;
+  }
+  __syncthreads();
+  // Picked logits, base 2: 32 lanes a dot product, 16 bytes a lane where rows allow it (a row of E = 200 in 16 bits is
+  // then one access), else single elements.
+  const T* x = static_cast<const T*>(p.X) + (long)n * p.E;
+  const T* W = static_cast<const T*>(p.W);
+  constexpr int VN = 16 / sizeof(T), FLY = 2;
+  const bool vec = p.E % VN == 0 && (((uintptr_t)p.X | (uintptr_t)p.W) & 15) == 0;
+  const int l32 = threadIdx.x & 31;
+  for (int k0 = threadIdx.x >> 5; k0 <= K; k0 += 8 * FLY) {
+    int id[FLY];
+    float dot[FLY];
+#pragma unroll
+    for (int q = 0; q < FLY; ++q) {
+      id[q] = k0 + 8 * q <= K ? sid[k0 + 8 * q] : -1;
+      dot[q] = 0.f;
+    }
+    if (vec) {
+      for (int e = l32 * VN; e < p.E; e += 32 * VN) {
+        const Packed<T, VN> r = *reinterpret_cast<const Packed<T, VN>*>(x + e);
+        Packed<T, VN> w[FLY];
+#pragma unroll
+        for (int q = 0; q < FLY; ++q)
+          w[q] = *reinterpret_cast<const Packed<T, VN>*>(W + (long)max(id[q], 0) * p.E + e);
+#pragma unroll
+        for (int q = 0; q < FLY; ++q)
+#pragma unroll
+            for (int j = 0; j < VN; ++j) dot[q] = fmaf(r.f(j), w[q].f(j), dot[q]);
+      }
+    } else {
+      for (int e = l32; e < p.E; e += 32) {
+        const float r = (float)x[e];
+#pragma unroll
+        for (int q = 0; q < FLY; ++q)
+          dot[q] = fmaf(r, (float)W[(long)max(id[q], 0) * p.E + e], dot[q]);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < FLY; ++q) {
+      dot[q] = half_sum(dot[q]);
+      if (l32 == 0 && k0 + 8 * q <= K) {
+        const float v = id[q] >= 0 ? (dot[q] + (float)static_cast<const T*>(p.bias)[id[q]]) * LOG2E : 0.f;
+        spick[k0 + 8 * q] = v;
+        p.pick[(long)i * (K + 1) + k0 + 8 * q] = v;
+      }
+    }
   }
   {
     const float mm = wave_max(m);
@@ -870,8 +887,7 @@ __global__ __launch_bounds__(256) void dt_combine_kernel(DistillArgs p) {
     if (TWO) b = wave_sum(b * __builtin_amdgcn_exp2f((m - mm) * p.itau));
     if (lane == 0) { red[wave][0] = mm; red[wave][1] = a; red[wave][2] = b; }
   }
-  __threadfence_block();
-  __syncthreads();                                                // also: pick[] is written
+  __syncthreads();
   if (wave != 0) return;
   m = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
   a = b = 0.f;
@@ -882,76 +898,52 @@ __global__ __launch_bounds__(256) void dt_combine_kernel(DistillArgs p) {
     if (TWO) b += red[w][2] * __builtin_amdgcn_exp2f(d * p.itau);
   }
   const float L1 = m + log2f(a), L2 = TWO ? fmaf(m, p.itau, log2f(b)) : L1;
+  float tm = -INFINITY;
+  bool bad = false;                                               // a NaN among the teacher's logits
+  for (int k = lane; k < K; k += 64)
+    if (sid[k] >= 0) { tm = fmaxf(tm, slog[k]); bad |= slog[k] != slog[k]; }
+  tm = wave_max(tm);
+  if (__any(bad)) tm = NAN;
+  const bool some = tm != -INFINITY;
   if (lane == 0) {
     p.L1[i] = L1;
     p.L2[i] = L2;
-    p.slive[r] = 1;
-    p.hard[n] = (L1 - pick[p.K]) * LN2;
+    p.slive[n % p.R] = 1;
+    p.hard[n] = (L1 - spick[K]) * LN2;
+    p.some[i] = K == 0 || !some ? 0.f : tm != tm ? NAN : 1.f;
   }
-  float* share = p.share + (long)i * (p.K + 1);
-  if (!p.K) {
-    if (lane == 0) { share[0] = 0.f; p.some[i] = 0.f; }
-    return;
-  }
-  float tm = -INFINITY;
-  bool bad = false;                                               // a NaN among the teacher's logits
-  for (int k = lane; k < p.K; k += 64) {
-    const int64_t id = ids[k];
-    if (id >= 0 && id < p.V) { tm = fmaxf(tm, top[k]); bad |= top[k] != top[k]; }
-  }
-  tm = wave_max(tm);
-  if (__any(bad)) tm = NAN;
+  float* share = p.share + (long)i * (K + 1);
   float sum = 0.f;
-  if (tm != -INFINITY)
-    for (int k = lane; k < p.K; k += 64) {
-      const int64_t id = ids[k];
-      if (id >= 0 && id < p.V) sum += __builtin_amdgcn_exp2f((top[k] - tm) * p.itau * LOG2E);
-    }
+  for (int k = lane; k < K; k += 64)
+    if (some && sid[k] >= 0) sum += __builtin_amdgcn_exp2f((slog[k] - tm) * p.itau * LOG2E);
   sum = wave_sum(sum);
   const float lsum = log2f(sum), inv = 1.0f / sum;
   float loss = 0.f;
-  const auto prob = [&](int k) { return __builtin_amdgcn_exp2f((top[k] - tm) * p.itau * LOG2E) * inv; };
   bool listed = false;
-  for (int k = lane; k < p.K; k += 64) {
-    const int64_t id = ids[k];
-    const bool in = id >= 0 && id < p.V, some = tm != -INFINITY;
-    if (in && some) {
-      const float lp = (top[k] - tm) * p.itau * LOG2E, pk = prob(k);
-      if (pk != 0.f) loss += pk * (lp - lsum - (pick[k] * p.itau - L2));
-    }
-    listed |= id == tg;
+  for (int k = lane; k < K; k += 64) {
+    const float lp = (slog[k] - tm) * p.itau * LOG2E, pk = some && sid[k] >= 0 ? __builtin_amdgcn_exp2f(lp) * inv : 0.f;
+    if (pk != 0.f) loss += pk * (lp - lsum - (spick[k] * p.itau - L2));
+    listed |= sid[k] >= 0 && sid[k] == sid[K];
+    slog[k] = pk;                                                 // (its own lane's entry) from here on: p_k
   }
+  loss = wave_sum(loss);
+  if (lane == 0 && K) p.soft[n] = p.tau * p.tau * LN2 * loss;
+  const bool tgt_listed = __any(listed);
+  if (lane == 0) share[K] = tgt_listed ? -1.f : 0.f;
   // an id listed several times is one entry of the gradient: its first place holds the sum of the shares, the others -1
   // (as does the target's own place, K, if the teacher lists it)
-  const int ne = (p.K + 63) / 64;
-  for (int c = 0; c < ne; ++c) {
-    const int k = c * 64 + lane;
-    const int64_t id = k < p.K ? ids[k] : -1;
-    const bool in = id >= 0 && id < p.V;
-    float sum2 = 0.f;
-    bool first = true;
-    for (int d = 0; d < ne; ++d) {
-      const int kq = d * 64 + lane;
-      const int64_t idq = kq < p.K ? ids[kq] : -1;
-      const float pq = (idq >= 0 && idq < p.V && tm != -INFINITY) ? prob(kq) : 0.f;
-      for (int q = 0; q < 64 && d * 64 + q < p.K; ++q) {
-        const int iq = __builtin_amdgcn_readlane((int)idq, q);    // ids inside the vocabulary fit 31 bits
-        const float sq = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, pq), q));
-        const int hq = __builtin_amdgcn_readlane((int)(idq >> 32), q);
-        if (in && hq == 0 && iq == (int)id) {
-          sum2 += sq;
-          if (d * 64 + q < k) first = false;
-        }
+  __builtin_amdgcn_wave_barrier();
+  for (int k = lane; k < K; k += 64) {
+    const int id = sid[k];
+    float all = 0.f;
+    bool first = id >= 0;
+    for (int q = 0; q < K; ++q)
+      if (sid[q] == id) {
+        all += slog[q];
+        if (q < k) first = false;
       }
-    }
-    if (k < p.K) share[k] = in && first ? sum2 : -1.f;
+    share[k] = first ? all : -1.f;
   }
-  const bool tgt_listed = __any(listed);
-  if (lane == 0) share[p.K] = tgt_listed ? -1.f : 0.f;
-  const float some = bad || tm != tm ? NAN : tm != -INFINITY ? 1.f : 0.f;
-  if (lane == 0) p.some[i] = some;
-  loss = wave_sum(loss);
-  if (lane == 0) p.soft[n] = p.tau * p.tau * LN2 * loss;
 }
 
 // a wave per sentence: out[r] = sum over t, of the hard rows and (blockIdx.y = 1) the soft ones
@@ -1306,7 +1298,7 @@ static DistillPlan dt_plan(int dtype, long N, int E, int V, int K) {
   return d;
 }
 static bool dt_sizes_ok(long N, long E, long V, long K) {
-  return N < (1L << 30) && E > 0 && E <= 65536 && V > 0 && V < (1L << 30) && K >= 0 && K <= V && K <= 65536;
+  return N < (1L << 30) && E > 0 && E <= 65536 && V > 0 && V < (1L << 30) && K >= 0 && K <= V && K <= DT_MOST_K;
 }
 // 0 where there are no rows, or for sizes that the calls refuse
 long distill_workspace_floats(int dtype, long N, long E, long V, long K) {

@@ -680,16 +680,16 @@ def _proj_check(final, W, b, eos):
 
 def proj_distill(final, W, b, eos, pad, teacher_ids, teacher_logits, tau):
     """Cross-entropy and distillation of one student projection, logits never stored: final (T,R,E), W (V,E), b (V,) in
-    fp32, bf16 or fp16; eos (B,T) int64 targets (rows at `pad` count nothing), R % B == 0; the teacher's K best of every
-    position: teacher_ids (B,T,K) int64, teacher_logits (B,T,K) float (ids outside the vocabulary and logits of -inf are
+    fp32, bf16 or fp16; eos (B,T) int64 targets (rows at `pad` count nothing), R % B == 0; the teacher's K <= 1024 best of
+    every position: teacher_ids (B,T,K) int64, teacher_logits (B,T,K) float (ids outside the vocabulary and logits of -inf are
     absent entries).  With p = softmax(teacher_logits / tau) over the K entries and q_tau = softmax(logits / tau) over
     the whole vocabulary:
       hard (R,) = sum_t -log softmax(logits)[target],   soft (R,) = sum_t tau^2 KL(p || q_tau)
     -> (hard, soft) fp32, differentiable in final, W and b."""
     _proj_check(final, W, b, eos)
     _need(teacher_ids.dim() == 3 and teacher_ids.dtype == torch.int64 and
-          tuple(teacher_ids.shape[:2]) == tuple(eos.shape) and 0 < teacher_ids.shape[2] <= W.shape[0],
-          'teacher_ids must be int64 (B,T,K) with 0 < K <= V')
+          tuple(teacher_ids.shape[:2]) == tuple(eos.shape) and 0 < teacher_ids.shape[2] <= min(W.shape[0], 1024),
+          'teacher_ids must be int64 (B,T,K) with 0 < K <= min(V, 1024)')
     _need(teacher_logits.shape == teacher_ids.shape and teacher_logits.is_floating_point(),
           'teacher_logits must be a float tensor of the shape of teacher_ids')
     _need(0.0 < tau < 1e6, 'tau must be positive')

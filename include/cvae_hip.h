@@ -269,7 +269,7 @@ int cvae_projce_backward_saved_n(int nd, const float* const* final, const float*
  * are fp32.  final[T*R,E] (rows n = t*R + r), W[V,E], b[V], eos[B,T] targets: row r reads sentence r % B, or r / (R / B)
  * if sentence_major (R % B == 0).  Rows whose target is `pad` have no loss and no gradient; a target outside [0,V) that
  * is not `pad` counts as a logit of 0 (as in cvae_projce_*).
- * K >= 0 entries of the teacher at every position: ids[B,T,K], top[B,T,K]; an entry whose id is outside [0,V) or whose
+ * 0 <= K <= min(V, 1024) entries of the teacher at every position: ids[B,T,K], top[B,T,K]; an entry whose id is outside [0,V) or whose
  * logit is -inf is absent, a row with no entry has soft = 0; an id may be listed twice.  K = 0: ids, top, soft (and
  * gsoft) are not read and tau is ignored.
  * -> hard[R], soft[R]: sums over t.  ws: cvae_distill_workspace(dtype, T*R, E, V, K) floats, 16-byte aligned; the backward

@@ -166,7 +166,7 @@ def compare(dev, a, tau, **kw):
 # more than one tile of rows; more splits than tiles
 SIZES = [(1, 1, 1, 1, 1, 1), (3, 2, 2, 8, 5, 5), (7, 5, 5, 75, 1003, 5), (4, 3, 3, 63, 127, 2), (4, 3, 3, 64, 128, 16),
          (5, 2, 2, 127, 129, 3), (2, 4, 2, 128, 300, 7), (3, 3, 3, 200, 513, 33), (11, 14, 7, 37, 260, 64),
-         (30, 12, 12, 201, 1500, 4), (2, 1, 1, 513, 400, 9)]
+         (30, 12, 12, 201, 1500, 4), (2, 1, 1, 513, 400, 9), (3, 2, 2, 24, 1030, 1024), (2, 2, 2, 300, 640, 130)]
 
 
 @pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])

@@ -27,6 +27,7 @@ def good():
     ('teacher_ids', dict(teacher_ids=torch.zeros(T, B, K, dtype=torch.int64))),
     ('teacher_ids', dict(teacher_ids=torch.zeros(B, T, V + 1, dtype=torch.int64))),
     ('teacher_ids', dict(teacher_ids=torch.zeros(B, T, 0, dtype=torch.int64))),
+    ('teacher_ids', dict(W=torch.zeros(2000, E), b=torch.zeros(2000), teacher_ids=torch.zeros(B, T, 1025, dtype=torch.int64))),
     ('teacher_logits', dict(teacher_logits=torch.zeros(B, T, K + 1))),
     ('teacher_logits', dict(teacher_logits=torch.zeros(B, T, K, dtype=torch.int64))),
     ('tau', dict(tau=0.0)), ('tau', dict(tau=-1.0)), ('tau', dict(tau=float('nan'))), ('tau', dict(tau=float('inf'))),
@@ -70,7 +71,7 @@ def test_c_entries_refuse_bad_arguments():
                   one, one, a['tau'], one, one, one, one, one, one, a['ws'], None)
     for f in (forward, backward):
         for bad in (dict(dtype=3), dict(B=0), dict(R=3), dict(T=-1), dict(T=1 << 20, R=1 << 12), dict(E=0), dict(V=0),
-                    dict(V=1 << 31), dict(K=-1), dict(K=11), dict(tau=0.0), dict(tau=float('nan')), dict(ws=None), dict(ws=24)):
+                    dict(V=1 << 31), dict(K=-1), dict(K=11), dict(K=1025, V=2000), dict(tau=0.0), dict(tau=float('nan')), dict(ws=None), dict(ws=24)):
             with pytest.raises(_lib.CvaeHipError, match='distill_'):
                 f(**bad)
     with pytest.raises(_lib.CvaeHipError, match='rows'):

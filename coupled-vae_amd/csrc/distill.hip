@@ -279,12 +279,13 @@ template <typename T, int NP> __global__ __launch_bounds__(256) void dt_image_ke
 // One operand's tile of RT rows / columns, copied to LDS by NW waves.  Memory holds 128-byte pieces: `row` bytes from a
 // row's piece to the next row's, `grp` bytes from a piece to the next one of the same row (images: grp = 128, a row is
 // contiguous; P: row = 128, the rows of one piece are contiguous).
-//   K along the rows (KS = false): RT rows; stage s is piece s of each.
-//   K down the rows (KS = true): RT columns, that is RT NP / 64 pieces, of 64 (two planes: 32) rows a stage.
+//   K along the rows (KS = false): RT rows; stage s is piece s of each, KR = 64 / NP values.
+//   K down the rows (KS = true): RT columns, that is RT NP / 64 pieces, of KR rows a stage.
 // In LDS, 16-byte chunk c of row r sits at chunk c ^ (r / 2 & 7) of its 128 bytes (KS: c ^ 4 (r & 3)): the chunks that
 // 16 lanes of a read take lie in different banks of the 64 (c ^ (r & 7) left two rows in each: half of all LDS cycles).
-template <int NP, bool KS, int RT, int NW> struct Operand {
-  static constexpr int PI = RT / 8 / NW;                          // copies of 1 KiB a wave and stage
+template <int NP, bool KS, int RT, int NW, int KR = 64 / NP> struct Operand {
+  static constexpr int PLANES = NP, KB = KR / 16;                 // K blocks of 16 in a stage
+  static constexpr int PI = RT * 2 * NP * KR / 1024 / NW;         // copies of 1 KiB a wave and stage
   static constexpr int ROW = RT * 2 * NP;                         // bytes of a K row in LDS (KS)
   const char* base;
   long row, grp;
@@ -307,7 +308,7 @@ template <int NP, bool KS, int RT, int NW> struct Operand {
     }
   }
   __device__ __forceinline__ void issue(int stage, char* lds, int wave) const {
-    const char* b = base + (KS ? (long)stage * (64 / NP) * row : (long)stage * grp);
+    const char* b = base + (KS ? (long)stage * KR * row : (long)stage * grp);
 #pragma unroll
     for (int i = 0; i < PI; ++i)
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(b + off[i]),
@@ -331,37 +332,35 @@ template <int NP, bool KS, int RT, int NW> struct Operand {
 };
 
 // acc[i][j] += (rows am + 32 i of A) x (rows bn + 32 j of B) over K block ks of the stage in LDS
-template <int NP, typename OA, typename OB>
+template <typename OA, typename OB>
 __device__ __forceinline__ void mfma_block(const char* la, const char* lb, int am, int bn, int ks, int lane,
                                            f32x16 (&acc)[2][2]) {
-  h8 a[2][NP], b[2][NP];
+  constexpr int NA = OA::PLANES, NB = OB::PLANES;
+  h8 a[2][NA], b[2][NB];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int q = 0; q < NA; ++q) a[i][q] = OA::frag(la, am + 32 * i, ks, q, lane);
+#pragma unroll
+    for (int q = 0; q < NB; ++q) b[i][q] = OB::frag(lb, bn + 32 * i, ks, q, lane);
+  }
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int q = 0; q < NP; ++q) {
-      a[i][q] = OA::frag(la, am + 32 * i, ks, q, lane);
-      b[i][q] = OB::frag(lb, bn + 32 * i, ks, q, lane);
-    }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      if (NP == 2) {                                              // the small products first
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][NP - 1], acc[i][j], 0, 0, 0);
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][NP - 1], b[j][0], acc[i][j], 0, 0, 0);
-      }
+    for (int j = 0; j < 2; ++j) {                                 // the small products first
+      if (NB == 2) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][NB - 1], acc[i][j], 0, 0, 0);
+      if (NA == 2) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][NA - 1], b[j][0], acc[i][j], 0, 0, 0);
       acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][0], acc[i][j], 0, 0, 0);
     }
 }
-template <int NP, typename OA, typename OB>
+template <typename OA, typename OB>
 __device__ __forceinline__ void stage_product(const char* la, const char* lb, int am, int bn, int blocks, int lane,
                                               f32x16 (&acc)[2][2]) {
-  constexpr int KB = 4 / NP;                                      // K blocks of 16 in a stage
-  if (blocks >= KB) {
+  if (blocks >= OA::KB) {
 #pragma unroll
-    for (int ks = 0; ks < KB; ++ks) mfma_block<NP, OA, OB>(la, lb, am, bn, ks, lane, acc);
+    for (int ks = 0; ks < OA::KB; ++ks) mfma_block<OA, OB>(la, lb, am, bn, ks, lane, acc);
   } else {
-    for (int ks = 0; ks < blocks; ++ks) mfma_block<NP, OA, OB>(la, lb, am, bn, ks, lane, acc);
+    for (int ks = 0; ks < blocks; ++ks) mfma_block<OA, OB>(la, lb, am, bn, ks, lane, acc);
   }
 }
 __device__ __forceinline__ void clear(f32x16 (&acc)[2][2]) {
@@ -392,7 +391,7 @@ __device__ __forceinline__ void stage_barrier() {
 // Stages [0, n), n > 0, of one tile, stage 0 already on its way into (la, lb); `last` K blocks of the last stage are used.
 // While a stage is multiplied the next one loads: behind the last one, whatever then(a, b) asks for the free pair.
 // (No stage is left out of the loop's middle: a `break` there cost 64 register moves a round.)
-template <int NP, typename OA, typename OB, typename Then>
+template <typename OA, typename OB, typename Then>
 __device__ __forceinline__ void stages(const OA& A, const OB& B, int n, int last, char* la,
                                        char* lb, char* na, char* nb, int am, int bn, int lane, int wave,
                                        f32x16 (&acc)[2][2], const Then& then) {
@@ -400,22 +399,22 @@ __device__ __forceinline__ void stages(const OA& A, const OB& B, int n, int last
   for (; s + 3 <= n; s += 2) {
     stage_barrier();
     A.issue(s + 1, na, wave); B.issue(s + 1, nb, wave);
-    stage_product<NP, OA, OB>(la, lb, am, bn, 4, lane, acc);
+    stage_product<OA, OB>(la, lb, am, bn, 4, lane, acc);
     stage_barrier();
     A.issue(s + 2, la, wave); B.issue(s + 2, lb, wave);
-    stage_product<NP, OA, OB>(na, nb, am, bn, 4, lane, acc);
+    stage_product<OA, OB>(na, nb, am, bn, 4, lane, acc);
   }
   if (s + 2 == n) {
     stage_barrier();
     A.issue(s + 1, na, wave); B.issue(s + 1, nb, wave);
-    stage_product<NP, OA, OB>(la, lb, am, bn, 4, lane, acc);
+    stage_product<OA, OB>(la, lb, am, bn, 4, lane, acc);
     stage_barrier();
     then(la, lb);
-    stage_product<NP, OA, OB>(na, nb, am, bn, last, lane, acc);
+    stage_product<OA, OB>(na, nb, am, bn, last, lane, acc);
   } else {
     stage_barrier();
     then(na, nb);
-    stage_product<NP, OA, OB>(la, lb, am, bn, last, lane, acc);
+    stage_product<OA, OB>(la, lb, am, bn, last, lane, acc);
   }
 }
 
@@ -428,7 +427,7 @@ template <int C> __device__ __forceinline__ void ring_barrier() {
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
-template <int NP, typename OA, typename OB>
+template <typename OA, typename OB>
 __device__ __forceinline__ void ring_product(const OA& A, const OB& B, int n, char* la0, char* lb0, char* la1, char* lb1,
                                              char* la2, char* lb2, int am, int bn, int lane, int wave, f32x16 (&acc)[2][2]) {
   constexpr int C = OA::PI + OB::PI;
@@ -442,7 +441,7 @@ __device__ __forceinline__ void ring_product(const OA& A, const OB& B, int n, ch
   const auto step = [&](int s, char* la, char* lb, char* fa, char* fb) {
     ring_barrier<C>();
     issue(s + 2, fa, fb);
-    stage_product<NP, OA, OB>(la, lb, am, bn, 4, lane, acc);
+    stage_product<OA, OB>(la, lb, am, bn, 4, lane, acc);
   };
   issue(0, la0, lb0);
   issue(1, la1, lb1);
@@ -583,7 +582,7 @@ __global__ __launch_bounds__(256, 2) void dt_forward_kernel(DistillArgs p) {
     if (t0 < t1) { A.issue(0, la0, wave); B.issue(0, lb0, wave); }
     const auto do_tile = [&](int tile, char* la, char* lb, char* na, char* nb) {
       clear(acc);
-      stages<NP, Op, Op>(A, B, nst, last, la, lb, na, nb, am, bn, lane, wave, acc, [&](char* fa, char* fb) {
+      stages<Op, Op>(A, B, nst, last, la, lb, na, nb, am, bn, lane, wave, acc, [&](char* fa, char* fb) {
         if (tile + 1 < t1) {                                      // the next tile of W loads under this one's fold
           A.base = wbase + (long)(tile + 1) * DT_TILE * ld;
           A.issue(0, fa, wave);
@@ -613,7 +612,7 @@ __global__ __launch_bounds__(256, 2) void dt_forward_kernel(DistillArgs p) {
 // at E = 200 spends its time on them.  Stages of 64 K values x 128 (64) words, four buffers, three in flight; K blocks
 // of 16: NK = 4, 8 or 13 (E up to 64, 128, 208; every shipped model has E = 200).  GRAD: instead of folding, the tile
 // leaves as P = a 2^(t - L1) + b 2^(t / tau - L2), through 2 KiB of LDS a wave so that rows leave in runs of 64 bytes.
-template <int NP, bool TWO, bool GRAD, int NK>
+template <int NP, int NQ, bool TWO, bool GRAD, int NK>
 __global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
   constexpr int NST = NK <= 4 ? 1 : NK <= 8 ? 2 : 4, VT = 128 / NP, NJ = 2 / NP, RB = 128 * NP;   // RB: bytes of a row's stage
   __shared__ __attribute__((aligned(16))) char w0[DT_STAGE + 512];
@@ -701,13 +700,13 @@ __global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
           for (int st = 0; st < NST; ++st) {
             const int g = u * NST + st;
             // Stages g + 1 and g + 2 stay in flight: four copies each, one more for a tile's last stage (its biases);
-            // and the 8 stores of every tile that ended within the last three steps (they count like copies, in order;
+            // and the stores of every tile that ended within the last three steps (they count like copies, in order;
             // at an item's first three steps there are none to count).
-            constexpr int two = 8 + (NST == 1 ? 2 : NST == 2 ? 1 : 0);
+            constexpr int two = 8 + (NST == 1 ? 2 : NST == 2 ? 1 : 0), out = NJ * 2 * NQ * 2;
             if (GRAD && (tl - t0) * NST + st >= 3) {
-              if (NST == 4) { if (st == 0) ring_barrier<16>(); else if (st == 3) ring_barrier<8>(); else ring_barrier<17>(); }
-              else if (NST == 2) { if (st == 0) ring_barrier<25>(); else ring_barrier<17>(); }
-              else ring_barrier<34>();
+              if (NST == 4) { if (st == 0) ring_barrier<8 + out>(); else if (st == 3) ring_barrier<8>(); else ring_barrier<9 + out>(); }
+              else if (NST == 2) { if (st == 0) ring_barrier<9 + 2 * out>(); else ring_barrier<9 + out>(); }
+              else ring_barrier<10 + 3 * out>();
             } else if (NST == 4 && (st == 1 || st == 2)) {
               ring_barrier<9>();
             } else {
@@ -741,38 +740,42 @@ __global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
             }
           }
           const float* bl = reinterpret_cast<const float*>(ring(u * NST + NST - 1) + DT_STAGE) + am;
-          float4 bias[2][4];
+          if (!GRAD) {
+            float4 bias[2][4];
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) bias[i][g] = *reinterpret_cast<const float4*>(bl + 32 * i + 8 * g + 4 * lhi);
+              for (int g = 0; g < 4; ++g) bias[i][g] = *reinterpret_cast<const float4*>(bl + 32 * i + 8 * g + 4 * lhi);
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) {
-            if (!GRAD) {
-              fold<TWO>(acc[0][j], acc[1][j], bias, c, p.itau, m[j], s1[j], s2[j]);
-              continue;
-            }
-            char* tr = turn + wave * 2048;
+            for (int j = 0; j < NJ; ++j) fold<TWO>(acc[0][j], acc[1][j], bias, c, p.itau, m[j], s1[j], s2[j]);
+            continue;
+          }
+          char* tr = turn + wave * 2048;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int v = tl * VT + am + 32 * i;                // in the range
-              char* out = reinterpret_cast<char*>(p.P) +
-                          ((long)(v * NP >> 6) * p.Np + n0 + bn + 32 * j + (lane >> 2)) * 128 + (NP == 1 ? (v & 32) * 2 : 0) + (lane & 3) * 16;
+          for (int i = 0; i < 2; ++i) {
+            const int v = tl * VT + am + 32 * i;                  // in the range
+            float4 bias[4];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) bias[g] = *reinterpret_cast<const float4*>(bl + 32 * i + 8 * g + 4 * lhi);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+              char* out = reinterpret_cast<char*>(p.P) + ((long)(v * NQ >> 6) * p.Np + n0 + bn + 32 * j + (lane >> 2)) * 128 +
+                          (NQ == 1 ? (v & 32) * 2 : 0) + (lane & 3) * 16;
               Packed<f16_t, 4> hi[4], lo[4];
 #pragma unroll
               for (int g = 0; g < 4; ++g) {
-                const float bv[4] = {bias[i][g].x, bias[i][g].y, bias[i][g].z, bias[i][g].w};
+                const float bv[4] = {bias[g].x, bias[g].y, bias[g].z, bias[g].w};
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                   const float t = fmaf(acc[i][j][4 * g + k], c, bv[k]);
                   float x = s1[j] * __builtin_amdgcn_exp2f(t - La[j]);
                   if (TWO) x = fmaf(s2[j], __builtin_amdgcn_exp2f(fmaf(t, p.itau, -Lb[j])), x);
                   hi[g].set(k, x);
-                  if (NP == 2) lo[g].set(k, x - hi[g].f(k));
+                  if (NQ == 2) lo[g].set(k, x - hi[g].f(k));
                 }
               }
 #pragma unroll
-              for (int pl = 0; pl < NP; ++pl) {
+              for (int pl = 0; pl < NQ; ++pl) {
 #pragma unroll
                 for (int g = 0; g < 4; ++g)
                   *reinterpret_cast<Packed<f16_t, 4>*>(tr + l31 * 64 + ((g ^ ((l31 >> 1) & 3)) << 4) + lhi * 8) = pl ? lo[g] : hi[g];
@@ -1027,7 +1030,7 @@ template <typename T, int NP> __global__ __launch_bounds__(256) void dt_gimage_k
 }
 
 // P[n][v] of a piece of the vocabulary without the picked entries: a 2^(t - L1) + b 2^(t / tau - L2)
-template <int NP, bool TWO>
+template <int NP, int NQ, bool TWO>
 __global__ __launch_bounds__(256, 2) void dt_grad_kernel(DistillArgs p) {
   DT_LDS
   const int nl = *p.nlive, nt = (nl + DT_TILE - 1) / DT_TILE, vt = (p.vc + DT_TILE - 1) / DT_TILE;
@@ -1053,7 +1056,7 @@ __global__ __launch_bounds__(256, 2) void dt_grad_kernel(DistillArgs p) {
   clear(acc);
   A.issue(0, la0, wave);
   B.issue(0, lb0, wave);
-  stages<NP, Op, Op>(A, B, nst, last, la0, lb0, la1, lb1, am, bn, lane, wave, acc, [](char*, char*) {});
+  stages<Op, Op>(A, B, nst, last, la0, lb0, la1, lb1, am, bn, lane, wave, acc, [](char*, char*) {});
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -1076,29 +1079,29 @@ __global__ __launch_bounds__(256, 2) void dt_grad_kernel(DistillArgs p) {
           if (TWO) x = fmaf(cb, __builtin_amdgcn_exp2f(fmaf(t, p.itau, -L2)), x);
           x = in ? x : 0.f;
           hi.set(k, x);
-          if (NP == 2) lo.set(k, x - hi.f(k));
+          if (NQ == 2) lo.set(k, x - hi.f(k));
         }
-        const int byte = NP == 1 ? v * 2 : (v >> 5) * 128 + (v & 31) * 2;
-        char* row = DT_AREA(nn * NP >> 6) + (nn * 256 * NP & (DT_STAGE - 1));
+        const int byte = NQ == 1 ? v * 2 : (v >> 5) * 128 + (v & 31) * 2;
+        char* row = DT_AREA(nn * NQ >> 6) + (nn * 256 * NQ & (DT_STAGE - 1));
         *reinterpret_cast<Packed<f16_t, 4>*>(row + ((((byte >> 4) ^ (nn & 15)) << 4) | (byte & 15))) = hi;
-        if (NP == 2) {
+        if (NQ == 2) {
           const int bl = byte + 64;
           *reinterpret_cast<Packed<f16_t, 4>*>(row + ((((bl >> 4) ^ (nn & 15)) << 4) | (bl & 15))) = lo;
         }
       }
   }
   __syncthreads();
-  char* P = reinterpret_cast<char*>(p.P) + ((long)tv * 2 * NP * p.Np + n0) * 128;
-  for (int k = threadIdx.x; k < DT_TILE * 16 * NP; k += 256) {    // piece by piece, its 128 rows in one run of memory
+  char* P = reinterpret_cast<char*>(p.P) + ((long)tv * 2 * NQ * p.Np + n0) * 128;
+  for (int k = threadIdx.x; k < DT_TILE * 16 * NQ; k += 256) {    // piece by piece, its 128 rows in one run of memory
     const int g = k >> 10, nn = (k >> 3) & 127, ch = g * 8 + (k & 7);
-    const uint4 x = *reinterpret_cast<const uint4*>(DT_AREA(nn * NP >> 6) + (nn * 256 * NP & (DT_STAGE - 1)) + ((ch ^ (nn & 15)) << 4));
+    const uint4 x = *reinterpret_cast<const uint4*>(DT_AREA(nn * NQ >> 6) + (nn * 256 * NQ & (DT_STAGE - 1)) + ((ch ^ (nn & 15)) << 4));
     *reinterpret_cast<uint4*>(P + (long)g * p.Np * 128 + (k & 1023) * 16) = x;
   }
 }
 
 // The picked entries of a row, from their own fp32 logits: softmax minus the target / the teacher's share (an id that
 // was listed before, or a target that the teacher lists, has share -1 here: its first place writes it).
-template <int NP, bool TWO>
+template <int NQ, bool TWO>
 __global__ __launch_bounds__(256) void dt_pick_kernel(DistillArgs p) {
   const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (i >= *p.nlive) return;
@@ -1113,10 +1116,10 @@ __global__ __launch_bounds__(256) void dt_pick_kernel(DistillArgs p) {
     float x = a * (__builtin_amdgcn_exp2f(pick - L1) - (id == tg ? 1.f : 0.f));
     if (p.K) x = fmaf(b, __builtin_amdgcn_exp2f(fmaf(pick, TWO ? p.itau : 1.f, -L2)) - share, x);
     const int v = (int)(id - p.v0);
-    _Float16* q = p.P + ((long)(v * NP >> 6) * p.Np + i) * 64 + (v & (64 / NP - 1));
+    _Float16* q = p.P + ((long)(v * NQ >> 6) * p.Np + i) * 64 + (v & (64 / NQ - 1));
     const _Float16 hi = (_Float16)x;
     q[0] = hi;
-    if (NP == 2) q[32] = (_Float16)(x - (float)hi);
+    if (NQ == 2) q[32] = (_Float16)(x - (float)hi);
   }
 }
 
@@ -1135,9 +1138,9 @@ __device__ __forceinline__ int dt_dx_splits(int tiles, int stages) {
 
 // dX: (W down its rows: K = vocabulary) x (P along its rows), tiles of RA columns of E x RB rows.  Items (tile, split of
 // the range): partial tiles in accumulator order, added to what an earlier range left there.
-template <int NP, int RA>
+template <int NP, int NQ, int RA>
 __global__ __launch_bounds__(512, 2) void dt_dx_kernel(DistillArgs p, int et, int add) {
-  constexpr int RB = 384 - RA, BK = 64 / NP;
+  constexpr int RB = 384 - RA, BK = 64 / NQ;
   DT_RING(RA, RB)
   const int nl = *p.nlive, tiles = (nl + RB - 1) / RB * et;
   const int splits = dt_dx_splits(tiles, p.vfull / BK);
@@ -1145,8 +1148,8 @@ __global__ __launch_bounds__(512, 2) void dt_dx_kernel(DistillArgs p, int et, in
   const int am = (RA == 256 ? wave >> 1 : wave & 1) * 64, bn = (RA == 256 ? wave & 1 : wave >> 1) * 64;
   const int stages = p.vc / BK, per = (stages + splits - 1) / splits;
   const long ldw = (long)p.Kp * NP * 2;
-  using OA = Operand<NP, true, RA, 8>;
-  using OB = Operand<NP, false, RB, 8>;
+  using OA = Operand<NP, true, RA, 8, BK>;
+  using OB = Operand<NQ, false, RB, 8>;
   OA A;
   OB B;
   A.init(nullptr, ldw, 128, lane, wave);
@@ -1157,7 +1160,7 @@ __global__ __launch_bounds__(512, 2) void dt_dx_kernel(DistillArgs p, int et, in
     A.base = reinterpret_cast<const char*>(p.Wimg) + (p.v0 + (long)s0 * BK) * ldw + (long)te * RA * 2 * NP;
     B.base = reinterpret_cast<const char*>(p.P) + ((long)s0 * p.Np + tn * RB) * 128;
     f32x16 acc[2][2];
-    ring_product<NP, OA, OB>(A, B, s1 - s0, la0, lb0, la1, lb1, la2, lb2, am, bn, lane, wave, acc);
+    ring_product<OA, OB>(A, B, s1 - s0, la0, lb0, la1, lb1, la2, lb2, am, bn, lane, wave, acc);
     float4* out = reinterpret_cast<float4*>(p.slab) + ((long)split * tiles + tile) * (RA * RB / 4) + wave * 1024 + lane;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -1172,13 +1175,13 @@ __global__ __launch_bounds__(512, 2) void dt_dx_kernel(DistillArgs p, int et, in
         }
   }
 }
-template <typename T, int NP, int RA>
+template <typename T, int NQ, int RA>
 __global__ __launch_bounds__(256) void dt_dx_sum_kernel(DistillArgs p, int et) {
   constexpr int RB = 384 - RA;
   const int nl = *p.nlive, tiles = (nl + RB - 1) / RB * et;
   const int tile = blockIdx.x >> 5;                               // 32 blocks a tile
   if (tile >= tiles) return;
-  const int splits = dt_dx_splits(tiles, p.vfull / (64 / NP));
+  const int splits = dt_dx_splits(tiles, p.vfull / (64 / NQ));
   const float w = ldexpf(1.f, -p.sexp[1] - P_EXP);
   const int slot = (blockIdx.x & 31) * 256 + threadIdx.x;
   const long step = (long)tiles * (RA * RB / 4);
@@ -1201,24 +1204,24 @@ __global__ __launch_bounds__(256) void dt_dx_sum_kernel(DistillArgs p, int et) {
 
 // dW and db: (s X down its rows: K = live rows) x (P down its rows), tiles of RA columns of E x RB words, whole K in one
 // block
-template <typename T, int NP, int RA>
+template <typename T, int NP, int NQ, int RA>
 __global__ __launch_bounds__(512, 2) void dt_dw_kernel(DistillArgs p, int et) {
-  constexpr int RB = 384 - RA, BK = 64 / NP;
+  constexpr int RB = 384 - RA, BK = 64 / NQ;
   DT_RING(RA, RB)
   const int nl = *p.nlive, vt = p.vc / RB;
   const int pv = (vt + 7) / 8, j0 = blockIdx.x >> 3, tv = (blockIdx.x & 7) * pv + j0 / et, te = j0 % et;
   if (j0 / et >= pv || tv >= vt) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int am = (RA == 256 ? wave >> 1 : wave & 1) * 64, bn = (RA == 256 ? wave & 1 : wave >> 1) * 64;
-  using OA = Operand<NP, true, RA, 8>;
-  using OB = Operand<NP, true, RB, 8>;
+  using OA = Operand<NP, true, RA, 8, BK>;
+  using OB = Operand<NQ, true, RB, 8>;
   OA A;
   OB B;
   A.init(reinterpret_cast<const char*>(p.Gimg) + (long)te * RA * 2 * NP, (long)p.Kg * NP * 2, 128, lane, wave);
   B.init(reinterpret_cast<const char*>(p.P) + (long)(tv * RB / BK) * p.Np * 128, 128, (long)p.Np * 128, lane, wave);
   const float fw = *p.gmax * ldexpf(1.f, -P_EXP - p.sexp[0]), fb = *p.gmax * ldexpf(1.f, -2 * P_EXP);
   f32x16 acc[2][2];
-  ring_product<NP, OA, OB>(A, B, (nl + BK - 1) / BK, la0, lb0, la1, lb1, la2, lb2, am, bn, lane, wave, acc);
+  ring_product<OA, OB>(A, B, (nl + BK - 1) / BK, la0, lb0, la1, lb1, la2, lb2, am, bn, lane, wave, acc);
   // a lane holds four neighbouring columns of a word's row at a time
   const bool vec = p.E % 4 == 0 && ((uintptr_t)p.dW % (4 * sizeof(T))) == 0;
 #pragma unroll
@@ -1255,12 +1258,13 @@ struct DistillPlan {
   long bytes, back_bytes;
   long hard, soft, counts, rows, inv, nlive, slive, amax, sexp, Ximg, Wimg, b2, L1, L2, some, pick, share, part;   // offsets in bytes
   long Gimg, coef, gmax, P, slab;
-  int np, Np, Vp, Kp, Kg, nb, nk, fvt, rax, raw, et, etw;
+  int np, nq, Np, Vp, Kp, Kg, nb, nk, fvt, rax, raw, et, etw;
   long vc, pplane;
 };
 static DistillPlan dt_plan(int dtype, long N, int E, int V, int K) {
   DistillPlan d = {};
   d.np = dtype == DT_F32 ? 2 : 1;
+  d.nq = dtype == DT_BF16 ? 1 : 2;                  // planes of P
   d.Np = (int)((N + 255) / 256 * 256); d.Vp = (V + 255) / 256 * 256; d.nk = E <= 64 ? 4 : E <= 128 ? 8 : E <= 208 ? 13 : 0;
   d.Kp = d.nk == 13 ? 256 : (E + 63) / 64 * 64; d.Kg = (E + 64) / 64 * 64;
   d.nb = cdiv(N, DT_CROWS);
@@ -1285,14 +1289,14 @@ static DistillPlan dt_plan(int dtype, long N, int E, int V, int K) {
   d.pick = take(at, 4L * N * (K + 1)); d.share = take(at, 4L * N * (K + 1));
   d.part = take(at, 12L * d.pplane);
   d.bytes = at;
-  long vc = DT_PIECE_BYTES / (2L * d.np * d.Np) / 256 * 256;
+  long vc = DT_PIECE_BYTES / (2L * d.nq * d.Np) / 256 * 256;
   if (vc < 1024) vc = 1024;
   const int pieces = cdiv(d.Vp, vc);
   d.vc = ((long)d.Vp / 256 + pieces - 1) / pieces * 256;          // ranges of equal size
   const int tiles = d.Np / (384 - d.rax) * d.et;
   at = 0;
   d.Gimg = take(at, 2L * d.Np * d.Kg * d.np + slack); d.coef = take(at, 12L * d.Np); d.gmax = take(at, 4);
-  d.P = take(at, 2L * d.Np * d.vc * d.np);
+  d.P = take(at, 2L * d.Np * d.vc * d.nq);
   d.slab = take(at, 4L * 32768 * (tiles > DT_DX_MOST ? tiles : DT_DX_MOST));
   d.back_bytes = at;
   return d;
@@ -1331,25 +1335,25 @@ static void dt_fill(DistillArgs& a, const DistillPlan& d, const DistillCall& c, 
   a.part = (float*)(w + d.part); a.pplane = d.pplane; a.fvt = d.fvt; a.least = d.nk ? 1 : 8;
 }
 
-template <int NP, bool TWO, bool GRAD> static void dt_rows(int nk, const DistillArgs& a, hipStream_t s) {
+template <int NP, int NQ, bool TWO, bool GRAD> static void dt_rows(int nk, const DistillArgs& a, hipStream_t s) {
   const dim3 grid(DT_WALK_BLOCKS);
-  if (nk == 4) hipLaunchKernelGGL((dt_rows_kernel<NP, TWO, GRAD, 4>), grid, dim3(256), 0, s, a);
-  else if (nk == 8) hipLaunchKernelGGL((dt_rows_kernel<NP, TWO, GRAD, 8>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((dt_rows_kernel<NP, TWO, GRAD, 13>), grid, dim3(256), 0, s, a);
+  if (nk == 4) hipLaunchKernelGGL((dt_rows_kernel<NP, NQ, TWO, GRAD, 4>), grid, dim3(256), 0, s, a);
+  else if (nk == 8) hipLaunchKernelGGL((dt_rows_kernel<NP, NQ, TWO, GRAD, 8>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((dt_rows_kernel<NP, NQ, TWO, GRAD, 13>), grid, dim3(256), 0, s, a);
 }
 template <typename T, int NP, bool TWO> static int dt_forward(const DistillPlan& d, const DistillArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((dt_count_kernel<T>), dim3(d.nb + 2 * DT_AMAX), dim3(256), 0, s, a, d.nb);
   CVAE_LAUNCH_CHECK("dt_count_kernel");
   hipLaunchKernelGGL((dt_image_kernel<T, NP>), dim3(cdiv(a.N, 16) + d.Np / 16 + d.Vp / 16), dim3(256), 0, s, a, cdiv(a.N, 16));
   CVAE_LAUNCH_CHECK("dt_image_kernel");
-  if (d.nk) dt_rows<NP, TWO, false>(d.nk, a, s);
+  if (d.nk) dt_rows<NP, 1, TWO, false>(d.nk, a, s);
   else hipLaunchKernelGGL((dt_forward_kernel<NP, TWO>), dim3(DT_WALK_BLOCKS), dim3(256), 0, s, a);
   CVAE_LAUNCH_CHECK("dt_forward_kernel");
   hipLaunchKernelGGL((dt_combine_kernel<T, TWO>), dim3(a.N), dim3(256), 0, s, a);
   CVAE_LAUNCH_CHECK("dt_combine_kernel");
   return 0;
 }
-template <typename T, int NP, bool TWO> static int dt_backward(const DistillPlan& d, DistillArgs a, hipStream_t s) {
+template <typename T, int NP, int NQ, bool TWO> static int dt_backward(const DistillPlan& d, DistillArgs a, hipStream_t s) {
   const int nx = cdiv(a.N, 16), nt = d.Np / DT_TILE;
   hipLaunchKernelGGL((dt_gimage_kernel<T, NP>), dim3(nx + d.Np / 16), dim3(256), 0, s, a, nx);
   CVAE_LAUNCH_CHECK("dt_gimage_kernel");
@@ -1357,33 +1361,33 @@ template <typename T, int NP, bool TWO> static int dt_backward(const DistillPlan
     a.v0 = (int)v0;
     a.vc = (int)(d.Vp - v0 < d.vc ? d.Vp - v0 : d.vc);
     const int vt = cdiv(a.vc, DT_TILE);
-    if (d.nk) dt_rows<NP, TWO, true>(d.nk, a, s);
-    else hipLaunchKernelGGL((dt_grad_kernel<NP, TWO>), dim3((unsigned)((long)cdiv(vt, 8) * 8 * nt)), dim3(256), 0, s, a);
+    if (d.nk) dt_rows<NP, NQ, TWO, true>(d.nk, a, s);
+    else hipLaunchKernelGGL((dt_grad_kernel<NP, NQ, TWO>), dim3((unsigned)((long)cdiv(vt, 8) * 8 * nt)), dim3(256), 0, s, a);
     CVAE_LAUNCH_CHECK("dt_grad_kernel");
-    hipLaunchKernelGGL((dt_pick_kernel<NP, TWO>), dim3(cdiv(a.N, 4)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((dt_pick_kernel<NQ, TWO>), dim3(cdiv(a.N, 4)), dim3(256), 0, s, a);
     CVAE_LAUNCH_CHECK("dt_pick_kernel");
     const dim3 gx(DT_DX_BLOCKS);
-    if (d.rax == 256) hipLaunchKernelGGL((dt_dx_kernel<NP, 256>), gx, dim3(512), 0, s, a, d.et, v0 > 0 ? 1 : 0);
-    else hipLaunchKernelGGL((dt_dx_kernel<NP, 128>), gx, dim3(512), 0, s, a, d.et, v0 > 0 ? 1 : 0);
+    if (d.rax == 256) hipLaunchKernelGGL((dt_dx_kernel<NP, NQ, 256>), gx, dim3(512), 0, s, a, d.et, v0 > 0 ? 1 : 0);
+    else hipLaunchKernelGGL((dt_dx_kernel<NP, NQ, 128>), gx, dim3(512), 0, s, a, d.et, v0 > 0 ? 1 : 0);
     CVAE_LAUNCH_CHECK("dt_dx_kernel");
     const dim3 gw((unsigned)((long)cdiv(a.vc / (384 - d.raw), 8) * 8 * d.etw));
-    if (d.raw == 256) hipLaunchKernelGGL((dt_dw_kernel<T, NP, 256>), gw, dim3(512), 0, s, a, d.etw);
-    else hipLaunchKernelGGL((dt_dw_kernel<T, NP, 128>), gw, dim3(512), 0, s, a, d.etw);
+    if (d.raw == 256) hipLaunchKernelGGL((dt_dw_kernel<T, NP, NQ, 256>), gw, dim3(512), 0, s, a, d.etw);
+    else hipLaunchKernelGGL((dt_dw_kernel<T, NP, NQ, 128>), gw, dim3(512), 0, s, a, d.etw);
     CVAE_LAUNCH_CHECK("dt_dw_kernel");
   }
   const dim3 gs((unsigned)((long)(d.Np / (384 - d.rax)) * d.et * 32));
-  if (d.rax == 256) hipLaunchKernelGGL((dt_dx_sum_kernel<T, NP, 256>), gs, dim3(256), 0, s, a, d.et);
-  else hipLaunchKernelGGL((dt_dx_sum_kernel<T, NP, 128>), gs, dim3(256), 0, s, a, d.et);
+  if (d.rax == 256) hipLaunchKernelGGL((dt_dx_sum_kernel<T, NQ, 256>), gs, dim3(256), 0, s, a, d.et);
+  else hipLaunchKernelGGL((dt_dx_sum_kernel<T, NQ, 128>), gs, dim3(256), 0, s, a, d.et);
   CVAE_LAUNCH_CHECK("dt_dx_sum_kernel");
   return 0;
 }
-template <typename T, int NP> static int dt_run(const DistillPlan& d, const DistillArgs& a, bool back, hipStream_t s) {
-  if (back) return a.two ? dt_backward<T, NP, true>(d, a, s) : dt_backward<T, NP, false>(d, a, s);
+template <typename T, int NP, int NQ> static int dt_run(const DistillPlan& d, const DistillArgs& a, bool back, hipStream_t s) {
+  if (back) return a.two ? dt_backward<T, NP, NQ, true>(d, a, s) : dt_backward<T, NP, NQ, false>(d, a, s);
   return a.two ? dt_forward<T, NP, true>(d, a, s) : dt_forward<T, NP, false>(d, a, s);
 }
 static int dt_dispatch(int dtype, const DistillPlan& d, const DistillArgs& a, bool back, hipStream_t s) {
-  if (dtype == DT_F32) return dt_run<float, 2>(d, a, back, s);
-  return dtype == DT_BF16 ? dt_run<bf16_t, 1>(d, a, back, s) : dt_run<f16_t, 1>(d, a, back, s);
+  if (dtype == DT_F32) return dt_run<float, 2, 2>(d, a, back, s);
+  return dtype == DT_BF16 ? dt_run<bf16_t, 1, 1>(d, a, back, s) : dt_run<f16_t, 1, 2>(d, a, back, s);
 }
 
 int launch_distill_forward(const DistillCall& c, float* hard, float* soft, void* ws, hipStream_t s) {

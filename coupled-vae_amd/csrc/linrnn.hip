@@ -436,12 +436,13 @@ __global__ __launch_bounds__(256) void linrnn_step_kernel(LinRnnArgs p) {
 
 // ---------------------------------------------------------------------------------------------- host side
 static int lr_channels_per_block(int dtype, int H) { return 64 * ((dtype != DT_F32 && H % 2 == 0) ? 2 : 1); }
-// segments of the time axis: enough blocks for two on every CU, of no less than two rounds (128 steps) each
+// segments of the time axis: enough blocks for two on every CU (8192 x 2000 channels bf16: forward 61 us with 512 blocks,
+// 76 with 256, 62 with 1024), of no less than one round (64 steps) each
 static void lr_plan(int dtype, int T, int B, int H, int* nseg, int* seg) {
   constexpr int R = LR_C * LR_W;
   const long cb = ((long)B * H + lr_channels_per_block(dtype, H) - 1) / lr_channels_per_block(dtype, H);
   long want = (512 + cb - 1) / (cb > 0 ? cb : 1);
-  const long most = T / (2 * R);
+  const long most = ((long)T + R - 1) / R;
   if (want > most) want = most;
   if (cb >= 256 || want < 1) want = 1;
   *seg = (int)((((long)T + want - 1) / want + R - 1) / R * R);

@@ -455,13 +455,8 @@ __device__ __forceinline__ void ring_product(const OA& A, const OB& B, int n, ch
   if (s + 1 < n) step(s + 1, la1, lb1, la0, lb0);
   ring_barrier<0>();                                              // no copy may land in LDS that the next block owns
 }
-#define DT_RING(RA, RB) \
-  __shared__ __attribute__((aligned(16))) char la0[(RA) * 128]; \
-  __shared__ __attribute__((aligned(16))) char la1[(RA) * 128]; \
-  __shared__ __attribute__((aligned(16))) char la2[(RA) * 128]; \
-  __shared__ __attribute__((aligned(16))) char lb0[(RB) * 128]; \
-  __shared__ __attribute__((aligned(16))) char lb1[(RB) * 128]; \
-  __shared__ __attribute__((aligned(16))) char lb2[(RB) * 128];
+// three buffers for the operand of 256 rows or columns, three for the one of 128
+struct Ring { char *x0, *x1, *x2, *y0, *y1, *y2; };
 // value r of an accumulator tile: row 4 (lane / 32) + 8 (r / 4) + r % 4, column lane % 32
 __device__ __forceinline__ int acc_row(int r, int lane) { return (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5); }
 
@@ -1139,9 +1134,8 @@ __device__ __forceinline__ int dt_dx_splits(int tiles, int stages) {
 // dX: (W down its rows: K = vocabulary) x (P along its rows), tiles of RA columns of E x RB rows.  Items (tile, split of
 // the range): partial tiles in accumulator order, added to what an earlier range left there.
 template <int NP, int NQ, int RA>
-__global__ __launch_bounds__(512, 2) void dt_dx_kernel(DistillArgs p, int et, int add) {
+__device__ __forceinline__ void dx_items(const DistillArgs& p, const Ring& m, int first, int et, int add) {
   constexpr int RB = 384 - RA, BK = 64 / NQ;
-  DT_RING(RA, RB)
   const int nl = *p.nlive, tiles = (nl + RB - 1) / RB * et;
   const int splits = dt_dx_splits(tiles, p.vfull / BK);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1154,13 +1148,14 @@ __global__ __launch_bounds__(512, 2) void dt_dx_kernel(DistillArgs p, int et, in
   OB B;
   A.init(nullptr, ldw, 128, lane, wave);
   B.init(nullptr, 128, (long)p.Np * 128, lane, wave);
-  for (int item = blockIdx.x; item < tiles * splits; item += DT_DX_BLOCKS) {
+  for (int item = first; item < tiles * splits; item += DT_DX_BLOCKS) {
     const int split = item % splits, tile = item / splits, te = tile % et, tn = tile / et;
     const int s0 = split * per, s1 = min(stages, s0 + per);
     A.base = reinterpret_cast<const char*>(p.Wimg) + (p.v0 + (long)s0 * BK) * ldw + (long)te * RA * 2 * NP;
     B.base = reinterpret_cast<const char*>(p.P) + ((long)s0 * p.Np + tn * RB) * 128;
     f32x16 acc[2][2];
-    ring_product<OA, OB>(A, B, s1 - s0, la0, lb0, la1, lb1, la2, lb2, am, bn, lane, wave, acc);
+    if (RA == 256) ring_product<OA, OB>(A, B, s1 - s0, m.x0, m.y0, m.x1, m.y1, m.x2, m.y2, am, bn, lane, wave, acc);
+    else ring_product<OA, OB>(A, B, s1 - s0, m.y0, m.x0, m.y1, m.x1, m.y2, m.x2, am, bn, lane, wave, acc);
     float4* out = reinterpret_cast<float4*>(p.slab) + ((long)split * tiles + tile) * (RA * RB / 4) + wave * 1024 + lane;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -1205,11 +1200,10 @@ __global__ __launch_bounds__(256) void dt_dx_sum_kernel(DistillArgs p, int et) {
 // dW and db: (s X down its rows: K = live rows) x (P down its rows), tiles of RA columns of E x RB words, whole K in one
 // block
 template <typename T, int NP, int NQ, int RA>
-__global__ __launch_bounds__(512, 2) void dt_dw_kernel(DistillArgs p, int et) {
+__device__ __forceinline__ void dw_tile(const DistillArgs& p, const Ring& m, int block, int et) {
   constexpr int RB = 384 - RA, BK = 64 / NQ;
-  DT_RING(RA, RB)
   const int nl = *p.nlive, vt = p.vc / RB;
-  const int pv = (vt + 7) / 8, j0 = blockIdx.x >> 3, tv = (blockIdx.x & 7) * pv + j0 / et, te = j0 % et;
+  const int pv = (vt + 7) / 8, j0 = block >> 3, tv = (block & 7) * pv + j0 / et, te = j0 % et;
   if (j0 / et >= pv || tv >= vt) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int am = (RA == 256 ? wave >> 1 : wave & 1) * 64, bn = (RA == 256 ? wave & 1 : wave >> 1) * 64;
@@ -1221,7 +1215,8 @@ __global__ __launch_bounds__(512, 2) void dt_dw_kernel(DistillArgs p, int et) {
   B.init(reinterpret_cast<const char*>(p.P) + (long)(tv * RB / BK) * p.Np * 128, 128, (long)p.Np * 128, lane, wave);
   const float fw = *p.gmax * ldexpf(1.f, -P_EXP - p.sexp[0]), fb = *p.gmax * ldexpf(1.f, -2 * P_EXP);
   f32x16 acc[2][2];
-  ring_product<OA, OB>(A, B, (nl + BK - 1) / BK, la0, lb0, la1, lb1, la2, lb2, am, bn, lane, wave, acc);
+  if (RA == 256) ring_product<OA, OB>(A, B, (nl + BK - 1) / BK, m.x0, m.y0, m.x1, m.y1, m.x2, m.y2, am, bn, lane, wave, acc);
+  else ring_product<OA, OB>(A, B, (nl + BK - 1) / BK, m.y0, m.x0, m.y1, m.x1, m.y2, m.x2, am, bn, lane, wave, acc);
   // a lane holds four neighbouring columns of a word's row at a time
   const bool vec = p.E % 4 == 0 && ((uintptr_t)p.dW % (4 * sizeof(T))) == 0;
 #pragma unroll
@@ -1249,6 +1244,21 @@ __global__ __launch_bounds__(512, 2) void dt_dw_kernel(DistillArgs p, int et) {
           if (e + k == p.E) static_cast<T*>(p.db)[v] = (T)(acc[i][j][4 * g + k] * fb);
       }
   }
+}
+
+// Both products of a range in one launch, dX's items in the first DT_DX_BLOCKS blocks (one a CU), dW's tiles behind them:
+// the CUs that one of them leaves idle at its end work on the other.
+template <typename T, int NP, int NQ, int RAX, int RAW>
+__global__ __launch_bounds__(512, 2) void dt_products_kernel(DistillArgs p, int etx, int etw, int add) {
+  __shared__ __attribute__((aligned(16))) char x0[32768];
+  __shared__ __attribute__((aligned(16))) char x1[32768];
+  __shared__ __attribute__((aligned(16))) char x2[32768];
+  __shared__ __attribute__((aligned(16))) char y0[16384];
+  __shared__ __attribute__((aligned(16))) char y1[16384];
+  __shared__ __attribute__((aligned(16))) char y2[16384];
+  const Ring m = {x0, x1, x2, y0, y1, y2};
+  if (blockIdx.x < DT_DX_BLOCKS) dx_items<NP, NQ, RAX>(p, m, blockIdx.x, etx, add);
+  else dw_tile<T, NP, NQ, RAW>(p, m, blockIdx.x - DT_DX_BLOCKS, etw);
 }
 
 // ------------------------------------------------------------------------------------------------- host side
@@ -1366,14 +1376,13 @@ template <typename T, int NP, int NQ, bool TWO> static int dt_backward(const Dis
     CVAE_LAUNCH_CHECK("dt_grad_kernel");
     hipLaunchKernelGGL((dt_pick_kernel<NQ, TWO>), dim3(cdiv(a.N, 4)), dim3(256), 0, s, a);
     CVAE_LAUNCH_CHECK("dt_pick_kernel");
-    const dim3 gx(DT_DX_BLOCKS);
-    if (d.rax == 256) hipLaunchKernelGGL((dt_dx_kernel<NP, NQ, 256>), gx, dim3(512), 0, s, a, d.et, v0 > 0 ? 1 : 0);
-    else hipLaunchKernelGGL((dt_dx_kernel<NP, NQ, 128>), gx, dim3(512), 0, s, a, d.et, v0 > 0 ? 1 : 0);
-    CVAE_LAUNCH_CHECK("dt_dx_kernel");
-    const dim3 gw((unsigned)((long)cdiv(a.vc / (384 - d.raw), 8) * 8 * d.etw));
-    if (d.raw == 256) hipLaunchKernelGGL((dt_dw_kernel<T, NP, NQ, 256>), gw, dim3(512), 0, s, a, d.etw);
-    else hipLaunchKernelGGL((dt_dw_kernel<T, NP, NQ, 128>), gw, dim3(512), 0, s, a, d.etw);
-    CVAE_LAUNCH_CHECK("dt_dw_kernel");
+    const dim3 grid((unsigned)(DT_DX_BLOCKS + (long)cdiv(a.vc / (384 - d.raw), 8) * 8 * d.etw));
+    const int add = v0 > 0 ? 1 : 0;
+    if (d.rax == 256 && d.raw == 256) hipLaunchKernelGGL((dt_products_kernel<T, NP, NQ, 256, 256>), grid, dim3(512), 0, s, a, d.et, d.etw, add);
+    else if (d.rax == 256) hipLaunchKernelGGL((dt_products_kernel<T, NP, NQ, 256, 128>), grid, dim3(512), 0, s, a, d.et, d.etw, add);
+    else if (d.raw == 256) hipLaunchKernelGGL((dt_products_kernel<T, NP, NQ, 128, 256>), grid, dim3(512), 0, s, a, d.et, d.etw, add);
+    else hipLaunchKernelGGL((dt_products_kernel<T, NP, NQ, 128, 128>), grid, dim3(512), 0, s, a, d.et, d.etw, add);
+    CVAE_LAUNCH_CHECK("dt_products_kernel");
   }
   const dim3 gs((unsigned)((long)(d.Np / (384 - d.rax)) * d.et * 32));
   if (d.rax == 256) hipLaunchKernelGGL((dt_dx_sum_kernel<T, NQ, 256>), gs, dim3(256), 0, s, a, d.et);

@@ -307,10 +307,11 @@ template <int NP, bool KS, int RT, int NW, int KR = 64 / NP> struct Operand {
       }
     }
   }
-  __device__ __forceinline__ void issue(int stage, char* lds, int wave) const {
+  // copies [i0, i1) of a stage
+  __device__ __forceinline__ void issue(int stage, char* lds, int wave, int i0 = 0, int i1 = PI) const {
     const char* b = base + (KS ? (long)stage * KR * row : (long)stage * grp);
 #pragma unroll
-    for (int i = 0; i < PI; ++i)
+    for (int i = i0; i < i1; ++i)
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(b + off[i]),
                                        (__attribute__((address_space(3))) void*)(lds + (wave * PI + i) * 1024), 16, 0, 0);
   }
@@ -331,36 +332,39 @@ template <int NP, bool KS, int RT, int NW, int KR = 64 / NP> struct Operand {
   }
 };
 
-// acc[i][j] += (rows am + 32 i of A) x (rows bn + 32 j of B) over K block ks of the stage in LDS
-template <typename OA, typename OB>
-__device__ __forceinline__ void mfma_block(const char* la, const char* lb, int am, int bn, int ks, int lane,
-                                           f32x16 (&acc)[2][2]) {
-  constexpr int NA = OA::PLANES, NB = OB::PLANES;
-  h8 a[2][NA], b[2][NB];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-#pragma unroll
-    for (int q = 0; q < NA; ++q) a[i][q] = OA::frag(la, am + 32 * i, ks, q, lane);
-#pragma unroll
-    for (int q = 0; q < NB; ++q) b[i][q] = OB::frag(lb, bn + 32 * i, ks, q, lane);
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {                                 // the small products first
-      if (NB == 2) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][NB - 1], acc[i][j], 0, 0, 0);
-      if (NA == 2) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][NA - 1], b[j][0], acc[i][j], 0, 0, 0);
-      acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i][0], b[j][0], acc[i][j], 0, 0, 0);
-    }
-}
-template <typename OA, typename OB>
+// acc[i][j] += (rows am + 32 i of A) x (rows bn + 32 j of B) over `blocks` K blocks of the stage in LDS.  The next block's
+// operands are read, and more(block) adds its share of the next stage's copies, while the matrix unit works on this one:
+// a CU takes a copy of 1 KiB every 16 cycles, so asked for all at once at a stage's start they hold its waves back.
+template <typename OA, typename OB, typename More>
 __device__ __forceinline__ void stage_product(const char* la, const char* lb, int am, int bn, int blocks, int lane,
-                                              f32x16 (&acc)[2][2]) {
-  if (blocks >= OA::KB) {
+                                              f32x16 (&acc)[2][2], const More& more) {
+  constexpr int NA = OA::PLANES, NB = OB::PLANES, KB = OA::KB;
+  h8 a[2][2][NA], b[2][2][NB];
+  const auto read = [&](int ks) {
 #pragma unroll
-    for (int ks = 0; ks < OA::KB; ++ks) mfma_block<OA, OB>(la, lb, am, bn, ks, lane, acc);
-  } else {
-    for (int ks = 0; ks < blocks; ++ks) mfma_block<OA, OB>(la, lb, am, bn, ks, lane, acc);
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int q = 0; q < NA; ++q) a[ks & 1][i][q] = OA::frag(la, am + 32 * i, ks, q, lane);
+#pragma unroll
+      for (int q = 0; q < NB; ++q) b[ks & 1][i][q] = OB::frag(lb, bn + 32 * i, ks, q, lane);
+    }
+  };
+  read(0);
+#pragma unroll
+  for (int ks = 0; ks < KB; ++ks) {
+    if (ks >= blocks) continue;
+    if (ks + 1 < KB) read(ks + 1);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {                               // the small products first
+        const int q = ks & 1;
+        if (NB == 2) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[q][i][0], b[q][j][NB - 1], acc[i][j], 0, 0, 0);
+        if (NA == 2) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[q][i][NA - 1], b[q][j][0], acc[i][j], 0, 0, 0);
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[q][i][0], b[q][j][0], acc[i][j], 0, 0, 0);
+      }
+    more(ks);
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 __device__ __forceinline__ void clear(f32x16 (&acc)[2][2]) {
@@ -395,26 +399,31 @@ template <typename OA, typename OB, typename Then>
 __device__ __forceinline__ void stages(const OA& A, const OB& B, int n, int last, char* la,
                                        char* lb, char* na, char* nb, int am, int bn, int lane, int wave,
                                        f32x16 (&acc)[2][2], const Then& then) {
+  constexpr int KB = OA::KB, PA = OA::PI, PB = OB::PI;
+  const auto copy = [&](int s, char* a, char* b) {
+    return [&, s, a, b](int ks) {
+      A.issue(s, a, wave, ks * PA / KB, (ks + 1) * PA / KB);
+      B.issue(s, b, wave, ks * PB / KB, (ks + 1) * PB / KB);
+    };
+  };
+  const auto none = [](int) {};
   int s = 0;
   for (; s + 3 <= n; s += 2) {
     stage_barrier();
-    A.issue(s + 1, na, wave); B.issue(s + 1, nb, wave);
-    stage_product<OA, OB>(la, lb, am, bn, 4, lane, acc);
+    stage_product<OA, OB>(la, lb, am, bn, KB, lane, acc, copy(s + 1, na, nb));
     stage_barrier();
-    A.issue(s + 2, la, wave); B.issue(s + 2, lb, wave);
-    stage_product<OA, OB>(na, nb, am, bn, 4, lane, acc);
+    stage_product<OA, OB>(na, nb, am, bn, KB, lane, acc, copy(s + 2, la, lb));
   }
   if (s + 2 == n) {
     stage_barrier();
-    A.issue(s + 1, na, wave); B.issue(s + 1, nb, wave);
-    stage_product<OA, OB>(la, lb, am, bn, 4, lane, acc);
+    stage_product<OA, OB>(la, lb, am, bn, KB, lane, acc, copy(s + 1, na, nb));
     stage_barrier();
     then(la, lb);
-    stage_product<OA, OB>(na, nb, am, bn, last, lane, acc);
+    stage_product<OA, OB>(na, nb, am, bn, last, lane, acc, none);
   } else {
     stage_barrier();
     then(na, nb);
-    stage_product<OA, OB>(la, lb, am, bn, last, lane, acc);
+    stage_product<OA, OB>(la, lb, am, bn, last, lane, acc, none);
   }
 }
 
@@ -430,7 +439,7 @@ template <int C> __device__ __forceinline__ void ring_barrier() {
 template <typename OA, typename OB>
 __device__ __forceinline__ void ring_product(const OA& A, const OB& B, int n, char* la0, char* lb0, char* la1, char* lb1,
                                              char* la2, char* lb2, int am, int bn, int lane, int wave, f32x16 (&acc)[2][2]) {
-  constexpr int C = OA::PI + OB::PI;
+  constexpr int C = OA::PI + OB::PI, KB = OA::KB;
   clear(acc);
   if (n <= 0) return;
   const auto issue = [&](int s, char* la, char* lb) {
@@ -440,8 +449,11 @@ __device__ __forceinline__ void ring_product(const OA& A, const OB& B, int n, ch
   };
   const auto step = [&](int s, char* la, char* lb, char* fa, char* fb) {
     ring_barrier<C>();
-    issue(s + 2, fa, fb);
-    stage_product<OA, OB>(la, lb, am, bn, 4, lane, acc);
+    const int f = s + 2 < n ? s + 2 : n - 1;
+    stage_product<OA, OB>(la, lb, am, bn, KB, lane, acc, [&](int ks) {
+      A.issue(f, fa, wave, ks * OA::PI / KB, (ks + 1) * OA::PI / KB);
+      B.issue(f, fb, wave, ks * OB::PI / KB, (ks + 1) * OB::PI / KB);
+    });
   };
   issue(0, la0, lb0);
   issue(1, la1, lb1);

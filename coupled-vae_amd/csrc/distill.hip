@@ -428,8 +428,9 @@ __device__ __forceinline__ void stages(const OA& A, const OB& B, int n, int last
 }
 
 // The same with three buffers, for tiles of 256 x 128 on 8 waves (one block on a CU): two stages are in flight under the
-// one that is multiplied.  Every step copies a stage (the last ones a stage that is already there), so that the count of
-// copies to wait for is a constant.
+// one that is multiplied.  A stage's barrier stands before its last K block, whose operands are in registers by then: the
+// next stage's first operands are read under that block's products, and the matrix unit does not wait for LDS behind a
+// barrier.  Past the end the last stage is copied again, so that the count of copies to wait for is a constant.
 template <int C> __device__ __forceinline__ void ring_barrier() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt(0x0070 | (C & 15) | (C >> 4) << 14);  // vmcnt(C) lgkmcnt(0)
@@ -439,32 +440,67 @@ template <int C> __device__ __forceinline__ void ring_barrier() {
 template <typename OA, typename OB>
 __device__ __forceinline__ void ring_product(const OA& A, const OB& B, int n, char* la0, char* lb0, char* la1, char* lb1,
                                              char* la2, char* lb2, int am, int bn, int lane, int wave, f32x16 (&acc)[2][2]) {
-  constexpr int C = OA::PI + OB::PI, KB = OA::KB;
+  constexpr int C = OA::PI + OB::PI, KB = OA::KB, NA = OA::PLANES, NB = OB::PLANES;
+  constexpr int SH = KB == 4 ? 3 : 2;                             // a stage's copies in SH shares
   clear(acc);
   if (n <= 0) return;
-  const auto issue = [&](int s, char* la, char* lb) {
+  h8 a[2][2][NA], b[2][2][NB];
+  const auto read = [&](int q, const char* la, const char* lb, int ks) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int pl = 0; pl < NA; ++pl) a[q][i][pl] = OA::frag(la, am + 32 * i, ks, pl, lane);
+#pragma unroll
+      for (int pl = 0; pl < NB; ++pl) b[q][i][pl] = OB::frag(lb, bn + 32 * i, ks, pl, lane);
+    }
+  };
+  const auto multiply = [&](int q) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {                               // the small products first
+        if (NB == 2) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[q][i][0], b[q][j][NB - 1], acc[i][j], 0, 0, 0);
+        if (NA == 2) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[q][i][NA - 1], b[q][j][0], acc[i][j], 0, 0, 0);
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[q][i][0], b[q][j][0], acc[i][j], 0, 0, 0);
+      }
+  };
+  const auto copy = [&](int s, char* la, char* lb, int share) {
     s = s < n ? s : n - 1;
-    A.issue(s, la, wave);
-    B.issue(s, lb, wave);
+    A.issue(s, la, wave, share * OA::PI / SH, (share + 1) * OA::PI / SH);
+    B.issue(s, lb, wave, share * OB::PI / SH, (share + 1) * OB::PI / SH);
   };
-  const auto step = [&](int s, char* la, char* lb, char* fa, char* fb) {
-    ring_barrier<C>();
-    const int f = s + 2 < n ? s + 2 : n - 1;
-    stage_product<OA, OB>(la, lb, am, bn, KB, lane, acc, [&](int ks) {
-      A.issue(f, fa, wave, ks * OA::PI / KB, (ks + 1) * OA::PI / KB);
-      B.issue(f, fb, wave, ks * OB::PI / KB, (ks + 1) * OB::PI / KB);
-    });
+  // stage s from (la, lb); stage s + 1 is in (na, nb); (fa, fb), stage s - 1's, still take stage s + 2's last shares
+  const auto step = [&](int s, char* la, char* lb, char* na, char* nb, char* fa, char* fb, bool first) {
+#pragma unroll
+    for (int ks = 0; ks + 1 < KB; ++ks) {
+      read((ks + 1) & 1, la, lb, ks + 1);
+      multiply(ks & 1);
+      if (!first && ks + 1 < SH) copy(s + 2, fa, fb, ks + 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    ring_barrier<C>();                                            // stage s + 1 is there, and all are done with stage s
+    read(0, na, nb, 0);
+    multiply((KB - 1) & 1);
+    copy(s + 3, la, lb, 0);
+    __builtin_amdgcn_sched_barrier(0);
   };
-  issue(0, la0, lb0);
-  issue(1, la1, lb1);
-  int s = 0;
+#pragma unroll
+  for (int i = 0; i < SH; ++i) copy(0, la0, lb0, i);
+#pragma unroll
+  for (int i = 0; i < SH; ++i) copy(1, la1, lb1, i);
+#pragma unroll
+  for (int i = 0; i < SH; ++i) copy(2, la2, lb2, i);
+  ring_barrier<2 * C>();
+  read(0, la0, lb0, 0);
+  step(0, la0, lb0, la1, lb1, la2, lb2, true);
+  int s = 1;
   for (; s + 3 <= n; s += 3) {
-    step(s, la0, lb0, la2, lb2);
-    step(s + 1, la1, lb1, la0, lb0);
-    step(s + 2, la2, lb2, la1, lb1);
+    step(s, la1, lb1, la2, lb2, la0, lb0, false);
+    step(s + 1, la2, lb2, la0, lb0, la1, lb1, false);
+    step(s + 2, la0, lb0, la1, lb1, la2, lb2, false);
   }
-  if (s < n) step(s, la0, lb0, la2, lb2);
-  if (s + 1 < n) step(s + 1, la1, lb1, la0, lb0);
+  if (s < n) step(s, la1, lb1, la2, lb2, la0, lb0, false);
+  if (s + 1 < n) step(s + 1, la2, lb2, la0, lb0, la1, lb1, false);
   ring_barrier<0>();                                              // no copy may land in LDS that the next block owns
 }
 // three buffers for the operand of 256 rows or columns, three for the one of 128

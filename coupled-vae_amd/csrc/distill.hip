@@ -71,7 +71,7 @@ __device__ __forceinline__ long position(const DistillArgs& p, int n) {
 __device__ __forceinline__ int scale_exp(float amax) {          // amax * 2^e in [2^13, 2^14)
   if (!(amax > 0.f)) return 0;
   const int e = P_EXP - (int)floorf(log2f(amax));
-  return e < -60 ? -60 : (e > 60 ? 60 : e);
+  return e < -110 ? -110 : (e > 110 ? 110 : e);
 }
 // largest finite magnitude of a tensor from its partials, by every thread of a block of 256
 __device__ __forceinline__ float block_amax(const float* part, float* red) {
@@ -1050,7 +1050,7 @@ template <typename T, int NP> __global__ __launch_bounds__(256) void dt_gimage_k
     ee[q] = 0;
     if (i < 0) {
       T* z = static_cast<T*>(p.dX) + (long)n * p.E;
-      if (n < p.N)
+      if (n < p.N && p.dX)
         for (int k = lane; k < p.E; k += 64) z[k] = (T)0.f;
       continue;
     }
@@ -1305,8 +1305,9 @@ __global__ __launch_bounds__(512, 2) void dt_products_kernel(DistillArgs p, int 
   __shared__ __attribute__((aligned(16))) char y1[16384];
   __shared__ __attribute__((aligned(16))) char y2[16384];
   const Ring m = {x0, x1, x2, y0, y1, y2};
-  if (blockIdx.x < DT_DX_BLOCKS) dx_items<NP, NQ, RAX>(p, m, blockIdx.x, etx, add);
-  else dw_tile<T, NP, NQ, RAW>(p, m, blockIdx.x - DT_DX_BLOCKS, etw);
+  const int behind = p.dX ? DT_DX_BLOCKS : 0;                     // either product may not be wanted
+  if ((int)blockIdx.x < behind) dx_items<NP, NQ, RAX>(p, m, blockIdx.x, etx, add);
+  else dw_tile<T, NP, NQ, RAW>(p, m, blockIdx.x - behind, etw);
 }
 
 // ------------------------------------------------------------------------------------------------- host side
@@ -1424,7 +1425,7 @@ template <typename T, int NP, int NQ, bool TWO> static int dt_backward(const Dis
     CVAE_LAUNCH_CHECK("dt_grad_kernel");
     hipLaunchKernelGGL((dt_pick_kernel<NQ, TWO>), dim3(cdiv(a.N, 4)), dim3(256), 0, s, a);
     CVAE_LAUNCH_CHECK("dt_pick_kernel");
-    const dim3 grid((unsigned)(DT_DX_BLOCKS + (long)cdiv(a.vc / (384 - d.raw), 8) * 8 * d.etw));
+    const dim3 grid((unsigned)((a.dX ? DT_DX_BLOCKS : 0) + (a.dW ? (long)cdiv(a.vc / (384 - d.raw), 8) * 8 * d.etw : 0)));
     const int add = v0 > 0 ? 1 : 0;
     if (d.rax == 256 && d.raw == 256) hipLaunchKernelGGL((dt_products_kernel<T, NP, NQ, 256, 256>), grid, dim3(512), 0, s, a, d.et, d.etw, add);
     else if (d.rax == 256) hipLaunchKernelGGL((dt_products_kernel<T, NP, NQ, 256, 128>), grid, dim3(512), 0, s, a, d.et, d.etw, add);
@@ -1432,6 +1433,7 @@ template <typename T, int NP, int NQ, bool TWO> static int dt_backward(const Dis
     else hipLaunchKernelGGL((dt_products_kernel<T, NP, NQ, 128, 128>), grid, dim3(512), 0, s, a, d.et, d.etw, add);
     CVAE_LAUNCH_CHECK("dt_products_kernel");
   }
+  if (!a.dX) return 0;
   const dim3 gs((unsigned)((long)(d.Np / (384 - d.rax)) * d.et * 32));
   if (d.rax == 256) hipLaunchKernelGGL((dt_dx_sum_kernel<T, NQ, 256>), gs, dim3(256), 0, s, a, d.et);
   else hipLaunchKernelGGL((dt_dx_sum_kernel<T, NQ, 128>), gs, dim3(256), 0, s, a, d.et);
@@ -1469,8 +1471,10 @@ int launch_distill_backward(const DistillCall& c, const float* ghard, const floa
   CVAE_TRY(dt_check("distill_backward", c));
   CVAE_REQUIRE((int64_t)c.T * c.R > 0, "distill_backward: no rows");
   CVAE_REQUIRE((int64_t)c.T * c.R <= (1 << 22), "distill_backward: more than %d rows", 1 << 22);   // 32-bit lane offsets in P
-  CVAE_REQUIRE(c.X && c.W && c.b && c.eos && ghard && saved && dX && dW && db && ws && (c.K == 0 || (c.ids && c.top && gsoft)),
+  CVAE_REQUIRE(c.X && c.W && c.b && c.eos && ghard && saved && ws && (c.K == 0 || (c.ids && c.top && gsoft)),
                "distill_backward: null operand");
+  CVAE_REQUIRE((dW == nullptr) == (db == nullptr), "distill_backward: dW and db go together");
+  if (!dX && !dW) return 0;
   CVAE_REQUIRE((((uintptr_t)ws | (uintptr_t)saved) & 15) == 0, "distill_backward: the workspaces must be 16-byte aligned");
   const DistillPlan d = dt_plan(c.dtype, (long)c.T * c.R, c.E, (int)c.V, c.K);
   DistillArgs a = {};

@@ -661,7 +661,10 @@ class ProjDistillFn(torch.autograd.Function):
         if T * R == 0:
             return (torch.zeros_like(final), torch.zeros_like(W), torch.zeros_like(b)) + (None,) * 6
         ghard, gsoft = _c(ghard), _c(gsoft)
-        dfinal, dW, db = torch.empty_like(final), torch.empty_like(W), torch.empty_like(b)
+        dfinal = torch.empty_like(final) if ctx.needs_input_grad[0] else None
+        dW = db = None
+        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+            dW, db = torch.empty_like(W), torch.empty_like(b)
         ws = _f((query('cvae_distill_backward_workspace', dt, T * R, E, V, K),), final)
         call('cvae_distill_backward', dt, ptr(final), ptr(W), ptr(b), ptr(eos), *args, ptr(ids), ptr(top), tau, ptr(ghard),
              ptr(gsoft), ptr(saved), ptr(dfinal), ptr(dW), ptr(db), ptr(ws), stream())
@@ -685,7 +688,7 @@ def proj_distill(final, W, b, eos, pad, teacher_ids, teacher_logits, tau):
     absent entries).  With p = softmax(teacher_logits / tau) over the K entries and q_tau = softmax(logits / tau) over
     the whole vocabulary:
       hard (R,) = sum_t -log softmax(logits)[target],   soft (R,) = sum_t tau^2 KL(p || q_tau)
-    -> (hard, soft) fp32, differentiable in final, W and b."""
+    -> (hard, soft) fp32, differentiable in final, W and b (no gradient reaches the teacher)."""
     _proj_check(final, W, b, eos)
     _need(teacher_ids.dim() == 3 and teacher_ids.dtype == torch.int64 and
           tuple(teacher_ids.shape[:2]) == tuple(eos.shape) and 0 < teacher_ids.shape[2] <= min(W.shape[0], 1024),

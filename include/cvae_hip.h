@@ -279,7 +279,7 @@ int cvae_distill_forward(int dtype, const void* final, const void* W, const void
                          int sentence_major, int B, int T, int R, int E, int64_t V, int K, const int64_t* ids,
                          const float* top, float tau, float* hard, float* soft, float* ws, void* stream);
 /* ghard[R], gsoft[R] = dL/dhard, dL/dsoft -> dfinal[T*R,E], dW[V,E], db[V] of `dtype`, overwritten.  The other arguments
- * as in the forward call; at most 2^22 rows.  ws: cvae_distill_backward_workspace floats, 16-byte aligned. */
+ * as in the forward call; at most 2^22 rows.  dfinal, or dW and db, may be NULL: not wanted, and not computed.  ws: cvae_distill_backward_workspace floats, 16-byte aligned. */
 int64_t cvae_distill_backward_workspace(int dtype, int64_t N, int64_t E, int64_t V, int K);
 int cvae_distill_backward(int dtype, const void* final, const void* W, const void* b, const int64_t* eos, int64_t pad,
                           int sentence_major, int B, int T, int R, int E, int64_t V, int K, const int64_t* ids,

@@ -254,3 +254,20 @@ def test_captured_and_replayed(dev):
         torch.cuda.synchronize()
         for k, v in work().items():
             assert torch.equal(out[k], v), (seed, k)
+
+
+def test_offsets_past_32_bits(dev):
+    """2.2e9 pre-activations: a row's results do not depend on how many rows there are (same kernels, same order of work)."""
+    T, B, H = 16800, 64, 1024
+    assert T * B * 2 * H > 2 ** 31
+    g = torch.Generator(device=dev).manual_seed(0)
+    u = torch.empty(T, B, 2 * H, dtype=torch.bfloat16, device=dev)
+    dy = torch.empty(T, B, H, dtype=torch.bfloat16, device=dev)
+    for t in range(0, T, 2100):
+        u[t:t + 2100] = torch.randn(2100, B, 2 * H, generator=g, device=dev).bfloat16()
+        dy[t:t + 2100] = torch.randn(2100, B, H, generator=g, device=dev).bfloat16()
+    h0, dlast = torch.randn(B, H, generator=g, device=dev), torch.randn(B, H, generator=g, device=dev)
+    whole = run(u, 2, h0, None, False, dy, dlast)
+    part = run(u[:, 32:].contiguous(), 2, h0[32:], None, False, dy[:, 32:].contiguous(), dlast[32:])
+    assert torch.equal(whole['y'][:, 32:], part['y']) and torch.equal(whole['du'][:, 32:], part['du'])
+    assert torch.equal(whole['last'][32:], part['last']) and torch.equal(whole['dh0'][32:], part['dh0'])

@@ -311,6 +311,30 @@ def test_one_loss_alone_and_a_second_backward(dev):
                 check(v, want[k], k, 40, 210, 24)
 
 
+def test_only_the_gradients_that_are_wanted(dev):
+    """Frozen weights, or a frozen decoder: the other gradients do not change."""
+    from cvae_amd import ops
+    a = inputs(6, 5, 5, 72, 900, 4, 'f32', 17)
+    full = run(dev, a, 2.0)
+    for wanted in (('final',), ('W', 'b'), ('W',), ('b', 'final')):
+        leaves = {k: a[k].to(dev).requires_grad_(k in wanted) for k in ('final', 'W', 'b')}
+        hard, soft = ops.proj_distill(*leaves.values(), a['eos'].to(dev), PAD, a['ids'].to(dev), a['top'].to(dev), 2.0)
+        grads = torch.autograd.grad([hard, soft], [leaves[k] for k in wanted], [a['gh'].to(dev), a['gs'].to(dev)])
+        for k, v in zip(wanted, grads):
+            assert torch.equal(v, full['d' + k]), (wanted, k)
+
+
+def test_a_teacher_that_is_not_a_number(dev):
+    """A NaN among a row's teacher logits makes its sentence's soft loss NaN, and only that."""
+    from cvae_amd import ops
+    a = inputs(4, 3, 3, 16, 60, 4, 'f32', 18)
+    a['eos'] = torch.where(a['eos'] == PAD, 3, a['eos'])
+    a['top'][1, 2, 3] = float('nan')
+    args = [a[k].to(dev) for k in ('final', 'W', 'b')]
+    hard, soft = ops.proj_distill(*args, a['eos'].to(dev), PAD, a['ids'].to(dev), a['top'].to(dev), 2.0)
+    assert bool(torch.isfinite(hard).all()) and torch.isnan(soft).tolist() == [False, True, False]
+
+
 def test_gradient_against_differences(dev):
     """fp32, along one direction of W, b and final: the quotient of differences and the gradient agree within the e^2 term
     (measured by halving e) and the noise of the losses themselves (their derived bounds over e)."""

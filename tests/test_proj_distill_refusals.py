@@ -74,6 +74,9 @@ def test_c_entries_refuse_bad_arguments():
                     dict(V=1 << 31), dict(K=-1), dict(K=11), dict(K=1025, V=2000), dict(tau=0.0), dict(tau=float('nan')), dict(ws=None), dict(ws=24)):
             with pytest.raises(_lib.CvaeHipError, match='distill_'):
                 f(**bad)
+    with pytest.raises(_lib.CvaeHipError, match='go together'):
+        _lib.call('cvae_distill_backward', 0, one, one, one, one, 0, 0, 2, 4, 2, 8, 10, 3, one, one, 2.0, one, one, one, one,
+                  None, one, one, None)
     with pytest.raises(_lib.CvaeHipError, match='rows'):
         backward(T=1 << 14, R=1 << 9)
     for name in ('cvae_distill_workspace', 'cvae_distill_backward_workspace'):      # sizes of nothing, or refused ones: 0

@@ -197,9 +197,9 @@ __global__ __launch_bounds__(64 * LR_W) void linrnn_maps_kernel(LinRnnArgs p) {
   }
 }
 
-// Bound by memory: u is read once, y written once.  2000 steps x 32 rows x 2048, three gates, bf16, ragged: 230 us, 3.7 TB/s of what
-// live steps need (a large copy: 4.7); 110 x 32 x 512 fp32 10.5 us.  Asking for the next round's rows early cost
-// registers, hence blocks on a CU: 292 us.
+// Bound by memory: u is read once, y written once.  2000 steps x 32 rows x 2048, three gates, bf16, ragged: 230 us, 3.7
+// TB/s of what live steps need (a large copy: 4.7); 110 x 32 x 512 fp32 10.5 us.  Asking for the next round's rows
+// early cost registers, hence blocks on a CU: 292 us.
 template <typename T, int VW, int G>
 __global__ __launch_bounds__(64 * LR_W) void linrnn_fwd_kernel(LinRnnArgs p) {
   __shared__ float lds[2][LR_W][2][64 * VW];
@@ -307,7 +307,7 @@ __global__ __launch_bounds__(64 * LR_W, 4) void linrnn_bwd_kernel(LinRnnArgs p) 
     enter_segment<VW>(p, L, seg, true, wave, nw, lane, reinterpret_cast<float (*)[2][64 * VW]>(&lds[0][0][0][0]), carry);
   int buf = 0;
   const int R = LR_C * nw;                        // steps of a round: 64, or the whole of a shorter sequence
-  for (int sc = s0 + (s1 - s0 - 1) / R * R; sc >= s0; sc -= R, buf ^= 1) {
+  for (int sc = s0 + (s1 - s0 + R - 1) / R * R - R; sc >= s0; sc -= R, buf ^= 1) {   // (no steps: no round)
     const int w0 = sc + wave * LR_C, w1 = min(s1, w0 + LR_C);
     const Steps st = steps_of<VW>(p, L, w0, w1);
     float hin[VW];
@@ -513,6 +513,8 @@ int launch_linrnn_forward(int dtype, int gates, int reverse, int T, int B, int H
   a.u = u; a.h0 = h0; a.len = len; a.y = y; a.h_last = h_last; a.bounds = bounds; a.agg = ws;
   lr_plan(dtype, T, B, H, &a.nseg, &a.seg);
   CVAE_REQUIRE(a.nseg == 1 || ws, "linrnn_forward: null workspace");
+  // every segment starts from h0, and the last one may end before another begins
+  CVAE_REQUIRE(a.nseg == 1 || h_last != h0, "linrnn_forward: h_last may be h0 only where no workspace is needed");
   return lr_dispatch(dtype, a, false, s);
 }
 

@@ -551,6 +551,10 @@ def linear_rnn(u, gates, h0=None, length=None, reverse=False):
     return LinearRnnFn.apply(_c(u), gates, _c(h0), _c(length), reverse)
 
 
+def _overlap(at, size, t):
+    return at < t.data_ptr() + t.numel() * t.element_size() and t.data_ptr() < at + size
+
+
 def linear_rnn_step(u, gates, h, out=None):
     """One decoding step of linear_rnn: u (B,gates*H), state h (B,H) fp32 -> y (B,H) of u's type, the new state
     (B,H) fp32 (written to `out` if given; out = h updates it in place).  No gradient."""
@@ -563,6 +567,9 @@ def linear_rnn_step(u, gates, h, out=None):
           'out must be contiguous float32 of shape (B, H)')
     _here(u, h, out)
     u, h = _c(u), _c(h)
+    at, size = out.data_ptr(), 4 * B * H
+    _need(at == h.data_ptr() or not _overlap(at, size, h), 'out must be h itself or must not overlap it')
+    _need(not _overlap(at, size, u), 'out must not overlap u')
     y = torch.empty((B, H), dtype=u.dtype, device=u.device)
     call('cvae_linrnn_forward', _DTYPE[u.dtype], gates, 0, 1, B, H, ptr(u), ptr(h), None, ptr(y), ptr(out), None, None,
          stream())

@@ -202,7 +202,8 @@ int cvae_decoder_backward_n(int nd, int cell, int B, int T, int E, int Hd, int64
  * dtype: storage of u, y, dy, du: 0 = fp32, 1 = bf16, 2 = fp16 (the state, h0, h_last and their gradients are fp32).
  * gates: 3 = rows z|n|o, 2 = rows z|n (y_t = h_t).  u[T,B,gates*H], h0[B,H] or NULL (zeros), len[B] or NULL (all T; a
  * value outside [0,T] counts as the nearer end): row b takes steps t < len[b] -- upwards, or with reverse != 0 downwards
- * from len[b]-1 -- and past them y = 0, the state is carried and du = 0.  y[T,B,H], h_last[B,H] (may be h0: in place).
+ * from len[b]-1 -- and past them y = 0, the state is carried and du = 0.  y[T,B,H], h_last[B,H] (may be h0, in place, where
+ * cvae_linrnn_workspace is 0; else that call is refused).
  * states: NULL, or cvae_linrnn_state_floats floats that the backward call reads (the state every 64 steps).
  * ws: cvae_linrnn_workspace floats (0: may be NULL). */
 int64_t cvae_linrnn_state_floats(int T, int B, int H);

@@ -271,3 +271,30 @@ def test_offsets_past_32_bits(dev):
     part = run(u[:, 32:].contiguous(), 2, h0[32:], None, False, dy[:, 32:].contiguous(), dlast[32:])
     assert torch.equal(whole['y'][:, 32:], part['y']) and torch.equal(whole['du'][:, 32:], part['du'])
     assert torch.equal(whole['last'][32:], part['last']) and torch.equal(whole['dh0'][32:], part['dh0'])
+
+
+def test_gradients_of_no_steps(dev):
+    """A sequence of length zero hands its initial state on, and the state's gradient back."""
+    from cvae_amd import ops
+    h0 = torch.randn(2, 4, device=dev, requires_grad=True)
+    u = torch.empty(0, 2, 8, device=dev, requires_grad=True)
+    y, last = ops.linear_rnn(u, 2, h0=h0)
+    g = torch.randn(2, 4, device=dev)
+    du, dh0 = torch.autograd.grad((y, last), (u, h0), (torch.empty(0, 2, 4, device=dev), g))
+    assert du.shape == u.shape and torch.equal(dh0, g)
+
+
+def test_step_refuses_an_overlapping_out(dev):
+    from cvae_amd import ops
+    B, H = 3, 8
+    room = torch.randn(2 * B * 3 * H, device=dev)
+    u, h = room[:B * 3 * H].view(B, 3 * H), room[B * 3 * H:B * 4 * H].view(B, H)
+    keep = room.clone()
+    for at in (B * 3 * H + 1, B * 3 * H + B * H - 1, B * 3 * H - 1, 0):
+        with pytest.raises(ValueError, match='overlap'):
+            ops.linear_rnn_step(u, 3, h, out=room[at:at + B * H].view(B, H))
+    assert torch.equal(room, keep)
+    want = ops.linear_rnn_step(u, 3, h)[1]
+    out = room[B * 4 * H:B * 5 * H].view(B, H)                    # right behind the state
+    ops.linear_rnn_step(u, 3, h, out=out)
+    assert torch.equal(out, want) and torch.equal(room[:B * 4 * H], keep[:B * 4 * H])

@@ -63,3 +63,10 @@ def test_c_entries_refuse_bad_arguments():
         _lib.call(name, 0, 3, 0, 4, 0, 8, *([None] * n))
     for sizes in ((0, 2, 8), (4, 0, 8), (4, 2, 0), (0, 0, 0), (1, 1, 1)):
         assert _lib.query('cvae_linrnn_workspace', 0, *sizes) == 0
+
+
+def test_in_place_state_of_a_segmented_sequence_is_refused():
+    """Segments run at once and each starts from h0, so the last one must not overwrite it."""
+    assert _lib.query('cvae_linrnn_workspace', 0, 1000, 1, 8) > 0
+    with pytest.raises(_lib.CvaeHipError, match='h_last may be h0'):
+        _lib.call('cvae_linrnn_forward', 0, 3, 0, 1000, 1, 8, 16, 16, None, 16, 16, None, 16, None)

@@ -135,7 +135,6 @@ template <typename T> __global__ __launch_bounds__(256) void dt_count_kernel(Dis
     return;
   }
   // (what stands in dropped rows does not set the scale of the others)
-  // (what stands in dropped rows does not set the scale of the others)
   const int b = blockIdx.x - nb, which = b / DT_AMAX, slot = b % DT_AMAX;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   float m = 0.f;

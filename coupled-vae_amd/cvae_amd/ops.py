@@ -557,19 +557,20 @@ def _overlap(at, size, t):
 
 def linear_rnn_step(u, gates, h, out=None):
     """One decoding step of linear_rnn: u (B,gates*H), state h (B,H) fp32 -> y (B,H) of u's type, the new state
-    (B,H) fp32 (written to `out` if given; out = h updates it in place).  No gradient."""
+    (B,H) fp32 (written to `out` if given; out = h updates it in place, no other overlap).  No gradient."""
     _linear_rnn_check(u, gates, h, 2)
     _need(h is not None, 'the state is missing')
     B, H = h.shape
-    if out is None:
-        out = _f((B, H), u)
-    _need(out.dtype == torch.float32 and out.shape == h.shape and out.is_contiguous(),
+    _need(out is None or (out.dtype == torch.float32 and out.shape == h.shape and out.is_contiguous()),
           'out must be contiguous float32 of shape (B, H)')
     _here(u, h, out)
     u, h = _c(u), _c(h)
-    at, size = out.data_ptr(), 4 * B * H
-    _need(at == h.data_ptr() or not _overlap(at, size, h), 'out must be h itself or must not overlap it')
-    _need(not _overlap(at, size, u), 'out must not overlap u')
+    if out is None:
+        out = _f((B, H), u)
+    else:
+        at, size = out.data_ptr(), 4 * B * H
+        _need(at == h.data_ptr() or not _overlap(at, size, h), 'out must be h itself or must not overlap it')
+        _need(not _overlap(at, size, u), 'out must not overlap u')
     y = torch.empty((B, H), dtype=u.dtype, device=u.device)
     call('cvae_linrnn_forward', _DTYPE[u.dtype], gates, 0, 1, B, H, ptr(u), ptr(h), None, ptr(y), ptr(out), None, None,
          stream())

@@ -270,9 +270,9 @@ int cvae_projce_backward_saved_n(int nd, const float* const* final, const float*
  * are fp32.  final[T*R,E] (rows n = t*R + r), W[V,E], b[V], eos[B,T] targets: row r reads sentence r % B, or r / (R / B)
  * if sentence_major (R % B == 0).  Rows whose target is `pad` have no loss and no gradient; a target outside [0,V) that
  * is not `pad` counts as a logit of 0 (as in cvae_projce_*).
- * 0 <= K <= min(V, 1024) entries of the teacher at every position: ids[B,T,K], top[B,T,K]; an entry whose id is outside [0,V) or whose
- * logit is -inf is absent, a row with no entry has soft = 0; an id may be listed twice.  K = 0: ids, top, soft (and
- * gsoft) are not read and tau is ignored.
+ * 0 <= K <= min(V, 1024) entries of the teacher at every position: ids[B,T,K], top[B,T,K]; an entry whose id is outside
+ * [0,V) or whose logit is -inf is absent, a row with no entry has soft = 0; an id may be listed twice.  K = 0: ids, top,
+ * soft (and gsoft) are not read and tau is ignored.
  * -> hard[R], soft[R]: sums over t.  ws: cvae_distill_workspace(dtype, T*R, E, V, K) floats, 16-byte aligned; the backward
  * call reads it (`saved`). */
 int64_t cvae_distill_workspace(int dtype, int64_t N, int64_t E, int64_t V, int K);
@@ -280,7 +280,8 @@ int cvae_distill_forward(int dtype, const void* final, const void* W, const void
                          int sentence_major, int B, int T, int R, int E, int64_t V, int K, const int64_t* ids,
                          const float* top, float tau, float* hard, float* soft, float* ws, void* stream);
 /* ghard[R], gsoft[R] = dL/dhard, dL/dsoft -> dfinal[T*R,E], dW[V,E], db[V] of `dtype`, overwritten.  The other arguments
- * as in the forward call; at most 2^22 rows.  dfinal, or dW and db, may be NULL: not wanted, and not computed.  ws: cvae_distill_backward_workspace floats, 16-byte aligned. */
+ * as in the forward call; at most 2^22 rows.  dfinal, or dW and db, may be NULL: not wanted, and not computed.
+ * ws: cvae_distill_backward_workspace floats, 16-byte aligned. */
 int64_t cvae_distill_backward_workspace(int dtype, int64_t N, int64_t E, int64_t V, int K);
 int cvae_distill_backward(int dtype, const void* final, const void* W, const void* b, const int64_t* eos, int64_t pad,
                           int sentence_major, int B, int T, int R, int E, int64_t V, int K, const int64_t* ids,

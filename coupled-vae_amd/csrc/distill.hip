@@ -712,32 +712,46 @@ __global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
       }
     }
     if (t0 < t1) {
+      const auto ring = [&](int g) -> char* { return (g & 3) == 0 ? w0 : (g & 3) == 1 ? w1 : (g & 3) == 2 ? w2 : w3; };
+      const auto copy = [&](const char* from, char* w) {          // a stage: 16 KiB
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + off[i]),
+                                           (__attribute__((address_space(3))) void*)(w + (wave * 4 + i) * 1024), 16, 0, 0);
+      };
+      // one operand of 32 rows from `r`, K block ks of a stage, plane pl
+      const auto frag = [&](const char* w, int r, int ks, int pl) {
+        const int ch = NP == 1 ? (ks * 2 + lhi) ^ ((r >> 1) & 7) : ((ks >> 1) * 8 + pl * 4 + (ks & 1) * 2 + lhi) ^ (r & 15);
+        return *reinterpret_cast<const h8*>(w + r * RB + ch * 16);
+      };
+      // the rows pass through the ring once: read from memory straight into operands they would come 32 bytes a row at a time
       h8 xf[NJ][NP][NK];
 #pragma unroll
-      for (int j = 0; j < NJ; ++j)
+      for (int half = 0; half < NP; ++half) {
 #pragma unroll
-        for (int pl = 0; pl < NP; ++pl)
+        for (int st = 0; st < NST; ++st)
+          copy(reinterpret_cast<const char*>(p.Ximg) + (n0 + half * 64) * ld + st * RB, ring(st));
+        ring_barrier<0>();
+        if (NP == 1 || wave >> 1 == half) {
 #pragma unroll
-          for (int kb = 0; kb < NK; ++kb) {
-            const int k = kb * 16 + lhi * 8;
-            xf[j][pl][kb] = *reinterpret_cast<const h8*>(reinterpret_cast<const char*>(p.Ximg) + (n0 + bn + 32 * j + l31) * ld +
-                                                         (NP == 1 ? k * 2 : (k >> 5) * 128 + pl * 64 + (k & 31) * 2));
-          }
+          for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int pl = 0; pl < NP; ++pl)
+#pragma unroll
+              for (int kb = 0; kb < NK; ++kb) xf[j][pl][kb] = frag(ring(kb / 4), (NP == 1 ? bn + 32 * j : bn & 32) + l31, kb & 3, pl);
+        }
+        ring_barrier<0>();
+      }
       const char* W = reinterpret_cast<const char*>(p.Wimg) + (long)(GRAD ? p.v0 : 0) * ld;
       const float* b2 = p.b2 + (GRAD ? p.v0 : 0);
       const auto issue = [&](int tile, int st, char* w) {         // (past the range: its last tile again)
         tile = tile < t1 ? tile : t1 - 1;
-        const char* b = W + (long)tile * VT * ld + st * RB;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(b + off[i]),
-                                           (__attribute__((address_space(3))) void*)(w + (wave * 4 + i) * 1024), 16, 0, 0);
+        copy(W + (long)tile * VT * ld + st * RB, w);
         if (st == NST - 1)
           __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(
                                                reinterpret_cast<const char*>(b2 + tile * VT) + boff + lane * 4),
                                            (__attribute__((address_space(3))) void*)(w + DT_STAGE + boff), 4, 0, 0);
       };
-      const auto ring = [&](int g) -> char* { return (g & 3) == 0 ? w0 : (g & 3) == 1 ? w1 : (g & 3) == 2 ? w2 : w3; };
 #pragma unroll
       for (int g = 0; g < 3; ++g) issue(t0 + g / NST, g % NST, ring(g));
       for (int tile = t0; tile < t1; tile += 4 / NST) {
@@ -777,11 +791,7 @@ __global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
 #pragma unroll
               for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int pl = 0; pl < NP; ++pl) {
-                  const int r = am + 32 * i + l31;
-                  const int ch = NP == 1 ? (ks * 2 + lhi) ^ ((r >> 1) & 7) : ((ks >> 1) * 8 + pl * 4 + (ks & 1) * 2 + lhi) ^ (r & 15);
-                  a[i][pl] = *reinterpret_cast<const h8*>(w + r * RB + ch * 16);
-                }
+                for (int pl = 0; pl < NP; ++pl) a[i][pl] = frag(w, am + 32 * i + l31, ks, pl);
 #pragma unroll
               for (int i = 0; i < 2; ++i)
 #pragma unroll

@@ -289,6 +289,15 @@ template <typename T, int NP> __global__ __launch_bounds__(256) void dt_image_ke
 //   K down the rows (KS = true): RT columns, that is RT NP / 64 pieces, of KR rows a stage.
 // In LDS, 16-byte chunk c of row r sits at chunk c ^ (r / 2 & 7) of its 128 bytes (KS: c ^ 4 (r & 3)): the chunks that
 // 16 lanes of a read take lie in different banks of the 64 (c ^ (r & 7) left two rows in each: half of all LDS cycles).
+//
+// A copy takes its address as a scalar base and 32 bits a lane (64-bit addresses a lane cost the walk at E = 200 two additions a
+// copy and the registers for them: 148 -> 135 us).
+template <int BYTES> __device__ __forceinline__ void copy_lds(const void* base, unsigned off, void* lds) {
+  const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, -1, 0x27000);
+  auto* to = (__attribute__((address_space(3))) void*)lds;
+  if constexpr (BYTES == 16) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, to, 16, off, 0, 0, 0);
+  else __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, to, 4, off, 0, 0, 0);
+}
 template <int NP, bool KS, int RT, int NW, int KR = 64 / NP> struct Operand {
   static constexpr int PLANES = NP, KB = KR / 16;                 // K blocks of 16 in a stage
   static constexpr int PI = RT * 2 * NP * KR / 1024 / NW;         // copies of 1 KiB a wave and stage
@@ -317,9 +326,7 @@ template <int NP, bool KS, int RT, int NW, int KR = 64 / NP> struct Operand {
   __device__ __forceinline__ void issue(int stage, char* lds, int wave, int i0 = 0, int i1 = PI) const {
     const char* b = base + (KS ? (long)stage * KR * row : (long)stage * grp);
 #pragma unroll
-    for (int i = i0; i < i1; ++i)
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(b + off[i]),
-                                       (__attribute__((address_space(3))) void*)(lds + (wave * PI + i) * 1024), 16, 0, 0);
+    for (int i = i0; i < i1; ++i) copy_lds<16>(b, off[i], lds + (wave * PI + i) * 1024);
   }
   // the 32 rows / columns from `c0`, K block `ks` of the stage, plane `pl`, as one MFMA operand
   static __device__ __forceinline__ h8 frag(const char* lds, int c0, int ks, int pl, int lane) {
@@ -535,8 +542,8 @@ __device__ __forceinline__ int dt_splits(int nt, int vt, int least) {
 // all 29 row tiles at once: 504).
 __device__ __forceinline__ void walk_order(int q, int nt, int ranges, int& tn, int& range) {
   const int group = q / (8 * ranges), rem = q - group * 8 * ranges, size = min(8, nt - 8 * group);
-  range = rem / size;
-  tn = group * 8 + rem - range * size;
+  range = __builtin_amdgcn_readfirstlane(rem / size);             // (scalar, for the copies' addresses)
+  tn = __builtin_amdgcn_readfirstlane(group * 8 + rem - range * size);
 }
 
 // Fold 64 vocabulary entries of a lane's row into its running (max, sum) pairs, base 2: two accumulator tiles of 32
@@ -608,7 +615,7 @@ __global__ __launch_bounds__(256, 2) void dt_forward_kernel(DistillArgs p) {
   DT_LDS
   const int nl = *p.nlive, nt = (nl + DT_TILE - 1) / DT_TILE, vt = p.fvt;
   if (nt == 0) return;
-  const int splits = dt_splits(nt, vt, p.least), per = (vt + splits - 1) / splits;
+  const int splits = dt_splits(nt, vt, p.least), per = __builtin_amdgcn_readfirstlane((vt + splits - 1) / splits);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int am = (wave >> 1) * 64, bn = (wave & 1) * 64;
   const int e = p.sexp[0] + p.sexp[1];
@@ -678,7 +685,7 @@ __global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
   __shared__ __attribute__((aligned(16))) char turn[GRAD ? 8192 : 3072];
   const int nl = *p.nlive, nt = (nl + DT_TILE - 1) / DT_TILE, vt = GRAD ? p.vc / VT : p.fvt;
   if (nt == 0) return;
-  const int splits = dt_splits(nt, vt, 1), per = (vt + splits - 1) / splits;
+  const int splits = dt_splits(nt, vt, 1), per = __builtin_amdgcn_readfirstlane((vt + splits - 1) / splits);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int am = NP == 1 ? (wave >> 1) * 64 : 0, bn = NP == 1 ? (wave & 1) * 64 : wave * 32;
   const int l31 = lane & 31, lhi = lane >> 5;
@@ -695,7 +702,7 @@ __global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
   const int boff = NP == 1 ? (wave & 1) * 256 : 0;                // each wave copies 64 of the tile's biases
   const int xcd = blockIdx.x & 7, per_xcd = nt * (splits / 8);
   for (int q = blockIdx.x >> 3; q < per_xcd; q += DT_WALK_BLOCKS / 8) {
-    const int split = xcd + 8 * (q / nt), n0 = (q % nt) * DT_TILE;
+    const int range = __builtin_amdgcn_readfirstlane(q / nt), split = xcd + 8 * range, n0 = (q - range * nt) * DT_TILE;
     const int t0 = split * per, t1 = min(vt, t0 + per);
     if (GRAD && t0 >= t1) continue;
     float m[NJ], s1[NJ], s2[NJ];                                  // GRAD: L1, a, then L2, b
@@ -715,9 +722,7 @@ __global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
       const auto ring = [&](int g) -> char* { return (g & 3) == 0 ? w0 : (g & 3) == 1 ? w1 : (g & 3) == 2 ? w2 : w3; };
       const auto copy = [&](const char* from, char* w) {          // a stage: 16 KiB
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + off[i]),
-                                           (__attribute__((address_space(3))) void*)(w + (wave * 4 + i) * 1024), 16, 0, 0);
+        for (int i = 0; i < 4; ++i) copy_lds<16>(from, off[i], w + (wave * 4 + i) * 1024);
       };
       // one operand of 32 rows from `r`, K block ks of a stage, plane pl
       const auto frag = [&](const char* w, int r, int ks, int pl) {
@@ -748,9 +753,7 @@ __global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
         tile = tile < t1 ? tile : t1 - 1;
         copy(W + (long)tile * VT * ld + st * RB, w);
         if (st == NST - 1)
-          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(
-                                               reinterpret_cast<const char*>(b2 + tile * VT) + boff + lane * 4),
-                                           (__attribute__((address_space(3))) void*)(w + DT_STAGE + boff), 4, 0, 0);
+          copy_lds<4>(b2 + tile * VT, boff + lane * 4, w + DT_STAGE + boff);
       };
 #pragma unroll
       for (int g = 0; g < 3; ++g) issue(t0 + g / NST, g % NST, ring(g));

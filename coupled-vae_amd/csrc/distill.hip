@@ -518,8 +518,6 @@ __device__ __forceinline__ void ring_product(const OA& A, const OB& B, int n, ch
 }
 // three buffers for the operand of 256 rows or columns, three for the one of 128
 struct Ring { char *x0, *x1, *x2, *y0, *y1, *y2; };
-// value r of an accumulator tile: row 4 (lane / 32) + 8 (r / 4) + r % 4, column lane % 32
-__device__ __forceinline__ int acc_row(int r, int lane) { return (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5); }
 
 // ------------------------------------------------------------------------------------------------- forward
 // Work items of the kernels that walk the vocabulary: (tile of 128 live rows) x (range of its vt tiles).  512 blocks, two

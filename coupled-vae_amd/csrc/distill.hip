@@ -16,8 +16,8 @@
 //
 // What bounds it: 8 N E V operations (S twice, dX, dW; fp32 three times that) against reads of X and W and writes of their
 // gradients, so from a few hundred rows on the matrix cores do, and beside them two exponentials an element and pass at small
-// E.  Measured on live rows, forward and backward: 3650 rows x 1024 x 50000 bf16 1.74 ms (1.49 TFLOP, 0.86 PFLOP/s of useful work;
-// a large library product runs at 1.38), 4815 x 200 x 50000 bf16 with 64 teacher entries at tau 2 0.75 ms.
+// E.  Measured on live rows, forward and backward: 3650 rows x 1024 x 50000 bf16 1.62 ms (1.49 TFLOP, 0.92 PFLOP/s of
+// useful work; a large library product runs at 1.38), 4815 x 200 x 50000 bf16 with 64 teacher entries at tau 2 0.72 ms.
 //
 // Image layout: rows of 128-byte pieces, one plane: 64 values, two planes: 32 hi values then 32 lo values.  A piece is
 // what one row adds to a pipeline stage, so one loop serves both.  Rows are padded to 128 with zeros, columns to 64.
@@ -606,8 +606,9 @@ __device__ __forceinline__ void store_pairs(const DistillArgs& p, float* x, cons
 
 // The forward walk for any E: both operands stream through LDS, a stage of 64 K values (two planes: 32) loading under the
 // one that is multiplied, four waves of 64 x 64 each, two blocks on a CU so that one's fold runs under the other's products.
-// 3650 rows x 1024 x 50000 bf16: 461 us, 0.81 PFLOP/s, matrix cores busy 45 % of the time at 1.93 GHz; fold and pipeline
-// restarts between tiles are the rest.  (256 x 128 tiles of eight waves, one block on a CU: 529, its fold stands alone.)
+// 3650 rows x 1024 x 50000 bf16: 415 us, 0.90 PFLOP/s, matrix cores busy 53 % of the time at 1.81 GHz; fold and pipeline
+// restarts between tiles are the rest.  (256 x 128 tiles of eight waves, one block on a CU: 529 where this took 461, its
+// fold stands alone.)
 template <int NP, bool TWO>
 __global__ __launch_bounds__(256, 2) void dt_forward_kernel(DistillArgs p) {
   DT_LDS
@@ -670,9 +671,10 @@ __global__ __launch_bounds__(256, 2) void dt_forward_kernel(DistillArgs p) {
 // at E = 200 spends its time on them.  Stages of 64 K values x 128 (64) words, four buffers, three in flight; K blocks
 // of 16: NK = 4, 8 or 13 (E up to 64, 128, 208; every shipped model has E = 200).  GRAD: instead of folding, the tile
 // leaves as P = a 2^(t - L1) + b 2^(t / tau - L2), through 2 KiB of LDS a wave so that rows leave in runs of 64 bytes.
-// 4815 rows x 200 x 50000 bf16, two exponentials an element: forward 150 us (0.64 PFLOP/s), gradient 237 (it writes 481 MB).
-// Left out one at a time from the forward walk: exponentials 35 us, copies 25, products 30: no one of them bounds it, what is
-// left is the wait for each other, and the fold of one tile between the products of the next did not shorten it (152).
+// 4815 rows x 200 x 50000 bf16, two exponentials an element: forward 143 us (0.67 PFLOP/s), gradient 216 (it writes 481 MB).
+// Nothing alone bounds it: left out one at a time when the forward walk took 155, exponentials were worth 35 us, copies 25,
+// products 30.  Standing the fold of one tile between the products of the next (two sets of accumulators) gained nothing there
+// and cost the gradient 10 %.
 template <int NP, int NQ, bool TWO, bool GRAD, int NK>
 __global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
   constexpr int NST = NK <= 4 ? 1 : NK <= 8 ? 2 : 4, VT = 128 / NP, NJ = 2 / NP, RB = 128 * NP;   // RB: bytes of a row's stage
@@ -1099,7 +1101,7 @@ template <typename T, int NP> __global__ __launch_bounds__(256) void dt_gimage_k
 
 // P[n][v] of a piece of the vocabulary without the picked entries: a 2^(t - L1) + b 2^(t / tau - L2), for any E: the forward
 // walk's product, once a 128 x 128 tile.  The tile goes through LDS so that rows leave whole.  3650 rows x 1024 x 50000 bf16:
-// 489 us, 0.76 PFLOP/s and 365 MB written.
+// 474 us, 0.79 PFLOP/s and 365 MB written.  (As a walk like the forward one 560: a stage's wait would count the stores.)
 template <int NP, int NQ, bool TWO>
 __global__ __launch_bounds__(256, 2) void dt_grad_kernel(DistillArgs p) {
   DT_LDS
@@ -1326,8 +1328,8 @@ __device__ __forceinline__ void dw_tile(const DistillArgs& p, const Ring& m, int
 
 // Both products of a range in one launch, dX's items in the first DT_DX_BLOCKS blocks (one a CU), dW's tiles behind them:
 // the CUs that one of them leaves idle at its end work on the other.  256 x 128 tiles of eight waves, three buffers, P read once
-// by each product from the caches that the range was sized for.  3650 x 1024 x 50000 bf16: 795 us for both, 0.94 PFLOP/s;
-// matrix cores busy 55 % of the time at the 1.81 GHz that their power leaves.  4815 x 200 x 50000: 289 us, 0.67 (0.85 with the
+// by each product from the caches that the range was sized for.  3650 x 1024 x 50000 bf16: 790 us for both, 0.95 PFLOP/s;
+// matrix cores busy 61 % of the time at the 1.72 GHz that their power leaves.  4815 x 200 x 50000: 279 us, 0.69 (0.88 with the
 // padding of 200 to 256 columns).
 template <typename T, int NP, int NQ, int RAX, int RAW>
 __global__ __launch_bounds__(512, 2) void dt_products_kernel(DistillArgs p, int etx, int etw, int add) {

@@ -450,31 +450,53 @@ template <int C> __device__ __forceinline__ void ring_barrier() {
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
-template <typename OA, typename OB>
+//
+// A tile is 8 x 4 fragments of 32 x 32 (columns of E by rows or words; RA = 128: 4 x 8), four to a wave, 2 x 2 of them: where a
+// tile of E has at most 224 (96) columns, the waves of its second half (all waves) take 3 x 1 instead, and nothing is
+// multiplied for the last 32 columns of padding.  Two waves share a SIMD, w and w + 4: each SIMD then has 7 fragments, not 8.
+template <int RA> struct Part {
+  bool tall;
+  int a, b, wave;                                                 // first column of E, first of the other operand
+  __device__ __forceinline__ Part(int cols, int w) : wave(w) {
+    tall = RA == 256 ? cols <= 224 && w >= 4 : cols <= 96;
+    a = RA == 256 ? (tall ? 128 : (w >> 1) * 64) : (tall ? 0 : (w & 1) * 64);
+    b = RA == 256 ? (tall ? (w - 4) * 32 : (w & 1) * 64) : (tall ? w * 32 : (w >> 1) * 64);
+  }
+  __device__ __forceinline__ bool has(int i) const { return !tall || i < 3; }
+  __device__ __forceinline__ int col(int i) const { return a + (tall ? i : i >> 1) * 32; }
+  __device__ __forceinline__ int row(int i) const { return b + (tall ? 0 : i & 1) * 32; }
+};
+template <bool TALL, typename OA, typename OB>
 __device__ __forceinline__ void ring_product(const OA& A, const OB& B, int n, char* la0, char* lb0, char* la1, char* lb1,
-                                             char* la2, char* lb2, int am, int bn, int lane, int wave, f32x16 (&acc)[2][2]) {
+                                             char* la2, char* lb2, int am, int bn, int lane, int wave, f32x16 (&acc)[4]) {
   constexpr int C = OA::PI + OB::PI, KB = OA::KB, NA = OA::PLANES, NB = OB::PLANES;
   constexpr int SH = KB == 4 ? 3 : 2;                             // a stage's copies in SH shares
-  clear(acc);
+  constexpr int FA = TALL ? 3 : 2, FB = TALL ? 1 : 2;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
   if (n <= 0) return;
-  h8 a[2][2][NA], b[2][2][NB];
+  h8 a[2][FA][NA], b[2][FB][NB];
   const auto read = [&](int q, const char* la, const char* lb, int ks) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < FA; ++i)
 #pragma unroll
       for (int pl = 0; pl < NA; ++pl) a[q][i][pl] = OA::frag(la, am + 32 * i, ks, pl, lane);
 #pragma unroll
+    for (int i = 0; i < FB; ++i)
+#pragma unroll
       for (int pl = 0; pl < NB; ++pl) b[q][i][pl] = OB::frag(lb, bn + 32 * i, ks, pl, lane);
-    }
   };
   const auto multiply = [&](int q) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < FA; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {                               // the small products first
-        if (NB == 2) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[q][i][0], b[q][j][NB - 1], acc[i][j], 0, 0, 0);
-        if (NA == 2) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[q][i][NA - 1], b[q][j][0], acc[i][j], 0, 0, 0);
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[q][i][0], b[q][j][0], acc[i][j], 0, 0, 0);
+      for (int j = 0; j < FB; ++j) {                              // the small products first
+        f32x16& x = acc[i * FB + j];
+        if (NB == 2) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[q][i][0], b[q][j][NB - 1], x, 0, 0, 0);
+        if (NA == 2) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[q][i][NA - 1], b[q][j][0], x, 0, 0, 0);
+        x = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[q][i][0], b[q][j][0], x, 0, 0, 0);
       }
   };
   const auto copy = [&](int s, char* la, char* lb, int share) {
@@ -518,6 +540,14 @@ __device__ __forceinline__ void ring_product(const OA& A, const OB& B, int n, ch
 }
 // three buffers for the operand of 256 rows or columns, three for the one of 128
 struct Ring { char *x0, *x1, *x2, *y0, *y1, *y2; };
+template <int RA, typename OA, typename OB>
+__device__ __forceinline__ void tile_product(const OA& A, const OB& B, int n, const Ring& m, const Part<RA>& t, int lane,
+                                             f32x16 (&acc)[4]) {
+  char *a0 = RA == 256 ? m.x0 : m.y0, *a1 = RA == 256 ? m.x1 : m.y1, *a2 = RA == 256 ? m.x2 : m.y2;
+  char *b0 = RA == 256 ? m.y0 : m.x0, *b1 = RA == 256 ? m.y1 : m.x1, *b2 = RA == 256 ? m.y2 : m.x2;
+  if (t.tall) ring_product<true>(A, B, n, a0, b0, a1, b1, a2, b2, t.a, t.b, lane, t.wave, acc);
+  else ring_product<false>(A, B, n, a0, b0, a1, b1, a2, b2, t.a, t.b, lane, t.wave, acc);
+}
 
 // ------------------------------------------------------------------------------------------------- forward
 // Work items of the kernels that walk the vocabulary: (tile of 128 live rows) x (range of its vt tiles).  512 blocks, two
@@ -1217,7 +1247,6 @@ __device__ __forceinline__ void dx_items(const DistillArgs& p, const Ring& m, in
   const int nl = *p.nlive, tiles = (nl + RB - 1) / RB * et;
   const int splits = dt_dx_splits(tiles, p.vfull / BK);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int am = (RA == 256 ? wave >> 1 : wave & 1) * 64, bn = (RA == 256 ? wave & 1 : wave >> 1) * 64;
   const int stages = p.vc / BK, per = (stages + splits - 1) / splits;
   const long ldw = (long)p.Kp * NP * 2;
   using OA = Operand<NP, true, RA, 8, BK>;
@@ -1231,21 +1260,21 @@ __device__ __forceinline__ void dx_items(const DistillArgs& p, const Ring& m, in
     const int s0 = split * per, s1 = min(stages, s0 + per);
     A.base = reinterpret_cast<const char*>(p.Wimg) + (p.v0 + (long)s0 * BK) * ldw + (long)te * RA * 2 * NP;
     B.base = reinterpret_cast<const char*>(p.P) + ((long)s0 * p.Np + tn * RB) * 128;
-    f32x16 acc[2][2];
-    if (RA == 256) ring_product<OA, OB>(A, B, s1 - s0, m.x0, m.y0, m.x1, m.y1, m.x2, m.y2, am, bn, lane, wave, acc);
-    else ring_product<OA, OB>(A, B, s1 - s0, m.y0, m.x0, m.y1, m.x1, m.y2, m.x2, am, bn, lane, wave, acc);
+    f32x16 acc[4];
+    const Part<RA> t(__builtin_amdgcn_readfirstlane(p.E - te * RA), wave);
+    tile_product<RA>(A, B, s1 - s0, m, t, lane, acc);
     float4* out = reinterpret_cast<float4*>(p.slab) + ((long)split * tiles + tile) * (RA * RB / 4) + wave * 1024 + lane;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 4; ++i) {
+      if (!t.has(i)) continue;
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          float4* q = out + ((i * 2 + j) * 4 + g) * 64;
-          float4 x = make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
-          if (add) { const float4 y = *q; x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w; }
-          *q = x;
-        }
+      for (int g = 0; g < 4; ++g) {
+        float4* q = out + (i * 4 + g) * 64;
+        float4 x = make_float4(acc[i][4 * g], acc[i][4 * g + 1], acc[i][4 * g + 2], acc[i][4 * g + 3]);
+        if (add) { const float4 y = *q; x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w; }
+        *q = x;
+      }
+    }
   }
 }
 // dX from the splits' partial tiles, always in the same order: the result does not depend on which block came first.  11 us for
@@ -1261,14 +1290,15 @@ __global__ __launch_bounds__(256) void dt_dx_sum_kernel(DistillArgs p, int et) {
   const int slot = (blockIdx.x & 31) * 256 + threadIdx.x;
   const long step = (long)tiles * (RA * RB / 4);
   const float4* q = reinterpret_cast<const float4*>(p.slab) + (long)tile * (RA * RB / 4) + slot;
+  const int lane = slot & 63, frag = (slot >> 6) & 15, wave = slot >> 10;
+  const int te = tile % et;
+  const Part<RA> t(p.E - te * RA, wave);
+  const int i = (tile / et) * RB + t.row(frag >> 2) + (lane & 31);
+  const int e = te * RA + t.col(frag >> 2) + (frag & 3) * 8 + (lane >> 5) * 4;
+  if (i >= nl || e >= p.E || !t.has(frag >> 2)) return;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
   for (int k = 0; k < splits; ++k) { const float4 y = q[k * step]; s.x += y.x; s.y += y.y; s.z += y.z; s.w += y.w; }
-  const int lane = slot & 63, frag = (slot >> 6) & 15, wave = slot >> 10;
-  const int am = (RA == 256 ? wave >> 1 : wave & 1) * 64, bn = (RA == 256 ? wave & 1 : wave >> 1) * 64;
-  const int i = (tile / et) * RB + bn + ((frag >> 2) & 1) * 32 + (lane & 31);
-  const int e = (tile % et) * RA + am + (frag >> 3) * 32 + (frag & 3) * 8 + (lane >> 5) * 4;
-  if (i >= nl) return;
   const float f = w * p.coef[2 * (long)p.Np + i];
   T* out = static_cast<T*>(p.dX) + (long)p.rows[i] * p.E + e;
   const float v[4] = {s.x, s.y, s.z, s.w};
@@ -1286,7 +1316,6 @@ __device__ __forceinline__ void dw_tile(const DistillArgs& p, const Ring& m, int
   const int pv = (vt + 7) / 8, j0 = block >> 3, tv = (block & 7) * pv + j0 / et, te = j0 % et;
   if (j0 / et >= pv || tv >= vt) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int am = (RA == 256 ? wave >> 1 : wave & 1) * 64, bn = (RA == 256 ? wave & 1 : wave >> 1) * 64;
   using OA = Operand<NP, true, RA, 8, BK>;
   using OB = Operand<NQ, true, RB, 8>;
   OA A;
@@ -1294,35 +1323,33 @@ __device__ __forceinline__ void dw_tile(const DistillArgs& p, const Ring& m, int
   A.init(reinterpret_cast<const char*>(p.Gimg) + (long)te * RA * 2 * NP, (long)p.Kg * NP * 2, 128, lane, wave);
   B.init(reinterpret_cast<const char*>(p.P) + (long)(tv * RB / BK) * p.Np * 128, 128, (long)p.Np * 128, lane, wave);
   const float fw = *p.gmax * ldexpf(1.f, -P_EXP - p.sexp[0]), fb = *p.gmax * ldexpf(1.f, -2 * P_EXP);
-  f32x16 acc[2][2];
-  if (RA == 256) ring_product<OA, OB>(A, B, (nl + BK - 1) / BK, m.x0, m.y0, m.x1, m.y1, m.x2, m.y2, am, bn, lane, wave, acc);
-  else ring_product<OA, OB>(A, B, (nl + BK - 1) / BK, m.y0, m.x0, m.y1, m.x1, m.y2, m.x2, am, bn, lane, wave, acc);
+  f32x16 acc[4];
+  const Part<RA> t(__builtin_amdgcn_readfirstlane(p.E + 1 - te * RA), wave);   // (the bias' column too)
+  tile_product<RA>(A, B, (nl + BK - 1) / BK, m, t, lane, acc);
   // a lane holds four neighbouring columns of a word's row at a time
   const bool vec = p.E % 4 == 0 && ((uintptr_t)p.dW % (4 * sizeof(T))) == 0;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int v = p.v0 + tv * RB + bn + 32 * j + (lane & 31);
-    if (v >= p.V) continue;
+  for (int i = 0; i < 4; ++i) {
+    const int v = p.v0 + tv * RB + t.row(i) + (lane & 31);
+    if (v >= p.V || !t.has(i)) continue;
     T* out = static_cast<T*>(p.dW) + (long)v * p.E;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int g = 0; g < 4; ++g) {
+      const int e = te * RA + t.col(i) + 8 * g + 4 * (lane >> 5);
+      if (vec && e + 3 < p.E) {
+        Packed<T, 4> x;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int e = te * RA + am + 32 * i + 8 * g + 4 * (lane >> 5);
-        if (vec && e + 3 < p.E) {
-          Packed<T, 4> x;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) x.set(k, acc[i][j][4 * g + k] * fw);
-          *reinterpret_cast<Packed<T, 4>*>(out + e) = x;
-        } else {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (e + k < p.E) out[e + k] = (T)(acc[i][j][4 * g + k] * fw);
-        }
+        for (int k = 0; k < 4; ++k) x.set(k, acc[i][4 * g + k] * fw);
+        *reinterpret_cast<Packed<T, 4>*>(out + e) = x;
+      } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (e + k == p.E) static_cast<T*>(p.db)[v] = (T)(acc[i][j][4 * g + k] * fb);
+          if (e + k < p.E) out[e + k] = (T)(acc[i][4 * g + k] * fw);
       }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (e + k == p.E) static_cast<T*>(p.db)[v] = (T)(acc[i][4 * g + k] * fb);
+    }
   }
 }
 

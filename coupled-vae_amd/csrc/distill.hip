@@ -62,7 +62,7 @@ struct DistillArgs {
   _Float16* Gimg; float* coef;             // s X image with a column of s; [3][Np]: a, b, s / gmax
   float* gmax;
   _Float16* P; int v0, vc;                 // a range of the vocabulary: [vc NP / 64 pieces][Np rows][128 bytes]
-  float* slab; int vfull;                  // partial tiles of dX; words of a full range
+  float* slab; int vfull, dwtiles;         // partial tiles of dX; words of a full range, and its tiles of dW
   void* dX; void* dW; void* db;
 };
 
@@ -1226,17 +1226,36 @@ __global__ __launch_bounds__(256) void dt_pick_kernel(DistillArgs p) {
   }
 }
 
-// Splits of the vocabulary for the dX product's tiles (known on the device alone): a block a CU, items in rounds of 256;
-// an item costs its stages and about 14 more for its partial tile's way out and back.
+// Splits of the vocabulary for the dX product's tiles (known on the device alone): a block a CU, items in rounds of 256; an
+// item costs its stages and about 14 more for its partial tile's way out and back.  dW's tiles follow on the same CUs and need
+// not come out even (157 of them for a vocabulary of 20000).  With two planes of W, where a stage is matrix work, as many splits
+// as there are CUs spared in dW's last round are therefore longer by a tile of dW, if dX's items are one round (also where only
+// dX is wanted: its bits do not depend on that): 3520 x 200 x 20000 fp32 131 -> 116 us for both products.  With one plane a
+// stage is memory work, twice as long in dX as in dW, and even splits are better (4815 x 200 x 50000 bf16: 140 us a range, 173).
 constexpr int DT_DX_BLOCKS = 256, DT_DX_MOST = 1024;
-__device__ __forceinline__ int dt_dx_splits(int tiles, int stages) {
-  const int k = (threadIdx.x & 63) + 1;
+struct Splits {
+  int n, even, size, most;                                        // splits; the first `even` of `size` stages, the others of `most`
+  __device__ __forceinline__ int begin(int s) const { return s <= even ? s * size : even * size + (s - even) * most; }
+};
+template <int NP> __device__ __forceinline__ Splits dt_dx_splits(const DistillArgs& p, int tiles, int stages, int nl, int bk) {
+  const int k = (threadIdx.x & 63) + 1, items = tiles * k;
+  const int d = (nl + bk - 1) / bk + 6, rounds = (p.dwtiles + DT_DX_BLOCKS - 1) / DT_DX_BLOCKS;   // a tile of dW, in stages
+  const int spared = NP == 2 && items <= DT_DX_BLOCKS ? min(k, (rounds * DT_DX_BLOCKS - p.dwtiles) / tiles) : 0;
+  const int more = spared > 0 ? max(0, min(d, (stages - 4 * k) / spared)) : 0;
+  const int size = more > 0 ? (stages - spared * more) / k : (stages + k - 1) / k;
   int best = 0x7fffffff;
-  if (k == 1 || (tiles * k <= DT_DX_MOST && k * 4 <= stages))
-    best = min(((tiles * k + DT_DX_BLOCKS - 1) / DT_DX_BLOCKS) * ((stages + k - 1) / k + 14), 0x1ffffff) * 64 + (k - 1);
+  if (k == 1 || (items <= DT_DX_MOST && k * 4 <= stages))
+    best = min(((items + DT_DX_BLOCKS - 1) / DT_DX_BLOCKS) * (size + 14), 0x1ffffff) * 64 + (k - 1);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) best = min(best, __shfl_xor(best, o, 64));
-  return __builtin_amdgcn_readfirstlane((best & 63) + 1);
+  const int lane = best & 63;
+  Splits r;
+  r.n = __builtin_amdgcn_readfirstlane(lane + 1);
+  r.size = __builtin_amdgcn_readfirstlane(__shfl(size, lane, 64));
+  const int longer = __builtin_amdgcn_readfirstlane(__shfl(more > 0 ? spared : 0, lane, 64));
+  r.even = r.n - longer;
+  r.most = longer ? __builtin_amdgcn_readfirstlane((stages - r.even * r.size + longer - 1) / longer) : 0;
+  return r;
 }
 
 // dX: (W down its rows: K = vocabulary) x (P along its rows), tiles of RA columns of E x RB rows.  Items (tile, split of
@@ -1245,9 +1264,9 @@ template <int NP, int NQ, int RA>
 __device__ __forceinline__ void dx_items(const DistillArgs& p, const Ring& m, int first, int et, int add) {
   constexpr int RB = 384 - RA, BK = 64 / NQ;
   const int nl = *p.nlive, tiles = (nl + RB - 1) / RB * et;
-  const int splits = dt_dx_splits(tiles, p.vfull / BK);
+  const Splits splits = dt_dx_splits<NP>(p, tiles, p.vfull / BK, nl, BK);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int stages = p.vc / BK, per = (stages + splits - 1) / splits;
+  const int stages = p.vc / BK;
   const long ldw = (long)p.Kp * NP * 2;
   using OA = Operand<NP, true, RA, 8, BK>;
   using OB = Operand<NQ, false, RB, 8>;
@@ -1255,9 +1274,9 @@ __device__ __forceinline__ void dx_items(const DistillArgs& p, const Ring& m, in
   OB B;
   A.init(nullptr, ldw, 128, lane, wave);
   B.init(nullptr, 128, (long)p.Np * 128, lane, wave);
-  for (int item = first; item < tiles * splits; item += DT_DX_BLOCKS) {
-    const int split = item % splits, tile = item / splits, te = tile % et, tn = tile / et;
-    const int s0 = split * per, s1 = min(stages, s0 + per);
+  for (int item = first; item < tiles * splits.n; item += DT_DX_BLOCKS) {
+    const int split = item / tiles, tile = item - split * tiles, te = tile % et, tn = tile / et;
+    const int s0 = min(stages, splits.begin(split)), s1 = min(stages, splits.begin(split + 1));   // (the last range may be shorter)
     A.base = reinterpret_cast<const char*>(p.Wimg) + (p.v0 + (long)s0 * BK) * ldw + (long)te * RA * 2 * NP;
     B.base = reinterpret_cast<const char*>(p.P) + ((long)s0 * p.Np + tn * RB) * 128;
     f32x16 acc[4];
@@ -1285,7 +1304,7 @@ __global__ __launch_bounds__(256) void dt_dx_sum_kernel(DistillArgs p, int et) {
   const int nl = *p.nlive, tiles = (nl + RB - 1) / RB * et;
   const int tile = blockIdx.x >> 5;                               // 32 blocks a tile
   if (tile >= tiles) return;
-  const int splits = dt_dx_splits(tiles, p.vfull / (64 / NQ));
+  const int splits = dt_dx_splits<sizeof(T) == 4 ? 2 : 1>(p, tiles, p.vfull / (64 / NQ), nl, 64 / NQ).n;
   const float w = ldexpf(1.f, -p.sexp[1] - P_EXP);
   const int slot = (blockIdx.x & 31) * 256 + threadIdx.x;
   const long step = (long)tiles * (RA * RB / 4);
@@ -1546,6 +1565,7 @@ int launch_distill_backward(const DistillCall& c, const float* ghard, const floa
   char* w = static_cast<char*>(ws);
   a.Gimg = (_Float16*)(w + d.Gimg); a.coef = (float*)(w + d.coef); a.gmax = (float*)(w + d.gmax);
   a.P = (_Float16*)(w + d.P); a.slab = (float*)(w + d.slab); a.vfull = (int)d.vc;
+  a.dwtiles = a.vfull / (384 - d.raw) * d.etw;
   return dt_dispatch(c.dtype, d, a, true, s);
 }
 

@@ -453,7 +453,8 @@ template <int C> __device__ __forceinline__ void ring_barrier() {
 //
 // A tile is 8 x 4 fragments of 32 x 32 (columns of E by rows or words; RA = 128: 4 x 8), four to a wave, 2 x 2 of them: where a
 // tile of E has at most 224 (96) columns, the waves of its second half (all waves) take 3 x 1 instead, and nothing is
-// multiplied for the last 32 columns of padding.  Two waves share a SIMD, w and w + 4: each SIMD then has 7 fragments, not 8.
+// multiplied for the last 32 columns of padding.  Two waves share a SIMD, w and w + 4: each SIMD then has 7 fragments, not 8
+// (both products of 3520 x 200 x 20000 fp32 142 -> 134 us, of 3650 x 1024 x 50000 bf16, whose bias column has a tile, 784 -> 756).
 template <int RA> struct Part {
   bool tall;
   int a, b, wave;                                                 // first column of E, first of the other operand
@@ -1374,9 +1375,9 @@ __device__ __forceinline__ void dw_tile(const DistillArgs& p, const Ring& m, int
 
 // Both products of a range in one launch, dX's items in the first DT_DX_BLOCKS blocks (one a CU), dW's tiles behind them:
 // the CUs that one of them leaves idle at its end work on the other.  256 x 128 tiles of eight waves, three buffers, P read once
-// by each product from the caches that the range was sized for.  3650 x 1024 x 50000 bf16: 790 us for both, 0.95 PFLOP/s;
-// matrix cores busy 61 % of the time at the 1.72 GHz that their power leaves.  4815 x 200 x 50000: 279 us, 0.69 (0.88 with the
-// padding of 200 to 256 columns).
+// by each product from the caches that the range was sized for.  3650 x 1024 x 50000 bf16: 755 us for both, 0.99 PFLOP/s;
+// matrix cores busy 61 % of the time at the 1.71 GHz that their power leaves.  4815 x 200 x 50000: 279 us, 0.69 PFLOP/s, bound by
+// P: 481 MB by each product at 3.4 TB/s.
 template <typename T, int NP, int NQ, int RAX, int RAW>
 __global__ __launch_bounds__(512, 2) void dt_products_kernel(DistillArgs p, int etx, int etw, int add) {
   __shared__ __attribute__((aligned(16))) char x0[32768];

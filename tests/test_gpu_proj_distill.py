@@ -176,6 +176,16 @@ def test_distillation(dev, size, tau, dtype):
     compare(dev, inputs(*size, dtype, sum(size)), tau)
 
 
+# the last tile of E around what its waves share differently (96, 224 columns, and one more for the bias), alone and behind
+# whole tiles; a vocabulary whose tiles leave part of the chip free
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('size', [(20, 7, 7, 95, 900, 3), (20, 7, 7, 96, 900, 3), (20, 7, 7, 223, 900, 2), (20, 7, 7, 224, 900, 2),
+                                  (9, 4, 4, 225, 700, 2), (9, 4, 4, 352, 700, 2), (9, 4, 4, 480, 700, 2),
+                                  (32, 8, 8, 200, 20000, 4)])
+def test_partly_filled_tiles(dev, size, dtype):
+    compare(dev, inputs(*size, dtype, sum(size)), 2.0)
+
+
 @pytest.mark.parametrize('dtype', ['bf16', 'f16'])
 @pytest.mark.parametrize('size', SIZES)
 def test_cross_entropy_16_bit(dev, size, dtype):
@@ -455,3 +465,26 @@ def test_a_text_decoder_of_the_new_operators(dev):
     check_rnn(y, rnn['y'], 'y')
     check_rnn(grads[0], rnn['du'], 'du')
     check_rnn(grads[1], rnn['dh0'], 'dh0')
+
+
+def test_most_rows_that_a_backward_pass_takes(dev):
+    """2^22 rows of which 300 are live: offsets inside a tile of P pass 2^31 bytes.  The same 300 rows alone give the same bits."""
+    from cvae_amd import ops
+    T, R, E, V, K, n = 2048, 2048, 75, 250, 3, 300
+    g = torch.Generator().manual_seed(4)
+    small = inputs(1, n, n, E, V, K, 'f16', 41)
+    small['eos'] = torch.randint(1, V, (n, 1), generator=g)
+    big = dict(small, final=torch.zeros(T, R, E, dtype=torch.float16), eos=torch.full((R, T), PAD), gh=torch.zeros(R), gs=torch.zeros(R),
+               ids=torch.zeros(R, T, K, dtype=torch.int64), top=torch.zeros(R, T, K))
+    big['final'][T - 1, :n] = small['final'][0]
+    for k in ('gh', 'gs'):
+        big[k][:n] = small[k]
+    for k in ('eos', 'ids', 'top'):
+        big[k][:n, T - 1] = small[k][:, 0]
+    want, got = run(dev, small, 2.0), run(dev, big, 2.0)
+    for k in ('hard', 'soft'):
+        assert torch.equal(got[k][:n], want[k]) and not got[k][n:].any(), k
+    for k in ('dW', 'db'):
+        assert torch.equal(got[k], want[k]), k
+    assert torch.equal(got['dfinal'][T - 1, :n], want['dfinal'][0])
+    assert not got['dfinal'][T - 1, n:].any() and not got['dfinal'][:T - 1].any()

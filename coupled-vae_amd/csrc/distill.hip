@@ -1443,8 +1443,9 @@ static DistillPlan dt_plan(int dtype, long N, int E, int V, int K) {
   d.back_bytes = at;
   return d;
 }
+// (a launch has fewer than 2^32 threads: 256 a row in the merge, 16 a word in the images)
 static bool dt_sizes_ok(long N, long E, long V, long K) {
-  return N < (1L << 30) && E > 0 && E <= 65536 && V > 0 && V < (1L << 30) && K >= 0 && K <= V && K <= DT_MOST_K;
+  return N <= (1L << 23) && E > 0 && E <= 65536 && V > 0 && V <= (1L << 26) && K >= 0 && K <= V && K <= DT_MOST_K;
 }
 // 0 where there are no rows, or for sizes that the calls refuse
 long distill_workspace_floats(int dtype, long N, long E, long V, long K) {
@@ -1560,6 +1561,7 @@ int launch_distill_backward(const DistillCall& c, const float* ghard, const floa
   if (!dX && !dW) return 0;
   CVAE_REQUIRE((((uintptr_t)ws | (uintptr_t)saved) & 15) == 0, "distill_backward: the workspaces must be 16-byte aligned");
   const DistillPlan d = dt_plan(c.dtype, (long)c.T * c.R, c.E, (int)c.V, c.K);
+  CVAE_REQUIRE((long)(d.Np / (384 - d.rax)) * d.et < (1 << 19), "distill_backward: too many rows of E = %d", c.E);   // 2^13 threads a tile
   DistillArgs a = {};
   dt_fill(a, d, c, const_cast<void*>(saved));
   a.ghard = ghard; a.gsoft = gsoft; a.dX = dX; a.dW = dW; a.db = db;

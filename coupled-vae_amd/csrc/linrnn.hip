@@ -498,7 +498,7 @@ static int lr_dispatch(int dtype, const LinRnnArgs& a, bool back, hipStream_t s)
 static int lr_check(const char* what, int dtype, int gates, int T, int B, int H) {
   CVAE_REQUIRE(dtype >= DT_F32 && dtype <= DT_F16, "%s: dtype %d is none of 0 (fp32), 1 (bf16), 2 (fp16)", what, dtype);
   CVAE_REQUIRE(gates == 2 || gates == 3, "%s: gates must be 2 or 3, not %d", what, gates);
-  CVAE_REQUIRE(T >= 0 && B >= 0 && H >= 0 && T < (1 << 30) && (int64_t)B * H < (1LL << 31) / 4, "%s: bad shape T=%d B=%d H=%d",
+  CVAE_REQUIRE(T >= 0 && B >= 0 && H >= 0 && T < (1 << 30) && (int64_t)B * H <= (1LL << 28), "%s: bad shape T=%d B=%d H=%d",
                what, T, B, H);
   return 0;
 }

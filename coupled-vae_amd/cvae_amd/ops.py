@@ -728,6 +728,7 @@ def proj_ce(final, W, b, eos, pad, cache=None):
         _proj_check(final, W, b, eos)
         _here(final, W, b, eos)
         return ProjDistillFn.apply(_c(final), _c(W), _c(b), _c(eos), pad, 0, None, None, 1.0)
+    _need(W.dtype == b.dtype == torch.float32, 'final, W and b must share one of float32, bfloat16, float16')
     return ProjCEFn.apply(final, W, b, _targets(eos, final.shape[1], cache), pad)
 
 
@@ -810,6 +811,7 @@ def proj_ce_sorted(final, W, b, eos, pad):
         _proj_check(final, W, b, eos)
         _here(final, W, b, eos)
         return ProjDistillFn.apply(_c(final), _c(W), _c(b), _c(eos), pad, 1, None, None, 1.0)
+    _need(W.dtype == b.dtype == torch.float32, 'final, W and b must share one of float32, bfloat16, float16')
     tgt = targets_sentence_major(eos, final.shape[1] // B)
     return ProjCEFn.apply(final, W, b, tgt, pad)
 

@@ -200,7 +200,7 @@ int cvae_decoder_backward_n(int nd, int cell, int B, int T, int E, int Hd, int64
  * the state, so a sequence is a scan and long ones run in parallel over time):
  *   z = sigmoid(u_z), n = tanh(u_n), o = sigmoid(u_o):  h_t = z h_(t-1) + (1 - z) n,  y_t = o h_t
  * dtype: storage of u, y, dy, du: 0 = fp32, 1 = bf16, 2 = fp16 (the state, h0, h_last and their gradients are fp32).
- * gates: 3 = rows z|n|o, 2 = rows z|n (y_t = h_t).  u[T,B,gates*H], h0[B,H] or NULL (zeros), len[B] or NULL (all T; a
+ * gates: 3 = rows z|n|o, 2 = rows z|n (y_t = h_t).  B*H <= 2^28.  u[T,B,gates*H], h0[B,H] or NULL (zeros), len[B] or NULL (all T; a
  * value outside [0,T] counts as the nearer end): row b takes steps t < len[b] -- upwards, or with reverse != 0 downwards
  * from len[b]-1 -- and past them y = 0, the state is carried and du = 0.  y[T,B,H], h_last[B,H] (may be h0, in place, where
  * cvae_linrnn_workspace is 0; else that call is refused).
@@ -270,7 +270,7 @@ int cvae_projce_backward_saved_n(int nd, const float* const* final, const float*
  * are fp32.  final[T*R,E] (rows n = t*R + r), W[V,E], b[V], eos[B,T] targets: row r reads sentence r % B, or r / (R / B)
  * if sentence_major (R % B == 0).  Rows whose target is `pad` have no loss and no gradient; a target outside [0,V) that
  * is not `pad` counts as a logit of 0 (as in cvae_projce_*).
- * 0 <= K <= min(V, 1024) entries of the teacher at every position: ids[B,T,K], top[B,T,K]; an entry whose id is outside
+ * At most 2^23 rows, V <= 2^26, E <= 65536.  0 <= K <= min(V, 1024) entries of the teacher at every position: ids[B,T,K], top[B,T,K]; an entry whose id is outside
  * [0,V) or whose logit is -inf is absent, a row with no entry has soft = 0; an id may be listed twice.  K = 0: ids, top,
  * soft (and gsoft) are not read and tau is ignored.
  * -> hard[R], soft[R]: sums over t.  ws: cvae_distill_workspace(dtype, T*R, E, V, K) floats, 16-byte aligned; the backward

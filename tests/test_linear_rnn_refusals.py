@@ -70,3 +70,8 @@ def test_in_place_state_of_a_segmented_sequence_is_refused():
     assert _lib.query('cvae_linrnn_workspace', 0, 1000, 1, 8) > 0
     with pytest.raises(_lib.CvaeHipError, match='h_last may be h0'):
         _lib.call('cvae_linrnn_forward', 0, 3, 0, 1000, 1, 8, 16, 16, None, 16, 16, None, 16, None)
+
+
+def test_more_channels_than_a_launch_are_refused():
+    with pytest.raises(_lib.CvaeHipError, match='bad shape'):
+        _lib.call('cvae_linrnn_forward', 0, 3, 0, 64, (1 << 14) + 1, 1 << 14, 16, None, None, 16, 16, None, None, None)

@@ -84,3 +84,26 @@ def test_c_entries_refuse_bad_arguments():
         for sizes in ((0, 8, 10, 3), (-1, 8, 10, 3), (5, 0, 10, 3), (5, 8, 0, 0), (5, 8, 10, 11), (5, 8, 10, -1),
                       (1 << 40, 8, 10, 3), (5, 1 << 40, 10, 3), (5, 8, 1 << 40, 3)):
             assert _lib.query(name, 1, *sizes) == 0, sizes
+
+
+def test_fp32_cross_entropy_refuses_16_bit_weights(monkeypatch):
+    monkeypatch.setattr(torch.cuda, 'current_device', lambda: 0)
+    a = good()
+    for k in ('W', 'b'):
+        bad = {n: a[n].float() if n in ('final', 'W', 'b') else a[n] for n in ('final', 'W', 'b', 'eos', 'pad')}
+        bad[k] = bad[k].to(torch.bfloat16)
+        for f in (ops.proj_ce, ops.proj_ce_sorted):
+            with pytest.raises(ValueError, match='must share'):
+                f(**bad)
+
+
+def test_sizes_beyond_a_launch_are_refused():
+    """A launch has fewer than 2^32 threads; the workspace of a refused size is 0."""
+    for N, E, V in (((1 << 23) + 1, 8, 100), (8, 8, (1 << 26) + 1), (8, 65537, 100)):
+        assert _lib.query('cvae_distill_workspace', 1, N, E, V, 0) == 0
+    assert _lib.query('cvae_distill_workspace', 1, 1 << 23, 8, 100, 0) > 0
+    with pytest.raises(_lib.CvaeHipError, match='bad shape'):
+        _lib.call('cvae_distill_forward', 1, 16, 16, 16, 16, 0, 0, 1, 1, (1 << 23) + 1, 8, 100, 0, None, None, 1.0, 16, None, 16, None)
+    with pytest.raises(_lib.CvaeHipError, match='too many rows'):
+        _lib.call('cvae_distill_backward', 1, 16, 16, 16, 16, 0, 0, 1, 1, 1 << 22, 8192, 100, 0, None, None, 1.0, 16, None, 16, 16,
+                  16, 16, 16, None)

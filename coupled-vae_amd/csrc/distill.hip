@@ -713,7 +713,7 @@ __global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
   __shared__ __attribute__((aligned(16))) char w1[DT_STAGE + 512];
   __shared__ __attribute__((aligned(16))) char w2[DT_STAGE + 512];
   __shared__ __attribute__((aligned(16))) char w3[DT_STAGE + 512];
-  __shared__ __attribute__((aligned(16))) char turn[GRAD ? 8192 : 3072];
+  __shared__ __attribute__((aligned(16))) char turn[GRAD ? 4 * 2048 : 2 * 128 * 3 * sizeof(float)];
   const int nl = *p.nlive, nt = (nl + DT_TILE - 1) / DT_TILE, vt = GRAD ? p.vc / VT : p.fvt;
   if (nt == 0) return;
   const int splits = dt_splits(nt, vt, 1), per = __builtin_amdgcn_readfirstlane((vt + splits - 1) / splits);

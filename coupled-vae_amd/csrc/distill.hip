@@ -20,7 +20,8 @@
 // useful work; a large library product runs at 1.38), 4815 x 200 x 50000 bf16 with 64 teacher entries at tau 2 0.72 ms.
 //
 // Image layout: rows of 128-byte pieces, one plane: 64 values, two planes: 32 hi values then 32 lo values.  A piece is
-// what one row adds to a pipeline stage, so one loop serves both.  Rows are padded to 128 with zeros, columns to 64.
+// what one row adds to a pipeline stage, so one loop serves both.  Rows are padded to 256 with zeros, columns to 64 (to
+// 256 for 129 to 208 columns).
 // Both orders that the products need are read from this one layout: rows along K with ds_read_b128, and K down the
 // rows with ds_read_b64_tr_b16, which transposes on its way to the registers.
 #include "common.hpp"
@@ -42,7 +43,7 @@ constexpr int P_EXP = 13;                  // |P| <= 1 is stored times 2^13
 
 struct DistillArgs {
   int N, T, R, B, E, V, K;
-  int Np, Vp, Kp, Kg;                      // N and V up to 256, E up to 64, E + 1 up to 64
+  int Np, Vp, Kp, Kg;                      // multiples of 256 for N and V, of 64 for E and E + 1
   float tau, itau;
   int two;                                 // tau != 1 and K > 0: a second normaliser
   const void* X; const void* W; const void* bias;

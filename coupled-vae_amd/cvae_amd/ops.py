@@ -724,11 +724,10 @@ def proj_ce(final, W, b, eos, pad, cache=None):
     """final (T,R,E), W (V,E), b (V,), eos (B,T) with R % B == 0 -> (R,) fp32.  fp32, or bf16 / fp16 throughout (then
     through the kernels of proj_distill).  `cache`: a dict shared by the losses of one forward pass
     (the two decoders of a training step read the same targets): the time-major targets are built once."""
+    _proj_check(final, W, b, eos)
+    _here(final, W, b, eos)
     if final.dtype != torch.float32:
-        _proj_check(final, W, b, eos)
-        _here(final, W, b, eos)
         return ProjDistillFn.apply(_c(final), _c(W), _c(b), _c(eos), pad, 0, None, None, 1.0)
-    _need(W.dtype == b.dtype == torch.float32, 'final, W and b must share one of float32, bfloat16, float16')
     return ProjCEFn.apply(final, W, b, _targets(eos, final.shape[1], cache), pad)
 
 
@@ -799,6 +798,10 @@ def proj_ce_pair_ok(finals, Ws):
 def proj_ce_pair(finals, Ws, bs, eos, pad, cache=None):
     """[final (T,R,E)] * nd, eos (B,T) -> nd per-sentence sums (R,), as nd proj_ce calls.  fp32."""
     _need(all(t.dtype == torch.float32 for t in (*finals, *Ws, *bs)), 'proj_ce_pair takes float32 (16-bit: proj_ce)')
+    for d, final in enumerate(finals):
+        _proj_check(final, Ws[d], bs[d], eos)
+        _need(final.shape == finals[0].shape and Ws[d].shape == Ws[0].shape, 'the decoders of a pair must have one shape')
+        _here(final, Ws[d], bs[d], eos)
     tgt = _targets(eos, finals[0].shape[1], cache)
     flat = [t for d in range(len(finals)) for t in (finals[d], Ws[d], bs[d])]
     return ProjCEPairFn.apply(pad, tgt, *flat)
@@ -806,13 +809,11 @@ def proj_ce_pair(finals, Ws, bs, eos, pad, cache=None):
 
 def proj_ce_sorted(final, W, b, eos, pad):
     """final (T,B*K,E) on sentence-major rows, eos (B,T) -> (B*K,).  fp32, or bf16 / fp16 throughout."""
-    B = eos.shape[0]
+    _proj_check(final, W, b, eos)
+    _here(final, W, b, eos)
     if final.dtype != torch.float32:
-        _proj_check(final, W, b, eos)
-        _here(final, W, b, eos)
         return ProjDistillFn.apply(_c(final), _c(W), _c(b), _c(eos), pad, 1, None, None, 1.0)
-    _need(W.dtype == b.dtype == torch.float32, 'final, W and b must share one of float32, bfloat16, float16')
-    tgt = targets_sentence_major(eos, final.shape[1] // B)
+    tgt = targets_sentence_major(eos, final.shape[1] // eos.shape[0])
     return ProjCEFn.apply(final, W, b, tgt, pad)
 
 

@@ -107,3 +107,33 @@ def test_sizes_beyond_a_launch_are_refused():
     with pytest.raises(_lib.CvaeHipError, match='too many rows'):
         _lib.call('cvae_distill_backward', 1, 16, 16, 16, 16, 0, 0, 1, 1, 1 << 22, 8192, 100, 0, None, None, 1.0, 16, None, 16, 16,
                   16, 16, 16, None)
+
+
+@pytest.mark.parametrize('what,change', [
+    ('must be \\(T,R,E\\)', dict(final=torch.zeros(T, B, E + 1))),
+    ('must be \\(T,R,E\\)', dict(W=torch.zeros(V, E - 1))),
+    ('must be \\(T,R,E\\)', dict(b=torch.zeros(V - 1))),
+    ('eos must be', dict(eos=torch.ones(B, T - 1, dtype=torch.int64))),
+    ('eos must be', dict(eos=torch.ones(3, T, dtype=torch.int64))),
+    ('eos must be', dict(eos=torch.ones(B, T, dtype=torch.int32))),
+    ('current GPU', dict()),
+])
+def test_fp32_cross_entropy_refuses_what_its_kernels_would_read_past(what, change, monkeypatch):
+    """Host tensors and sizes that do not belong together, refused in fp32 as in 16 bits: the kernels would read past the
+    operands' ends."""
+    monkeypatch.setattr(torch.cuda, 'current_device', lambda: 0)
+    a = dict(good(), **change)
+    a = {k: a[k] for k in ('final', 'W', 'b', 'eos', 'pad')}
+    for f in (ops.proj_ce, ops.proj_ce_sorted):
+        with pytest.raises(ValueError, match=what):
+            f(**a)
+    with pytest.raises(ValueError, match=what):
+        ops.proj_ce_pair([a['final']] * 2, [a['W']] * 2, [a['b']] * 2, a['eos'], 0)
+
+
+@pytest.mark.parametrize('change', [dict(final=torch.zeros(T, 2 * B, E)), dict(W=torch.zeros(V + 1, E), b=torch.zeros(V + 1))])
+def test_paired_cross_entropy_refuses_two_shapes(change, monkeypatch):
+    monkeypatch.setattr(torch.cuda, 'current_device', lambda: -1)      # (host tensors pass: the shapes are looked at)
+    a, o = good(), dict(good(), **change)
+    with pytest.raises(ValueError, match='one shape'):
+        ops.proj_ce_pair([a['final'], o['final']], [a['W'], o['W']], [a['b'], o['b']], a['eos'], 0)

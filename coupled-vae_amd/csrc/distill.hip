@@ -27,6 +27,7 @@
 #include "common.hpp"
 #include "misc.hpp"
 #include "dtype.hpp"
+#include "dx_splits.hpp"
 
 namespace cvae {
 
@@ -1234,30 +1235,14 @@ __global__ __launch_bounds__(256) void dt_pick_kernel(DistillArgs p) {
 // as there are CUs spared in dW's last round are therefore longer by a tile of dW, if dX's items are one round (also where only
 // dX is wanted: its bits do not depend on that): 3520 x 200 x 20000 fp32 131 -> 116 us for both products.  With one plane a
 // stage is memory work, twice as long in dX as in dW, and even splits are better (4815 x 200 x 50000 bf16: 140 us a range, 173).
-constexpr int DT_DX_BLOCKS = 256, DT_DX_MOST = 1024;
-struct Splits {
-  int n, even, size, most;                                        // splits; the first `even` of `size` stages, the others of `most`
-  __device__ __forceinline__ int begin(int s) const { return s <= even ? s * size : even * size + (s - even) * most; }
-};
 template <int NP> __device__ __forceinline__ Splits dt_dx_splits(const DistillArgs& p, int tiles, int stages, int nl, int bk) {
-  const int k = (threadIdx.x & 63) + 1, items = tiles * k;
-  const int d = (nl + bk - 1) / bk + 6, rounds = (p.dwtiles + DT_DX_BLOCKS - 1) / DT_DX_BLOCKS;   // a tile of dW, in stages
-  const int spared = NP == 2 && items <= DT_DX_BLOCKS ? min(k, (rounds * DT_DX_BLOCKS - p.dwtiles) / tiles) : 0;
-  const int more = spared > 0 ? max(0, min(d, (stages - 4 * k) / spared)) : 0;
-  const int size = more > 0 ? (stages - spared * more) / k : (stages + k - 1) / k;
-  int best = 0x7fffffff;
-  if (k == 1 || (items <= DT_DX_MOST && k * 4 <= stages))
-    best = min(((items + DT_DX_BLOCKS - 1) / DT_DX_BLOCKS) * (size + 14), 0x1ffffff) * 64 + (k - 1);
+  const DxSplit mine = dx_split((threadIdx.x & 63) + 1, tiles, stages, (nl + bk - 1) / bk + 6, p.dwtiles, NP == 2);
+  int best = mine.cost;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) best = min(best, __shfl_xor(best, o, 64));
   const int lane = best & 63;
-  Splits r;
-  r.n = __builtin_amdgcn_readfirstlane(lane + 1);
-  r.size = __builtin_amdgcn_readfirstlane(__shfl(size, lane, 64));
-  const int longer = __builtin_amdgcn_readfirstlane(__shfl(more > 0 ? spared : 0, lane, 64));
-  r.even = r.n - longer;
-  r.most = longer ? __builtin_amdgcn_readfirstlane((stages - r.even * r.size + longer - 1) / longer) : 0;
-  return r;
+  return dx_splits_of(__builtin_amdgcn_readfirstlane(lane + 1), __builtin_amdgcn_readfirstlane(__shfl(mine.size, lane, 64)),
+                      __builtin_amdgcn_readfirstlane(__shfl(mine.longer, lane, 64)), stages);
 }
 
 // dX: (W down its rows: K = vocabulary) x (P along its rows), tiles of RA columns of E x RB rows.  Items (tile, split of

@@ -488,3 +488,14 @@ def test_most_rows_that_a_backward_pass_takes(dev):
         assert torch.equal(got[k], want[k]), k
     assert torch.equal(got['dfinal'][T - 1, :n], want['dfinal'][0])
     assert not got['dfinal'][T - 1, n:].any() and not got['dfinal'][:T - 1].any()
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('E,V', [(20, 90), (200, 20000), (300, 700)])
+def test_nothing_live_of_every_type(dev, E, V, dtype):
+    """A batch of padding alone, by storage type and width: the number of live rows is known on the device only."""
+    a = inputs(4, 3, 3, E, V, 3, dtype, 1)
+    a['eos'][:] = PAD
+    got = run(dev, a, 2.0)
+    for k, v in got.items():
+        assert not bool(v.any()), k

@@ -532,6 +532,8 @@ def _linear_rnn_check(u, gates, h0, dims):
     _need(u.dim() == dims, 'u must have %d dimensions' % dims)
     _need(u.dtype in _DTYPE, 'u must be float32, bfloat16 or float16, not %s' % u.dtype)
     _need(u.shape[-1] % gates == 0, 'the last dimension of u (%d) is no multiple of gates' % u.shape[-1])
+    # (here too: the library's arguments are 32-bit, a larger size would reach it as another one)
+    _need(u.shape[0] < 2 ** 30 and u.shape[-2] * (u.shape[-1] // gates) <= 2 ** 28, 'u is too large: 2^30 steps, 2^28 channels')
     if h0 is not None:
         _need(h0.dtype == torch.float32 and tuple(h0.shape) == (u.shape[-2], u.shape[-1] // gates),
               'the state must be float32 of shape (B, H)')
@@ -685,6 +687,8 @@ def _proj_check(final, W, b, eos):
     _need(final.dtype in _DTYPE and W.dtype == final.dtype and b.dtype == final.dtype,
           'final, W and b must share one of float32, bfloat16, float16')
     _need(W.shape[0] > 0 and W.shape[1] > 0, 'W is empty')
+    # (the library's sizes are 32-bit: a larger one would reach it as another one)
+    _need(max(*final.shape, final.shape[0] * final.shape[1]) < 2 ** 31, 'final is too large: 2^31 rows or columns')
     _need(eos.dim() == 2 and eos.dtype == torch.int64 and eos.shape[0] > 0 and eos.shape[1] == final.shape[0] and
           final.shape[1] % eos.shape[0] == 0, 'eos must be int64 (B,T) with R a multiple of B')
 

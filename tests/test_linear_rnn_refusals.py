@@ -75,3 +75,14 @@ def test_in_place_state_of_a_segmented_sequence_is_refused():
 def test_more_channels_than_a_launch_are_refused():
     with pytest.raises(_lib.CvaeHipError, match='bad shape'):
         _lib.call('cvae_linrnn_forward', 0, 3, 0, 64, (1 << 14) + 1, 1 << 14, 16, None, None, 16, 16, None, None, None)
+
+
+@pytest.mark.parametrize('shape', [((1 << 32) + 3, 1, 2), (1 << 30, 1, 2), (4, (1 << 32) + 1, 2), (4, 1, (1 << 33) + 2)])
+def test_sizes_past_32_bits_are_refused(shape, monkeypatch):
+    """The C entries take 32-bit sizes: 2^32 + 3 steps must not run as 3."""
+    monkeypatch.setattr(torch.cuda, 'current_device', lambda: 0)
+    with pytest.raises(ValueError, match='too large'):
+        ops.linear_rnn(z(1).expand(shape), 2)
+    if shape[0] == 4:
+        with pytest.raises(ValueError, match='too large'):
+            ops.linear_rnn_step(z(1).expand(shape[1:]), 2, z(1).expand(shape[1], shape[2] // 2))

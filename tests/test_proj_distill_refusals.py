@@ -137,3 +137,14 @@ def test_paired_cross_entropy_refuses_two_shapes(change, monkeypatch):
     a, o = good(), dict(good(), **change)
     with pytest.raises(ValueError, match='one shape'):
         ops.proj_ce_pair([a['final'], o['final']], [a['W'], o['W']], [a['b'], o['b']], a['eos'], 0)
+
+
+@pytest.mark.parametrize('t,r,e', [((1 << 32) + 1, 1, E), (0, (1 << 32) + 2, E), (1 << 20, 1 << 12, E), (1, 1, (1 << 32) + 8)])
+def test_sizes_past_32_bits_are_refused(t, r, e, monkeypatch):
+    """The C entries take 32-bit sizes: 2^32 + 8 columns must not run as 8."""
+    monkeypatch.setattr(torch.cuda, 'current_device', lambda: 0)
+    for dtype in (torch.float32, torch.bfloat16):
+        z = torch.zeros(1, dtype=dtype)
+        for f in (ops.proj_ce, ops.proj_ce_sorted):
+            with pytest.raises(ValueError, match='too large'):
+                f(z.expand(t, r, e), z.expand(V, e), z.expand(V), torch.ones(1, 1, dtype=torch.int64).expand(1, t), 0)

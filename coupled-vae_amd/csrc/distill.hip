@@ -1446,7 +1446,8 @@ static int dt_check(const char* what, const DistillCall& c) {
   CVAE_REQUIRE(c.B > 0 && c.T >= 0 && c.R >= 0 && c.R % c.B == 0, "%s: R = %d must be a multiple of B = %d", what, c.R, c.B);
   CVAE_REQUIRE(dt_sizes_ok((int64_t)c.T * c.R, c.E, c.V, c.K), "%s: bad shape T=%d R=%d E=%d V=%lld K=%d", what, c.T, c.R,
                c.E, (long long)c.V, c.K);
-  CVAE_REQUIRE(c.K == 0 || (c.tau > 0.f && c.tau < 1e6f), "%s: tau must be positive", what);
+  // (below, S / tau has no bits left in fp32, and its exponentials overflow in the gradient)
+  CVAE_REQUIRE(c.K == 0 || (c.tau >= 1e-6f && c.tau < 1e6f), "%s: tau must be in [1e-6, 1e6)", what);
   return 0;
 }
 static void dt_fill(DistillArgs& a, const DistillPlan& d, const DistillCall& c, void* ws) {

@@ -698,7 +698,7 @@ def proj_distill(final, W, b, eos, pad, teacher_ids, teacher_logits, tau):
     fp32, bf16 or fp16; eos (B,T) int64 targets (rows at `pad` count nothing), R % B == 0; the teacher's K <= 1024 best of
     every position: teacher_ids (B,T,K) int64, teacher_logits (B,T,K) float (ids outside the vocabulary and logits of -inf are
     absent entries).  With p = softmax(teacher_logits / tau) over the K entries and q_tau = softmax(logits / tau) over
-    the whole vocabulary:
+    the whole vocabulary (1e-6 <= tau < 1e6):
       hard (R,) = sum_t -log softmax(logits)[target],   soft (R,) = sum_t tau^2 KL(p || q_tau)
     -> (hard, soft) fp32, differentiable in final, W and b (no gradient reaches the teacher)."""
     _proj_check(final, W, b, eos)
@@ -707,7 +707,7 @@ def proj_distill(final, W, b, eos, pad, teacher_ids, teacher_logits, tau):
           'teacher_ids must be int64 (B,T,K) with 0 < K <= min(V, 1024)')
     _need(teacher_logits.shape == teacher_ids.shape and teacher_logits.is_floating_point(),
           'teacher_logits must be a float tensor of the shape of teacher_ids')
-    _need(0.0 < tau < 1e6, 'tau must be positive')
+    _need(1e-6 <= tau < 1e6, 'tau must be in [1e-6, 1e6)')
     _here(final, W, b, eos, teacher_ids, teacher_logits)
     return ProjDistillFn.apply(_c(final), _c(W), _c(b), _c(eos), pad, 0, _c(teacher_ids), _c(teacher_logits.float()),
                                float(tau))

@@ -272,7 +272,7 @@ int cvae_projce_backward_saved_n(int nd, const float* const* final, const float*
  * is not `pad` counts as a logit of 0 (as in cvae_projce_*).
  * At most 2^23 rows, V <= 2^26, E <= 65536.  0 <= K <= min(V, 1024) entries of the teacher at every position: ids[B,T,K], top[B,T,K]; an entry whose id is outside
  * [0,V) or whose logit is -inf is absent, a row with no entry has soft = 0; an id may be listed twice.  K = 0: ids, top,
- * soft (and gsoft) are not read and tau is ignored.
+ * soft (and gsoft) are not read and tau is ignored; else 1e-6 <= tau < 1e6.
  * -> hard[R], soft[R]: sums over t.  ws: cvae_distill_workspace(dtype, T*R, E, V, K) floats, 16-byte aligned; the backward
  * call reads it (`saved`). */
 int64_t cvae_distill_workspace(int dtype, int64_t N, int64_t E, int64_t V, int K);

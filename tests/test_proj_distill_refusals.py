@@ -148,3 +148,16 @@ def test_sizes_past_32_bits_are_refused(t, r, e, monkeypatch):
         for f in (ops.proj_ce, ops.proj_ce_sorted):
             with pytest.raises(ValueError, match='too large'):
                 f(z.expand(t, r, e), z.expand(V, e), z.expand(V), torch.ones(1, 1, dtype=torch.int64).expand(1, t), 0)
+
+
+@pytest.mark.parametrize('tau', [1e-40, 1e-20, 9e-7])
+def test_a_temperature_that_leaves_no_bits_is_refused(tau, monkeypatch):
+    """S / tau times 2^-24 is then more than the logits' differences, and 1 / tau ends in infinity."""
+    monkeypatch.setattr(torch.cuda, 'current_device', lambda: 0)
+    with pytest.raises(ValueError, match='tau'):
+        ops.proj_distill(**dict(good(), tau=tau))
+    for name, n in (('cvae_distill_forward', 4), ('cvae_distill_backward', 8)):
+        with pytest.raises(_lib.CvaeHipError, match='tau'):
+            _lib.call(name, 0, 16, 16, 16, 16, 0, 0, B, T, B, E, V, K, 16, 16, tau, *([None] * n))
+    with pytest.raises(ValueError, match='current GPU'):              # the smallest that is taken gets as far as the devices
+        ops.proj_distill(**dict(good(), tau=1e-6))

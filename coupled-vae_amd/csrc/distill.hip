@@ -75,11 +75,15 @@ __device__ __forceinline__ long position(const DistillArgs& p, int n) {
 }
 
 // ------------------------------------------------------------------------------------------------- scales and images
-__device__ __forceinline__ int scale_exp(float amax) {          // amax * 2^e in [2^13, 2^14)
+// amax * 2^e in [2^13, 2^14), up to the largest float (e = -114); a tensor of less than 2^-97 altogether keeps e = 110, so that the
+// powers that undo it stay floats
+__device__ __forceinline__ int scale_exp(float amax) {
   if (!(amax > 0.f)) return 0;
   const int e = P_EXP - (int)floorf(log2f(amax));
-  return e < -110 ? -110 : (e > 110 ? 110 : e);
+  return e > 110 ? 110 : e;
 }
+// from a product of images to a base-2 logit (finite, so that a product of zero stays zero beside tensors of 2^64 and more)
+__device__ __forceinline__ float unscale(const int* e) { return fminf(ldexpf(LOG2E, -(e[0] + e[1])), 3.0e38f); }
 // largest finite magnitude of a tensor from its partials, by every thread of a block of 256
 __device__ __forceinline__ float block_amax(const float* part, float* red) {
   static_assert(DT_AMAX == 512, "two partials a thread");
@@ -140,7 +144,7 @@ template <typename T> __global__ __launch_bounds__(256) void dt_count_kernel(Dis
   const int b = blockIdx.x - nb, which = b / DT_AMAX, slot = b % DT_AMAX;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   float m = 0.f;
-  const auto take = [&](float v) { v = fabsf(v); m = v < 3.4e38f ? fmaxf(m, v) : m; };
+  const auto take = [&](float v) { v = fabsf(v); m = v < INFINITY ? fmaxf(m, v) : m; };
   if (which) {
     const T* x = static_cast<const T*>(p.W);
     constexpr int VN = 16 / sizeof(T);
@@ -650,8 +654,7 @@ __global__ __launch_bounds__(256, 2) void dt_forward_kernel(DistillArgs p) {
   const int splits = dt_splits(nt, vt, p.least), per = __builtin_amdgcn_readfirstlane((vt + splits - 1) / splits);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int am = (wave >> 1) * 64, bn = (wave & 1) * 64;
-  const int e = p.sexp[0] + p.sexp[1];
-  const float c = ldexpf(LOG2E, -e);
+  const float c = unscale(p.sexp);
   const long ld = (long)p.Kp * NP * 2;
   const int nst = (p.E + 64 / NP - 1) / (64 / NP), last = ((p.E + 15) / 16) - (nst - 1) * (4 / NP);
   const int xcd = blockIdx.x & 7, per_xcd = nt * (splits / 8);
@@ -722,7 +725,7 @@ __global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int am = NP == 1 ? (wave >> 1) * 64 : 0, bn = NP == 1 ? (wave & 1) * 64 : wave * 32;
   const int l31 = lane & 31, lhi = lane >> 5;
-  const float c = ldexpf(LOG2E, -(p.sexp[0] + p.sexp[1]));
+  const float c = unscale(p.sexp);
   const long ld = (long)p.Kp * NP * 2;
   unsigned off[4];
 #pragma unroll
@@ -1155,8 +1158,7 @@ __global__ __launch_bounds__(256, 2) void dt_grad_kernel(DistillArgs p) {
   A.init(reinterpret_cast<const char*>(p.Wimg) + w0 * ld, ld, 128, lane, wave);
   B.init(reinterpret_cast<const char*>(p.Ximg) + n0 * ld, ld, 128, lane, wave);
   const int nst = (p.E + 64 / NP - 1) / (64 / NP), last = ((p.E + 15) / 16) - (nst - 1) * (4 / NP);
-  const int e = p.sexp[0] + p.sexp[1];
-  const float c = ldexpf(LOG2E, -e);
+  const float c = unscale(p.sexp);
   f32x16 acc[2][2];
   clear(acc);
   A.issue(0, la0, wave);

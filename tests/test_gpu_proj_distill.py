@@ -499,3 +499,23 @@ def test_nothing_live_of_every_type(dev, E, V, dtype):
     got = run(dev, a, 2.0)
     for k, v in got.items():
         assert not bool(v.any()), k
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+@pytest.mark.parametrize('E,V', [(16, 300), (224, 300)])
+def test_states_up_to_the_largest_float(dev, E, V, dtype):
+    """A column of 2^127 that no word weighs, beside states near 2^95 and weights near 2^-95.  The images scale by 2^-114 and keep
+    2^-25 of what is then the unit: a logit is off by 2^89 sum |w| at most, a loss and its logit's share in lse by twice that."""
+    T, B, K, tau = 3, 2, 3, 2.0
+    a = inputs(T, B, B, E, V, K, dtype, 21)
+    a['eos'] = a['eos'] % (V - 1) + 1
+    a['final'], a['W'] = a['final'] * 2.0 ** 95, a['W'] * 2.0 ** -95
+    a['final'][:, :, 0], a['W'][:, 0] = 2.0 ** 127, 0.0
+    a['gh'], a['gs'] = a['gh'] * 0.01, a['gs'] * 0.01                  # (dW's first column stays below the largest float)
+    got, want = run(dev, a, tau), oracle(a, tau)
+    off = 2 * 2.0 ** 89 * float(a['W'].double().abs().sum(1).max())
+    for k, f in (('hard', 1.0), ('soft', tau)):                        # soft: tau^2 times a difference of logits over tau
+        value, bound = want[k]
+        assert bool(((got[k].detach().double().cpu() - value).abs() <= bound + f * T * off).all()), k
+    for k, v in got.items():
+        assert bool(torch.isfinite(v).all()), k

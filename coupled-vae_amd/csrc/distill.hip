@@ -902,6 +902,13 @@ __global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
   }
 }
 
+// log2 of a picked word's softmax: at most 0, also where its logit (a product of its own) and the normaliser (the walk's) are
+// large enough that their roundings say otherwise; a NaN stays one
+__device__ __forceinline__ float log_share(float pick, float lse) {
+  const float d = pick - lse;
+  return d > 0.f ? 0.f : d;
+}
+
 // sum over the 32 lanes of a half-wave: four steps inside rows of 16 lanes on the vector ALU, one through LDS
 __device__ __forceinline__ float half_sum(float v) {
   const auto step = [](float x, int y) { return x + __builtin_bit_cast(float, y); };
@@ -1005,7 +1012,10 @@ __global__ __launch_bounds__(256) void dt_combine_kernel(DistillArgs p) {
     a += red[w][1] * __builtin_amdgcn_exp2f(d);
     if (TWO) b += red[w][2] * __builtin_amdgcn_exp2f(d * p.itau);
   }
-  const float L1 = m + log2f(a), L2 = TWO ? fmaf(m, p.itau, log2f(b)) : L1;
+  // (a, b >= 1, so L1 >= m; where rounding leaves L2 below m / tau, the next float: no share of the gradient walk passes 1)
+  const float L1 = m + log2f(a);
+  float L2 = TWO ? fmaf(m, p.itau, log2f(b)) : L1;
+  if (TWO && fmaf(m, p.itau, -L2) > 0.f) L2 = fmaf(fabsf(L2), 0x1p-23f, L2);
   float tm = -INFINITY;
   bool bad = false;                                               // a NaN among the teacher's logits
   for (int k = lane; k < K; k += 64)
@@ -1017,7 +1027,7 @@ __global__ __launch_bounds__(256) void dt_combine_kernel(DistillArgs p) {
     p.L1[i] = L1;
     p.L2[i] = L2;
     p.slive[n % p.R] = 1;
-    p.hard[n] = (L1 - spick[K]) * LN2;
+    p.hard[n] = (sid[K] >= 0 ? -log_share(spick[K], L1) : L1) * LN2;   // (outside the vocabulary: a logit of 0)
     p.some[i] = K == 0 || !some ? 0.f : tm != tm ? NAN : 1.f;
   }
   float* share = p.share + (long)i * (K + 1);
@@ -1030,7 +1040,7 @@ __global__ __launch_bounds__(256) void dt_combine_kernel(DistillArgs p) {
   bool listed = false;
   for (int k = lane; k < K; k += 64) {
     const float lp = (slog[k] - tm) * p.itau * LOG2E, pk = some && sid[k] >= 0 ? __builtin_amdgcn_exp2f(lp) * inv : 0.f;
-    if (pk != 0.f) loss += pk * (lp - lsum - (spick[k] * p.itau - L2));
+    if (pk != 0.f) loss += pk * (lp - lsum - log_share(spick[k] * p.itau, L2));
     listed |= sid[k] >= 0 && sid[k] == sid[K];
     slog[k] = pk;                                                 // (its own lane's entry) from here on: p_k
   }
@@ -1221,8 +1231,8 @@ __global__ __launch_bounds__(256) void dt_pick_kernel(DistillArgs p) {
     const int64_t id = k < p.K ? ids[k] : tg;
     const float share = p.share[(long)i * (p.K + 1) + k], pick = p.pick[(long)i * (p.K + 1) + k];
     if (id < p.v0 || id >= (int64_t)p.v0 + p.vc || id >= p.V || share == -1.f) continue;
-    float x = a * (__builtin_amdgcn_exp2f(pick - L1) - (id == tg ? 1.f : 0.f));
-    if (p.K) x = fmaf(b, __builtin_amdgcn_exp2f(fmaf(pick, TWO ? p.itau : 1.f, -L2)) - share, x);
+    float x = a * (__builtin_amdgcn_exp2f(log_share(pick, L1)) - (id == tg ? 1.f : 0.f));
+    if (p.K) x = fmaf(b, __builtin_amdgcn_exp2f(log_share(pick * (TWO ? p.itau : 1.f), L2)) - share, x);
     const int v = (int)(id - p.v0);
     _Float16* q = p.P + ((long)(v * NQ >> 6) * p.Np + i) * 64 + (v & (64 / NQ - 1));
     const _Float16 hi = (_Float16)x;

@@ -519,3 +519,27 @@ def test_states_up_to_the_largest_float(dev, E, V, dtype):
         assert bool(((got[k].detach().double().cpu() - value).abs() <= bound + f * T * off).all()), k
     for k, v in got.items():
         assert bool(torch.isfinite(v).all()), k
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('E', [24, 200, 224])
+@pytest.mark.parametrize('tau', [2.0, 1.3])
+def test_no_word_has_more_than_the_whole(dev, tau, E, dtype):
+    """Logits so large that their rounding is more than what tells the best word from the normaliser: lse >= S[target] all the
+    same, so no loss is negative, and no gradient outgrows its upstream one."""
+    T, B, V, K = 4, 16, 300, 3
+    for scale in (1e3, 1e4) if dtype == 'f16' else (1e3, 1e7, 1e12):
+        a = inputs(T, B, B, E, V, K, dtype, 22, scale=scale)
+        best = (a['final'].double() @ a['W'].double().t() + a['b'].double()).argmax(2).t().contiguous()     # (B,T)
+        best[B // 2:] = (best[B // 2:] + 31) % V                       # half of the rows pick other words
+        best = torch.where(best == PAD, 1, best)
+        a['eos'] = best
+        a['ids'][:, :, 0] = best
+        a['ids'][:, :, 1:] = (best[..., None] + torch.tensor([7, 19])) % V
+        got = run(dev, a, tau)
+        assert bool((got['hard'] >= 0).all()) and bool((got['soft'] >= 0).all()), (scale, got['hard'].min(), got['soft'].min())
+        for k, v in got.items():
+            assert bool(torch.isfinite(v).all()), (scale, k)
+        # |db| of a word: its rows' (|gh| + tau |gs|), to the sum's rounding
+        most = T * (a['gh'].abs() + tau * a['gs'].abs()).sum()
+        assert float(got['db'].float().abs().max()) <= float(most) * 1.01, scale

@@ -35,13 +35,29 @@ struct LinRnnArgs {
   int nseg, seg;                  // segments and their steps (a multiple of 64)
 };
 
-// sigmoid(x) and 1 - sigmoid(x), each to ~2 ulp (1 - z is formed from e^-|x|, not by subtraction: forget gates near 1
-// decide how much enters a long-lived state)
-__device__ __forceinline__ void sigmoid_pair(float x, float& s, float& c) {
-  const float e = __builtin_amdgcn_exp2f(-1.4426950408889634f * fabsf(x));
+// sigmoid(x) and 1 - sigmoid(x) (1 - z is formed from e^-|x|, not by subtraction: forget gates near 1 decide how much enters a
+// long-lived state).  The larger of the two is good to ~2 ulp.  The smaller one is e^-|x| nearly, and as the exponent is rounded
+// before it is raised, off by up to (2 + |x|) 2^-24 of itself: 16-bit storage stops there, as |x| 2^-24 is nothing beside what its
+// own rounding of x does.  fp32 storage takes the rounding back: with t = |x| log2 e as rounded, e^-|x| = 2^-t e^-(|x| - t ln 2),
+// ~2 ulp.  (r is a NaN at an infinity, where 2^-t = 0 has the last word.)  For 16-bit types that would be 650 us in place of 635
+// for both passes of 2000 x 32 x 2048.
+template <typename T> __device__ __forceinline__ void sigmoid_pair(float x, float& s, float& c) {
+  const float a = fabsf(x), t = 1.4426950408889634f * a;
+  float e = __builtin_amdgcn_exp2f(-t);
+  if (sizeof(T) == 4) {
+    const float r = fminf(fmaf(t, 1.9046542999577679e-9f, fmaf(t, -0.693147182464599609f, a)), 1.0f);   // -ln 2 in two parts
+    e = fmaf(-r, e, e);
+  }
   const float big = __builtin_amdgcn_rcpf(1.0f + e), small = e * big;
   s = x >= 0.f ? big : small;
   c = x >= 0.f ? small : big;
+}
+// the output gate: sigmoid(x) to the same bounds
+template <typename T> __device__ __forceinline__ float sigmoid_of(float x) {
+  if (sizeof(T) != 4) return sigmoid_fast(x);
+  float s, c;
+  sigmoid_pair<T>(x, s, c);
+  return s;
 }
 // tanh: its series to x^9 below 0.3 (next term < 6e-8 relative), else from exp (1 - 2 / (1 + e^2x) keeps only an
 // absolute 1e-7, too little near zero)
@@ -170,8 +186,8 @@ __global__ __launch_bounds__(64 * LR_W) void linrnn_maps_kernel(LinRnnArgs p) {
 #pragma unroll
       for (int v = 0; v < VW; ++v) {
         float z, c, in;
-        sigmoid_pair(rz[i].f(v), z, c);
-        if (BACK) in = z * (G == 3 ? rn[i].f(v) * sigmoid_fast(ro[i].f(v)) : rn[i].f(v));
+        sigmoid_pair<T>(rz[i].f(v), z, c);
+        if (BACK) in = z * (G == 3 ? rn[i].f(v) * sigmoid_of<T>(ro[i].f(v)) : rn[i].f(v));
         else in = c * tanh_full(rn[i].f(v));
         if (live) { x[v] = fmaf(z, x[v], in); a[v] *= z; }
       }
@@ -232,7 +248,7 @@ __global__ __launch_bounds__(64 * LR_W) void linrnn_fwd_kernel(LinRnnArgs p) {
 #pragma unroll
         for (int v = 0; v < VW; ++v) {
           float c;
-          sigmoid_pair(rz[i].f(v), a[i][v], c);
+          sigmoid_pair<T>(rz[i].f(v), a[i][v], c);
           x[i][v] = c * tanh_full(rn[i].f(v));
         }
       if (st == ST_MIXED) {
@@ -277,7 +293,7 @@ __global__ __launch_bounds__(64 * LR_W) void linrnn_fwd_kernel(LinRnnArgs p) {
 #pragma unroll
       for (int v = 0; v < VW; ++v) {
         h[v] = fmaf(a[i][v], h[v], x[i][v]);
-        out.set(v, G == 3 ? sigmoid_fast(ro[i].f(v)) * h[v] : h[v]);
+        out.set(v, G == 3 ? sigmoid_of<T>(ro[i].f(v)) * h[v] : h[v]);
       }
       if (st == ST_MIXED && t >= L.len) out = Packed<T, VW>{};
       if (s < w1 && L.valid) *reinterpret_cast<Packed<T, VW>*>(y + (long)t * p.n + (unsigned)L.hbase) = out;
@@ -328,9 +344,9 @@ __global__ __launch_bounds__(64 * LR_W, 4) void linrnn_bwd_kernel(LinRnnArgs p) 
       for (int i = 0; i < LR_C; ++i)
 #pragma unroll
         for (int v = 0; v < VW; ++v) {
-          sigmoid_pair(rz[i].f(v), z[i][v], c[i][v]);
+          sigmoid_pair<T>(rz[i].f(v), z[i][v], c[i][v]);
           n[i][v] = tanh_full(rn[i].f(v));
-          o[i][v] = G == 3 ? sigmoid_fast(ro[i].f(v)) : 1.f;
+          o[i][v] = G == 3 ? sigmoid_of<T>(ro[i].f(v)) : 1.f;
         }
       if (st == ST_MIXED) {
 #pragma unroll
@@ -433,9 +449,9 @@ __global__ __launch_bounds__(256) void linrnn_step_kernel(LinRnnArgs p) {
 #pragma unroll
   for (int v = 0; v < VW; ++v) {
     float z, k, o = 1.f, oc;
-    sigmoid_pair(rz.f(v), z, k);
+    sigmoid_pair<T>(rz.f(v), z, k);
     h[v] = fmaf(z, h[v], k * tanh_full(rn.f(v)));
-    if (p.gates == 3) sigmoid_pair(ro.f(v), o, oc);
+    if (p.gates == 3) sigmoid_pair<T>(ro.f(v), o, oc);
     out.set(v, o * h[v]);
     p.h_last[c + v] = h[v];
   }

@@ -298,3 +298,50 @@ def test_step_refuses_an_overlapping_out(dev):
     out = room[B * 4 * H:B * 5 * H].view(B, H)                    # right behind the state
     ops.linear_rnn_step(u, 3, h, out=out)
     assert torch.equal(out, want) and torch.equal(room[:B * 4 * H], keep[:B * 4 * H])
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+@pytest.mark.parametrize('gates', [2, 3])
+def test_the_small_side_of_saturated_gates(dev, gates, dtype):
+    """Gates of 5 to 80 either way, no sums to hide in: with h0 = 0 the state is (1 - z) n, the gradient of a gate near 1 is made of
+    1 - z, the gradient of h0 of a z near 0.  Each is held to the same few units of its own value; with 16-bit storage to |x| units
+    more for a gate at x, whose exponent is rounded once (to x 2^-24) before it is raised."""
+    B, H = 8, 256
+    g = torch.Generator().manual_seed(31)
+    u, h0, dy, dlast = inputs(dev, 1, B, H, gates, 'f32', 31)
+    gate = (5 + 75 * torch.rand(B, H, generator=g)) * torch.where(torch.rand(B, H, generator=g) < 0.5, 1.0, -1.0)
+    u[0, :, :H] = gate.to(dev)
+    if gates == 3:
+        u[0, :, 2 * H:] = gate.flip(1).to(dev)
+    u = u.to(DT[dtype])
+    for h in (torch.zeros_like(h0), h0):
+        got, want = run(u, gates, h, None, False, dy.to(DT[dtype]), dlast), oracle(u, gates, h, None, False, dy.to(DT[dtype]), dlast)
+        for k in got:
+            value, bound = want[k]
+            if dtype != 'f32':
+                x = u[0, :, :H].double().abs().cpu() + (u[0, :, 2 * H:].double().abs().cpu() if gates == 3 else 0)
+                bound = bound + U * value.abs() * (x if k != 'du' else x.repeat(1, gates))
+            check(got[k], (value, bound), k)
+
+
+def test_infinite_gates(dev):
+    """A gate of +inf keeps the state, one of -inf replaces it, exactly; a NaN reaches its own channel only."""
+    from cvae_amd import ops
+    H = 6
+    u = torch.zeros(2, 1, 3 * H, device=dev)
+    u[:, 0, H:2 * H] = 0.5
+    u[:, 0, 0], u[:, 0, 1], u[:, 0, 2] = float('inf'), float('-inf'), float('nan')
+    u[:, 0, H + 3], u[:, 0, H + 4] = float('inf'), float('-inf')
+    u[:, 0, 2 * H + 5] = float('-inf')
+    h0 = torch.full((1, H), 0.25, device=dev)
+    for step in (False, True):
+        h = h0
+        if step:
+            for t in range(2):
+                y, h = ops.linear_rnn_step(u[t], 3, h)
+        else:
+            y, h = ops.linear_rnn(u, 3, h0=h0)
+            y = y[-1]
+        assert h[0, 0] == 0.25 and abs(float(h[0, 1]) - 0.46211715726) < 1e-6 and torch.isnan(h[0, 2])
+        assert float(h[0, 3]) == 0.25 * 0.25 + 0.5 * 1.5 and float(h[0, 4]) == 0.25 * 0.25 - 0.5 * 1.5 and float(y[0, 5]) == 0
+        assert torch.isnan(y[0]).tolist() == [False, False, True, False, False, False]

@@ -543,3 +543,23 @@ def test_no_word_has_more_than_the_whole(dev, tau, E, dtype):
         # |db| of a word: its rows' (|gh| + tau |gs|), to the sum's rounding
         most = T * (a['gh'].abs() + tau * a['gs'].abs()).sum()
         assert float(got['db'].float().abs().max()) <= float(most) * 1.01, scale
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('K', [0, 3])
+def test_flat_batch_of_many_sentences(dev, K, dtype):
+    """T = 1: as many sentences as rows, whose upstream gradients span 2^30; what an empty one carries counts nowhere."""
+    T, R, E, V = 1, 3001, 24, 60
+    if dtype == 'f32' and not K:
+        K = 1                                                            # (fp32 without a teacher has kernels of its own)
+    a = inputs(T, R, R, E, V, K, dtype, 23)
+    a['eos'] = torch.where(torch.arange(R)[:, None] % 7 == 3, PAD, a['eos'].clamp_min(1))
+    for k in ('gh', 'gs') if K else ('gh',):
+        a[k] = a[k] * 2.0 ** -(torch.arange(R) % 31)
+    want = oracle(a, 2.0)
+    dead = a['eos'][:, 0] == PAD
+    for k in ('gh', 'gs') if K else ('gh',):
+        a[k] = torch.where(dead, 1e30, a[k])
+    got = run(dev, a, 2.0)
+    for k in got:
+        check(got[k], want[k], k, E, V, T * R)

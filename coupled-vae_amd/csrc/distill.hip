@@ -1462,7 +1462,9 @@ static DistillPlan dt_plan(int dtype, long N, int E, int V, int K) {
   d.et = cdiv(E, d.rax); d.etw = cdiv(E + 1, d.raw);
   const int nt = d.Np / DT_TILE;
   d.fvt = d.Vp / (d.nk ? DT_TILE / d.np : DT_TILE);
-  d.pplane = 8L * (nt > DT_MOST_ITEMS ? nt : DT_MOST_ITEMS) * 128;
+  const int ranges = d.fvt / 8 < 1 ? 1 : (d.fvt / 8 > 64 ? 64 : d.fvt / 8);        // of an XCD at most (dt_splits)
+  const long items = (long)nt * ranges < DT_MOST_ITEMS ? (long)nt * ranges : DT_MOST_ITEMS;
+  d.pplane = 8L * (nt > items ? nt : items) * 128;
   auto take = [](long& at, long bytes) { const long o = at; at += (bytes + 255) / 256 * 256; return o; };
   long at = 0;
   d.hard = take(at, 4 * N); d.soft = take(at, K ? 4 * N : 0);
@@ -1485,7 +1487,7 @@ static DistillPlan dt_plan(int dtype, long N, int E, int V, int K) {
   at = 0;
   d.Gimg = take(at, 2L * d.Np * d.Kg * d.np + slack); d.coef = take(at, 12L * d.Np); d.gmax = take(at, 4); d.gpart = take(at, 4L * DT_GPART);
   d.P = take(at, 2L * d.Np * d.vc * d.nq);
-  d.slab = take(at, 4L * 32768 * (tiles > DT_DX_MOST ? tiles : DT_DX_MOST));
+  d.slab = take(at, 4L * 32768 * dx_partial_tiles(tiles, (int)(d.vc * d.nq / 64)));
   d.back_bytes = at;
   return d;
 }

@@ -40,6 +40,13 @@ DX_FN DxSplit dx_split(int k, int tiles, int stages, int d, int dwtiles, bool sp
   return r;
 }
 
+// partial tiles that any number of live rows can ask for: one split of every tile, or more of fewer
+DX_FN int dx_partial_tiles(int tiles, int stages) {
+  const int k = stages / 4 < 1 ? 1 : (stages / 4 > 64 ? 64 : stages / 4);
+  const long many = (long)tiles * k < DT_DX_MOST ? (long)tiles * k : DT_DX_MOST;
+  return tiles > many ? tiles : (int)many;
+}
+
 struct Splits {
   int n, even, size, most;                                        // splits; the first `even` of `size` stages, the others of `most`
   DX_FN int begin(int s) const { return s <= even ? s * size : even * size + (s - even) * most; }

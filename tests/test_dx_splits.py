@@ -1,5 +1,6 @@
 """The rule that cuts the dX product's range into splits (csrc/dx_splits.hpp), built by the host compiler with its integer checks on:
-over sizes of all kinds, none of them live rows among them, the splits cover the range once and nothing is divided by zero."""
+over sizes of all kinds, no live rows among them, the splits cover the range once, their partial tiles fit what is reserved, and
+nothing is divided by zero."""
 import os
 import shutil
 import subprocess
@@ -25,6 +26,9 @@ int main() {
     }
     const int k = lane + 1;
     if (lane < 0 || (k > 1 && (k * 4 > s || (long)t * k > DT_DX_MOST))) { printf("k %d of %d tiles, %d stages\n", k, t, s); return 1; }
+    const int rows_at_most[] = {t, t + 1, 3 * t + 2, 50000};
+    for (int m : rows_at_most)
+      if ((long)t * k > dx_partial_tiles(m, s)) { printf("slab: %d of %d tiles, %d stages, k %d\n", t, m, s, k); return 1; }
     const Splits r = dx_splits_of(k, all[k].size, all[k].longer, s);
     if (r.n != k || r.begin(0) != 0 || r.begin(r.n) < s) { printf("not covered: %d tiles, %d stages, k %d\n", t, s, k); return 1; }
     for (int i = 0; i < r.n; ++i)

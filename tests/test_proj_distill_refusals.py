@@ -161,3 +161,19 @@ def test_a_temperature_that_leaves_no_bits_is_refused(tau, monkeypatch):
             _lib.call(name, 0, 16, 16, 16, 16, 0, 0, B, T, B, E, V, K, 16, 16, tau, *([None] * n))
     with pytest.raises(ValueError, match='current GPU'):              # the smallest that is taken gets as far as the devices
         ops.proj_distill(**dict(good(), tau=1e-6))
+
+
+@pytest.mark.parametrize('dtype', [0, 1, 2])
+def test_workspaces_follow_the_sizes(dtype):
+    """P of a range, the partial tiles of dX, an image of the rows: what is documented, and little for little."""
+    def parts(N, E, V):
+        planes, np_ = (1 if dtype == 1 else 2), (2 if dtype == 0 else 1)
+        rows, words = (N + 255) // 256 * 256, (V + 255) // 256 * 256
+        most = max(1024, (400 << 20) // (2 * planes * rows) // 256 * 256)
+        words = min(words, most)
+        return 2 * planes * rows * words, 131072 * max(1024, (rows // 128) * ((E + 127) // 128)), 2 * np_ * rows * (E + 64)
+    for N, E, V in ((1, 8, 10), (35, 75, 1003), (7680, 200, 50000), (1 << 20, 200, 20000), (1 << 22, 75, 250)):
+        got = 4 * _lib.query('cvae_distill_backward_workspace', dtype, N, E, V, 3)
+        assert got <= sum(parts(N, E, V)) + 16 * N + (1 << 16), (N, E, V, got)
+    for name in ('cvae_distill_workspace', 'cvae_distill_backward_workspace'):
+        assert 4 * _lib.query(name, dtype, 1, 8, 10, 3) <= 2 << 20

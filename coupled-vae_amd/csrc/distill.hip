@@ -503,7 +503,9 @@ template <int RA> struct Part {
   __device__ __forceinline__ int col(int i) const { return a + (tall ? i : i >> 1) * 32; }
   __device__ __forceinline__ int row(int i) const { return b + (tall ? 0 : i & 1) * 32; }
 };
-template <bool TALL, typename OA, typename OB>
+// FOLD > 0: what FOLD stages added up is put aside and the next ones start from zero, so that a long K is no single chain of
+// additions (whose error grows with the root of its length).
+template <bool TALL, int FOLD, typename OA, typename OB>
 __device__ __forceinline__ void ring_product(const OA& A, const OB& B, int n, char* la0, char* lb0, char* la1, char* lb1,
                                              char* la2, char* lb2, int am, int bn, int lane, int wave, f32x16 (&acc)[4]) {
   constexpr int C = OA::PI + OB::PI, KB = OA::KB, NA = OA::PLANES, NB = OB::PLANES;
@@ -514,6 +516,7 @@ __device__ __forceinline__ void ring_product(const OA& A, const OB& B, int n, ch
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
   if (n <= 0) return;
+  f32x16 sum[4] = {};
   h8 a[2][FA][NA], b[2][FB][NB];
   const auto read = [&](int q, const char* la, const char* lb, int ks) {
 #pragma unroll
@@ -570,20 +573,29 @@ __device__ __forceinline__ void ring_product(const OA& A, const OB& B, int n, ch
     step(s, la1, lb1, la2, lb2, la0, lb0, false);
     step(s + 1, la2, lb2, la0, lb0, la1, lb1, false);
     step(s + 2, la0, lb0, la1, lb1, la2, lb2, false);
+    static_assert(FOLD % 3 == 0, "whole rounds of the three buffers");
+    if (FOLD && s % (FOLD ? FOLD : 1) == 1) {
+#pragma unroll
+      for (int i = 0; i < FA * FB; ++i) { sum[i] += acc[i]; acc[i] = f32x16{}; }
+    }
   }
   if (s < n) step(s, la1, lb1, la2, lb2, la0, lb0, false);
   if (s + 1 < n) step(s + 1, la2, lb2, la0, lb0, la1, lb1, false);
   ring_barrier<0>();                                              // no copy may land in LDS that the next block owns
+  if (FOLD) {
+#pragma unroll
+    for (int i = 0; i < FA * FB; ++i) acc[i] += sum[i];
+  }
 }
 // three buffers for the operand of 256 rows or columns, three for the one of 128
 struct Ring { char *x0, *x1, *x2, *y0, *y1, *y2; };
-template <int RA, typename OA, typename OB>
+template <int RA, int FOLD, typename OA, typename OB>
 __device__ __forceinline__ void tile_product(const OA& A, const OB& B, int n, const Ring& m, const Part<RA>& t, int lane,
                                              f32x16 (&acc)[4]) {
   char *a0 = RA == 256 ? m.x0 : m.y0, *a1 = RA == 256 ? m.x1 : m.y1, *a2 = RA == 256 ? m.x2 : m.y2;
   char *b0 = RA == 256 ? m.y0 : m.x0, *b1 = RA == 256 ? m.y1 : m.x1, *b2 = RA == 256 ? m.y2 : m.x2;
-  if (t.tall) ring_product<true>(A, B, n, a0, b0, a1, b1, a2, b2, t.a, t.b, lane, t.wave, acc);
-  else ring_product<false>(A, B, n, a0, b0, a1, b1, a2, b2, t.a, t.b, lane, t.wave, acc);
+  if (t.tall) ring_product<true, FOLD>(A, B, n, a0, b0, a1, b1, a2, b2, t.a, t.b, lane, t.wave, acc);
+  else ring_product<false, FOLD>(A, B, n, a0, b0, a1, b1, a2, b2, t.a, t.b, lane, t.wave, acc);
 }
 
 // ------------------------------------------------------------------------------------------------- forward
@@ -1328,7 +1340,7 @@ __device__ __forceinline__ void dx_items(const DistillArgs& p, const Ring& m, in
     B.base = reinterpret_cast<const char*>(p.P) + ((long)s0 * p.Np + tn * RB) * 128;
     f32x16 acc[4];
     const Part<RA> t(__builtin_amdgcn_readfirstlane(p.E - te * RA), wave);
-    tile_product<RA>(A, B, s1 - s0, m, t, lane, acc);
+    tile_product<RA, 0>(A, B, s1 - s0, m, t, lane, acc);
     float4* out = reinterpret_cast<float4*>(p.slab) + ((long)split * tiles + tile) * (RA * RB / 4) + wave * 1024 + lane;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -1374,7 +1386,8 @@ __global__ __launch_bounds__(256) void dt_dx_sum_kernel(DistillArgs p, int et) {
 }
 
 // dW and db: (s X down its rows: K = live rows) x (P down its rows), tiles of RA columns of E x RB words, whole K in one
-// block
+// block.  fp32: chains of 24 stages (768 rows), joined: relative error of dW and db at 131072 x 200 x 512 3.6e-7 and 1.9e-7 (one chain
+// 5.5e-6 and 5.9e-7; at 8192 rows 3.1e-7 and 6e-8 against 9.9e-7 and 4.2e-7), no time measured for it.  16-bit gradients round by more.
 template <typename T, int NP, int NQ, int RA>
 __device__ __forceinline__ void dw_tile(const DistillArgs& p, const Ring& m, int block, int et) {
   constexpr int RB = 384 - RA, BK = 64 / NQ;
@@ -1391,7 +1404,7 @@ __device__ __forceinline__ void dw_tile(const DistillArgs& p, const Ring& m, int
   const float fw = *p.gmax * ldexpf(1.f, -P_EXP - p.sexp[0]), fb = *p.gmax * ldexpf(1.f, -2 * P_EXP);
   f32x16 acc[4];
   const Part<RA> t(__builtin_amdgcn_readfirstlane(p.E + 1 - te * RA), wave);   // (the bias' column too)
-  tile_product<RA>(A, B, (nl + BK - 1) / BK, m, t, lane, acc);
+  tile_product<RA, sizeof(T) == 4 ? 24 : 0>(A, B, (nl + BK - 1) / BK, m, t, lane, acc);
   // a lane holds four neighbouring columns of a word's row at a time
   const bool vec = p.E % 4 == 0 && ((uintptr_t)p.dW % (4 * sizeof(T))) == 0;
 #pragma unroll

@@ -597,3 +597,30 @@ def test_more_rows_than_their_counts_are_added_up_in_every_block(dev):
         tol = 1.01 * bound + 40 * U * bound + half * (value.abs() + bound) + 1e-30
         assert bool(((got.double() - value).abs() <= tol).all())
     assert not bool(dX[0][tgt == PAD].any())
+
+
+def test_gradients_of_the_weights_do_not_lose_bits_with_the_rows(dev):
+    """fp32, 131072 rows: the sums over the rows are chains of 768 rows, joined by one of 171, and random roundings grow with the
+    root of a chain's length: sqrt(768) + sqrt(171) units, and 12 for the operands' 22 bits as in `oracle`.  (One chain of all of
+    them: 362 units, of which 83 were seen.)"""
+    from cvae_amd import ops
+    R, E, V, K, tau = 131072, 24, 60, 2, 2.0
+    g = torch.Generator(device=dev).manual_seed(6)
+    final = torch.tanh(torch.randn(1, R, E, generator=g, device=dev)).requires_grad_()
+    W = (torch.randn(V, E, generator=g, device=dev) * 0.3).requires_grad_()
+    b = (torch.randn(V, generator=g, device=dev) * 0.2).requires_grad_()
+    eos = torch.randint(1, V, (R, 1), generator=g, device=dev)
+    ids = torch.stack([torch.randint(0, V // 2, (R, 1), generator=g, device=dev), torch.randint(V // 2, V, (R, 1), generator=g, device=dev)], 2)
+    top = torch.randn(R, 1, K, generator=g, device=dev)
+    gh, gs = (torch.rand(R, generator=g, device=dev) + 0.5 for _ in range(2))
+    hard, soft = ops.proj_distill(final, W, b, eos, PAD, ids, top, tau)
+    dW, db = torch.autograd.grad([hard, soft], [W, b], [gh, gs])
+    x, w = final.detach()[0].double(), W.detach().double()
+    S = (x[:, None, :] * w[None]).sum(2) + b.detach().double()
+    P = torch.softmax(S, 1) * gh.double()[:, None] + torch.softmax(S / tau, 1) * (gs.double() * tau)[:, None]
+    P.scatter_add_(1, eos, -gh.double()[:, None])
+    P.scatter_add_(1, ids[:, 0], -torch.softmax(top[:, 0].double() / tau, 1) * (gs.double() * tau)[:, None])
+    units = math.sqrt(768) + math.sqrt(171) + 12
+    for name, got, value in (('dW', dW, torch.stack([(P[:, v:v + 1] * x).sum(0) for v in range(V)])), ('db', db, P.sum(0))):
+        off = float((got.double() - value).norm() / value.norm()) / U
+        assert off <= units, (name, off)

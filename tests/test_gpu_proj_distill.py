@@ -624,3 +624,63 @@ def test_gradients_of_the_weights_do_not_lose_bits_with_the_rows(dev):
     for name, got, value in (('dW', dW, torch.stack([(P[:, v:v + 1] * x).sum(0) for v in range(V)])), ('db', db, P.sum(0))):
         off = float((got.double() - value).norm() / value.norm()) / U
         assert off <= units, (name, off)
+
+
+# Wide rows over more than a tile everywhere: an odd and an even number of stages in one plane (300: 5, 330: 6, 513: 9) and in two
+# (10, 11, 17), more than eight tiles of rows, several tiles of words to a range, several ranges to an XCD
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('E,V,K', [(300, 20000, 3), (330, 9001, 3), (513, 9001, 3), (513, 12000, 0)])
+def test_wide_rows_over_many_tiles(dev, E, V, K, dtype):
+    if dtype == 'f32' and not K:
+        K = 2
+    T, R = 18, 70
+    a = inputs(T, R, R, E, V, K, dtype, E + V)
+    a['eos'] = torch.where(a['eos'] == PAD, 3, a['eos'])
+    a['eos'][5, 7:] = PAD
+    assert int((a['eos'] != PAD).sum()) > 8 * 128
+    compare(dev, a, 2.0)
+
+
+# (words: an odd number of blocks of 256, so that two ranges of P are not equally long)
+@pytest.mark.parametrize('dtype,T,R,E,V', [('f32', 64, 80, 300, 24700), ('f32', 64, 80, 200, 24700), ('bf16', 64, 128, 300, 25800),
+                                           ('bf16', 64, 128, 120, 25800), ('f16', 64, 80, 513, 24700), ('f16', 64, 80, 200, 24700)])
+def test_ranges_of_unequal_length(dev, dtype, T, R, E, V):
+    """Two ranges of the vocabulary, the last one shorter, against float64 on the GPU: every 128 rows of dX and every 128 words of dW
+    and db by the norm of what they are off, so that no single tile hides in the others.  fp32: root-mean-square growth as in
+    `check`; 16 bits: the output's half step."""
+    N, words = T * R, (V + 255) // 256 * 256
+    most = (400 << 20) // ((2 if dtype == 'bf16' else 4) * N) // 256 * 256
+    assert most < words <= 2 * most and words // 256 % 2 == 1
+    a = inputs(T, R, R, E, V, 0, dtype, E)
+    a['eos'] = torch.where(a['eos'] == PAD, 3, a['eos'])
+    K, tau = 3, 2.0
+    g = torch.Generator().manual_seed(7)
+    a['ids'] = (torch.randint(0, V, (R, T, 1), generator=g) + torch.tensor([0, 5000, 15001])) % V
+    a['top'], a['gs'] = torch.randn(R, T, K, generator=g), torch.rand(R, generator=g) + 0.5
+    got = run(dev, a, tau)
+    x, w, b = (a[k].to(dev).double() for k in ('final', 'W', 'b'))
+    x = x.reshape(N, E)
+    S = x @ w.t().contiguous() + b
+    tgt, ids = a['eos'].to(dev).t().reshape(N, 1), a['ids'].to(dev).transpose(0, 1).reshape(N, K)
+    sent = torch.arange(R, device=dev).repeat(T)
+    gh, gs = (a[k].to(dev).double()[sent][:, None] for k in ('gh', 'gs'))
+    lse, lse2 = torch.logsumexp(S, 1, keepdim=True), torch.logsumexp(S / tau, 1, keepdim=True)
+    p = torch.softmax(a['top'].to(dev).double().transpose(0, 1).reshape(N, K) / tau, 1)
+    add = lambda v: torch.zeros(R, dtype=torch.float64, device=dev).index_add(0, sent, v)
+    want = dict(hard=add((lse - S.gather(1, tgt))[:, 0]),
+                soft=add(tau ** 2 * (p * (torch.log(p) - S.gather(1, ids) / tau + lse2)).sum(1)))
+    P = torch.exp(S - lse).mul_(gh)
+    P += torch.exp(S / tau - lse2).mul_(gs * tau)
+    del S
+    P.scatter_add_(1, tgt, -gh)
+    P.scatter_add_(1, ids, -p * gs * tau)
+    want['dfinal'], want['dW'], want['db'] = P @ w, P.t().contiguous() @ x, P.sum(0)
+    rel = 2 * (math.sqrt(E) + math.sqrt(max(V, N)) + 64) * U
+    half = torch.finfo(DT[dtype]).eps / 2
+    for k, v in want.items():
+        u = got[k].detach().double().reshape(v.shape)
+        n = 1 if k in ('hard', 'soft') else 128
+        bound = rel if dtype == 'f32' or n == 1 else half
+        for i in range(0, v.shape[0], n):
+            off, size = float((u[i:i + n] - v[i:i + n]).norm()), float(v[i:i + n].norm())
+            assert off <= bound * size, (k, i, off / size, bound)

@@ -808,7 +808,10 @@ __global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
         return *reinterpret_cast<const h8*>(w + r * RB + ch * 16);
       };
       // the rows pass through the ring once: read from memory straight into operands they would come 32 bytes a row at a time
+      // (`row` hides that their places in LDS are the same for every item: kept in registers they would push others into memory)
       h8 xf[NJ][NP][NK];
+      int row = l31;
+      asm volatile("" : "+v"(row));
 #pragma unroll
       for (int half = 0; half < NP; ++half) {
 #pragma unroll
@@ -821,7 +824,7 @@ __global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
 #pragma unroll
             for (int pl = 0; pl < NP; ++pl)
 #pragma unroll
-              for (int kb = 0; kb < NK; ++kb) xf[j][pl][kb] = frag(ring(kb / 4), (NP == 1 ? bn + 32 * j : bn & 32) + l31, kb & 3, pl);
+              for (int kb = 0; kb < NK; ++kb) xf[j][pl][kb] = frag(ring(kb / 4), (NP == 1 ? bn + 32 * j : bn & 32) + row, kb & 3, pl);
         }
         ring_barrier<0>();
       }

@@ -327,6 +327,9 @@ __global__ __launch_bounds__(64 * LR_W, 4) void linrnn_bwd_kernel(LinRnnArgs p) 
   for (int sc = s0 + (s1 - s0 + R - 1) / R * R - R; sc >= s0; sc -= R, buf ^= 1) {   // (no steps: no round)
     const int w0 = sc + wave * LR_C, w1 = min(s1, w0 + LR_C);
     const Steps st = steps_of<VW>(p, L, w0, w1);
+    // (hides that these are the same every round: the addresses made of them, kept in registers, would push others into memory)
+    int ubase = L.base, ybase = L.hbase;
+    asm volatile("" : "+v"(ubase), "+v"(ybase));
     float hin[VW];
 #pragma unroll
     for (int v = 0; v < VW; ++v) hin[v] = p.bounds[(long)(sc / (LR_C * LR_W)) * p.n + L.c + v];
@@ -336,10 +339,10 @@ __global__ __launch_bounds__(64 * LR_W, 4) void linrnn_bwd_kernel(LinRnnArgs p) 
     for (int v = 0; v < VW; ++v) { A[v] = 1.f; X[v] = 0.f; Q[v] = 0.f; }
     if (st != ST_DEAD) {
       Packed<T, VW> rz[LR_C], rn[LR_C], ro[LR_C];
-      load_steps<T, VW>(p, L, st == ST_FULL, p.u, ustep, L.base, w0, rz);
-      load_steps<T, VW>(p, L, st == ST_FULL, p.u, ustep, L.base + p.H, w0, rn);
-      if (G == 3) load_steps<T, VW>(p, L, st == ST_FULL, p.u, ustep, L.base + 2 * p.H, w0, ro);
-      load_steps<T, VW>(p, L, st == ST_FULL, p.dy, p.n, L.hbase, w0, rd);
+      load_steps<T, VW>(p, L, st == ST_FULL, p.u, ustep, ubase, w0, rz);
+      load_steps<T, VW>(p, L, st == ST_FULL, p.u, ustep, ubase + p.H, w0, rn);
+      if (G == 3) load_steps<T, VW>(p, L, st == ST_FULL, p.u, ustep, ubase + 2 * p.H, w0, ro);
+      load_steps<T, VW>(p, L, st == ST_FULL, p.dy, p.n, ybase, w0, rd);
 #pragma unroll
       for (int i = 0; i < LR_C; ++i)
 #pragma unroll
@@ -390,7 +393,7 @@ __global__ __launch_bounds__(64 * LR_W, 4) void linrnn_bwd_kernel(LinRnnArgs p) 
     if (st == ST_DEAD) {
       for (int s = w0; s < w1; ++s)
         if (L.valid) {
-          T* q = du + (long)time_of(p, s) * ustep + (unsigned)L.base;
+          T* q = du + (long)time_of(p, s) * ustep + (unsigned)ubase;
 #pragma unroll
           for (int g = 0; g < G; ++g) *reinterpret_cast<Packed<T, VW>*>(q + g * p.H) = Packed<T, VW>{};
         }
@@ -419,7 +422,7 @@ __global__ __launch_bounds__(64 * LR_W, 4) void linrnn_bwd_kernel(LinRnnArgs p) 
       }
       if (st == ST_MIXED && t >= L.len) gz = gn = go = Packed<T, VW>{};   // exact zeros, whatever the carry holds
       if (s < w1 && L.valid) {
-        T* q = du + (long)t * ustep + (unsigned)L.base;
+        T* q = du + (long)t * ustep + (unsigned)ubase;
         *reinterpret_cast<Packed<T, VW>*>(q) = gz;
         *reinterpret_cast<Packed<T, VW>*>(q + p.H) = gn;
         if (G == 3) *reinterpret_cast<Packed<T, VW>*>(q + 2 * p.H) = go;

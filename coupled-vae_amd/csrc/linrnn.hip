@@ -390,6 +390,7 @@ __global__ __launch_bounds__(64 * LR_W, 4) void linrnn_bwd_kernel(LinRnnArgs p) 
       for (int v = 0; v < VW; ++v)
         carry[v] = fmaf(lds[buf][w][0][lane * VW + v], carry[v], lds[buf][w][2][lane * VW + v]);
     }
+    if (!du) continue;                            // (not wanted: the carry alone goes on, to dh0)
     if (st == ST_DEAD) {
       for (int s = w0; s < w1; ++s)
         if (L.valid) {
@@ -543,7 +544,8 @@ int launch_linrnn_backward(int dtype, int gates, int reverse, int T, int B, int 
                            hipStream_t s) {
   CVAE_TRY(lr_check("linrnn_backward", dtype, gates, T, B, H));
   if ((long)B * H == 0) return 0;
-  CVAE_REQUIRE(T == 0 || (u && dy && du && bounds), "linrnn_backward: null operand");
+  if (!du && !dh0) return 0;
+  CVAE_REQUIRE(T == 0 || (u && dy && bounds), "linrnn_backward: null operand");
   LinRnnArgs a = {};
   a.T = T; a.B = B; a.H = H; a.gates = gates; a.reverse = reverse != 0; a.n = (long)B * H;
   a.u = u; a.len = len; a.bounds = const_cast<float*>(bounds); a.dy = dy; a.dlast = dlast; a.du = du; a.dh0 = dh0;

@@ -519,7 +519,7 @@ class LinearRnnFn(torch.autograd.Function):
         u, length, states = ctx.saved_tensors
         T, B, H = ctx.dims[3:]
         dy, dlast = _c(dy), _c(dlast)
-        du = torch.empty_like(u)
+        du = torch.empty_like(u) if ctx.needs_input_grad[0] else None
         dh0 = _f((B, H), u) if ctx.needs_input_grad[2] else None
         ws = _f((query('cvae_linrnn_workspace', ctx.dims[0], T, B, H),), u)
         call('cvae_linrnn_backward', *ctx.dims, ptr(u), ptr(length), ptr(states), ptr(dy), ptr(dlast), ptr(du),

@@ -210,7 +210,7 @@ int64_t cvae_linrnn_state_floats(int T, int B, int H);
 int64_t cvae_linrnn_workspace(int dtype, int T, int B, int H);
 int cvae_linrnn_forward(int dtype, int gates, int reverse, int T, int B, int H, const void* u, const float* h0,
                         const int64_t* len, void* y, float* h_last, float* states, float* ws, void* stream);
-/* dy[T,B,H], dh_last[B,H] or NULL (zeros) -> du[T,B,gates*H], dh0[B,H] (may be NULL), both overwritten. */
+/* dy[T,B,H], dh_last[B,H] or NULL (zeros) -> du[T,B,gates*H], dh0[B,H], both overwritten; either may be NULL: not wanted. */
 int cvae_linrnn_backward(int dtype, int gates, int reverse, int T, int B, int H, const void* u, const int64_t* len,
                          const float* states, const void* dy, const float* dh_last, void* du, float* dh0, float* ws,
                          void* stream);

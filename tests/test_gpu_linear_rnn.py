@@ -345,3 +345,25 @@ def test_infinite_gates(dev):
         assert h[0, 0] == 0.25 and abs(float(h[0, 1]) - 0.46211715726) < 1e-6 and torch.isnan(h[0, 2])
         assert float(h[0, 3]) == 0.25 * 0.25 + 0.5 * 1.5 and float(h[0, 4]) == 0.25 * 0.25 - 0.5 * 1.5 and float(y[0, 5]) == 0
         assert torch.isnan(y[0]).tolist() == [False, False, True, False, False, False]
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+@pytest.mark.parametrize('T,B,H,gates,ragged', [(9, 3, 20, 3, True), (300, 2, 34, 3, True), (130, 5, 33, 2, False), (1, 4, 8, 2, False)])
+def test_only_the_gradients_that_are_wanted(dev, T, B, H, gates, ragged, dtype):
+    """Frozen pre-activations, or a frozen initial state: the other gradient does not change, and nothing is kept for the one that
+    nobody wants."""
+    from cvae_amd import ops
+    u, h0, dy, dlast = inputs(dev, T, B, H, gates, dtype, 41)
+    length = torch.arange(B, device=dev) * T // B if ragged else None
+    full = run(u, gates, h0, length, False, dy, dlast)
+    for wanted in ('u', 'h0'):
+        leaves = dict(u=u.detach().requires_grad_(wanted == 'u'), h0=h0.detach().requires_grad_(wanted == 'h0'))
+        y, last = ops.linear_rnn(leaves['u'], gates, h0=leaves['h0'], length=length)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        got, = torch.autograd.grad([y, last], [leaves[wanted]], [dy, dlast])
+        assert torch.equal(got, full['d' + wanted]), wanted
+        if wanted == 'h0':
+            spare = torch.cuda.max_memory_allocated() - before          # (its own gradient and the maps of segments, in 512-byte blocks)
+            assert spare < max(u.numel() * u.element_size(), 64 << 10), spare

@@ -107,6 +107,9 @@ template <typename T> __device__ __forceinline__ void load4(const T* row, int k,
     for (int i = 0; i < 4; ++i) x[i] = k + i < E ? (float)row[k + i] : 0.f;
   }
 }
+// x as one rounded fp32 value, whose two planes belong together: the compiler may form hi from x's last product or sum in one
+// instruction that rounds once, and lo from x itself; where the two hi differ (one x in some 2^14), lo mends nothing
+__device__ __forceinline__ void one_value(float& x) { asm("" : "+v"(x)); }
 template <int NP> __device__ __forceinline__ long image_at(int k) { return NP == 1 ? k : (long)(k >> 5) * 64 + (k & 31); }
 template <int NP> __device__ __forceinline__ void store4(_Float16* row, int k, const float (&x)[4]) {
   Packed<f16_t, 4> hi, lo;
@@ -920,6 +923,7 @@ __global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
                   const float t = fmaf(acc[i][j][4 * g + k], c, bv[k]);
                   float x = s1[j] * __builtin_amdgcn_exp2f(t - La[j]);
                   if (TWO) x = fmaf(s2[j], __builtin_amdgcn_exp2f(fmaf(t, p.itau, -Lb[j])), x);
+                  if (NQ == 2) one_value(x);
                   hi[g].set(k, x);
                   if (NQ == 2) lo[g].set(k, x - hi[g].f(k));
                 }
@@ -1258,6 +1262,7 @@ __global__ __launch_bounds__(256, 2) void dt_grad_kernel(DistillArgs p) {
           float x = ca * __builtin_amdgcn_exp2f(t - L1);
           if (TWO) x = fmaf(cb, __builtin_amdgcn_exp2f(fmaf(t, p.itau, -L2)), x);
           x = in ? x : 0.f;
+          if (NQ == 2) one_value(x);
           hi.set(k, x);
           if (NQ == 2) lo.set(k, x - hi.f(k));
         }
@@ -1298,6 +1303,7 @@ __global__ __launch_bounds__(256) void dt_pick_kernel(DistillArgs p) {
     if (p.K) x = fmaf(b, __builtin_amdgcn_exp2f(log_share(pick * (TWO ? p.itau : 1.f), L2)) - share, x);
     const int v = (int)(id - p.v0);
     _Float16* q = p.P + ((long)(v * NQ >> 6) * p.Np + i) * 64 + (v & (64 / NQ - 1));
+    if (NQ == 2) one_value(x);
     const _Float16 hi = (_Float16)x;
     q[0] = hi;
     if (NQ == 2) q[32] = (_Float16)(x - (float)hi);

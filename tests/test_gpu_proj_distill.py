@@ -684,3 +684,15 @@ def test_ranges_of_unequal_length(dev, dtype, T, R, E, V):
         for i in range(0, v.shape[0], n):
             off, size = float((u[i:i + n] - v[i:i + n]).norm()), float(v[i:i + n].norm())
             assert off <= bound * size, (k, i, off / size, bound)
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'f16'])
+@pytest.mark.parametrize('tau', [1.0, 2.5])
+@pytest.mark.parametrize('E', [40, 100, 200, 224])
+def test_both_planes_of_every_entry(dev, E, tau, dtype):
+    """States that are the unit vectors: dW then is d loss / d S itself, transposed, and every one of its 1500 E entries shows both
+    of its fp16 planes alone, with nothing to average it out."""
+    a = inputs(1, E, E, E, 1500, 3, dtype, 26)
+    a['final'] = torch.eye(E)[None].to(DT[dtype])
+    a['eos'] = torch.where(a['eos'] == PAD, 3, a['eos'])
+    compare(dev, a, tau)

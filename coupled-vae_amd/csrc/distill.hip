@@ -973,11 +973,28 @@ __device__ __forceinline__ float half_sum(float v) {
 // does not wait for another load is asked for at once: the ids and teacher logits first.  (Two picked rows of W in flight
 // a group of lanes: with 64 entries a row 47 us for 4815 rows, four 54, eight 74.)
 constexpr int DT_MOST_K = 1024;
+// Ids listed more than once are found through a table of first places, at most half full (comparing all pairs took, for 3520 rows x
+// 200 bf16, 34 us with 64 entries, 178 with 256 and 1950 with 1024; this 26, 66 and 248).
+constexpr int DT_FREE = 0x7fffffff;
+__host__ __device__ __forceinline__ int dt_table_bits(int K) {
+  int bits = 5;
+  while ((1 << bits) < 2 * K) ++bits;
+  return bits;
+}
+__host__ __device__ __forceinline__ int dt_combine_words(int K) {  // of LDS: ids, picked logits, teacher logits, table, repeats
+  return 3 * K + 2 + (1 << dt_table_bits(K)) + (K + 31) / 32;
+}
+__device__ __forceinline__ unsigned table_slot(int id, int bits) { return (unsigned)id * 2654435769u >> (32 - bits); }
 template <typename T, bool TWO>
 __global__ __launch_bounds__(256) void dt_combine_kernel(DistillArgs p) {
   __shared__ float red[4][3];
-  __shared__ int sid[DT_MOST_K + 1];                              // ids inside the vocabulary, else -1; [K]: the target
-  __shared__ float slog[DT_MOST_K], spick[DT_MOST_K + 1];
+  extern __shared__ __attribute__((aligned(16))) char words[];
+  int* sid = reinterpret_cast<int*>(words);                       // ids inside the vocabulary, else -1; [K]: the target
+  float* spick = reinterpret_cast<float*>(sid + p.K + 1);
+  float* slog = spick + p.K + 1;
+  int* table = reinterpret_cast<int*>(slog + p.K);                // first place of an id, at its slot or the next free one
+  const int bits = dt_table_bits(p.K), size = 1 << bits;
+  unsigned* multi = reinterpret_cast<unsigned*>(table + size);    // a bit per entry: its id is listed again
   const int i = blockIdx.x;
   const int nl = *p.nlive;
   if (i >= nl) return;
@@ -989,6 +1006,8 @@ __global__ __launch_bounds__(256) void dt_combine_kernel(DistillArgs p) {
     sid[k] = id >= 0 && id < p.V ? (int)id : -1;
     if (k < K) slog[k] = p.top[at * K + k];
   }
+  for (int i = threadIdx.x; i < size; i += 256) table[i] = DT_FREE;
+  for (int i = threadIdx.x; i < (K + 31) / 32; i += 256) multi[i] = 0;
   // normalisers: every thread a share of the walk's ranges
   const int nt = (nl + DT_TILE - 1) / DT_TILE, splits = dt_splits(nt, p.fvt, p.least);
   float m = -1e30f, a = 0.f, b = 0.f;
@@ -1000,6 +1019,15 @@ __global__ __launch_bounds__(256) void dt_combine_kernel(DistillArgs p) {
     m = mm;
   }
   __syncthreads();
+  for (int k = threadIdx.x; k < K; k += 256) {                    // (a slot holds places of one id for good; the least of them stays)
+    const int id = sid[k];
+    if (id < 0) continue;
+    for (unsigned h = table_slot(id, bits);; h = (h + 1) & (size - 1)) {
+      const int old = atomicCAS(&table[h], DT_FREE, k);
+      if (old == DT_FREE) break;
+      if (sid[old] == id) { atomicMin(&table[h], k); break; }
+    }
+  }
   // Picked logits, base 2: 32 lanes a dot product, 16 bytes a lane where rows allow it (a row of E = 200 in 16 bits is
   // then one access), else single elements.
   const T* x = static_cast<const T*>(p.X) + (long)n * p.E;
@@ -1099,16 +1127,26 @@ __global__ __launch_bounds__(256) void dt_combine_kernel(DistillArgs p) {
   if (lane == 0) share[K] = tgt_listed ? -1.f : 0.f;
   // an id listed several times is one entry of the gradient: its first place holds the sum of the shares, the others -1
   // (as does the target's own place, K, if the teacher lists it)
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
   for (int k = lane; k < K; k += 64) {
     const int id = sid[k];
-    float all = 0.f;
-    bool first = id >= 0;
-    for (int q = 0; q < K; ++q)
-      if (sid[q] == id) {
-        all += slog[q];
-        if (q < k) first = false;
-      }
+    int f = -1;
+    if (id >= 0) {
+      unsigned h = table_slot(id, bits);
+      while (sid[f = table[h]] != id) h = (h + 1) & (size - 1);
+      if (f != k) atomicOr(&multi[f >> 5], 1u << (f & 31));
+    }
+    spick[k] = __int_as_float(f);                                 // (its own lane's entry, no longer needed)
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  for (int k = lane; k < K; k += 64) {
+    const bool first = __float_as_int(spick[k]) == k;
+    float all = slog[k];
+    if (first && (multi[k >> 5] >> (k & 31) & 1))
+      for (int q = k + 1; q < K; ++q)
+        if (sid[q] == sid[k]) all += slog[q];
     share[k] = first ? all : -1.f;
   }
 }
@@ -1567,7 +1605,7 @@ template <typename T, int NP, bool TWO> static int dt_forward(const DistillPlan&
   if (d.nk) dt_rows<NP, 1, TWO, false>(d.nk, a, s);
   else hipLaunchKernelGGL((dt_forward_kernel<NP, TWO>), dim3(DT_WALK_BLOCKS), dim3(256), 0, s, a);
   CVAE_LAUNCH_CHECK("dt_forward_kernel");
-  hipLaunchKernelGGL((dt_combine_kernel<T, TWO>), dim3(a.N), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((dt_combine_kernel<T, TWO>), dim3(a.N), dim3(256), 4 * dt_combine_words(a.K), s, a);
   CVAE_LAUNCH_CHECK("dt_combine_kernel");
   return 0;
 }

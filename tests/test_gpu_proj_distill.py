@@ -696,3 +696,21 @@ def test_both_planes_of_every_entry(dev, E, tau, dtype):
     a['final'] = torch.eye(E)[None].to(DT[dtype])
     a['eos'] = torch.where(a['eos'] == PAD, 3, a['eos'])
     compare(dev, a, tau)
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+@pytest.mark.parametrize('K,V', [(1, 3), (2, 2), (16, 17), (17, 40), (64, 70), (65, 70), (100, 130), (128, 1100), (129, 1100), (513, 600), (1024, 1100)])
+def test_many_entries_with_repeats(dev, K, V, dtype):
+    """Entries drawn with replacement (and some outside the vocabulary), around the sizes at which the table of ids grows; one
+    position lists one id K times, one lists no id twice, one the target last."""
+    T, B, E = 3, 4, 40
+    a = inputs(T, B, B, E, V, K, dtype, 24)
+    g = torch.Generator().manual_seed(25)
+    distinct = a['ids'].clone()
+    a['ids'] = torch.randint(-2, V + 2, (B, T, K), generator=g)
+    a['ids'][0, 0], a['ids'][0, 1] = 5, distinct[0, 1]
+    a['eos'][0] = torch.tensor([7, 9, 11])
+    a['ids'][0, 2, K - 1] = 11
+    a['top'][1, 0, ::3] = float('-inf')
+    compare(dev, a, 2.0)
+    compare(dev, a, 1.0)

@@ -567,7 +567,8 @@ def linear_rnn_step(u, gates, h, out=None):
           'out must be contiguous float32 of shape (B, H)')
     _here(u, h, out)
     u, h = _c(u), _c(h)
-    if out is None:
+    given = out is not None
+    if not given:
         out = _f((B, H), u)
     else:
         at, size = out.data_ptr(), 4 * B * H
@@ -576,6 +577,8 @@ def linear_rnn_step(u, gates, h, out=None):
     y = torch.empty((B, H), dtype=u.dtype, device=u.device)
     call('cvae_linrnn_forward', _DTYPE[u.dtype], gates, 0, 1, B, H, ptr(u), ptr(h), None, ptr(y), ptr(out), None, None,
          stream())
+    if given:
+        torch.autograd.graph.increment_version(out)     # a graph that saved it says so, instead of taking the new values
     return y, out
 
 

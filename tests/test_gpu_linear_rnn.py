@@ -367,3 +367,19 @@ def test_only_the_gradients_that_are_wanted(dev, T, B, H, gates, ragged, dtype):
         if wanted == 'h0':
             spare = torch.cuda.max_memory_allocated() - before          # (its own gradient and the maps of segments, in 512-byte blocks)
             assert spare < max(u.numel() * u.element_size(), 64 << 10), spare
+
+
+def test_a_graph_notices_that_its_saved_state_was_stepped(dev):
+    """out = h is written in place: autograd refuses to use the old state's saved value, as behind torch's own in-place calls."""
+    from cvae_amd import ops
+    w = torch.ones(2, 8, device=dev, requires_grad=True)
+    u, h = torch.randn(2, 24, device=dev), torch.randn(2, 8, device=dev)
+    z = (w * h).sum()
+    ops.linear_rnn_step(u, 3, h)                             # a new state: the old one stays
+    z.backward(retain_graph=True)
+    ops.linear_rnn_step(u, 3, h, out=h)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        z.backward()
+    with torch.inference_mode():
+        g = torch.randn(2, 8, device=dev)
+        assert ops.linear_rnn_step(u, 3, g, out=g)[1] is g

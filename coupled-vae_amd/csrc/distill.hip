@@ -16,8 +16,8 @@
 //
 // What bounds it: 8 N E V operations (S twice, dX, dW; fp32 three times that) against reads of X and W and writes of their
 // gradients, so from a few hundred rows on the matrix cores do, and beside them two exponentials an element and pass at small
-// E.  Measured on live rows, forward and backward: 3650 rows x 1024 x 50000 bf16 1.62 ms (1.49 TFLOP, 0.92 PFLOP/s of
-// useful work; a large library product runs at 1.38), 4815 x 200 x 50000 bf16 with 64 teacher entries at tau 2 0.72 ms.
+// E.  Measured on live rows, forward and backward: 3650 rows x 1024 x 50000 bf16 1.68 ms (1.49 TFLOP, 0.89 PFLOP/s of
+// useful work; a large library product runs at 1.38), 4815 x 200 x 50000 bf16 with 64 teacher entries at tau 2 0.73 ms.
 //
 // Image layout: rows of 128-byte pieces, one plane: 64 values, two planes: 32 hi values then 32 lo values.  A piece is
 // what one row adds to a pipeline stage, so one loop serves both.  Rows are padded to 256 with zeros, columns to 64 (to
@@ -752,7 +752,8 @@ __global__ __launch_bounds__(256, 2) void dt_forward_kernel(DistillArgs p) {
 // at E = 200 spends its time on them.  Stages of 64 K values x 128 (64) words, four buffers, three in flight; K blocks
 // of 16: NK = 4, 8 or 13 (E up to 64, 128, 208; every shipped model has E = 200).  GRAD: instead of folding, the tile
 // leaves as P = a 2^(t - L1) + b 2^(t / tau - L2), through 2 KiB of LDS a wave so that rows leave in runs of 64 bytes.
-// 4815 rows x 200 x 50000 bf16, two exponentials an element: forward 143 us (0.67 PFLOP/s), gradient 216 (it writes 481 MB).
+// 4815 rows x 200 x 50000 bf16, two exponentials an element: forward 143 us (0.67 PFLOP/s), gradient 220 in two ranges (527 MB
+// written and 214 read by the memory counters, 3.4 TB/s); fp16, whose P has two planes, 360 in four.
 // Nothing alone bounds it: left out one at a time when the forward walk took 155, exponentials were worth 35 us, copies 25,
 // products 30.  Standing the fold of one tile between the products of the next (two sets of accumulators) gained nothing there
 // and cost the gradient 10 %.
@@ -971,7 +972,8 @@ __device__ __forceinline__ float half_sum(float v) {
 // One block per live row: the picked logits, the merge of the walk's pairs, the teacher's distribution, the two losses,
 // and the teacher's shares as the backward pass wants them.  A row is one chain of dependent loads, so everything that
 // does not wait for another load is asked for at once: the ids and teacher logits first.  (Two picked rows of W in flight
-// a group of lanes: with 64 entries a row 47 us for 4815 rows, four 54, eight 74.)
+// a group of lanes: with 64 entries a row 41 us for 4815 rows, by the memory counters 159 MB at 4.0 TB/s; four took a seventh more,
+// eight a half.)
 constexpr int DT_MOST_K = 1024;
 // Ids listed more than once are found through a table of first places, at most half full (comparing all pairs took, for 3520 rows x
 // 200 bf16, 34 us with 64 entries, 178 with 256 and 1950 with 1024; this 26, 66 and 248).
@@ -1482,8 +1484,9 @@ __device__ __forceinline__ void dw_tile(const DistillArgs& p, const Ring& m, int
 // Both products of a range in one launch, dX's items in the first DT_DX_BLOCKS blocks (one a CU), dW's tiles behind them:
 // the CUs that one of them leaves idle at its end work on the other.  256 x 128 tiles of eight waves, three buffers, P read once
 // by each product from the caches that the range was sized for.  3650 x 1024 x 50000 bf16: 755 us for both, 0.99 PFLOP/s;
-// matrix cores busy 61 % of the time at the 1.71 GHz that their power leaves.  4815 x 200 x 50000: 279 us, 0.69 PFLOP/s, bound by
-// P: 481 MB by each product at 3.4 TB/s.
+// matrix cores busy 61 % of the time at the 1.71 GHz that their power leaves.  By the memory counters 3.5 GB read
+// and 0.14 written, 4.9 TB/s.  4815 x 200 x 50000: 290 us in two ranges, 0.66 PFLOP/s, matrix cores busy 33 %, bound by P: a range of
+// 240 MB is read by each product, with W and the partial tiles 652 MB read and 36 written, 4.7 TB/s.
 template <typename T, int NP, int NQ, int RAX, int RAW>
 __global__ __launch_bounds__(512, 2) void dt_products_kernel(DistillArgs p, int etx, int etw, int add) {
   __shared__ __attribute__((aligned(16))) char x0[32768];
@@ -1499,8 +1502,8 @@ __global__ __launch_bounds__(512, 2) void dt_products_kernel(DistillArgs p, int 
 }
 
 // ------------------------------------------------------------------------------------------------- host side
-constexpr long DT_PIECE_BYTES = 400L << 20;        // of P: it is written, then read twice (4815 x 50000: 192 MiB 1210 us, 800 MiB 1131,
-                                                   // against 1147, but twice the workspace)
+constexpr long DT_PIECE_BYTES = 400L << 20;        // of P: it is written, then read twice (4815 x 200 x 50000 bf16, both passes: 110 MiB
+                                                   // 1045 us, 200 868, 300 798, 400 773, 900 777 and twice the workspace)
 
 struct DistillPlan {
   long bytes, back_bytes;

@@ -152,7 +152,7 @@ __device__ __forceinline__ void load_steps(const LinRnnArgs& p, const Lane<VW>& 
 }
 
 // The maps of every segment.  BACK: of the backward carry (z, o, dy), else of the state (z, n).  Only where channels are
-// few: 8192 steps x 2 rows x 1000 bf16, 25 us before the pass itself (36 forward, 66 backward).
+// few: 8192 steps x 2 rows x 1000 bf16, 25 us before the pass itself (36 forward, 51 backward).
 template <typename T, int VW, int G, bool BACK>
 __global__ __launch_bounds__(64 * LR_W) void linrnn_maps_kernel(LinRnnArgs p) {
   __shared__ float lds[LR_W][2][64 * VW];
@@ -214,8 +214,9 @@ __global__ __launch_bounds__(64 * LR_W) void linrnn_maps_kernel(LinRnnArgs p) {
 }
 
 // Bound by memory, and by its two sigmoids and the tanh beside it: u is read once, y written once.  2000 steps x 32 rows x
-// 2048, three gates, bf16, ragged: 230 us, 3.7 TB/s of what live steps need (a large copy: 4.7; without the tanh's series 215,
-// without any exponential 197); 110 x 32 x 512 fp32 10.5 us.  Asking for the next round's rows early cost registers,
+// 2048, three gates, bf16, ragged: 236 us with 0.59 GB read and 0.27 written, which is what live steps need and the zeros behind
+// them, 3.7 TB/s by the memory counters (a large copy: 4.7; without the tanh's series 215 us, without any exponential 197);
+// 110 x 32 x 512 fp32 11 us.  Asking for the next round's rows early cost registers,
 // hence blocks on a CU: 292 us.
 template <typename T, int VW, int G>
 __global__ __launch_bounds__(64 * LR_W) void linrnn_fwd_kernel(LinRnnArgs p) {
@@ -306,8 +307,9 @@ __global__ __launch_bounds__(64 * LR_W) void linrnn_fwd_kernel(LinRnnArgs p) {
 }
 
 // Two scans from opposite ends in one pass over u and dy: the state again from the one saved every 64 steps, the carry
-// downwards.  Four waves on a SIMD (two blocks on a CU): 128 registers.  2000 x 32 x 2048, three gates, bf16, ragged: 422 us,
-// 3.7 TB/s (without that bound on the registers 702).
+// downwards.  Four waves on a SIMD (two blocks on a CU): 128 registers.  2000 x 32 x 2048, three gates, bf16, ragged: 377 us with
+// 0.80 GB read and 0.79 written, 4.2 TB/s by the memory counters (without that bound on the registers 702 us; with the addresses
+// of a round kept through all of them, and 21 values in private memory for it, 422).
 template <typename T, int VW, int G>
 __global__ __launch_bounds__(64 * LR_W, 4) void linrnn_bwd_kernel(LinRnnArgs p) {
   __shared__ float lds[2][LR_W][3][64 * VW];      // A (both directions), X of the state, X of the carry

@@ -125,12 +125,19 @@ class CvaeHipError(RuntimeError):
     pass
 
 
+def reachable(t):
+    """The tensor, if a kernel can read it."""
+    if not (t.is_cuda or t.is_pinned()):
+        raise ValueError('tensor on %s, but the library works on GPU memory' % t.device)
+    return t
+
+
 def ptr(t):
-    """Device pointer of a contiguous tensor (None -> NULL)."""
+    """Pointer of a contiguous tensor that the GPU can reach: its own memory or pinned host memory (None -> NULL)."""
     if t is None:
         return None
     assert t.is_contiguous(), 'libcvae_hip needs contiguous tensors'
-    return t.data_ptr()
+    return reachable(t).data_ptr()
 
 
 _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)

@@ -10,7 +10,7 @@ import torch
 
 from . import _lib
 from .settings import settings
-from ._lib import call, ptr, ptr_array, query, stream
+from ._lib import call, ptr, ptr_array, query, reachable, stream
 
 GRU, LSTM = 0, 1
 SKINNY_MAX_ROWS = 256      # csrc/common.hpp: above this row count the recurrence runs as tiled GEMM + cell kernel
@@ -90,6 +90,7 @@ def gemm(A, B, transA=False, transB=False, bias=None, act=ACT_NONE, out=None, be
         out = _f((M, N), A)
     for t in (A, B, out):      # row-strided views are fine: the ABI takes leading dimensions
         assert t.dim() == 2 and t.stride(1) == 1
+        reachable(t)
     call('cvae_gemm', int(transA), int(transB), M, N, K, A.data_ptr(), A.stride(0), B.data_ptr(), B.stride(0),
          out.data_ptr(), out.stride(0), ptr(bias), act, beta, stream())
     return out

@@ -86,3 +86,13 @@ def test_sizes_past_32_bits_are_refused(shape, monkeypatch):
     if shape[0] == 4:
         with pytest.raises(ValueError, match='too large'):
             ops.linear_rnn_step(z(1).expand(shape[1:]), 2, z(1).expand(shape[1], shape[2] // 2))
+
+
+def test_no_operator_hands_pageable_host_memory_to_a_kernel():
+    """A kernel that is given it reads an address that the GPU has not mapped.  Every pointer passes through one place."""
+    x, w, b = z(3, 8), z(4, 8), z(4)
+    for bad in (lambda: _lib.ptr(x), lambda: _lib.ptr_array([x, w]), lambda: ops.linear(x, w, b), lambda: ops.sort_resort(torch.ones(3, dtype=torch.int64)),
+                lambda: ops.gemm(x, w, transB=True)):
+        with pytest.raises(ValueError, match='GPU memory'):
+            bad()
+    assert _lib.ptr(None) is None

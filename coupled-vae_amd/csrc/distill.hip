@@ -952,12 +952,9 @@ __global__ __launch_bounds__(256, 2) void dt_rows_kernel(DistillArgs p) {
   }
 }
 
-// log2 of a picked word's softmax: at most 0, also where its logit (a product of its own) and the normaliser (the walk's) are
+// log2 of a picked word's softmax, its logit (a product of its own) less the normaliser (the walk's): at most 0, also where they are
 // large enough that their roundings say otherwise; a NaN stays one
-__device__ __forceinline__ float log_share(float pick, float lse) {
-  const float d = pick - lse;
-  return d > 0.f ? 0.f : d;
-}
+__device__ __forceinline__ float log_share(float d) { return d > 0.f ? 0.f : d; }
 
 // sum over the 32 lanes of a half-wave: four steps inside rows of 16 lanes on the vector ALU, one through LDS
 __device__ __forceinline__ float half_sum(float v) {
@@ -1106,7 +1103,7 @@ __global__ __launch_bounds__(256) void dt_combine_kernel(DistillArgs p) {
     p.L1[i] = L1;
     p.L2[i] = L2;
     p.slive[n % p.R] = 1;
-    p.hard[n] = (sid[K] >= 0 ? -log_share(spick[K], L1) : L1) * LN2;   // (outside the vocabulary: a logit of 0)
+    p.hard[n] = (sid[K] >= 0 ? -log_share(spick[K] - L1) : L1) * LN2;   // (outside the vocabulary: a logit of 0)
     p.some[i] = K == 0 || !some ? 0.f : tm != tm ? NAN : 1.f;
   }
   float* share = p.share + (long)i * (K + 1);
@@ -1119,7 +1116,7 @@ __global__ __launch_bounds__(256) void dt_combine_kernel(DistillArgs p) {
   bool listed = false;
   for (int k = lane; k < K; k += 64) {
     const float lp = (slog[k] - tm) * p.itau * LOG2E, pk = some && sid[k] >= 0 ? __builtin_amdgcn_exp2f(lp) * inv : 0.f;
-    if (pk != 0.f) loss += pk * (lp - lsum - log_share(spick[k] * p.itau, L2));
+    if (pk != 0.f) loss += pk * (lp - lsum - log_share(fmaf(spick[k], p.itau, -L2)));
     listed |= sid[k] >= 0 && sid[k] == sid[K];
     slog[k] = pk;                                                 // (its own lane's entry) from here on: p_k
   }
@@ -1339,8 +1336,8 @@ __global__ __launch_bounds__(256) void dt_pick_kernel(DistillArgs p) {
     const int64_t id = k < p.K ? ids[k] : tg;
     const float share = p.share[(long)i * (p.K + 1) + k], pick = p.pick[(long)i * (p.K + 1) + k];
     if (id < p.v0 || id >= (int64_t)p.v0 + p.vc || id >= p.V || share == -1.f) continue;
-    float x = a * (__builtin_amdgcn_exp2f(log_share(pick, L1)) - (id == tg ? 1.f : 0.f));
-    if (p.K) x = fmaf(b, __builtin_amdgcn_exp2f(log_share(pick * (TWO ? p.itau : 1.f), L2)) - share, x);
+    float x = a * (__builtin_amdgcn_exp2f(log_share(pick - L1)) - (id == tg ? 1.f : 0.f));
+    if (p.K) x = fmaf(b, __builtin_amdgcn_exp2f(log_share(fmaf(pick, TWO ? p.itau : 1.f, -L2))) - share, x);
     const int v = (int)(id - p.v0);
     _Float16* q = p.P + ((long)(v * NQ >> 6) * p.Np + i) * 64 + (v & (64 / NQ - 1));
     if (NQ == 2) one_value(x);
